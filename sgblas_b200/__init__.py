@@ -21,7 +21,7 @@ __all__ = [
     "SGBLAS_STATUS_INVALID_VALUE", "SGBLAS_STATUS_ARCH_MISMATCH",
     "SGBLAS_STATUS_EXECUTION_FAILED", "SGBLAS_STATUS_INTERNAL_ERROR",
     "SGBLAS_STATUS_NOT_SUPPORTED", "SGBLAS_OP_N", "SGBLAS_OP_T", "SGBLAS_MATH_FP32",
-    "SGBLAS_MATH_TF32", "EXPORTED_SYMBOLS", "MgHandle", "mg_unique_id", "get_device_errors",
+    "SGBLAS_MATH_TF32", "SGBLAS_TYPE_FP32", "SGBLAS_TYPE_BF16", "SGBLAS_MAX_GROUPS", "EXPORTED_SYMBOLS", "MgHandle", "mg_unique_id", "get_device_errors",
 ]
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "lib" / "libsgblas.so"
@@ -39,6 +39,9 @@ SGBLAS_OP_N = 0
 SGBLAS_OP_T = 1
 SGBLAS_MATH_FP32 = 0
 SGBLAS_MATH_TF32 = 1
+SGBLAS_TYPE_FP32 = 0
+SGBLAS_TYPE_BF16 = 1
+SGBLAS_MAX_GROUPS = 1024
 
 _c_int_p = ctypes.POINTER(ctypes.c_int)
 _c_float_p = ctypes.POINTER(ctypes.c_float)
@@ -74,6 +77,32 @@ _SIGNATURES = {
                                            ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
                                            ctypes.c_int, _c_float_p, ctypes.c_void_p,
                                            ctypes.c_int]),
+    # products of language models (include/sgblas/sgblas_lm.h)
+    "sgblasGroupedGemmN": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+        ctypes.c_void_p, _c_float_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong,
+        ctypes.c_void_p, ctypes.c_int, _c_float_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
+    "sgblasGroupedGemmK": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        _c_float_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, _c_float_p,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_longlong]),
+    "sgblasQuantizeFp8": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong]),
+    "sgblasGemmFp8": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
+    "sgblasGroupedGemmFp8": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
+    "sgblasOrthogonalize": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_float_p,
+        ctypes.c_float, ctypes.c_float, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+        ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong]),
     # multi-GPU extension (include/sgblas/sgblas_mg.h)
     "sgblasMgGetUniqueId": (ctypes.c_int, [ctypes.c_void_p]),
     "sgblasMgCreate": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int,
@@ -215,6 +244,66 @@ class Handle:
 
     def sgemm_batched(self, *args) -> None:
         _check("sgblasSgemmBatched", self.sgemm_batched_status(*args))
+
+    # ---- products of language models (sgblas_lm.h): device arguments are
+    # torch tensors or integer addresses; types are SGBLAS_TYPE_*.
+
+    def grouped_gemm_n_status(self, transa, m, n, k, groups, offsets, alpha, a, lda, stride_a, b,
+                              ldb, beta, c, ctype, ldc) -> int:
+        """Raw sgblasGroupedGemmN: offsets is an int32 device array of groups + 1 columns."""
+        return lib.sgblasGroupedGemmN(self._h, transa, m, n, k, groups, _ptr(offsets), _fp(alpha),
+                                      _ptr(a), lda, stride_a, _ptr(b), ldb, _fp(beta), _ptr(c),
+                                      ctype, ldc)
+
+    def grouped_gemm_n(self, *args) -> None:
+        _check("sgblasGroupedGemmN", self.grouped_gemm_n_status(*args))
+
+    def grouped_gemm_k_status(self, m, n, k, groups, offsets, alpha, a, lda, b, ldb, beta, c, ctype,
+                              ldc, stride_c) -> int:
+        """Raw sgblasGroupedGemmK: offsets divide k, the columns of both operands."""
+        return lib.sgblasGroupedGemmK(self._h, m, n, k, groups, _ptr(offsets), _fp(alpha), _ptr(a),
+                                      lda, _ptr(b), ldb, _fp(beta), _ptr(c), ctype, ldc, stride_c)
+
+    def grouped_gemm_k(self, *args) -> None:
+        _check("sgblasGroupedGemmK", self.grouped_gemm_k_status(*args))
+
+    def quantize_fp8_status(self, k, n, block_n, x, xtype, ldx, q, ldq, scale, ldscale, batch=1,
+                            stride_x=0, stride_q=0, stride_scale=0) -> int:
+        """Raw sgblasQuantizeFp8 of one k x n matrix, or of a strided batch."""
+        return lib.sgblasQuantizeFp8(self._h, k, n, batch, block_n, _ptr(x), xtype, ldx, stride_x,
+                                     _ptr(q), ldq, stride_q, _ptr(scale), ldscale, stride_scale)
+
+    def quantize_fp8(self, *args, **kwargs) -> None:
+        _check("sgblasQuantizeFp8", self.quantize_fp8_status(*args, **kwargs))
+
+    def gemm_fp8_status(self, m, n, k, a, lda, scale_a, ldsa, b, ldb, scale_b, ldsb, c, ctype,
+                        ldc) -> int:
+        """Raw sgblasGemmFp8: C = A^T B with e4m3 operands and block scales."""
+        return lib.sgblasGemmFp8(self._h, m, n, k, _ptr(a), lda, _ptr(scale_a), ldsa, _ptr(b), ldb,
+                                 _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
+
+    def gemm_fp8(self, *args) -> None:
+        _check("sgblasGemmFp8", self.gemm_fp8_status(*args))
+
+    def grouped_gemm_fp8_status(self, m, n, k, groups, offsets, a, lda, stride_a, scale_a, ldsa,
+                                stride_sa, b, ldb, scale_b, ldsb, c, ctype, ldc) -> int:
+        """Raw sgblasGroupedGemmFp8."""
+        return lib.sgblasGroupedGemmFp8(self._h, m, n, k, groups, _ptr(offsets), _ptr(a), lda,
+                                        stride_a, _ptr(scale_a), ldsa, stride_sa, _ptr(b), ldb,
+                                        _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
+
+    def grouped_gemm_fp8(self, *args) -> None:
+        _check("sgblasGroupedGemmFp8", self.grouped_gemm_fp8_status(*args))
+
+    def orthogonalize_status(self, m, n, batch, steps, coefficients, eps, scale, g, gtype, ldg,
+                             stride_g, o, ldo, stride_o) -> int:
+        """Raw sgblasOrthogonalize: coefficients are three floats (or None)."""
+        abc = None if coefficients is None else (ctypes.c_float * 3)(*coefficients)
+        return lib.sgblasOrthogonalize(self._h, m, n, batch, steps, abc, eps, scale, _ptr(g), gtype,
+                                       ldg, stride_g, _ptr(o), ldo, stride_o)
+
+    def orthogonalize(self, *args) -> None:
+        _check("sgblasOrthogonalize", self.orthogonalize_status(*args))
 
 
 MG_UNIQUE_ID_BYTES = 128

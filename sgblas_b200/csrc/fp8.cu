@@ -1,0 +1,285 @@
+// Entry points of the e4m3 products, and the quantisation to e4m3 with a
+// scale for each block of 128 (sgblas_lm.h).
+#include "product.hpp"
+
+#include "device.hpp"
+#include "ptx.cuh"
+#include "sgemm_launch.hpp"
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <climits>
+
+namespace sgblas::detail {
+namespace {
+
+namespace t = kern::prod;
+
+constexpr float kFp8Max = 448.0F;
+constexpr unsigned kAmaxFloorBits = 0x0D800000u;   // 2^-100
+constexpr int kBlock = 128;
+constexpr int kPer = 8;             // consecutive values of one thread
+constexpr int kLanes = kBlock / kPer;
+
+struct QuantParams {
+  const void *x;
+  unsigned char *q;
+  float *scale;
+  int k, n, kblocks, ldx, ldq, ldscale;
+  long long stride_x, stride_q, stride_scale;
+  long long blocks;   // of the whole batch
+};
+
+__device__ __forceinline__ float toFloat(float v) { return v; }
+__device__ __forceinline__ float toFloat(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// kPer values at `at` (of `live` that exist; the rest are zero).
+template <typename T, bool kVector>
+__device__ __forceinline__ void loadValues(const T *at, int live, float (&v)[kPer]) {
+  if (kVector && live == kPer) {
+    alignas(16) T raw[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer * static_cast<int>(sizeof(T)) / 16; ++j)
+      reinterpret_cast<uint4 *>(raw)[j] = __ldg(reinterpret_cast<const uint4 *>(at) + j);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = toFloat(raw[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = j < live ? toFloat(at[j]) : 0.0F;
+  }
+}
+
+// Largest magnitude as bits: an integer maximum, which a NaN wins.
+__device__ __forceinline__ unsigned magnitude(const float (&v)[kPer]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  return m;
+}
+
+__device__ __forceinline__ float scaleOf(unsigned amax_bits) {
+  return __fdiv_rn(__uint_as_float(max(amax_bits, kAmaxFloorBits)), kFp8Max);
+}
+
+template <bool kVector>
+__device__ __forceinline__ void storeValues(unsigned char *at, int live, const float (&v)[kPer],
+                                            float scale) {
+  alignas(8) __nv_fp8x2_storage_t q[kPer / 2];
+#pragma unroll
+  for (int j = 0; j < kPer; j += 2)
+    q[j / 2] = __nv_cvt_float2_to_fp8x2(
+        make_float2(__fdiv_rn(v[j], scale), __fdiv_rn(v[j + 1], scale)), __NV_SATFINITE,
+        __NV_E4M3);
+  if (kVector && live == kPer) {
+    *reinterpret_cast<uint2 *>(at) = *reinterpret_cast<const uint2 *>(q);
+  } else {
+    const auto *bytes = reinterpret_cast<const unsigned char *>(q);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (j < live) at[j] = bytes[j];
+  }
+}
+
+// A scale for each 128 values of one column: sixteen lanes per block.
+template <typename T, bool kVector>
+__global__ void __launch_bounds__(256) quantizeColumnsKernel(const QuantParams p) {
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const long long block = (blockIdx.x * 256LL + threadIdx.x) / kLanes;
+  const int part = threadIdx.x % kLanes;
+  const bool in = block < p.blocks;
+  const long long column = in ? block / p.kblocks : 0;
+  const int kb = in ? static_cast<int>(block - column * p.kblocks) : 0;
+  const long long matrix = column / p.n;
+  const long long col = column - matrix * p.n;
+  const int k0 = kb * kBlock + part * kPer;
+  const int live = in ? min(kPer, max(0, p.k - k0)) : 0;
+  float v[kPer];
+  loadValues<T, kVector>(static_cast<const T *>(p.x) + matrix * p.stride_x + col * p.ldx + k0, live,
+                         v);
+  unsigned m = magnitude(v);
+#pragma unroll
+  for (int d = kLanes / 2; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const float scale = scaleOf(m);
+  storeValues<kVector>(p.q + matrix * p.stride_q + col * p.ldq + k0, live, v, scale);
+  if (in && part == 0) p.scale[matrix * p.stride_scale + col * p.ldscale + kb] = scale;
+}
+
+// A scale for each 128 x 128 block: one CTA per block, values in registers.
+template <typename T, bool kVector>
+__global__ void __launch_bounds__(256) quantizeBlocksKernel(const QuantParams p) {
+  __shared__ unsigned warp_max[8];
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const int nblocks = (p.n + kBlock - 1) / kBlock;
+  const long long block = blockIdx.x;
+  const int kb = static_cast<int>(block % p.kblocks);
+  const int nb = static_cast<int>(block / p.kblocks % nblocks);
+  const long long matrix = block / p.kblocks / nblocks;
+  const int part = threadIdx.x % kLanes, row = threadIdx.x / kLanes;   // 16 columns at a time
+  const int k0 = kb * kBlock + part * kPer;
+  const int live_k = min(kPer, max(0, p.k - k0));
+  const T *x = static_cast<const T *>(p.x) + matrix * p.stride_x + k0;
+  constexpr int kPasses = kBlock / (256 / kLanes);
+  float v[kPasses][kPer];
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const long long col = nb * static_cast<long long>(kBlock) + row + i * (256 / kLanes);
+    loadValues<T, kVector>(x + col * p.ldx, col < p.n ? live_k : 0, v[i]);
+    m = max(m, magnitude(v[i]));
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = max(m, warp_max[w]);
+  const float scale = scaleOf(m);
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const long long col = nb * static_cast<long long>(kBlock) + row + i * (256 / kLanes);
+    storeValues<kVector>(p.q + matrix * p.stride_q + col * p.ldq + k0, col < p.n ? live_k : 0, v[i],
+                         scale);
+  }
+  if (threadIdx.x == 0)
+    p.scale[matrix * p.stride_scale + static_cast<long long>(nb) * p.ldscale + kb] = scale;
+}
+
+template <typename T, bool kVector>
+cudaError_t launchQuantize(const QuantParams &p, int block_n, unsigned grid, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return block_n == 1 ? cudaLaunchKernelEx(&cfg, quantizeColumnsKernel<T, kVector>, p)
+                      : cudaLaunchKernelEx(&cfg, quantizeBlocksKernel<T, kVector>, p);
+}
+
+bool isType(sgblasDataType_t type) { return type == SGBLAS_TYPE_FP32 || type == SGBLAS_TYPE_BF16; }
+
+sgblasStatus_t gemmFp8(sgblasHandle_t handle, int m, int n, int k, int groups, const int *offsets,
+                       bool grouped, const void *a, int lda, long long stride_a,
+                       const float *scale_a, int ldsa, long long stride_sa, const void *b, int ldb,
+                       const float *scale_b, int ldsb, void *c, sgblasDataType_t ctype, int ldc) {
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  const int kblocks = k > 0 ? (k - 1) / kBlock + 1 : 0;
+  if (m < 0 || n < 0 || k < 0 || groups < 0 || !isType(ctype) || lda < std::max(1, k) ||
+      ldb < std::max(1, k) || ldc < std::max(1, m) || ldsa < std::max(1, kblocks) ||
+      ldsb < std::max(1, kblocks))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (m == 0 || n == 0 || groups == 0) return SGBLAS_STATUS_SUCCESS;
+  if (c == nullptr || (grouped && offsets == nullptr) ||
+      (k > 0 && (a == nullptr || b == nullptr || scale_a == nullptr || scale_b == nullptr)))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (groups > SGBLAS_MAX_GROUPS) return SGBLAS_STATUS_NOT_SUPPORTED;
+  DeviceInfo dev;
+  const sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  t::Params p = {};
+  p.offsets = offsets;
+  p.groups = groups;
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.c = c;
+  p.c_bf16 = ctype == SGBLAS_TYPE_BF16;
+  p.ldc = ldc;
+  p.alpha = 1.0F;
+  p.scale_a = scale_a;
+  p.scale_b = scale_b;
+  p.ldsa = ldsa;
+  p.ldsb = ldsb;
+  p.stride_sa = stride_sa;
+  p.format = t::kFormatE4m3;
+  NarrowOperand oa, ob;
+  oa.ptr = a;
+  oa.dim0 = k;
+  oa.dim1 = m;
+  oa.ld = lda;
+  oa.count = groups;
+  oa.stride = stride_a;
+  ob.ptr = b;
+  ob.dim0 = k;
+  ob.dim1 = n;
+  ob.ld = ldb;
+  return launchNarrow(handle, dev, 1, t::Ragged::kN, oa, false, ob, false, p);
+}
+
+}  // namespace
+}  // namespace sgblas::detail
+
+extern "C" sgblasStatus_t sgblasQuantizeFp8(sgblasHandle_t handle, int k, int n, int batch,
+                                            int block_n, const void *x, sgblasDataType_t xtype,
+                                            int ldx, long long stride_x, void *q, int ldq,
+                                            long long stride_q, float *scale, int ldscale,
+                                            long long stride_scale) {
+  using namespace sgblas::detail;
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  const int kblocks = k > 0 ? (k - 1) / kBlock + 1 : 0;
+  if (k < 0 || n < 0 || batch < 0 || (block_n != 1 && block_n != kBlock) || !isType(xtype) ||
+      ldx < std::max(1, k) || ldq < std::max(1, k) || ldscale < std::max(1, kblocks))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (k == 0 || n == 0 || batch == 0) return SGBLAS_STATUS_SUCCESS;
+  if (x == nullptr || q == nullptr || scale == nullptr) return SGBLAS_STATUS_INVALID_VALUE;
+  DeviceInfo dev;
+  const sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  QuantParams p = {};
+  p.x = x;
+  p.q = static_cast<unsigned char *>(q);
+  p.scale = scale;
+  p.k = k;
+  p.n = n;
+  p.kblocks = kblocks;
+  p.ldx = ldx;
+  p.ldq = ldq;
+  p.ldscale = ldscale;
+  if (batch > 1) {
+    p.stride_x = stride_x;
+    p.stride_q = stride_q;
+    p.stride_scale = stride_scale;
+  }
+  const long long nblocks = block_n == 1 ? n : (n - 1) / kBlock + 1;
+  p.blocks = nblocks * kblocks * batch;
+  const long long grid = block_n == 1 ? (p.blocks + 256 / kLanes - 1) / (256 / kLanes) : p.blocks;
+  if (grid > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  const auto stream = static_cast<cudaStream_t>(handle->stream);
+  // Whole vectors where every block of kPer values starts on 16 bytes of x
+  // and 8 bytes of q.
+  const int xsize = xtype == SGBLAS_TYPE_BF16 ? 2 : 4;
+  const bool vector = aligned16(x) && ldx * static_cast<long long>(xsize) % 16 == 0 &&
+                      p.stride_x * xsize % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 &&
+                      ldq % 8 == 0 && p.stride_q % 8 == 0;
+  const auto g = static_cast<unsigned>(grid);
+  if (xtype == SGBLAS_TYPE_BF16)
+    return launchStatus(vector ? launchQuantize<__nv_bfloat16, true>(p, block_n, g, stream)
+                               : launchQuantize<__nv_bfloat16, false>(p, block_n, g, stream));
+  return launchStatus(vector ? launchQuantize<float, true>(p, block_n, g, stream)
+                             : launchQuantize<float, false>(p, block_n, g, stream));
+}
+
+extern "C" sgblasStatus_t sgblasGemmFp8(sgblasHandle_t handle, int m, int n, int k, const void *a,
+                                        int lda, const float *scale_a, int ldsa, const void *b,
+                                        int ldb, const float *scale_b, int ldsb, void *c,
+                                        sgblasDataType_t ctype, int ldc) {
+  return sgblas::detail::gemmFp8(handle, m, n, k, 1, nullptr, false, a, lda, 0, scale_a, ldsa, 0, b,
+                                 ldb, scale_b, ldsb, c, ctype, ldc);
+}
+
+extern "C" sgblasStatus_t sgblasGroupedGemmFp8(sgblasHandle_t handle, int m, int n, int k,
+                                               int groups, const int *offsets, const void *a,
+                                               int lda, long long stride_a, const float *scale_a,
+                                               int ldsa, long long stride_sa, const void *b,
+                                               int ldb, const float *scale_b, int ldsb, void *c,
+                                               sgblasDataType_t ctype, int ldc) {
+  return sgblas::detail::gemmFp8(handle, m, n, k, groups, offsets, true, a, lda, stride_a, scale_a,
+                                 ldsa, stride_sa, b, ldb, scale_b, ldsb, c, ctype, ldc);
+}

@@ -1,0 +1,283 @@
+// sgblasOrthogonalize (sgblas_lm.h): Newton-Schulz steps on pairs of fp16
+// matrices.
+//
+// With X scaled to Frobenius norm 1, one step is X <- (c0 I + c1 A + c2 A A) X,
+// A the smaller Gram matrix of X. Three products: A (symmetric, half its
+// tiles), P = c0 I + c1 A + c2 A A (symmetric, half its tiles, the polynomial
+// in the epilogue) and P X. The iteration multiplies small singular values by
+// |c0| per step (3.4^5 = 485 for the usual five steps), and an error in X with
+// them, so single bf16 or fp16 iterates cost digits; pairs hi + lo of fp16
+// keep 22 bits for three products of the tensor core.
+//
+// X stays in G's orientation. m >= n: A = X^T X (both operands contiguous
+// along k), X P (X contiguous along m). m < n: A = X X^T (both contiguous along
+// m and n), P X (both contiguous along k; P is symmetric).
+#include "product.hpp"
+
+#include "device.hpp"
+#include "sgemm_launch.hpp"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <utility>
+
+namespace sgblas::detail {
+namespace {
+
+namespace t = kern::prod;
+
+constexpr int kNormThreads = 256;
+constexpr int kMaxPartials = 256;   // partial sums of squares per matrix
+
+struct NormParams {
+  const void *g;
+  int bf16;
+  int m, n, ldg;
+  long long stride_g;
+  int partials;        // per matrix
+  float *sums;         // [batch][partials]
+  float eps;
+  __half *hi, *lo;     // written by splitKernel
+  int ldx;
+  long long stride_x;
+};
+
+__device__ __forceinline__ float loadG(const NormParams &p, long long matrix, int row, int col) {
+  const long long at = matrix * p.stride_g + static_cast<long long>(col) * p.ldg + row;
+  return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.g)[at])
+                : static_cast<const float *>(p.g)[at];
+}
+
+// Sum over the block, the same in every thread; the order is fixed.
+__device__ __forceinline__ float blockSum(float v) {
+  __shared__ float part[kNormThreads / 32];
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
+  __syncthreads();
+  float s = 0.0F;
+#pragma unroll
+  for (int w = 0; w < kNormThreads / 32; ++w) s += part[w];
+  return s;
+}
+
+// sums[matrix][i] = sum of squares of the columns i, i + partials, ...
+__global__ void __launch_bounds__(kNormThreads) squaresKernel(const NormParams p) {
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  float s = 0.0F;
+  for (int col = blockIdx.x; col < p.n; col += p.partials)
+    for (int row = threadIdx.x; row < p.m; row += kNormThreads) {
+      const float v = loadG(p, blockIdx.y, row, col);
+      s = fmaf(v, v, s);
+    }
+  s = blockSum(s);
+  if (threadIdx.x == 0) p.sums[static_cast<size_t>(blockIdx.y) * p.partials + blockIdx.x] = s;
+}
+
+// X = G / (norm + eps) as pairs.
+__global__ void __launch_bounds__(kNormThreads) splitKernel(const NormParams p) {
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const float *sums = p.sums + static_cast<size_t>(blockIdx.y) * p.partials;
+  const float norm =
+      sqrtf(blockSum(static_cast<int>(threadIdx.x) < p.partials ? sums[threadIdx.x] : 0.0F));
+  const float divisor = norm + p.eps;
+  for (int col = blockIdx.x; col < p.n; col += gridDim.x)
+    for (int row = threadIdx.x; row < p.m; row += kNormThreads) {
+      const float v = loadG(p, blockIdx.y, row, col) / divisor * t::kPairScale;
+      const size_t at = blockIdx.y * static_cast<size_t>(p.stride_x) +
+                        static_cast<size_t>(col) * p.ldx + row;
+      t::splitPair(v, &p.hi[at], &p.lo[at]);
+    }
+}
+
+// One pair matrix of the workspace: `batch` matrices of dim0 x dim1.
+struct PairMatrix {
+  __half *hi = nullptr, *lo = nullptr;
+  int dim0 = 0, dim1 = 0;
+  long long ld = 0, stride = 0;
+};
+
+bool encodePair(CUtensorMap *hi, CUtensorMap *lo, const PairMatrix &x, int batch, bool mn,
+                int rows) {
+  const unsigned long long s1 = x.ld * 2ULL, s2 = x.stride * 2ULL;
+  const unsigned box1 = mn ? 64u : static_cast<unsigned>(rows);
+  return encodeTyped3d(hi, CU_TENSOR_MAP_DATA_TYPE_UINT16, x.hi, x.dim0, x.dim1, batch, s1, s2, 64,
+                       box1, CU_TENSOR_MAP_SWIZZLE_128B) &&
+         encodeTyped3d(lo, CU_TENSOR_MAP_DATA_TYPE_UINT16, x.lo, x.dim0, x.dim1, batch, s1, s2, 64,
+                       box1, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+cudaError_t launchWith(const void *kernel, dim3 grid, int threads, int smem, cudaStream_t stream,
+                       void **args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, kernel, args);
+}
+
+// p.m x p.n product of depth p.k over the batch; the epilogue is p.pair.out.
+template <bool kAMN, bool kBMN, bool kSymmetric>
+sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMatrix &a,
+                                 const PairMatrix &b, t::Params p, cudaStream_t stream) {
+  constexpr int kBN = 128;
+  using G = t::Cfg<2, t::Ragged::kBatch, kBN, kAMN, kBMN, 2, kSymmetric>;
+  auto kernel = t::productKernel<2, t::Ragged::kBatch, kBN, kAMN, kBMN, 2, kSymmetric>;
+  static std::atomic<uint64_t> configured{0};
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes,
+                       &configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  if (!encodePair(&p.tma_a, &p.pair.tma_a_lo, a, batch, kAMN, t::kBM) ||
+      !encodePair(&p.tma_b, &p.pair.tma_b_lo, b, batch, kBMN, kBN))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  p.groups = batch;
+  p.format = t::kFormatFp16;
+  p.err = dev.err;
+  p.tiles_m = (p.m + t::kBM - 1) / t::kBM;
+  p.tiles_n = (p.n + kBN - 1) / kBN;
+  const long long per = kSymmetric ? p.tiles_m * (p.tiles_m + 1LL) / 2
+                                   : static_cast<long long>(p.tiles_m) * p.tiles_n;
+  if (per * batch > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  void *args[] = {&p};
+  return launchStatus(launchWith(reinterpret_cast<const void *>(kernel),
+                                 dim3(static_cast<unsigned>(std::min<long long>(per * batch, dev.sms))),
+                                 t::kThreads, G::kSmemBytes, stream, args));
+}
+
+constexpr size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace sgblas::detail
+
+extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int n, int batch,
+                                              int steps, const float *coefficients, float eps,
+                                              float scale, const void *g, sgblasDataType_t gtype,
+                                              int ldg, long long stride_g, void *o, int ldo,
+                                              long long stride_o) {
+  using namespace sgblas::detail;
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  if (m < 0 || n < 0 || batch < 0 || steps < 1 || steps > 32 ||
+      (gtype != SGBLAS_TYPE_FP32 && gtype != SGBLAS_TYPE_BF16) || ldg < std::max(1, m) ||
+      ldo < std::max(1, m))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (m == 0 || n == 0 || batch == 0) return SGBLAS_STATUS_SUCCESS;
+  if (coefficients == nullptr || g == nullptr || o == nullptr || !(eps >= 0.0F))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (batch > 65535) return SGBLAS_STATUS_NOT_SUPPORTED;   // grid y
+  DeviceInfo dev;
+  sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  const auto stream = static_cast<cudaStream_t>(handle->stream);
+
+  // Workspace: partial sums; X twice (an update cannot overwrite what it
+  // reads), A and P, each a pair.
+  const bool tall = m >= n;
+  const int s = std::min(m, n), l = std::max(m, n);
+  const long long ldx = (m + 63LL) / 64 * 64, lds = (s + 63LL) / 64 * 64;
+  const int partials = std::min(n, kMaxPartials);
+  const size_t sum_bytes = align256(static_cast<size_t>(batch) * partials * sizeof(float));
+  const size_t x_bytes = static_cast<size_t>(ldx) * n * batch * sizeof(__half);   // 128-byte units
+  const size_t s_bytes = static_cast<size_t>(lds) * s * batch * sizeof(__half);
+  if (!ensureWorkspace(handle, kCounterRegionBytes + sum_bytes + 4 * x_bytes + 4 * s_bytes,
+                       dev.device, stream))
+    return SGBLAS_STATUS_NOT_SUPPORTED;
+  auto *base = static_cast<unsigned char *>(handle->workspace) + kCounterRegionBytes;
+  auto *sums = reinterpret_cast<float *>(base);
+  base += sum_bytes;
+  auto take = [&](int dim0, int dim1, long long ld, size_t bytes) {
+    PairMatrix x;
+    x.hi = reinterpret_cast<__half *>(base);
+    x.lo = reinterpret_cast<__half *>(base + bytes);
+    base += 2 * bytes;
+    x.dim0 = dim0;
+    x.dim1 = dim1;
+    x.ld = ld;
+    x.stride = ld * dim1;
+    return x;
+  };
+  PairMatrix x = take(m, n, ldx, x_bytes), next = take(m, n, ldx, x_bytes);
+  PairMatrix gram = take(s, s, lds, s_bytes), poly = take(s, s, lds, s_bytes);
+
+  NormParams q = {};
+  q.g = g;
+  q.bf16 = gtype == SGBLAS_TYPE_BF16;
+  q.m = m;
+  q.n = n;
+  q.ldg = ldg;
+  q.stride_g = batch > 1 ? stride_g : 0;
+  q.partials = partials;
+  q.sums = sums;
+  q.eps = eps;
+  q.hi = x.hi;
+  q.lo = x.lo;
+  q.ldx = static_cast<int>(ldx);
+  q.stride_x = x.stride;
+  void *qargs[] = {&q};
+  st = launchStatus(launchWith(reinterpret_cast<const void *>(squaresKernel),
+                               dim3(partials, batch), kNormThreads, 0, stream, qargs));
+  if (st == SGBLAS_STATUS_SUCCESS)
+    st = launchStatus(launchWith(reinterpret_cast<const void *>(splitKernel),
+                                 dim3(std::min(n, 4 * dev.sms), batch), kNormThreads, 0, stream,
+                                 qargs));
+  for (int step = 0; step < steps && st == SGBLAS_STATUS_SUCCESS; ++step) {
+    t::Params p = {};
+    // A = X^T X or X X^T.
+    p.m = p.n = s;
+    p.k = l;
+    p.ldc = static_cast<int>(lds);
+    p.stride_c = gram.stride;
+    p.pair.out = t::PairOut::kGram;
+    p.pair.hi = gram.hi;
+    p.pair.lo = gram.lo;
+    st = tall ? launchPairProduct<false, false, true>(dev, batch, x, x, p, stream)
+              : launchPairProduct<true, true, true>(dev, batch, x, x, p, stream);
+    if (st != SGBLAS_STATUS_SUCCESS) break;
+    // P = c0 I + c1 A + c2 A A.
+    p.k = s;
+    p.pair.out = t::PairOut::kPoly;
+    p.pair.hi = poly.hi;
+    p.pair.lo = poly.lo;
+    p.pair.prev_hi = gram.hi;
+    p.pair.prev_lo = gram.lo;
+    p.pair.c0 = coefficients[0];
+    p.pair.c1 = coefficients[1];
+    p.pair.c2 = coefficients[2];
+    st = launchPairProduct<false, false, true>(dev, batch, gram, gram, p, stream);
+    if (st != SGBLAS_STATUS_SUCCESS) break;
+    // X P or P X; the last one is the result.
+    p.m = m;
+    p.n = n;
+    if (step == steps - 1) {
+      p.pair.out = t::PairOut::kFinal;
+      p.c = o;
+      p.ldc = ldo;
+      p.stride_c = batch > 1 ? stride_o : 0;
+      p.alpha = scale;
+    } else {
+      p.pair.out = t::PairOut::kUpdate;
+      p.pair.hi = next.hi;
+      p.pair.lo = next.lo;
+      p.ldc = static_cast<int>(ldx);
+      p.stride_c = next.stride;
+    }
+    st = tall ? launchPairProduct<true, false, false>(dev, batch, x, poly, p, stream)
+              : launchPairProduct<false, false, false>(dev, batch, poly, x, p, stream);
+    std::swap(x, next);
+  }
+  if (!markWorkspaceUse(handle, stream) && st == SGBLAS_STATUS_SUCCESS)
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  return st;
+}

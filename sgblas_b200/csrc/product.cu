@@ -1,0 +1,196 @@
+// Launch of the 16- and 8-bit tensor-core products: operand copies, tensor
+// maps, tile width, persistent grid.
+#include "product.hpp"
+
+#include "device.hpp"
+#include "sgemm_launch.hpp"
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+
+namespace sgblas::detail {
+
+namespace t = kern::prod;
+
+sgblasStatus_t currentDevice(DeviceInfo *info) {
+  if (cudaGetDevice(&info->device) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  }
+  const int arch = isSm100(info->device);
+  if (arch < 0) return SGBLAS_STATUS_EXECUTION_FAILED;
+  if (arch == 0) return SGBLAS_STATUS_ARCH_MISMATCH;
+  info->err = deviceErrorWord(info->device);
+  info->sms = smCount(info->device);
+  return info->err == nullptr || info->sms <= 0 ? SGBLAS_STATUS_EXECUTION_FAILED
+                                                : SGBLAS_STATUS_SUCCESS;
+}
+
+namespace {
+
+// Copies rows of `dim0` elements to rows a multiple of 16 bytes apart, so
+// that TMA can read them; eight elements per thread, whose writes are whole
+// vectors. The elements beyond dim0 up to the padded row are not read by TMA.
+template <typename T>
+__global__ void __launch_bounds__(256) copyRowsKernel(const T *__restrict__ src, int dim0,
+                                                      long long rows_per_matrix, long long ld,
+                                                      long long stride, T *__restrict__ dst,
+                                                      long long ldp, long long rows) {
+  constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const long long per_row = (dim0 + kVec - 1) / kVec;
+  const long long total = rows * per_row;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const long long row = i / per_row;
+    const int x = static_cast<int>(i - row * per_row) * kVec;
+    const long long matrix = row / rows_per_matrix;
+    const T *sp = src + matrix * stride + (row - matrix * rows_per_matrix) * ld + x;
+    alignas(16) T v[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v[j] = x + j < dim0 ? sp[j] : T{0};
+    *reinterpret_cast<uint4 *>(dst + row * ldp + x) = *reinterpret_cast<const uint4 *>(v);
+  }
+}
+
+bool tmaReadable(const NarrowOperand &o, int elem_bytes) {
+  return aligned16(o.ptr) && o.ld * elem_bytes % 16 == 0 &&
+         (o.count == 1 || (o.stride * elem_bytes % 16 == 0 && o.stride > 0));
+}
+
+long long copyLd(const NarrowOperand &o, int elem_bytes) {
+  const int unit = 128 / elem_bytes;   // whole 128-byte lines
+  return (o.dim0 + unit - 1LL) / unit * unit;
+}
+
+size_t copyBytes(const NarrowOperand &o, int elem_bytes) {
+  return static_cast<size_t>(copyLd(o, elem_bytes)) * elem_bytes * o.dim1 * o.count;
+}
+
+// Copies the operand to dst and points it there.
+sgblasStatus_t copyOperand(NarrowOperand *o, int elem_bytes, void *dst, int sms,
+                           cudaStream_t stream) {
+  const long long ldp = copyLd(*o, elem_bytes);
+  const long long rows = static_cast<long long>(o->dim1) * o->count;
+  const long long vectors = rows * ((o->dim0 * elem_bytes + 15LL) / 16);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>((vectors + 255) / 256, 8LL * sms)));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e =
+      elem_bytes == 2
+          ? cudaLaunchKernelEx(&cfg, copyRowsKernel<uint16_t>,
+                               static_cast<const uint16_t *>(o->ptr), o->dim0,
+                               static_cast<long long>(o->dim1), o->ld, o->stride,
+                               static_cast<uint16_t *>(dst), ldp, rows)
+          : cudaLaunchKernelEx(&cfg, copyRowsKernel<uint8_t>, static_cast<const uint8_t *>(o->ptr),
+                               o->dim0, static_cast<long long>(o->dim1), o->ld, o->stride,
+                               static_cast<uint8_t *>(dst), ldp, rows);
+  o->ptr = dst;
+  o->ld = ldp;
+  o->stride = ldp * o->dim1;
+  return launchStatus(e);
+}
+
+bool encodeOperand(CUtensorMap *map, const NarrowOperand &o, int elem_bytes, bool mn, int rows) {
+  const auto type = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const unsigned long long stride1 = static_cast<unsigned long long>(o.ld) * elem_bytes;
+  const unsigned long long stride2 =
+      o.count == 1 ? stride1 * o.dim1 : static_cast<unsigned long long>(o.stride) * elem_bytes;
+  if (stride1 >= (1ULL << 40) || stride2 >= (1ULL << 40)) return false;
+  const unsigned box0 = static_cast<unsigned>(t::kRowBytes / elem_bytes);
+  return encodeTyped3d(map, type, o.ptr, o.dim0, o.dim1, o.count, stride1, stride2, box0,
+                       mn ? 64u : static_cast<unsigned>(rows), CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int kElemBytes, t::Ragged kRagged, int kBN, bool kAMN, bool kBMN>
+sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+                           t::Params &p, cudaStream_t stream) {
+  using G = t::Cfg<kElemBytes, kRagged, kBN, kAMN, kBMN, 1, false>;
+  if (p.k > 0 && (!encodeOperand(&p.tma_a, a, kElemBytes, kAMN, t::kBM) ||
+                  !encodeOperand(&p.tma_b, b, kElemBytes, kBMN, kBN)))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  p.tiles_m = (p.m + t::kBM - 1) / t::kBM;
+  p.tiles_n = (p.n + kBN - 1) / kBN;
+  // Tiles, or for ragged columns a bound on them: each group adds at most
+  // one partial tile.
+  const long long tiles =
+      kRagged == t::Ragged::kN
+          ? static_cast<long long>(p.tiles_m) * (p.n / kBN + std::min<long long>(p.groups, p.n))
+          : static_cast<long long>(p.tiles_m) * p.tiles_n * p.groups;
+  if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  auto kernel = t::productKernel<kElemBytes, kRagged, kBN, kAMN, kBMN>;
+  static std::atomic<uint64_t> configured{0};
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes,
+                       &configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, dev.sms)));
+  cfg.blockDim = dim3(t::kThreads);
+  cfg.dynamicSmemBytes = G::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+// Tile width by the tokens a group has on average.
+template <int kElemBytes, bool kAMN>
+sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+                             t::Params &p, cudaStream_t stream) {
+  constexpr auto kN = t::Ragged::kN;
+  const long long mean = p.n / std::max(p.groups, 1);
+  if (mean <= 32) return launchTyped<kElemBytes, kN, 32, kAMN, false>(dev, a, b, p, stream);
+  if (mean <= 64) return launchTyped<kElemBytes, kN, 64, kAMN, false>(dev, a, b, p, stream);
+  if (mean <= 128) return launchTyped<kElemBytes, kN, 128, kAMN, false>(dev, a, b, p, stream);
+  return launchTyped<kElemBytes, kN, 256, kAMN, false>(dev, a, b, p, stream);
+}
+
+}  // namespace
+
+sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_bytes,
+                            t::Ragged ragged, NarrowOperand a, bool a_mn, NarrowOperand b,
+                            bool b_mn, t::Params p) {
+  const auto stream = static_cast<cudaStream_t>(ctx->stream);
+  p.err = dev.err;
+  bool used_workspace = false;
+  if (p.k > 0) {
+    const bool copy_a = !tmaReadable(a, elem_bytes), copy_b = !tmaReadable(b, elem_bytes);
+    const size_t bytes_a = copy_a ? copyBytes(a, elem_bytes) : 0;
+    const size_t bytes_b = copy_b ? copyBytes(b, elem_bytes) : 0;
+    if (copy_a || copy_b) {
+      if (!ensureWorkspace(ctx, kCounterRegionBytes + bytes_a + bytes_b, dev.device, stream))
+        return SGBLAS_STATUS_NOT_SUPPORTED;
+      used_workspace = true;
+      auto *base = static_cast<unsigned char *>(ctx->workspace) + kCounterRegionBytes;
+      sgblasStatus_t st = SGBLAS_STATUS_SUCCESS;
+      if (copy_a) st = copyOperand(&a, elem_bytes, base, dev.sms, stream);
+      if (copy_b && st == SGBLAS_STATUS_SUCCESS)
+        st = copyOperand(&b, elem_bytes, base + bytes_a, dev.sms, stream);
+      if (st != SGBLAS_STATUS_SUCCESS) return st;
+    }
+  }
+  sgblasStatus_t st = SGBLAS_STATUS_INTERNAL_ERROR;
+  if (ragged == t::Ragged::kN && elem_bytes == 2 && a_mn && !b_mn)
+    st = launchRaggedN<2, true>(dev, a, b, p, stream);
+  else if (ragged == t::Ragged::kN && elem_bytes == 2 && !a_mn && !b_mn)
+    st = launchRaggedN<2, false>(dev, a, b, p, stream);
+  else if (ragged == t::Ragged::kN && elem_bytes == 1 && !a_mn && !b_mn)
+    st = launchRaggedN<1, false>(dev, a, b, p, stream);
+  else if (ragged == t::Ragged::kK && elem_bytes == 2 && a_mn && b_mn)
+    st = launchTyped<2, t::Ragged::kK, 256, true, true>(dev, a, b, p, stream);
+  if (used_workspace && !markWorkspaceUse(ctx, stream) && st == SGBLAS_STATUS_SUCCESS)
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  return st;
+}
+
+}  // namespace sgblas::detail

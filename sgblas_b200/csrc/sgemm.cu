@@ -136,24 +136,33 @@ bool encodeMatrix(CUtensorMap *map, const float *ptr, int rows, int cols, int ld
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encodeTyped3d(CUtensorMap *map, CUtensorMapDataType type, const void *ptr,
+                   unsigned long long dim0, unsigned long long dim1, unsigned long long dim2,
+                   unsigned long long stride1_bytes, unsigned long long stride2_bytes,
+                   unsigned box0, unsigned box1, CUtensorMapSwizzle swizzle) {
+  const EncodeTiledFn fn = encodeTiled();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {dim0, dim1, dim2};
+  const cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
+  const cuuint32_t box[3] = {box0, box1, 1};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  return fn(map, type, 3, const_cast<void *>(ptr), dims, strides, box, elem_strides,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encodeTiled3d(CUtensorMap *map, const float *ptr, unsigned long long dim0,
                    unsigned long long dim1, unsigned long long stride1_bytes, int batch,
                    long long stride_elems, unsigned box0, unsigned box1,
                    CUtensorMapSwizzle swizzle) {
-  const EncodeTiledFn fn = encodeTiled();
-  if (fn == nullptr) return false;
   // A single matrix is a batch of one with an unused, valid batch stride.
   const long long stride2 = batch == 1
                                 ? static_cast<long long>((dim1 * stride1_bytes + 15) / 16 * 16)
                                 : stride_elems * 4;
   if (stride2 <= 0 || stride2 % 16 != 0 || stride2 >= (1LL << 40)) return false;
-  const cuuint64_t dims[3] = {dim0, dim1, static_cast<cuuint64_t>(batch)};
-  const cuuint64_t strides[2] = {stride1_bytes, static_cast<cuuint64_t>(stride2)};
-  const cuuint32_t box[3] = {box0, box1, 1};
-  const cuuint32_t elem_strides[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(ptr), dims, strides, box,
-            elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encodeTyped3d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, ptr, dim0, dim1,
+                       static_cast<unsigned long long>(batch), stride1_bytes,
+                       static_cast<unsigned long long>(stride2), box0, box1, swizzle);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

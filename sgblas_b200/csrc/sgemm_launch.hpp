@@ -35,9 +35,14 @@ bool encodeTiled3d(CUtensorMap *map, const float *ptr, unsigned long long dim0,
                    long long stride_elems, unsigned box0, unsigned box1,
                    CUtensorMapSwizzle swizzle);
 
+// The general form: dim2 matrices of dim0 x dim1 elements of `type`, both
+// strides in bytes (multiples of 16), read in box0 x box1 boxes.
+bool encodeTyped3d(CUtensorMap *map, CUtensorMapDataType type, const void *ptr,
+                   unsigned long long dim0, unsigned long long dim1, unsigned long long dim2,
+                   unsigned long long stride1_bytes, unsigned long long stride2_bytes,
+                   unsigned box0, unsigned box1, CUtensorMapSwizzle swizzle);
+
 bool aligned16(const void *p);
-
-
 
 int smCount(int device);
 
