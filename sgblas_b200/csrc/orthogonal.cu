@@ -23,7 +23,6 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cmath>
 #include <utility>
 
 namespace sgblas::detail {
@@ -130,31 +129,37 @@ cudaError_t launchWith(const void *kernel, dim3 grid, int threads, int smem, cud
 }
 
 // p.m x p.n product of depth p.k over the batch; the epilogue is p.pair.out.
-template <bool kAMN, bool kBMN, bool kSymmetric>
-sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMatrix &a,
-                                 const PairMatrix &b, t::Params p, cudaStream_t stream) {
-  constexpr int kBN = 128;
-  using G = t::Cfg<2, t::Ragged::kBatch, kBN, kAMN, kBMN, 2, kSymmetric>;
-  auto kernel = t::productKernel<2, t::Ragged::kBatch, kBN, kAMN, kBMN, 2, kSymmetric>;
-  static std::atomic<uint64_t> configured{0};
-  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes,
-                       &configured))
-    return SGBLAS_STATUS_EXECUTION_FAILED;
-  if (!encodePair(&p.tma_a, &p.pair.tma_a_lo, a, batch, kAMN, t::kBM) ||
-      !encodePair(&p.tma_b, &p.pair.tma_b_lo, b, batch, kBMN, kBN))
+template <class G>
+sgblasStatus_t launchPairTyped(const DeviceInfo &dev, int batch, const PairMatrix &a,
+                               const PairMatrix &b, t::Params &p, cudaStream_t stream) {
+  if (!encodePair(&p.tma_a, &p.pair.tma_a_lo, a, batch, G::kAMN, t::kBM) ||
+      !encodePair(&p.tma_b, &p.pair.tma_b_lo, b, batch, G::kBMN, G::kBRows))
     return SGBLAS_STATUS_EXECUTION_FAILED;
   p.groups = batch;
   p.format = t::kFormatFp16;
+  p.chunk_iters = 4;   // 256 of k: 48 instructions
   p.err = dev.err;
-  p.tiles_m = (p.m + t::kBM - 1) / t::kBM;
-  p.tiles_n = (p.n + kBN - 1) / kBN;
-  const long long per = kSymmetric ? p.tiles_m * (p.tiles_m + 1LL) / 2
-                                   : static_cast<long long>(p.tiles_m) * p.tiles_n;
-  if (per * batch > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
-  void *args[] = {&p};
-  return launchStatus(launchWith(reinterpret_cast<const void *>(kernel),
-                                 dim3(static_cast<unsigned>(std::min<long long>(per * batch, dev.sms))),
-                                 t::kThreads, G::kSmemBytes, stream, args));
+  p.tiles_m = (p.m + G::kTileM - 1) / G::kTileM;
+  p.tiles_n = (p.n + G::kBN - 1) / G::kBN;
+  const long long tiles = batch * (G::kSymmetric ? p.tiles_m * (p.tiles_m + 1LL) / 2
+                                                 : static_cast<long long>(p.tiles_m) * p.tiles_n);
+  if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  return launchProductKernel<G>(dev, p, tiles, stream);
+}
+
+// Pairs of CTAs where their 256 x 256 tiles are at least half as many as the
+// pairs; 128 x 128 tiles of single CTAs below.
+template <bool kAMN, bool kBMN, bool kSymmetric>
+sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMatrix &a,
+                                 const PairMatrix &b, t::Params p, cudaStream_t stream) {
+  constexpr auto kB = t::Ragged::kBatch;
+  const long long tm = (p.m + 255) / 256, tn = (p.n + 255) / 256;
+  const long long tiles = batch * (kSymmetric ? tm * (tm + 1) / 2 : tm * tn);
+  if (4 * tiles >= dev.sms)
+    return launchPairTyped<t::Cfg<2, kB, 256, kAMN, kBMN, true, 2, kSymmetric>>(dev, batch, a, b, p,
+                                                                                stream);
+  return launchPairTyped<t::Cfg<2, kB, 128, kAMN, kBMN, false, 2, kSymmetric>>(dev, batch, a, b, p,
+                                                                               stream);
 }
 
 constexpr size_t align256(size_t v) { return (v + 255) / 256 * 256; }
@@ -263,9 +268,10 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
     if (step == steps - 1) {
       p.pair.out = t::PairOut::kFinal;
       p.c = o;
+      p.c_bf16 = 1;
       p.ldc = ldo;
       p.stride_c = batch > 1 ? stride_o : 0;
-      p.alpha = scale;
+      p.alpha = scale / (t::kPairScale * t::kPairScale);
     } else {
       p.pair.out = t::PairOut::kUpdate;
       p.pair.hi = next.hi;

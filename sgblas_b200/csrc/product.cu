@@ -109,38 +109,22 @@ bool encodeOperand(CUtensorMap *map, const NarrowOperand &o, int elem_bytes, boo
                        mn ? 64u : static_cast<unsigned>(rows), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int kElemBytes, t::Ragged kRagged, int kBN, bool kAMN, bool kBMN>
+template <class G>
 sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
                            t::Params &p, cudaStream_t stream) {
-  using G = t::Cfg<kElemBytes, kRagged, kBN, kAMN, kBMN, 1, false>;
-  if (p.k > 0 && (!encodeOperand(&p.tma_a, a, kElemBytes, kAMN, t::kBM) ||
-                  !encodeOperand(&p.tma_b, b, kElemBytes, kBMN, kBN)))
+  if (p.k > 0 && (!encodeOperand(&p.tma_a, a, G::kElemBytes, G::kAMN, t::kBM) ||
+                  !encodeOperand(&p.tma_b, b, G::kElemBytes, G::kBMN, G::kBRows)))
     return SGBLAS_STATUS_EXECUTION_FAILED;
-  p.tiles_m = (p.m + t::kBM - 1) / t::kBM;
-  p.tiles_n = (p.n + kBN - 1) / kBN;
+  p.tiles_m = (p.m + G::kTileM - 1) / G::kTileM;
+  p.tiles_n = (p.n + G::kBN - 1) / G::kBN;
   // Tiles, or for ragged columns a bound on them: each group adds at most
   // one partial tile.
   const long long tiles =
-      kRagged == t::Ragged::kN
-          ? static_cast<long long>(p.tiles_m) * (p.n / kBN + std::min<long long>(p.groups, p.n))
+      G::kRagged == t::Ragged::kN
+          ? static_cast<long long>(p.tiles_m) * (p.n / G::kBN + std::min<long long>(p.groups, p.n))
           : static_cast<long long>(p.tiles_m) * p.tiles_n * p.groups;
   if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
-  auto kernel = t::productKernel<kElemBytes, kRagged, kBN, kAMN, kBMN>;
-  static std::atomic<uint64_t> configured{0};
-  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes,
-                       &configured))
-    return SGBLAS_STATUS_EXECUTION_FAILED;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, dev.sms)));
-  cfg.blockDim = dim3(t::kThreads);
-  cfg.dynamicSmemBytes = G::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1] = {};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p));
+  return launchProductKernel<G>(dev, p, tiles, stream);
 }
 
 // Tile width by the tokens a group has on average.
@@ -149,10 +133,13 @@ sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, cons
                              t::Params &p, cudaStream_t stream) {
   constexpr auto kN = t::Ragged::kN;
   const long long mean = p.n / std::max(p.groups, 1);
-  if (mean <= 32) return launchTyped<kElemBytes, kN, 32, kAMN, false>(dev, a, b, p, stream);
-  if (mean <= 64) return launchTyped<kElemBytes, kN, 64, kAMN, false>(dev, a, b, p, stream);
-  if (mean <= 128) return launchTyped<kElemBytes, kN, 128, kAMN, false>(dev, a, b, p, stream);
-  return launchTyped<kElemBytes, kN, 256, kAMN, false>(dev, a, b, p, stream);
+  if (mean <= 32)
+    return launchTyped<t::Cfg<kElemBytes, kN, 32, kAMN, false, false>>(dev, a, b, p, stream);
+  if (mean <= 64)
+    return launchTyped<t::Cfg<kElemBytes, kN, 64, kAMN, false, false>>(dev, a, b, p, stream);
+  if (mean <= 128)
+    return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false>>(dev, a, b, p, stream);
+  return launchTyped<t::Cfg<kElemBytes, kN, 256, kAMN, false, true>>(dev, a, b, p, stream);
 }
 
 }  // namespace
@@ -162,6 +149,9 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
                             bool b_mn, t::Params p) {
   const auto stream = static_cast<cudaStream_t>(ctx->stream);
   p.err = dev.err;
+  // Chains of one block of 128 (e4m3) or 512 of k; a BF16 result of BF16
+  // operands is rounded at 2^-9, a thousand times a whole chain's error.
+  p.chunk_iters = elem_bytes == 1 ? 1 : p.c_bf16 ? INT_MAX : 8;
   bool used_workspace = false;
   if (p.k > 0) {
     const bool copy_a = !tmaReadable(a, elem_bytes), copy_b = !tmaReadable(b, elem_bytes);
@@ -187,7 +177,7 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
   else if (ragged == t::Ragged::kN && elem_bytes == 1 && !a_mn && !b_mn)
     st = launchRaggedN<1, false>(dev, a, b, p, stream);
   else if (ragged == t::Ragged::kK && elem_bytes == 2 && a_mn && b_mn)
-    st = launchTyped<2, t::Ragged::kK, 256, true, true>(dev, a, b, p, stream);
+    st = launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true>>(dev, a, b, p, stream);
   if (used_workspace && !markWorkspaceUse(ctx, stream) && st == SGBLAS_STATUS_SUCCESS)
     return SGBLAS_STATUS_EXECUTION_FAILED;
   return st;

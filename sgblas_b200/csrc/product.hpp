@@ -3,13 +3,18 @@
 #define SGBLAS_B200_PRODUCT_HPP_
 
 #include "context.hpp"
+#include "device.hpp"
 #include "product_tile.cuh"
+#include "sgemm_launch.hpp"
 
 #include <sgblas/sgblas_lm.h>
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cstddef>
+#include <cstdint>
 
 namespace sgblas::detail {
 
@@ -30,6 +35,35 @@ struct DeviceInfo {
   unsigned *err = nullptr;
 };
 sgblasStatus_t currentDevice(DeviceInfo *info);
+
+// Persistent launch of productKernel<G> over at most `tiles` tiles: a worker
+// (a CTA, or a cluster of two) per SM (or two).
+template <class G>
+sgblasStatus_t launchProductKernel(const DeviceInfo &dev, const kern::prod::Params &p,
+                                   long long tiles, cudaStream_t stream) {
+  auto kernel = kern::prod::productKernel<G>;
+  static std::atomic<uint64_t> configured{0};
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes,
+                       &configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  constexpr int kCtas = G::kTwo ? 2 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim =
+      dim3(static_cast<unsigned>(kCtas * std::min<long long>(tiles, dev.sms / kCtas)));
+  cfg.blockDim = dim3(kern::prod::kThreads);
+  cfg.dynamicSmemBytes = G::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kCtas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = G::kTwo ? 2 : 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p));
+}
 
 // Launches a product of `elem_bytes` operands (1: e4m3, 2: 16-bit). `mn`
 // operands are contiguous along m (or n) instead of k. p carries the sizes,

@@ -1,19 +1,27 @@
 // Tensor-core products with 16- and 8-bit operands (bf16, pairs of fp16,
 // e4m3): C = op(A) * op(B) per group or matrix, FP32 sums.
 //
-// One persistent CTA per SM walks 128 x N tiles of C: rows (m) on the 128
-// TMEM lanes, columns (n; tokens, where the groups are ragged along n) on the
-// instruction's N. A ragged group's last tile costs what it holds: N is set
-// per tile in steps of 16. Warp roles (12 warps):
+// One persistent CTA per SM walks 128 x N tiles of C, or a pair of CTAs
+// (cta_group::2) 256 x 256 ones: rows (m) on the TMEM lanes, columns (n;
+// tokens, where the groups are ragged along n) on the instruction's N. A
+// ragged group's last tile costs what it holds: N is set per tile in steps of
+// 16 (32 for a pair). Warp roles (12 warps):
 //   warp 0      TMA producer: 128-byte wide k slices of A and B into a ring;
 //   warp 1      MMA issuer: tcgen05.mma into one of two TMEM accumulators;
 //   warp 2      allocates and frees TMEM;
 //   warps 4-11  epilogue: two warps per TMEM lane quarter, half the columns
-//               each, keep the tile's sums in registers.
+//               each, keep the tile's sums in registers and write them out
+//               through shared memory.
+// In a pair, CTA r loads and holds rows [128 r, 128 r + 128) of the tile and
+// half of its columns' operand; the even CTA issues for both. A k slice then
+// costs each SM 32 KiB of operands instead of 48 for the same work, which
+// is what a single CTA's 128 x 256 tile is bound by (96 bytes per clock at
+// the tensor core's rate).
 //
 // Sums. The tensor core's FP32 adder truncates: the relative error of a chain
 // grows with its length (measured 3e-7 after 32 instructions, 3e-6 after 512).
-// So the k range is cut into chunks of kChunkIters slices; the issuer
+// So the k range is cut into chunks (128 to 512 of k; none for a
+// BF16 result of BF16 operands, whose rounding is a thousand times larger); the issuer
 // alternates between the two accumulators, and the epilogue adds each chunk
 // to the registers with rounding to nearest. For e4m3 the chunk is one block
 // of 128, and the same addition applies the block's scales.
@@ -40,9 +48,11 @@ constexpr int kRowBytes = 128;      // one 128-byte swizzle row
 constexpr int kAccums = 2;
 constexpr int kThreads = 384;
 constexpr int kEpilogueWarp0 = 4;
-constexpr int kEpilogueThreads = 256;
+constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueThreads = 32 * kEpilogueWarps;
+constexpr int kOutCols = 32;         // columns a warp passes through shared memory at once
 constexpr int kMaxGroups = 1024;
-constexpr int kScaleBatch = 8;      // blocks of 128 whose scales are staged at once
+constexpr int kScaleBatch = 4;      // blocks of 128 whose scales are staged at once
 
 // Which index the groups divide: n (columns of B and C), k (columns of A and
 // B), or none (a strided batch).
@@ -50,35 +60,46 @@ enum class Ragged { kN, kK, kBatch };
 
 // kPlanes 2: every operand is a pair of fp16 matrices, hi + lo, and a product
 // is hi hi + hi lo + lo hi. kSymmetric: C is symmetric; only tiles on and
-// below the diagonal are computed, and stored twice.
-template <int kElemBytes, Ragged kRagged, int kBN_, bool kAMN, bool kBMN, int kPlanes,
-          bool kSymmetric>
+// below the diagonal are computed, and stored twice. kTwo: a pair of CTAs.
+template <int kElemBytes_, Ragged kRagged_, int kBN_, bool kAMN_, bool kBMN_, bool kTwo_,
+          int kPlanes_ = 1, bool kSymmetric_ = false>
 struct Cfg {
+  static constexpr int kElemBytes = kElemBytes_;
+  static constexpr Ragged kRagged = kRagged_;
+  static constexpr int kBN = kBN_;                     // columns of the tile
+  static constexpr bool kAMN = kAMN_, kBMN = kBMN_;
+  static constexpr bool kTwo = kTwo_;
+  static constexpr int kPlanes = kPlanes_;
+  static constexpr bool kSymmetric = kSymmetric_;
   static constexpr bool kBytes = kElemBytes == 1;
-  static constexpr int kBN = kBN_;
+  static constexpr int kTileM = kTwo ? 2 * kBM : kBM;  // rows of the tile
+  static constexpr int kBRows = kTwo ? kBN / 2 : kBN;  // columns whose operand this CTA loads
+  static constexpr int kNStep = kTwo ? 32 : 16;        // granularity of the instruction's N
   static constexpr int kBK = kRowBytes / kElemBytes;   // 64 or 128
   static constexpr int kMmaK = 32 / kElemBytes;        // 16 or 32
-  static constexpr int kChunkIters = kBytes ? 1 : kPlanes == 2 ? 4 : 8;   // 128, 256 or 512 of k
   static constexpr int kABytes = kBM * kRowBytes;
-  static constexpr int kBBytes = kBN * kRowBytes;
+  static constexpr int kBBytes = kBRows * kRowBytes;
   static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
   static constexpr int kScaleBytes = kBytes ? 2 * kScaleBatch * kBN * 4 : 0;
-  static constexpr int kFit = (208 * 1024 - kScaleBytes) / kStageBytes;
+  static constexpr int kOutBytes = kEpilogueWarps * kOutCols * 64;
+  static constexpr int kFit = (217 * 1024 - kScaleBytes - kOutBytes) / kStageBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
-  static constexpr int kTmemColumns = kAccums * kBN < 32 ? 32 : kAccums * kBN;
-  static constexpr int kBarrierBytes = 8 * (2 * kStages + 2 * kAccums);
-  static constexpr int kSmemBytes = kStages * kStageBytes + kScaleBytes + kBarrierBytes + 1024;
+  static constexpr int kTmemColumns = kAccums * kBN;
+  static constexpr int kBarrierBytes = 8 * (3 * kStages + 2 * kAccums);
+  static constexpr int kSmemBytes =
+      kStages * kStageBytes + kScaleBytes + kOutBytes + kBarrierBytes + 1024;
   static_assert(kBN == 32 || kBN == 64 || kBN == 128 || kBN == 256, "tile width");
-  static_assert(!kSymmetric || kBN == kBM, "square tiles");
+  static_assert(!kSymmetric || kBN == kTileM, "square tiles");
   static_assert(!kBytes || (!kAMN && !kBMN), "8-bit operands are K-major");
-  static_assert(kSmemBytes <= 218 * 1024, "shared memory per CTA, beside the group table");
+  static_assert(!kBMN || kBRows % 64 == 0, "whole boxes");
+  static_assert(kStages >= 2 && kSmemBytes <= 218 * 1024 + 512, "shared memory beside the table");
 };
 
 // What the epilogue of a pair product writes (values v of the sum):
 //   kGram    hi + lo of v * 2^-12
 //   kPoly    hi + lo of c2 v 2^-12 + c1 A + c0 2^12 I, A the pair at prev
 //   kUpdate  hi + lo of v * 2^-12
-//   kFinal   bf16 of v * 2^-24 * alpha
+//   kFinal   bf16 of v * alpha
 // Pairs hold 2^12 times their value: fp16 then keeps 22 bits of every value
 // above 2^-16 and an absolute 2^-37 below, and reaches 15.99.
 enum class PairOut { kGram, kPoly, kUpdate, kFinal };
@@ -106,6 +127,7 @@ struct Params {
   const float *scale_a, *scale_b;   // e4m3: per (128 of k, 128 of m) and (128 of k, column)
   int ldsa, ldsb;
   long long stride_sa;
+  int chunk_iters;            // k slices of one chain
   unsigned format;            // the instruction descriptor's type bits
   unsigned *err;
   PairParams pair;
@@ -133,11 +155,11 @@ __device__ __forceinline__ uint64_t smemDesc(uint32_t addr) {
   return d;
 }
 
-template <bool kAMN, bool kBMN>
+template <class G>
 __device__ __forceinline__ uint32_t instrDesc(unsigned format, int n) {
-  return (1u << 4) | format | (static_cast<uint32_t>(kAMN) << 15) |
-         (static_cast<uint32_t>(kBMN) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(kBM >> 4) << 24);
+  return (1u << 4) | format | (static_cast<uint32_t>(G::kAMN) << 15) |
+         (static_cast<uint32_t>(G::kBMN) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(G::kTileM >> 4) << 24);
 }
 
 // The groups as one CTA sees them: offsets clamped to [0, total], and for
@@ -152,17 +174,17 @@ struct Tile {
   int group, m0, n0, cols, k0, klen;
 };
 
-template <Ragged kRagged, int kBN, bool kSymmetric>
+template <class G>
 __device__ __forceinline__ int tileCount(const Params &p, const GroupTable &t) {
-  if constexpr (kSymmetric) return p.tiles_m * (p.tiles_m + 1) / 2 * p.groups;
-  if constexpr (kRagged == Ragged::kN) return p.tiles_m * t.first[p.groups];
+  if constexpr (G::kSymmetric) return p.tiles_m * (p.tiles_m + 1) / 2 * p.groups;
+  if constexpr (G::kRagged == Ragged::kN) return p.tiles_m * t.first[p.groups];
   return p.tiles_m * p.tiles_n * p.groups;
 }
 
-template <Ragged kRagged, int kBN, bool kSymmetric>
+template <class G>
 __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int index) {
   Tile r;
-  if constexpr (kSymmetric) {
+  if constexpr (G::kSymmetric) {
     const int per = p.tiles_m * (p.tiles_m + 1) / 2;
     r.group = index / per;
     const int i = index - r.group * per;
@@ -170,14 +192,14 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
     int tm = static_cast<int>((sqrtf(8.0F * static_cast<float>(i) + 1.0F) - 1.0F) * 0.5F);
     while (tm * (tm + 1) / 2 > i) --tm;
     while ((tm + 1) * (tm + 2) / 2 <= i) ++tm;
-    r.m0 = tm * kBM;
-    r.n0 = (i - tm * (tm + 1) / 2) * kBN;
-    r.cols = min(kBN, p.n - r.n0);
+    r.m0 = tm * G::kTileM;
+    r.n0 = (i - tm * (tm + 1) / 2) * G::kBN;
+    r.cols = min(G::kBN, p.n - r.n0);
     r.k0 = 0;
     r.klen = p.k;
-  } else if constexpr (kRagged == Ragged::kN) {
+  } else if constexpr (G::kRagged == Ragged::kN) {
     const int nt = index / p.tiles_m;
-    r.m0 = (index - nt * p.tiles_m) * kBM;
+    r.m0 = (index - nt * p.tiles_m) * G::kTileM;
     int lo = 0, hi = p.groups;   // the last group whose first tile is <= nt
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -185,8 +207,8 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
       else hi = mid;
     }
     r.group = lo;
-    r.n0 = t.offset[lo] + (nt - t.first[lo]) * kBN;
-    r.cols = min(kBN, t.offset[lo + 1] - r.n0);
+    r.n0 = t.offset[lo] + (nt - t.first[lo]) * G::kBN;
+    r.cols = min(G::kBN, t.offset[lo + 1] - r.n0);
     r.k0 = 0;
     r.klen = p.k;
   } else {
@@ -194,12 +216,12 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
     r.group = index / per;
     const int i = index - r.group * per;
     const int tn = i / p.tiles_m;
-    r.m0 = (i - tn * p.tiles_m) * kBM;
-    r.n0 = tn * kBN;
-    r.cols = min(kBN, p.n - r.n0);
+    r.m0 = (i - tn * p.tiles_m) * G::kTileM;
+    r.n0 = tn * G::kBN;
+    r.cols = min(G::kBN, p.n - r.n0);
     r.k0 = 0;
     r.klen = p.k;
-    if constexpr (kRagged == Ragged::kK) {
+    if constexpr (G::kRagged == Ragged::kK) {
       r.k0 = t.offset[r.group];
       r.klen = max(0, t.offset[r.group + 1] - r.k0);
     }
@@ -208,10 +230,10 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
 }
 
 // Fills the table (all threads; ends with a barrier).
-template <Ragged kRagged, int kBN>
+template <class G>
 __device__ __forceinline__ void readGroups(const Params &p, GroupTable *t) {
-  if constexpr (kRagged == Ragged::kBatch) return;
-  const int total = kRagged == Ragged::kN ? p.n : p.k;
+  if constexpr (G::kRagged == Ragged::kBatch) return;
+  const int total = G::kRagged == Ragged::kN ? p.n : p.k;
   if (p.offsets == nullptr) {
     if (threadIdx.x == 0) {
       t->offset[0] = 0;
@@ -222,13 +244,13 @@ __device__ __forceinline__ void readGroups(const Params &p, GroupTable *t) {
       t->offset[g] = min(max(p.offsets[g], 0), total);
   }
   __syncthreads();
-  if constexpr (kRagged == Ragged::kN) {
+  if constexpr (G::kRagged == Ragged::kN) {
     if (threadIdx.x < 32) {
       int sum = 0;
       for (int g0 = 0; g0 < p.groups; g0 += 32) {
         const int g = g0 + static_cast<int>(threadIdx.x);
         int v = 0;
-        if (g < p.groups) v = (max(0, t->offset[g + 1] - t->offset[g]) + kBN - 1) / kBN;
+        if (g < p.groups) v = (max(0, t->offset[g + 1] - t->offset[g]) + G::kBN - 1) / G::kBN;
         int scan = v;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -262,56 +284,238 @@ __device__ __forceinline__ void splitPair(float v, __half *hi, __half *lo) {
   *lo = __float2half_rn(v - __half2float(*hi));
 }
 
-// Epilogue of a pair product: this thread's row, kHalf columns from col_begin.
-template <int kHalf, bool kSymmetric>
-__device__ __forceinline__ void storePair(const Params &p, const Tile &t, int row, int col_begin,
-                                          const float (&acc)[kHalf]) {
-  if (row >= p.m) return;
-  const size_t matrix = static_cast<size_t>(t.group) * static_cast<size_t>(p.stride_c);
-  const bool mirror = kSymmetric && t.m0 != t.n0;
+// A warp's share of a tile in registers: 32 rows by 8 * kBlocks columns, as
+// tmemFragments gives them. acc[4 * i + r] holds columns 8 i + 2 (t % 4) + {0, 1}
+// of row 8 r + t / 4.
+//
+// 16-bit results pass through shared memory, 32 columns at a time: stmatrix
+// transposes each 8 x 8 block, so that a column's 32 rows (64 bytes) lie
+// together and leave in vectors. The 16-byte pieces of a column are rotated by
+// the column's pair, which spreads eight columns over all banks.
+__device__ __forceinline__ uint32_t outSlot(int col, int piece) {
+  return static_cast<uint32_t>(col * 64 + ((piece ^ (col / 2 % 4)) * 16));
+}
+
+// Block i of the columns (8 of them) into the staging area.
+__device__ __forceinline__ void stageBlock(unsigned char *out, int block, int lane,
+                                           const uint32_t (&w)[4]) {
+  storeMatrixTrans4(smemAddr(out) + outSlot(block * 8 + lane % 8, lane / 8), w[0], w[1], w[2], w[3]);
+}
+
+// kOutCols staged columns (of which `cols` exist) to c: vectors of eight rows
+// where the address allows, else a row per lane.
+__device__ __forceinline__ void copyOut(const unsigned char *out, uint16_t *c, long long ldc,
+                                        int cols, int rows, int lane, bool vector) {
+  __syncwarp();
+  if (vector && rows >= 32) {
 #pragma unroll
-  for (int j0 = 0; j0 < kHalf; j0 += 8) {
-    if (col_begin + j0 >= t.cols) break;
-    alignas(16) __half hi[8], lo[8];
+    for (int i = 0; i < kOutCols / 8; ++i) {
+      const int col = i * 8 + lane / 4;
+      if (col < cols)
+        *reinterpret_cast<uint4 *>(c + col * ldc + lane % 4 * 8) =
+            *reinterpret_cast<const uint4 *>(out + outSlot(col, lane % 4));
+    }
+  } else if (lane < rows) {
+#pragma unroll 4
+    for (int col = 0; col < min(cols, kOutCols); ++col)
+      c[col * ldc + lane] =
+          *reinterpret_cast<const uint16_t *>(out + outSlot(col, lane / 8) + lane % 8 * 2);
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ uint32_t packBf16(float2 v) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(v);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// C = alpha * acc + beta * C in BF16.
+template <int kBlocks>
+__device__ __forceinline__ void storeBf16(const Params &p, __nv_bfloat16 *c, int cols, int rows,
+                                          const float2 (&acc)[kBlocks * 4], unsigned char *out,
+                                          int lane, bool vector) {
+  constexpr int kPass = kBlocks < kOutCols / 8 ? kBlocks : kOutCols / 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int col = t.n0 + col_begin + j0 + j;
-      const bool in = col_begin + j0 + j < t.cols;
-      const size_t at = matrix + static_cast<size_t>(col) * p.ldc + row;
-      if (p.pair.out == PairOut::kFinal) {
-        if (in)
-          static_cast<__nv_bfloat16 *>(p.c)[at] =
-              __float2bfloat16(acc[j0 + j] * (1.0F / (kPairScale * kPairScale)) * p.alpha);
-        continue;
+  for (int i0 = 0; i0 < kBlocks; i0 += kPass) {
+    if (i0 * 8 >= cols) break;
+#pragma unroll
+    for (int i = 0; i < kPass; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float2 v = acc[(i0 + i) * 4 + r];
+        v.x *= p.alpha;
+        v.y *= p.alpha;
+        if (p.beta != 0.0F) {
+          const int row = r * 8 + lane / 4, col = (i0 + i) * 8 + lane % 4 * 2;
+          const __nv_bfloat16 *at = c + static_cast<long long>(col) * p.ldc + row;
+          if (row < rows && col < cols) v.x = fmaf(p.beta, __bfloat162float(at[0]), v.x);
+          if (row < rows && col + 1 < cols) v.y = fmaf(p.beta, __bfloat162float(at[p.ldc]), v.y);
+        }
+        w[r] = packBf16(v);
       }
-      float v = acc[j0 + j] * (1.0F / kPairScale);
-      if (p.pair.out == PairOut::kPoly) {
-        v *= p.pair.c2;
-        if (in)
-          v = fmaf(p.pair.c1, __half2float(p.pair.prev_hi[at]) + __half2float(p.pair.prev_lo[at]),
-                   v);
-        if (col == row) v = fmaf(p.pair.c0, kPairScale, v);
+      stageBlock(out, i, lane, w);
+    }
+    copyOut(out, reinterpret_cast<uint16_t *>(c) + static_cast<long long>(i0) * 8 * p.ldc, p.ldc,
+            min(cols - i0 * 8, kPass * 8), rows, lane, vector);
+  }
+}
+
+// The same in FP32, from registers: a warp's store covers four whole sectors
+// (eight rows) of four columns.
+template <int kBlocks>
+__device__ __forceinline__ void storeFp32(const Params &p, float *c, int cols, int rows,
+                                          const float2 (&acc)[kBlocks * 4], int lane) {
+  float *at = c + static_cast<long long>(lane % 4 * 2) * p.ldc + lane / 4;
+  const int row = lane / 4, col = lane % 4 * 2;
+#pragma unroll
+  for (int i = 0; i < kBlocks; ++i) {
+    if (i * 8 >= cols) break;
+    const bool in0 = i * 8 + col < cols, in1 = i * 8 + col + 1 < cols;
+    float *next = at + p.ldc;
+    if (p.beta == 0.0F) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool live = r * 8 + row < rows;
+        if (live && in0) at[r * 8] = p.alpha * acc[i * 4 + r].x;
+        if (live && in1) next[r * 8] = p.alpha * acc[i * 4 + r].y;
       }
-      splitPair(v, &hi[j], &lo[j]);
-      if (in) {
-        p.pair.hi[at] = hi[j];
-        p.pair.lo[at] = lo[j];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool live = r * 8 + row < rows;
+        if (live && in0) at[r * 8] = fmaf(p.beta, at[r * 8], p.alpha * acc[i * 4 + r].x);
+        if (live && in1) next[r * 8] = fmaf(p.beta, next[r * 8], p.alpha * acc[i * 4 + r].y);
       }
     }
-    // The mirrored tile: rows are padded to 64 elements, so a vector may
-    // reach past n into the padding, which nothing reads.
-    if (mirror) {
-      const size_t at = matrix + static_cast<size_t>(row) * p.ldc + t.n0 + col_begin + j0;
-      *reinterpret_cast<uint4 *>(p.pair.hi + at) = *reinterpret_cast<const uint4 *>(hi);
-      *reinterpret_cast<uint4 *>(p.pair.lo + at) = *reinterpret_cast<const uint4 *>(lo);
+    at += 8LL * p.ldc;
+  }
+}
+
+// A pair product's result (PairOut). `at` is this warp's first element in
+// hi, lo, prev (or c); row0 and col0 are its place in the matrix. The
+// polynomial reads A across (A is symmetric, and two columns of a row lie
+// together); the mirrored tile is written the same way. Rows of the pair
+// matrices are padded to 64 elements, so whole pairs and vectors may reach
+// past the last row or column into padding that nothing reads.
+template <int kBlocks, bool kSymmetric>
+__device__ __forceinline__ void storePair(const Params &p, size_t matrix, bool mirror, int row0,
+                                          int col0, int cols, const float2 (&acc)[kBlocks * 4],
+                                          unsigned char *out, int lane, bool vector) {
+  const size_t at = matrix + static_cast<size_t>(col0) * p.ldc + row0;
+  const int rows = p.m - row0;
+  if (p.pair.out == PairOut::kFinal) {
+    storeBf16<kBlocks>(p, static_cast<__nv_bfloat16 *>(p.c) + at, cols, rows, acc, out, lane,
+                       vector);
+    return;
+  }
+  constexpr int kPass = kOutCols / 2 / 8;   // half the staging area each for hi and lo
+  unsigned char *out_lo = out + kOutCols / 2 * 64;
+  const bool poly = kSymmetric && p.pair.out == PairOut::kPoly;
+#pragma unroll
+  for (int i0 = 0; i0 < kBlocks; i0 += kPass) {
+    if (i0 * 8 >= cols) break;
+#pragma unroll
+    for (int i = 0; i < kPass; ++i) {
+      const int col = (i0 + i) * 8 + lane % 4 * 2;
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = r * 8 + lane / 4;
+        const bool live = row < rows && col < cols;
+        const size_t across = matrix + static_cast<size_t>(row0 + row) * p.ldc + col0 + col;
+        float2 v = acc[(i0 + i) * 4 + r];
+        v.x *= 1.0F / kPairScale;
+        v.y *= 1.0F / kPairScale;
+        if (poly) {
+          float2 h = make_float2(0.0F, 0.0F), l = h;
+          if (live) {
+            h = __half22float2(*reinterpret_cast<const __half2 *>(p.pair.prev_hi + across));
+            l = __half22float2(*reinterpret_cast<const __half2 *>(p.pair.prev_lo + across));
+          }
+          v.x = fmaf(p.pair.c1, h.x + l.x, v.x * p.pair.c2);
+          v.y = fmaf(p.pair.c1, h.y + l.y, v.y * p.pair.c2);
+          if (col0 + col == row0 + row) v.x = fmaf(p.pair.c0, kPairScale, v.x);
+          if (col0 + col + 1 == row0 + row) v.y = fmaf(p.pair.c0, kPairScale, v.y);
+        }
+        const __half2 h2 = __float22half2_rn(v);
+        const float2 hf = __half22float2(h2);
+        const __half2 l2 = __float22half2_rn(make_float2(v.x - hf.x, v.y - hf.y));
+        hi[r] = *reinterpret_cast<const uint32_t *>(&h2);
+        lo[r] = *reinterpret_cast<const uint32_t *>(&l2);
+        if (mirror && live) {
+          *reinterpret_cast<uint32_t *>(p.pair.hi + across) = hi[r];
+          *reinterpret_cast<uint32_t *>(p.pair.lo + across) = lo[r];
+        }
+      }
+      stageBlock(out, i, lane, hi);
+      stageBlock(out_lo, i, lane, lo);
+    }
+    const size_t to = at + static_cast<size_t>(i0) * 8 * p.ldc;
+    const int left = min(cols - i0 * 8, kPass * 8);
+    copyOut(out, reinterpret_cast<uint16_t *>(p.pair.hi + to), p.ldc, left, rows, lane, true);
+    copyOut(out_lo, reinterpret_cast<uint16_t *>(p.pair.lo + to), p.ldc, left, rows, lane, true);
+  }
+}
+
+// The MMA of either form, and its completion signal to this CTA or both.
+template <class G>
+__device__ __forceinline__ void issueMma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                         bool accumulate) {
+  if constexpr (G::kTwo) mmaNarrowPair<G::kBytes>(d_tmem, a, b, idesc, accumulate);
+  else mmaNarrow<G::kBytes>(d_tmem, a, b, idesc, accumulate);
+}
+template <class G>
+__device__ __forceinline__ void commitMma(uint64_t *bar) {
+  if constexpr (G::kTwo) mmaCommitBoth(bar);
+  else mmaCommit(bar);
+}
+// A box of operand `map` into this CTA's shared memory, counted on `bar` of
+// this CTA, or (kShared, a pair) of the even CTA.
+template <class G, bool kShared>
+__device__ __forceinline__ void loadBox(unsigned char *dst, const CUtensorMap *map, uint64_t *bar,
+                                        int x, int y, int z) {
+  if constexpr (kShared) tmaLoad3dPair(dst, map, clusterAddr(smemAddr(bar), 0), x, y, z);
+  else tmaLoad3d(dst, map, bar, x, y, z);
+}
+template <class G, bool kShared>
+__device__ __forceinline__ void loadStage(const Params &p, unsigned char *stage, uint64_t *bar,
+                                          int m0, int n0, int k0, int za, int zb) {
+#pragma unroll
+  for (int plane = 0; plane < G::kPlanes; ++plane) {
+    unsigned char *sa = stage + plane * G::kABytes;
+    unsigned char *sb = stage + G::kPlanes * G::kABytes + plane * G::kBBytes;
+    const CUtensorMap *map_a = plane == 0 ? &p.tma_a : &p.pair.tma_a_lo;
+    const CUtensorMap *map_b = plane == 0 ? &p.tma_b : &p.pair.tma_b_lo;
+    if constexpr (G::kAMN) {
+      for (int j = 0; j < kBM / 64; ++j)
+        loadBox<G, kShared>(sa + j * 64 * kRowBytes, map_a, bar, m0 + 64 * j, k0, za);
+    } else {
+      loadBox<G, kShared>(sa, map_a, bar, k0, m0, za);
+    }
+    if constexpr (G::kBMN) {
+      for (int j = 0; j < G::kBRows / 64; ++j)
+        loadBox<G, kShared>(sb + j * 64 * kRowBytes, map_b, bar, n0 + 64 * j, k0, zb);
+    } else {
+      loadBox<G, kShared>(sb, map_b, bar, k0, n0, zb);
     }
   }
 }
 
-template <int kElemBytes, Ragged kRagged, int kBN, bool kAMN, bool kBMN, int kPlanes = 1,
-          bool kSymmetric = false>
+// mbarriers (all waits bounded; in a pair the even CTA's, except where noted):
+//   full[s]       stage s loaded: TMA bytes of both CTAs
+//   empty[s]      the MMAs reading stage s completed (each CTA its own)
+//   acc_full[b]   accumulator b holds a chunk (each CTA its own)
+//   acc_empty[b]  every epilogue warp has read accumulator b
+//   tail[s]       a pair's odd CTA has cut off the last slice of a group, in stage s
+// A slice that ends a group ragged along k holds rows of the next group. The
+// issuer's warp zeroes them in both operands (zero times a NaN is a NaN) up to
+// the next multiple of 16, and multiplies no further. In a pair the odd CTA
+// does the same for its half: such a slice is counted on its own full[s], and
+// tail[s] tells the even CTA.
+template <class G>
 __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_constant__ Params p) {
-  using G = Cfg<kElemBytes, kRagged, kBN, kAMN, kBMN, kPlanes, kSymmetric>;
+  constexpr int kBN = G::kBN;
   constexpr int kStages = G::kStages;
   constexpr int kStageBytes = G::kStageBytes;
   extern __shared__ unsigned char smem_raw[];
@@ -319,12 +523,18 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
   __shared__ GroupTable table;
   unsigned char *smem = smem_raw + ((1024 - (smemAddr(smem_raw) & 1023)) & 1023);
   float *scales = reinterpret_cast<float *>(smem + kStages * kStageBytes);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStageBytes + G::kScaleBytes);
+  unsigned char *out_smem = smem + kStages * kStageBytes + G::kScaleBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(out_smem + G::kOutBytes);
   uint64_t *empty = full + kStages;
   uint64_t *acc_full = empty + kStages;
   uint64_t *acc_empty = acc_full + kAccums;
+  uint64_t *tail = acc_empty + kAccums;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // A worker is a CTA, or a pair: its position among them, and this CTA's in it.
+  const int rank = G::kTwo ? static_cast<int>(blockIdx.x & 1) : 0;
+  const int worker = G::kTwo ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int workers = G::kTwo ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
   if (threadIdx.x == 0) {
     if (p.k > 0) {
       prefetchTensorMap(&p.tma_a);
@@ -333,62 +543,61 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
     for (int s = 0; s < kStages; ++s) {
       mbarInit(&full[s], 1);
       mbarInit(&empty[s], 1);
+      mbarInit(&tail[s], 1);
     }
     for (int b = 0; b < kAccums; ++b) {
       mbarInit(&acc_full[b], 1);
-      mbarInit(&acc_empty[b], kEpilogueThreads);
+      mbarInit(&acc_empty[b], (G::kTwo ? 2 : 1) * kEpilogueWarps);
     }
     fenceBarrierInit();
   }
   if (warp == 2) {
-    tmemAlloc(&tmem_base_slot, G::kTmemColumns);
-    tmemRelinquish();
+    if constexpr (G::kTwo) {
+      tmemAllocPair(&tmem_base_slot, G::kTmemColumns);
+      tmemRelinquishPair();
+    } else {
+      tmemAlloc(&tmem_base_slot, G::kTmemColumns);
+      tmemRelinquish();
+    }
   }
   gridDependencyWait();
-  readGroups<kRagged, kBN>(p, &table);
+  readGroups<G>(p, &table);
   tcgenFenceBefore();
   __syncthreads();
+  if constexpr (G::kTwo) clusterSync();   // both CTAs' barriers and TMEM exist
   tcgenFenceAfter();
   allowDependentLaunch();
   const uint32_t tmem_base = tmem_base_slot;
-  const int tiles = tileCount<kRagged, kBN, kSymmetric>(p, table);
+  const int tiles = tileCount<G>(p, table);
 
   bool ok = true;
   auto wait = [&](uint64_t *bar, int parity) {
     if (ok) ok = mbarWait(bar, static_cast<uint32_t>(parity), p.err);
   };
+  // The instruction's N for a tile's valid columns.
+  auto widthOf = [](int cols) { return (cols + G::kNStep - 1) / G::kNStep * G::kNStep; };
 
   if (warp < kEpilogueWarp0) {
-    regDealloc<56>();
+    regDealloc<72>();
     if (warp == 0 && lane == 0) {
       // ---------------- TMA producer ----------------
       int s = 0, parity = 1;   // the first pass over the ring waits for nothing
-      for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-        const Tile t = tileAt<kRagged, kBN, kSymmetric>(p, table, i);
-        const int za = kRagged == Ragged::kK ? 0 : t.group;
-        const int zb = kRagged == Ragged::kBatch ? t.group : 0;
+      for (int i = worker; i < tiles; i += workers) {
+        const Tile t = tileAt<G>(p, table, i);
+        const int za = G::kRagged == Ragged::kK ? 0 : t.group;
+        const int zb = G::kRagged == Ragged::kBatch ? t.group : 0;
+        const int m0 = t.m0 + rank * kBM;
+        const int n0 = t.n0 + (G::kTwo ? rank * (widthOf(t.cols) / 2) : 0);
         for (int kk = 0; kk < t.klen; kk += G::kBK) {
           wait(&empty[s], parity);
-          const int k0 = t.k0 + kk;
-          mbarArriveExpectTx(&full[s], kStageBytes);
-#pragma unroll
-          for (int plane = 0; plane < kPlanes; ++plane) {
-            unsigned char *sa = smem + s * kStageBytes + plane * G::kABytes;
-            unsigned char *sb = smem + s * kStageBytes + kPlanes * G::kABytes + plane * G::kBBytes;
-            const CUtensorMap *map_a = plane == 0 ? &p.tma_a : &p.pair.tma_a_lo;
-            const CUtensorMap *map_b = plane == 0 ? &p.tma_b : &p.pair.tma_b_lo;
-            if constexpr (kAMN) {
-              for (int j = 0; j < kBM / 64; ++j)
-                tmaLoad3d(sa + j * 64 * kRowBytes, map_a, &full[s], t.m0 + 64 * j, k0, za);
-            } else {
-              tmaLoad3d(sa, map_a, &full[s], k0, t.m0, za);
-            }
-            if constexpr (kBMN) {
-              for (int j = 0; j < kBN / 64; ++j)
-                tmaLoad3d(sb + j * 64 * kRowBytes, map_b, &full[s], t.n0 + 64 * j, k0, zb);
-            } else {
-              tmaLoad3d(sb, map_b, &full[s], k0, t.n0, zb);
-            }
+          unsigned char *stage = smem + s * kStageBytes;
+          const bool cut = G::kRagged == Ragged::kK && t.klen - kk < G::kBK;
+          if (!G::kTwo || cut) {
+            mbarArriveExpectTx(&full[s], kStageBytes);
+            loadStage<G, false>(p, stage, &full[s], m0, n0, t.k0 + kk, za, zb);
+          } else {
+            if (rank == 0) mbarArriveExpectTx(&full[s], 2 * kStageBytes);
+            loadStage<G, G::kTwo>(p, stage, &full[s], m0, n0, t.k0 + kk, za, zb);
           }
           if (++s == kStages) {
             s = 0;
@@ -396,55 +605,75 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
           }
         }
       }
-    } else if (warp == 1) {
+      if constexpr (G::kTwo) {
+        // Every signal of the even CTA has landed before the pair ends.
+        for (int j = 0; j < kStages; ++j) {
+          wait(&empty[s], parity);
+          if (++s == kStages) {
+            s = 0;
+            parity ^= 1;
+          }
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
       // ---------------- MMA issuer ----------------
       int s = 0, parity = 0;
       int b = 0, acc_parity = 1;
-      for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-        const Tile t = tileAt<kRagged, kBN, kSymmetric>(p, table, i);
-        const uint32_t idesc = instrDesc<kAMN, kBMN>(p.format, (t.cols + 15) / 16 * 16);
+      unsigned tails = 0;   // bit s: parity of the next cut slice in stage s
+      const uint64_t desc_a = smemDesc<G::kAMN>(smemAddr(smem));
+      const uint64_t desc_b = smemDesc<G::kBMN>(smemAddr(smem) + G::kPlanes * G::kABytes);
+      for (int i = worker; i < tiles; i += workers) {
+        const Tile t = tileAt<G>(p, table, i);
+        const uint32_t idesc = instrDesc<G>(p.format, widthOf(t.cols));
         const int iters = (t.klen + G::kBK - 1) / G::kBK;
+        int in_chunk = 0;
         for (int kb = 0; kb < iters; ++kb) {
-          const bool first = kb % G::kChunkIters == 0;
-          const bool last = kb % G::kChunkIters == G::kChunkIters - 1 || kb == iters - 1;
+          const bool first = in_chunk == 0;
+          const bool last = ++in_chunk == p.chunk_iters || kb == iters - 1;
+          if (last) in_chunk = 0;
           if (first) wait(&acc_empty[b], acc_parity);
           wait(&full[s], parity);
-          unsigned char *stage = smem + s * kStageBytes;
           int steps = G::kBK / G::kMmaK;
-          if constexpr (kRagged == Ragged::kK) {
-            // The group's last slice: rows of k beyond it belong to the next
-            // group. Both operands' rows up to the next multiple of 16 are
-            // zeroed (zero times a NaN is a NaN), the rest is not multiplied.
+          if constexpr (G::kRagged == Ragged::kK) {
             const int rows = t.klen - kb * G::kBK;
             if (rows < G::kBK) {
+              unsigned char *stage = smem + s * kStageBytes;
               steps = (rows + G::kMmaK - 1) / G::kMmaK;
               zeroRows<kBM / 64>(stage, rows, steps * G::kMmaK, lane);
-              zeroRows<kBN / 64>(stage + G::kABytes, rows, steps * G::kMmaK, lane);
+              zeroRows<G::kBRows / 64>(stage + G::kABytes, rows, steps * G::kMmaK, lane);
               fenceProxyAsyncShared();
               __syncwarp();
+              if constexpr (G::kTwo) {
+                wait(&tail[s], (tails >> s) & 1);
+                tails ^= 1u << s;
+                fenceCluster();
+              }
             }
           }
           if (lane == 0) {
             tcgenFenceAfter();
-            const uint32_t sa = smemAddr(stage);
-            const uint32_t sb = sa + kPlanes * G::kABytes;
             const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * kBN);
-            for (int j = 0; j < steps; ++j) {
-              // K-major: the next instruction's k are 32 bytes further along
-              // each row; MN-major: 16 rows of 128 bytes further.
-              const uint32_t a0 = sa + (kAMN ? j * 16u * kRowBytes : j * 32u);
-              const uint32_t b0 = sb + (kBMN ? j * 16u * kRowBytes : j * 32u);
-              mmaNarrow<G::kBytes>(d_tmem, smemDesc<kAMN>(a0), smemDesc<kBMN>(b0), idesc,
-                                   !first || j > 0);
-              if constexpr (kPlanes == 2) {
-                mmaNarrow<false>(d_tmem, smemDesc<kAMN>(a0), smemDesc<kBMN>(b0 + G::kBBytes), idesc,
-                                 true);
-                mmaNarrow<false>(d_tmem, smemDesc<kAMN>(a0 + G::kABytes), smemDesc<kBMN>(b0), idesc,
-                                 true);
+            // Descriptors count 16 bytes. K-major: the next instruction's k
+            // are 32 bytes further along each row; MN-major: 16 rows of 128
+            // bytes further.
+            constexpr uint64_t kNextA = (G::kAMN ? 16 * kRowBytes : 32) / 16;
+            constexpr uint64_t kNextB = (G::kBMN ? 16 * kRowBytes : 32) / 16;
+            uint64_t ad = desc_a + static_cast<uint64_t>(s) * (kStageBytes / 16);
+            uint64_t bd = desc_b + static_cast<uint64_t>(s) * (kStageBytes / 16);
+#pragma unroll
+            for (int j = 0; j < G::kBK / G::kMmaK; ++j) {
+              if (j < steps) {
+                issueMma<G>(d_tmem, ad, bd, idesc, !first || j > 0);
+                if constexpr (G::kPlanes == 2) {
+                  issueMma<G>(d_tmem, ad, bd + G::kBBytes / 16, idesc, true);
+                  issueMma<G>(d_tmem, ad + G::kABytes / 16, bd, idesc, true);
+                }
               }
+              ad += kNextA;
+              bd += kNextB;
             }
-            mmaCommit(&empty[s]);
-            if (last) mmaCommit(&acc_full[b]);
+            commitMma<G>(&empty[s]);
+            if (last) commitMma<G>(&acc_full[b]);
           }
           __syncwarp();
           if (last) {
@@ -457,49 +686,87 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
           }
         }
       }
+    } else if (warp == 1 && G::kRagged == Ragged::kK) {
+      // ---------------- the odd CTA's cut slices ----------------
+      int s = 0;
+      unsigned seen = 0;   // bit s: parity of the next cut slice in stage s
+      for (int i = worker; i < tiles; i += workers) {
+        const Tile t = tileAt<G>(p, table, i);
+        const int iters = (t.klen + G::kBK - 1) / G::kBK;
+        if (iters == 0) continue;
+        const int at = (s + iters - 1) % kStages;
+        s = (s + iters) % kStages;
+        const int rows = t.klen - (iters - 1) * G::kBK;
+        if (rows == G::kBK) continue;
+        wait(&full[at], (seen >> at) & 1);
+        seen ^= 1u << at;
+        unsigned char *stage = smem + at * kStageBytes;
+        const int end = (rows + G::kMmaK - 1) / G::kMmaK * G::kMmaK;
+        zeroRows<kBM / 64>(stage, rows, end, lane);
+        zeroRows<G::kBRows / 64>(stage + G::kABytes, rows, end, lane);
+        fenceProxyAsyncShared();
+        __syncwarp();
+        if (lane == 0) mbarArriveCluster(clusterAddr(smemAddr(&tail[at]), 0));
+      }
     }
   } else {
     // ---------------- epilogue ----------------
-    regAlloc<224>();
+    regAlloc<216>();
     constexpr int kHalf = kBN / 2;                     // columns of this warp
+    constexpr int kBlocks = kHalf / 8;
     constexpr int kLoad = kHalf < 32 ? kHalf : 32;     // columns of one TMEM load
     const int quarter = warp % 4;
     const int col_begin = (warp - kEpilogueWarp0) / 4 * kHalf;
-    const int row_in_tile = quarter * 32 + lane;
     const int etid = threadIdx.x - 32 * kEpilogueWarp0;
+    unsigned char *out = out_smem + (warp - kEpilogueWarp0) * kOutCols * 64;
+    // Vectors of eight 16-bit rows: columns aligned to 16 bytes.
+    const bool vector = reinterpret_cast<uintptr_t>(p.c) % 16 == 0 && p.ldc % 8 == 0 &&
+                        p.stride_c % 8 == 0;
     int b = 0, acc_parity = 0;
+    // Scales of kScaleBatch blocks of one column per thread, one batch ahead;
+    // scale_a * scale_b per (block, column) is staged in shared memory.
     int scale_batches = 0;
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-      const Tile t = tileAt<kRagged, kBN, kSymmetric>(p, table, i);
-      const int row = t.m0 + row_in_tile;
-      const int iters = (t.klen + G::kBK - 1) / G::kBK;
-      const int chunks = (iters + G::kChunkIters - 1) / G::kChunkIters;
-      float acc[kHalf];
+    float sa_next[kScaleBatch] = {}, sb_next[kScaleBatch] = {};
+    auto fetchScales = [&](const Tile &t, int ch) {
+      const int m0 = t.m0 + rank * kBM;
+      if (etid >= t.cols || m0 >= p.m) return;
+      const int live = (t.klen + G::kBK - 1) / G::kBK - ch;
+      const float *sb = p.scale_b + static_cast<size_t>(t.n0 + etid) * p.ldsb + ch;
+      const float *sa = p.scale_a + t.group * p.stride_sa + static_cast<size_t>(m0 / 128) * p.ldsa + ch;
 #pragma unroll
-      for (int j = 0; j < kHalf; ++j) acc[j] = 0.0F;
+      for (int q = 0; q < kScaleBatch; ++q) {
+        sa_next[q] = q < live ? __ldg(sa + q) : 0.0F;
+        sb_next[q] = q < live ? __ldg(sb + q) : 0.0F;
+      }
+    };
+    if constexpr (G::kBytes) {
+      if (worker < tiles) fetchScales(tileAt<G>(p, table, worker), 0);
+    }
+    for (int i = worker; i < tiles; i += workers) {
+      const Tile t = tileAt<G>(p, table, i);
+      const int m0 = t.m0 + rank * kBM;
+      const int iters = (t.klen + G::kBK - 1) / G::kBK;
+      const int chunks = iters > 0 ? (iters - 1) / p.chunk_iters + 1 : 0;
+      float2 acc[kBlocks * 4];
+#pragma unroll
+      for (int j = 0; j < kBlocks * 4; ++j) acc[j] = make_float2(0.0F, 0.0F);
       for (int ch = 0; ch < chunks; ++ch) {
         const float *sc = nullptr;
         if constexpr (G::kBytes) {
-          // Scales of the next kScaleBatch blocks: scale_a * scale_b per
-          // (block, column), staged by one thread per column.
           if (ch % kScaleBatch == 0) {
+            // Stage this batch, fetched during the last one, and fetch the next.
             float *dst = scales + (scale_batches & 1) * kScaleBatch * kBN;
             if (etid < kBN) {
-              const bool in = etid < t.cols;
-              const float *sb = p.scale_b + static_cast<size_t>(in ? t.n0 + etid : 0) * p.ldsb;
-              const float *sa = p.scale_a + t.group * p.stride_sa +
-                                static_cast<size_t>(t.m0 / 128) * p.ldsa;
-              float v[kScaleBatch];
 #pragma unroll
-              for (int q = 0; q < kScaleBatch; ++q) {
-                const bool live = in && ch + q < chunks;
-                v[q] = live ? sb[ch + q] * sa[ch + q] : 0.0F;
-              }
-#pragma unroll
-              for (int q = 0; q < kScaleBatch; ++q) dst[q * kBN + etid] = v[q];
+              for (int q = 0; q < kScaleBatch; ++q) dst[q * kBN + etid] = sa_next[q] * sb_next[q];
             }
             namedBarrier<1, kEpilogueThreads>();
             ++scale_batches;
+            if (ch + kScaleBatch < chunks) {
+              fetchScales(t, ch + kScaleBatch);
+            } else if (i + workers < tiles) {
+              fetchScales(tileAt<G>(p, table, i + workers), 0);
+            }
           }
           sc = scales + ((scale_batches - 1) & 1) * kScaleBatch * kBN +
                (ch % kScaleBatch) * kBN + col_begin;
@@ -508,65 +775,82 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
         tcgenFenceAfter();
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                                static_cast<uint32_t>(b * kBN + col_begin);
+        // v: rows 0-15 of kLoad columns from c, then rows 16-31.
+        auto accumulate = [&](int c, const uint32_t (&v)[kLoad]) {
 #pragma unroll
-        for (int c = 0; c < kHalf; c += kLoad) {
-          if (col_begin + c >= t.cols) break;
-          uint32_t v[32];
-          if constexpr (kLoad == 32) tmemLoad32(taddr + c, v);
-          else tmemLoad16(taddr + c, v);
-          if constexpr (G::kBytes) {
+          for (int i = 0; i < kLoad / 8; ++i) {
+            float2 scale = make_float2(0.0F, 0.0F);
+            if constexpr (G::kBytes)
+              scale = *reinterpret_cast<const float2 *>(sc + c + i * 8 + lane % 4 * 2);
 #pragma unroll
-            for (int j = 0; j < kLoad; j += 4) {
-              const float4 s4 = *reinterpret_cast<const float4 *>(sc + c + j);
-              acc[c + j] = fmaf(__uint_as_float(v[j]), s4.x, acc[c + j]);
-              acc[c + j + 1] = fmaf(__uint_as_float(v[j + 1]), s4.y, acc[c + j + 1]);
-              acc[c + j + 2] = fmaf(__uint_as_float(v[j + 2]), s4.z, acc[c + j + 2]);
-              acc[c + j + 3] = fmaf(__uint_as_float(v[j + 3]), s4.w, acc[c + j + 3]);
+            for (int r = 0; r < 4; ++r) {
+              const int at = r / 2 * (kLoad / 2) + i * 4 + r % 2 * 2;
+              const float2 x = make_float2(__uint_as_float(v[at]), __uint_as_float(v[at + 1]));
+              float2 &a = acc[(c / 8 + i) * 4 + r];
+              if constexpr (G::kBytes) a = __ffma2_rn(x, scale, a);
+              else a = __fadd2_rn(a, x);
             }
-          } else {
+          }
+        };
+        // The next load is in flight while one is added. Columns past the
+        // tile's width hold what an earlier tile left; they are not written.
+        constexpr uint32_t kLower = 16u << 16;   // the quarter's lanes 16-31
+        if constexpr (kLoad == 16) {
+          uint32_t v[16];
+          tmemFragments<16>(taddr, v, 0);
+          tmemFragments<16>(taddr + kLower, v, 8);
+          tmemWait16(v);
+          accumulate(0, v);
+        } else {
+          uint32_t v[2][32];
+          tmemFragments<32>(taddr, v[0], 0);
+          tmemFragments<32>(taddr + kLower, v[0], 16);
 #pragma unroll
-            for (int j = 0; j < kLoad; ++j) acc[c + j] += __uint_as_float(v[j]);
+          for (int c = 0; c < kHalf; c += 32) {
+            uint32_t(&now)[32] = v[c / 32 % 2];
+            uint32_t(&next)[32] = v[(c / 32 + 1) % 2];
+            tmemWait32(now);
+            if (c + 32 < kHalf) {
+              tmemFragments<32>(taddr + c + 32, next, 0);
+              tmemFragments<32>(taddr + kLower + c + 32, next, 16);
+            }
+            accumulate(c, now);
           }
         }
         tcgenFenceBefore();
-        mbarArrive(&acc_empty[b]);
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (G::kTwo) mbarArriveCluster(clusterAddr(smemAddr(&acc_empty[b]), 0));
+          else mbarArrive(&acc_empty[b]);
+        }
         b ^= 1;
         if (b == 0) acc_parity ^= 1;
       }
-      if constexpr (kPlanes == 2) {
-        storePair<kHalf, kSymmetric>(p, t, row, col_begin, acc);
-        continue;
-      }
-      // C = alpha * acc + beta * C; a warp writes 32 consecutive rows of a column.
-      if (row < p.m) {
-        const long long matrix = kRagged == Ragged::kN ? 0 : t.group * p.stride_c;
-#pragma unroll
-        for (int j = 0; j < kHalf; ++j) {
-          const int col = col_begin + j;
-          if (col < t.cols) {
-            const size_t at = static_cast<size_t>(matrix) +
-                              static_cast<size_t>(t.n0 + col) * p.ldc + row;
-            float v = p.alpha * acc[j];
-            if (p.c_bf16) {
-              __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + at;
-              if (p.beta != 0.0F) v = fmaf(p.beta, __bfloat162float(*c), v);
-              *c = __float2bfloat16(v);
-            } else {
-              float *c = static_cast<float *>(p.c) + at;
-              if (p.beta != 0.0F) v = fmaf(p.beta, *c, v);
-              *c = v;
-            }
-          }
-        }
+      const size_t matrix =
+          G::kRagged == Ragged::kN ? 0 : static_cast<size_t>(t.group * p.stride_c);
+      const int row0 = m0 + quarter * 32;
+      const int col0 = t.n0 + col_begin, cols = t.cols - col_begin;
+      if (row0 < p.m && cols > 0) {
+        const size_t at = matrix + static_cast<size_t>(col0) * p.ldc + row0;
+        if constexpr (G::kPlanes == 2)
+          storePair<kBlocks, G::kSymmetric>(p, matrix, G::kSymmetric && t.m0 != t.n0, row0, col0,
+                                            cols, acc, out, lane, vector);
+        else if (p.c_bf16)
+          storeBf16<kBlocks>(p, static_cast<__nv_bfloat16 *>(p.c) + at, cols, p.m - row0, acc, out,
+                             lane, vector);
+        else
+          storeFp32<kBlocks>(p, static_cast<float *>(p.c) + at, cols, p.m - row0, acc, lane);
       }
     }
   }
 
   tcgenFenceBefore();
   __syncthreads();
+  if constexpr (G::kTwo) clusterSync();   // neither CTA leaves while the pair still works
   if (warp == 2) {
     tcgenFenceAfter();
-    tmemDealloc(tmem_base, G::kTmemColumns);
+    if constexpr (G::kTwo) tmemDeallocPair(tmem_base, G::kTmemColumns);
+    else tmemDealloc(tmem_base, G::kTmemColumns);
   }
 }
 

@@ -257,33 +257,82 @@ __device__ __forceinline__ void mmaCommit(uint64_t *bar) {
                : "memory");
 }
 // 32 consecutive TMEM columns of the warp's 32 lanes (lane i of the warp
-// reads TMEM lane (warp % 4) * 32 + i); then wait for the load.
-__device__ __forceinline__ void tmemLoad32(uint32_t taddr, uint32_t (&v)[32]) {
+// reads TMEM lane (warp % 4) * 32 + i). The values may be used after
+// tmemWait32 on them.
+__device__ __forceinline__ void tmemLoadAsync32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
       "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
       "%28, %29, %30, %31}, [%32];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
         "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
-        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Waits for the warp's TMEM loads; naming the registers keeps their uses
+// behind the wait.
+__device__ __forceinline__ void tmemWait32(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
+                 "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                 "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),
+                 "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
+                 "+r"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmemLoad32(uint32_t taddr, uint32_t (&v)[32]) {
+  tmemLoadAsync32(taddr, v);
+  tmemWait32(v);
 }
 
-// 16 consecutive TMEM columns, as tmemLoad32.
-__device__ __forceinline__ void tmemLoad16(uint32_t taddr, uint32_t *v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// Sixteen TMEM lanes (from the one in taddr) by 8 or 16 or 32 consecutive
+// columns as fragments: for the 8 columns from 8 i, lane t of the warp gets
+// columns 8 i + 2 (t % 4) + {0, 1} of row t / 4 in v[at + 4 i + {0, 1}] and of
+// row t / 4 + 8 in v[at + 4 i + {2, 3}]. Usable after tmemWait.
+template <int kColumns, int kRegs>
+__device__ __forceinline__ void tmemFragments(uint32_t taddr, uint32_t (&v)[kRegs], int at) {
+  static_assert(kColumns == 16 || kColumns == 32, "fragment width");
+  if constexpr (kColumns == 16) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(v[at + 0]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]),
+          "=r"(v[at + 5]), "=r"(v[at + 6]), "=r"(v[at + 7])
+        : "r"(taddr)
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[at + 0]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]),
+          "=r"(v[at + 5]), "=r"(v[at + 6]), "=r"(v[at + 7]), "=r"(v[at + 8]), "=r"(v[at + 9]),
+          "=r"(v[at + 10]), "=r"(v[at + 11]), "=r"(v[at + 12]), "=r"(v[at + 13]), "=r"(v[at + 14]),
+          "=r"(v[at + 15])
+        : "r"(taddr)
+        : "memory");
+  }
+}
+__device__ __forceinline__ void tmemWait16(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
+                 "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+
+// Four 8 x 8 matrices of 16-bit values to shared memory, transposed: lane t
+// holds elements (t / 4, 2 (t % 4) + {0, 1}) of each; lane 8 i + j gives the
+// address (16 bytes) where column j of matrix i goes.
+__device__ __forceinline__ void storeMatrixTrans4(uint32_t smem, uint32_t a, uint32_t b, uint32_t c,
+                                                  uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem),
+               "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 
 // ---- CTA pairs (clusters of two) and cta_group::2 ---------------------------
@@ -317,6 +366,11 @@ __device__ __forceinline__ float4 ldCluster4(uint32_t cluster_addr) {
 __device__ __forceinline__ void clusterSync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Orders this thread's memory accesses at cluster scope (an mbarrier wait
+// acquires at CTA scope only).
+__device__ __forceinline__ void fenceCluster() {
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
 }
 // Arrive on an mbarrier in any CTA of the cluster (cluster address).
 __device__ __forceinline__ void mbarArriveCluster(uint32_t cluster_bar) {
@@ -364,12 +418,40 @@ __device__ __forceinline__ void mmaTf32Pair(uint32_t d_tmem, uint64_t a_desc, ui
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
       : "memory");
 }
+// The same with 16- or 8-bit inputs (mmaNarrow).
+template <bool kBytes>
+__device__ __forceinline__ void mmaNarrowPair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                              uint32_t idesc, bool accumulate) {
+  if constexpr (kBytes) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+  }
+}
 // Arrives once on the mbarrier at `cluster_bar` (either CTA of the pair)
 // when every pair MMA this thread issued so far has completed.
 __device__ __forceinline__ void mmaCommitPair(uint32_t cluster_bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    cluster_bar)
                : "memory");
+}
+// The same on the mbarrier at this shared-memory offset in both CTAs.
+__device__ __forceinline__ void mmaCommitBoth(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smemAddr(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
 }
 
 // Asynchronous prefetch of [ptr, ptr + bytes) from global memory into L2.
