@@ -74,9 +74,9 @@ sgblasStatus_t sgblasGroupedGemmK(sgblasHandle_t handle, int m, int n, int k, in
  * scale for each block of 128 (along k) by block_n (1 or 128) columns:
  *
  *   scale = max(largest magnitude of the block, 2^-100) / 448
- *   q     = x / scale, rounded to the nearest e4m3 value
+ *   q     = x * (1 / scale), rounded to the nearest e4m3 value
  *
- * Both divisions are IEEE FP32. A NaN or an infinity in a block makes its
+ * The divisions and the product are rounded to nearest in FP32. A NaN or an infinity in a block makes its
  * scale NaN or infinite. scale is a column-major ceil(k/128) x ceil(n/block_n)
  * FP32 matrix. Strides in elements of each array (unused for batch == 1). */
 sgblasStatus_t sgblasQuantizeFp8(sgblasHandle_t handle, int k, int n, int batch, int block_n,

@@ -20,60 +20,80 @@ namespace t = kern::prod;
 constexpr float kFp8Max = 448.0F;
 constexpr unsigned kAmaxFloorBits = 0x0D800000u;   // 2^-100
 constexpr int kBlock = 128;
-constexpr int kPer = 8;             // consecutive values of one thread
+constexpr int kPer = 16;            // consecutive values of one thread
 constexpr int kLanes = kBlock / kPer;
+constexpr int kQuantThreads = 256;
+constexpr int kUnroll = 2;
+constexpr int kQuantBlocks = kUnroll * kQuantThreads / kLanes;   // of one CTA
 
 struct QuantParams {
   const void *x;
   unsigned char *q;
   float *scale;
-  int k, n, kblocks, ldx, ldq, ldscale;
+  int k, n, batch, kblocks, ldx, ldq, ldscale;
   long long stride_x, stride_q, stride_scale;
-  long long blocks;   // of the whole batch
+  unsigned blocks;   // of the whole batch
 };
 
 __device__ __forceinline__ float toFloat(float v) { return v; }
 __device__ __forceinline__ float toFloat(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// kPer values at `at` (of `live` that exist; the rest are zero).
+// kPer values at `at` (of `live` that exist; the rest are zero), as they lie
+// in memory.
+template <typename T>
+struct Values {
+  uint4 raw[kPer * sizeof(T) / 16];
+  __device__ __forceinline__ T operator[](int j) const {
+    return reinterpret_cast<const T *>(raw)[j];
+  }
+};
 template <typename T, bool kVector>
-__device__ __forceinline__ void loadValues(const T *at, int live, float (&v)[kPer]) {
+__device__ __forceinline__ void loadValues(const T *at, int live, Values<T> *v) {
   if (kVector && live == kPer) {
-    alignas(16) T raw[kPer];
 #pragma unroll
     for (int j = 0; j < kPer * static_cast<int>(sizeof(T)) / 16; ++j)
-      reinterpret_cast<uint4 *>(raw)[j] = __ldg(reinterpret_cast<const uint4 *>(at) + j);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = toFloat(raw[j]);
+      v->raw[j] = __ldg(reinterpret_cast<const uint4 *>(at) + j);
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = j < live ? toFloat(at[j]) : 0.0F;
+    for (int j = 0; j < kPer; ++j)
+      reinterpret_cast<T *>(v->raw)[j] = j < live ? at[j] : static_cast<T>(0.0F);
   }
 }
 
-// Largest magnitude as bits: an integer maximum, which a NaN wins.
-__device__ __forceinline__ unsigned magnitude(const float (&v)[kPer]) {
+// Largest magnitude as the bits of an FP32 value: an integer maximum, which a
+// NaN wins. BF16 values are compared two at a time, as halves of words.
+__device__ __forceinline__ unsigned magnitude(const Values<float> &v) {
   unsigned m = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
   return m;
+}
+__device__ __forceinline__ unsigned magnitude(const Values<__nv_bfloat16> &v) {
+  unsigned m = 0;
+#pragma unroll
+  for (int j = 0; j < kPer / 8; ++j) {
+    const unsigned ab = __vmaxu2(v.raw[j].x & 0x7FFF7FFFu, v.raw[j].y & 0x7FFF7FFFu);
+    const unsigned cd = __vmaxu2(v.raw[j].z & 0x7FFF7FFFu, v.raw[j].w & 0x7FFF7FFFu);
+    m = __vmaxu2(m, __vmaxu2(ab, cd));
+  }
+  return max(m << 16, m & 0xFFFF0000u);
 }
 
 __device__ __forceinline__ float scaleOf(unsigned amax_bits) {
   return __fdiv_rn(__uint_as_float(max(amax_bits, kAmaxFloorBits)), kFp8Max);
 }
 
-template <bool kVector>
-__device__ __forceinline__ void storeValues(unsigned char *at, int live, const float (&v)[kPer],
-                                            float scale) {
-  alignas(8) __nv_fp8x2_storage_t q[kPer / 2];
+template <typename T, bool kVector>
+__device__ __forceinline__ void storeValues(unsigned char *at, int live, const Values<T> &v,
+                                            float inverse) {
+  alignas(16) __nv_fp8x2_storage_t q[kPer / 2];
 #pragma unroll
   for (int j = 0; j < kPer; j += 2)
     q[j / 2] = __nv_cvt_float2_to_fp8x2(
-        make_float2(__fdiv_rn(v[j], scale), __fdiv_rn(v[j + 1], scale)), __NV_SATFINITE,
+        make_float2(toFloat(v[j]) * inverse, toFloat(v[j + 1]) * inverse), __NV_SATFINITE,
         __NV_E4M3);
   if (kVector && live == kPer) {
-    *reinterpret_cast<uint2 *>(at) = *reinterpret_cast<const uint2 *>(q);
+    *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(q);
   } else {
     const auto *bytes = reinterpret_cast<const unsigned char *>(q);
 #pragma unroll
@@ -82,67 +102,83 @@ __device__ __forceinline__ void storeValues(unsigned char *at, int live, const f
   }
 }
 
-// A scale for each 128 values of one column: sixteen lanes per block.
+// A scale for each 128 values of one column: eight lanes per block, kUnroll
+// blocks per thread, whose loads are issued together. Memory-bound: one read
+// and one write of each value.
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(256) quantizeColumnsKernel(const QuantParams p) {
+__global__ void __launch_bounds__(kQuantThreads) quantizeColumnsKernel(const QuantParams p) {
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
-  const long long block = (blockIdx.x * 256LL + threadIdx.x) / kLanes;
   const int part = threadIdx.x % kLanes;
-  const bool in = block < p.blocks;
-  const long long column = in ? block / p.kblocks : 0;
-  const int kb = in ? static_cast<int>(block - column * p.kblocks) : 0;
-  const long long matrix = column / p.n;
-  const long long col = column - matrix * p.n;
-  const int k0 = kb * kBlock + part * kPer;
-  const int live = in ? min(kPer, max(0, p.k - k0)) : 0;
-  float v[kPer];
-  loadValues<T, kVector>(static_cast<const T *>(p.x) + matrix * p.stride_x + col * p.ldx + k0, live,
-                         v);
-  unsigned m = magnitude(v);
+  const unsigned first =
+      blockIdx.x * static_cast<unsigned>(kQuantBlocks) + threadIdx.x / static_cast<unsigned>(kLanes);
+  Values<T> v[kUnroll];
+  size_t to[kUnroll];
+  float *scale_to[kUnroll];
+  int live[kUnroll];
 #pragma unroll
-  for (int d = kLanes / 2; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const float scale = scaleOf(m);
-  storeValues<kVector>(p.q + matrix * p.stride_q + col * p.ldq + k0, live, v, scale);
-  if (in && part == 0) p.scale[matrix * p.stride_scale + col * p.ldscale + kb] = scale;
+  for (int u = 0; u < kUnroll; ++u) {
+    const unsigned block = first + u * (kQuantThreads / kLanes);
+    const bool in = block < p.blocks;
+    const unsigned column = in ? block / static_cast<unsigned>(p.kblocks) : 0;
+    const int kb = in ? static_cast<int>(block - column * p.kblocks) : 0;
+    const unsigned matrix = p.batch > 1 ? column / static_cast<unsigned>(p.n) : 0;
+    const long long col = column - matrix * static_cast<unsigned>(p.n);
+    const int k0 = kb * kBlock + part * kPer;
+    live[u] = in ? min(kPer, max(0, p.k - k0)) : 0;
+    loadValues<T, kVector>(static_cast<const T *>(p.x) + matrix * p.stride_x + col * p.ldx + k0,
+                           live[u], &v[u]);
+    to[u] = static_cast<size_t>(matrix * p.stride_q + col * p.ldq + k0);
+    scale_to[u] = in && part == 0 ? p.scale + matrix * p.stride_scale + col * p.ldscale + kb : nullptr;
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    unsigned m = magnitude(v[u]);
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float scale = scaleOf(m);
+    storeValues<T, kVector>(p.q + to[u], live[u], v[u], __frcp_rn(scale));
+    if (scale_to[u] != nullptr) *scale_to[u] = scale;
+  }
 }
 
 // A scale for each 128 x 128 block: one CTA per block, values in registers.
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(256) quantizeBlocksKernel(const QuantParams p) {
-  __shared__ unsigned warp_max[8];
+__global__ void __launch_bounds__(kQuantThreads) quantizeBlocksKernel(const QuantParams p) {
+  __shared__ unsigned warp_max[kQuantThreads / 32];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
-  const int nblocks = (p.n + kBlock - 1) / kBlock;
-  const long long block = blockIdx.x;
-  const int kb = static_cast<int>(block % p.kblocks);
-  const int nb = static_cast<int>(block / p.kblocks % nblocks);
-  const long long matrix = block / p.kblocks / nblocks;
-  const int part = threadIdx.x % kLanes, row = threadIdx.x / kLanes;   // 16 columns at a time
+  const unsigned nblocks = static_cast<unsigned>((p.n + kBlock - 1) / kBlock);
+  const unsigned kblocks = static_cast<unsigned>(p.kblocks);
+  const int kb = static_cast<int>(blockIdx.x % kblocks);
+  const int nb = static_cast<int>(blockIdx.x / kblocks % nblocks);
+  const long long matrix = blockIdx.x / kblocks / nblocks;
+  const int part = threadIdx.x % kLanes, row = threadIdx.x / kLanes;   // 32 columns at a time
   const int k0 = kb * kBlock + part * kPer;
   const int live_k = min(kPer, max(0, p.k - k0));
   const T *x = static_cast<const T *>(p.x) + matrix * p.stride_x + k0;
-  constexpr int kPasses = kBlock / (256 / kLanes);
-  float v[kPasses][kPer];
-  unsigned m = 0;
+  constexpr int kPasses = kBlock / (kQuantThreads / kLanes);
+  Values<T> v[kPasses];
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
-    const long long col = nb * static_cast<long long>(kBlock) + row + i * (256 / kLanes);
-    loadValues<T, kVector>(x + col * p.ldx, col < p.n ? live_k : 0, v[i]);
-    m = max(m, magnitude(v[i]));
+    const long long col = nb * static_cast<long long>(kBlock) + row + i * (kQuantThreads / kLanes);
+    loadValues<T, kVector>(x + col * p.ldx, col < p.n ? live_k : 0, &v[i]);
   }
+  unsigned m = 0;
 #pragma unroll
-  for (int d = 16; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  for (int i = 0; i < kPasses; ++i) m = max(m, magnitude(v[i]));
+  m = __reduce_max_sync(0xffffffffu, m);
   if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) m = max(m, warp_max[w]);
+  for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, warp_max[w]);
   const float scale = scaleOf(m);
+  const float inverse = __frcp_rn(scale);
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
-    const long long col = nb * static_cast<long long>(kBlock) + row + i * (256 / kLanes);
-    storeValues<kVector>(p.q + matrix * p.stride_q + col * p.ldq + k0, col < p.n ? live_k : 0, v[i],
-                         scale);
+    const long long col = nb * static_cast<long long>(kBlock) + row + i * (kQuantThreads / kLanes);
+    storeValues<T, kVector>(p.q + matrix * p.stride_q + col * p.ldq + k0, col < p.n ? live_k : 0,
+                            v[i], inverse);
   }
   if (threadIdx.x == 0)
     p.scale[matrix * p.stride_scale + static_cast<long long>(nb) * p.ldscale + kb] = scale;
@@ -152,7 +188,7 @@ template <typename T, bool kVector>
 cudaError_t launchQuantize(const QuantParams &p, int block_n, unsigned grid, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(kQuantThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -238,6 +274,7 @@ extern "C" sgblasStatus_t sgblasQuantizeFp8(sgblasHandle_t handle, int k, int n,
   p.scale = scale;
   p.k = k;
   p.n = n;
+  p.batch = batch;
   p.kblocks = kblocks;
   p.ldx = ldx;
   p.ldq = ldq;
@@ -248,22 +285,21 @@ extern "C" sgblasStatus_t sgblasQuantizeFp8(sgblasHandle_t handle, int k, int n,
     p.stride_scale = stride_scale;
   }
   const long long nblocks = block_n == 1 ? n : (n - 1) / kBlock + 1;
-  p.blocks = nblocks * kblocks * batch;
-  const long long grid = block_n == 1 ? (p.blocks + 256 / kLanes - 1) / (256 / kLanes) : p.blocks;
-  if (grid > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  const double blocks = static_cast<double>(nblocks) * kblocks * batch;
+  if (blocks > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;   // 256 GiB of values
+  p.blocks = static_cast<unsigned>(blocks);
+  const unsigned grid = block_n == 1 ? (p.blocks + kQuantBlocks - 1) / kQuantBlocks : p.blocks;
   const auto stream = static_cast<cudaStream_t>(handle->stream);
-  // Whole vectors where every block of kPer values starts on 16 bytes of x
-  // and 8 bytes of q.
+  // Whole vectors where every kPer values start on 16 bytes of x and of q.
   const int xsize = xtype == SGBLAS_TYPE_BF16 ? 2 : 4;
   const bool vector = aligned16(x) && ldx * static_cast<long long>(xsize) % 16 == 0 &&
-                      p.stride_x * xsize % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 &&
-                      ldq % 8 == 0 && p.stride_q % 8 == 0;
-  const auto g = static_cast<unsigned>(grid);
+                      p.stride_x * xsize % 16 == 0 && aligned16(q) && ldq % 16 == 0 &&
+                      p.stride_q % 16 == 0;
   if (xtype == SGBLAS_TYPE_BF16)
-    return launchStatus(vector ? launchQuantize<__nv_bfloat16, true>(p, block_n, g, stream)
-                               : launchQuantize<__nv_bfloat16, false>(p, block_n, g, stream));
-  return launchStatus(vector ? launchQuantize<float, true>(p, block_n, g, stream)
-                             : launchQuantize<float, false>(p, block_n, g, stream));
+    return launchStatus(vector ? launchQuantize<__nv_bfloat16, true>(p, block_n, grid, stream)
+                               : launchQuantize<__nv_bfloat16, false>(p, block_n, grid, stream));
+  return launchStatus(vector ? launchQuantize<float, true>(p, block_n, grid, stream)
+                             : launchQuantize<float, false>(p, block_n, grid, stream));
 }
 
 extern "C" sgblasStatus_t sgblasGemmFp8(sgblasHandle_t handle, int m, int n, int k, const void *a,
