@@ -3,6 +3,7 @@
 #include "product.hpp"
 
 #include "device.hpp"
+#include "product_thin.cuh"
 #include "sgemm_launch.hpp"
 
 #include <algorithm>
@@ -127,16 +128,87 @@ sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const 
   return launchProductKernel<G>(dev, p, tiles, stream);
 }
 
+// The thin kernel: clusters of `split` CTAs per 128 x kBN tile.
+template <class G>
+sgblasStatus_t launchThin(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+                          t::Params &p, cudaStream_t stream) {
+  if (p.k > 0 && (!encodeOperand(&p.tma_a, a, G::kElemBytes, G::kAMN, t::kBM) ||
+                  !encodeOperand(&p.tma_b, b, G::kElemBytes, false, t::kThinBox)))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  p.tiles_m = (p.m + t::kBM - 1) / t::kBM;
+  const long long most =
+      static_cast<long long>(p.tiles_m) * (p.n / G::kBN + std::min<long long>(p.groups, p.n));
+  if (most > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  // About as many as there will be: every group has a tile, few have two.
+  const long long tiles = static_cast<long long>(p.tiles_m) *
+                          std::max<long long>(std::min(p.groups, p.n), p.n / G::kBN);
+  auto kernel = t::thinProductKernel<G>;
+  static std::atomic<uint64_t> configured{0};
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes,
+                       &configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(t::kThinThreads);
+  cfg.dynamicSmemBytes = G::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  // The split with the shortest run: waves of tiles over the clusters that
+  // fit the GPU at once, each 1 / split of a tile long. A CTA keeps at least
+  // four slices of k, and 32 where clusters take several tiles in turn and
+  // the hand-overs add up (measured: 32 experts of 2048 x 2048 e4m3, 16 slices,
+  // 28.1 us whole and 29.8 in halves; of 2048 x 4096 bf16, 64 slices, 86.2 us
+  // whole and 80.1 in halves; 4096 x 4096 e4m3, one token, 11.3 us whole and
+  // 6.7 in quarters).
+  static std::atomic<int> resident[kMaxDevices][4];   // clusters of 2^i CTAs
+  const int iters = (p.k + G::kBK - 1) / G::kBK;
+  int split = 1, grid = 0;
+  double best = 1e30;
+  for (int i = 0, s = 1; s <= t::kMaxSplit; ++i, s *= 2) {
+    if (s > 1 && iters < 4 * s) break;
+    int clusters = s == 1 ? dev.sms : resident[dev.device][i].load(std::memory_order_relaxed);
+    if (clusters == 0) {
+      attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+      cfg.gridDim = dim3(static_cast<unsigned>(s));
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        clusters = 0;
+      }
+      if (clusters <= 0) clusters = -1;
+      resident[dev.device][i].store(clusters, std::memory_order_relaxed);
+    }
+    if (clusters < 0) break;
+    if (s > 1 && tiles > clusters && iters < 32 * s) continue;
+    const double run = static_cast<double>((tiles + clusters - 1) / clusters) / s;
+    if (run < 0.97 * best) {
+      best = run;
+      split = s;
+      grid = static_cast<int>(std::min<long long>(most, clusters));
+    }
+  }
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  cfg.gridDim = dim3(static_cast<unsigned>(split * grid));
+  // Without a split there is no cluster to launch.
+  cfg.attrs = split > 1 ? attr : attr + 1;
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p, split));
+}
+
 // Tile width by the tokens a group has on average.
 template <int kElemBytes, bool kAMN>
 sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
                              t::Params &p, cudaStream_t stream) {
   constexpr auto kN = t::Ragged::kN;
   const long long mean = p.n / std::max(p.groups, 1);
-  if (mean <= 32)
-    return launchTyped<t::Cfg<kElemBytes, kN, 32, kAMN, false, false>>(dev, a, b, p, stream);
-  if (mean <= 64)
-    return launchTyped<t::Cfg<kElemBytes, kN, 64, kAMN, false, false>>(dev, a, b, p, stream);
+  if (mean <= 3) return launchThin<t::ThinCfg<kElemBytes, 16, kAMN>>(dev, a, b, p, stream);
+  if (mean <= 12) return launchThin<t::ThinCfg<kElemBytes, 32, kAMN>>(dev, a, b, p, stream);
+  if (mean <= 40) return launchThin<t::ThinCfg<kElemBytes, 64, kAMN>>(dev, a, b, p, stream);
   if (mean <= 128)
     return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false>>(dev, a, b, p, stream);
   return launchTyped<t::Cfg<kElemBytes, kN, 256, kAMN, false, true>>(dev, a, b, p, stream);

@@ -229,41 +229,40 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
   return r;
 }
 
-// Fills the table (all threads; ends with a barrier).
+// Fills the table (one warp; a barrier of the CTA must follow).
 template <class G>
-__device__ __forceinline__ void readGroups(const Params &p, GroupTable *t) {
+__device__ __forceinline__ void readGroups(const Params &p, GroupTable *t, int lane) {
   if constexpr (G::kRagged == Ragged::kBatch) return;
   const int total = G::kRagged == Ragged::kN ? p.n : p.k;
-  if (p.offsets == nullptr) {
-    if (threadIdx.x == 0) {
+  if (p.offsets == nullptr) {   // one group
+    if (lane == 0) {
       t->offset[0] = 0;
       t->offset[1] = total;
+      t->first[0] = 0;
+      t->first[1] = (total + G::kBN - 1) / G::kBN;
     }
-  } else {
-    for (int g = threadIdx.x; g <= p.groups; g += kThreads)
-      t->offset[g] = min(max(p.offsets[g], 0), total);
+    return;
   }
-  __syncthreads();
-  if constexpr (G::kRagged == Ragged::kN) {
-    if (threadIdx.x < 32) {
-      int sum = 0;
-      for (int g0 = 0; g0 < p.groups; g0 += 32) {
-        const int g = g0 + static_cast<int>(threadIdx.x);
-        int v = 0;
-        if (g < p.groups) v = (max(0, t->offset[g + 1] - t->offset[g]) + G::kBN - 1) / G::kBN;
-        int scan = v;
+  int sum = 0;   // column tiles of the groups so far
+  for (int g0 = 0; g0 < p.groups; g0 += 32) {
+    const int g = g0 + lane;
+    const int begin = min(max(p.offsets[min(g, p.groups)], 0), total);
+    const int end = min(max(p.offsets[min(g + 1, p.groups)], 0), total);
+    const int v = (max(0, end - begin) + G::kBN - 1) / G::kBN;
+    int scan = v;
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-          const int o = __shfl_up_sync(0xffffffffu, scan, d);
-          if (static_cast<int>(threadIdx.x) >= d) scan += o;
-        }
-        if (g < p.groups) t->first[g] = sum + scan - v;
-        sum += __shfl_sync(0xffffffffu, scan, 31);
-      }
-      if (threadIdx.x == 0) t->first[p.groups] = sum;
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, scan, d);
+      if (lane >= d) scan += o;
     }
-    __syncthreads();
+    if (g < p.groups) {
+      t->offset[g] = begin;
+      t->first[g] = sum + scan - v;
+    }
+    if (g == p.groups - 1) t->offset[p.groups] = end;
+    sum += __shfl_sync(0xffffffffu, scan, 31);
   }
+  if (lane == 0) t->first[p.groups] = sum;
 }
 
 // Zeroes the 128-byte rows [row0, row1) of each 64-row box of an MN-major
@@ -530,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
   uint64_t *acc_empty = acc_full + kAccums;
   uint64_t *tail = acc_empty + kAccums;
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniformWarp(), lane = threadIdx.x % 32;
   // A worker is a CTA, or a pair: its position among them, and this CTA's in it.
   const int rank = G::kTwo ? static_cast<int>(blockIdx.x & 1) : 0;
   const int worker = G::kTwo ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
@@ -560,13 +559,16 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       tmemRelinquish();
     }
   }
-  gridDependencyWait();
-  readGroups<G>(p, &table);
   tcgenFenceBefore();
   __syncthreads();
   if constexpr (G::kTwo) clusterSync();   // both CTAs' barriers and TMEM exist
   tcgenFenceAfter();
   allowDependentLaunch();
+  gridDependencyWait();
+  if constexpr (G::kRagged != Ragged::kBatch) {
+    if (warp == 0) readGroups<G>(p, &table, lane);
+    __syncthreads();
+  }
   const uint32_t tmem_base = tmem_base_slot;
   const int tiles = tileCount<G>(p, table);
 
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
 
   if (warp < kEpilogueWarp0) {
     regDealloc<72>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && electOne()) {
       // ---------------- TMA producer ----------------
       int s = 0, parity = 1;   // the first pass over the ring waits for nothing
       for (int i = worker; i < tiles; i += workers) {
@@ -617,6 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       }
     } else if (warp == 1 && rank == 0) {
       // ---------------- MMA issuer ----------------
+      const bool leader = electOne();
       int s = 0, parity = 0;
       int b = 0, acc_parity = 1;
       unsigned tails = 0;   // bit s: parity of the next cut slice in stage s
@@ -644,13 +647,12 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
               fenceProxyAsyncShared();
               __syncwarp();
               if constexpr (G::kTwo) {
-                wait(&tail[s], (tails >> s) & 1);
+                if (ok) ok = mbarWaitCluster(&tail[s], (tails >> s) & 1, p.err);
                 tails ^= 1u << s;
-                fenceCluster();
               }
             }
           }
-          if (lane == 0) {
+          if (leader) {
             tcgenFenceAfter();
             const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * kBN);
             // Descriptors count 16 bytes. K-major: the next instruction's k

@@ -192,6 +192,23 @@ __device__ __forceinline__ void allowDependentLaunch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// One lane of a converged warp. Tensor-core instructions issued by the lane
+// it picks, in a warp whose number the compiler knows to be uniform
+// (uniformWarp), cost 40 clocks each; behind a `lane == 0` test 57 (measured
+// with narrow instructions, which end sooner).
+__device__ __forceinline__ bool electOne() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ int uniformWarp() {
+  return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0);
+}
+
 // ---- tcgen05: tensor memory and the 5th-generation tensor cores ------------
 // Tensor memory (TMEM) is allocated in columns (a power of two, 32..512) by
 // one whole warp; the allocated base address is written to shared memory.
@@ -290,7 +307,29 @@ __device__ __forceinline__ void tmemLoad32(uint32_t taddr, uint32_t (&v)[32]) {
   tmemWait32(v);
 }
 
-// Sixteen TMEM lanes (from the one in taddr) by 8 or 16 or 32 consecutive
+__device__ __forceinline__ void tmemWait16(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
+                 "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+
+// 16 consecutive TMEM columns, as tmemLoad32.
+__device__ __forceinline__ void tmemLoad16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+  tmemWait16(v);
+}
+
+// Sixteen TMEM lanes (from the one in taddr) by 16 or 32 consecutive
 // columns as fragments: for the 8 columns from 8 i, lane t of the warp gets
 // columns 8 i + 2 (t % 4) + {0, 1} of row t / 4 in v[at + 4 i + {0, 1}] and of
 // row t / 4 + 8 in v[at + 4 i + {2, 3}]. Usable after tmemWait.
@@ -316,15 +355,6 @@ __device__ __forceinline__ void tmemFragments(uint32_t taddr, uint32_t (&v)[kReg
         : "memory");
   }
 }
-__device__ __forceinline__ void tmemWait16(uint32_t (&v)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
-                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
-                 "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-               :
-               : "memory");
-}
-
 // Four 8 x 8 matrices of 16-bit values to shared memory, transposed: lane t
 // holds elements (t / 4, 2 (t % 4) + {0, 1}) of each; lane 8 i + j gives the
 // address (16 bytes) where column j of matrix i goes.
@@ -367,10 +397,33 @@ __device__ __forceinline__ void clusterSync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Orders this thread's memory accesses at cluster scope (an mbarrier wait
-// acquires at CTA scope only).
-__device__ __forceinline__ void fenceCluster() {
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+// mbarWait for a barrier that other CTAs of the cluster arrive on: acquires at
+// cluster scope what they released.
+__device__ __forceinline__ bool mbarWaitCluster(uint64_t *bar, uint32_t parity, unsigned *err) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smemAddr(bar)), "r"(parity)
+        : "memory");
+    if (done != 0) return true;
+  }
+  if (err != nullptr) atomicOr(err, kErrBarrierTimeout);
+  return false;
+}
+// Asynchronous 16-byte store to distributed shared memory, counted in bytes on
+// an mbarrier of the CTA it goes to (both cluster addresses).
+__device__ __forceinline__ void storeAsyncCluster4(uint32_t to, uint32_t bar, float x, float y,
+                                                   float z, float w) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, "
+      "[%5];" ::"r"(to),
+      "r"(__float_as_uint(x)), "r"(__float_as_uint(y)), "r"(__float_as_uint(z)),
+      "r"(__float_as_uint(w)), "r"(bar)
+      : "memory");
 }
 // Arrive on an mbarrier in any CTA of the cluster (cluster address).
 __device__ __forceinline__ void mbarArriveCluster(uint32_t cluster_bar) {
