@@ -200,6 +200,27 @@ sgblasStatus_t launchThin(const DeviceInfo &dev, const NarrowOperand &a, const N
   return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p, split));
 }
 
+// e4m3 products with the tokens on the rows of the tile.
+sgblasStatus_t launchRows(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+                          t::Params &p, cudaStream_t stream) {
+  using G = t::Cfg<1, t::Ragged::kM, 256, false, false, true>;
+  if (p.k > 0 && (!encodeOperand(&p.tma_a, b, 1, false, t::kBM) ||
+                  !encodeOperand(&p.tma_b, a, 1, false, G::kBRows)))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  p.tiles_n = (p.m + G::kBN - 1) / G::kBN;
+  const long long tiles = static_cast<long long>(p.tiles_n) *
+                          (p.n / G::kTileM + std::min<long long>(p.groups, p.n));
+  if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  p.c_tma = p.c_bf16 && aligned16(p.c) && p.ldc % 8 == 0;
+  if (p.c_tma) {
+    const unsigned long long column = static_cast<unsigned long long>(p.ldc) * 2;
+    if (!encodeTyped3d(&p.tma_c, CU_TENSOR_MAP_DATA_TYPE_UINT16, p.c, p.m, p.n, 1, column,
+                       column * p.n, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+      return SGBLAS_STATUS_EXECUTION_FAILED;
+  }
+  return launchProductKernel<G>(dev, p, tiles, stream);
+}
+
 // Tile width by the tokens a group has on average.
 template <int kElemBytes, bool kAMN>
 sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
@@ -211,7 +232,8 @@ sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, cons
   if (mean <= 40) return launchThin<t::ThinCfg<kElemBytes, 64, kAMN>>(dev, a, b, p, stream);
   if (mean <= 128)
     return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false>>(dev, a, b, p, stream);
-  return launchTyped<t::Cfg<kElemBytes, kN, 256, kAMN, false, true>>(dev, a, b, p, stream);
+  if constexpr (kElemBytes == 1) return launchRows(dev, a, b, p, stream);
+  else return launchTyped<t::Cfg<kElemBytes, kN, 256, kAMN, false, true>>(dev, a, b, p, stream);
 }
 
 }  // namespace

@@ -52,11 +52,14 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kEpilogueThreads = 32 * kEpilogueWarps;
 constexpr int kOutCols = 32;         // columns a warp passes through shared memory at once
 constexpr int kMaxGroups = 1024;
-constexpr int kScaleBatch = 4;      // blocks of 128 whose scales are staged at once
+constexpr int kScaleBatch = 8;      // blocks of 128 whose scales are staged at once
 
 // Which index the groups divide: n (columns of B and C), k (columns of A and
-// B), or none (a strided batch).
-enum class Ragged { kN, kK, kBatch };
+// B), or none (a strided batch). kM is kN with the operands' places exchanged
+// (e4m3 only): tokens on the TMEM lanes, so that a thread's row has one scale
+// per block instead of one per column, and C's contiguous rows of features
+// lie along a thread's registers.
+enum class Ragged { kN, kK, kBatch, kM };
 
 // kPlanes 2: every operand is a pair of fp16 matrices, hi + lo, and a product
 // is hi hi + hi lo + lo hi. kSymmetric: C is symmetric; only tiles on and
@@ -80,8 +83,13 @@ struct Cfg {
   static constexpr int kABytes = kBM * kRowBytes;
   static constexpr int kBBytes = kBRows * kRowBytes;
   static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
-  static constexpr int kScaleBytes = kBytes ? 2 * kScaleBatch * kBN * 4 : 0;
-  static constexpr int kOutBytes = kEpilogueWarps * kOutCols * 64;
+  static constexpr bool kRows = kRagged == Ragged::kM;
+  // Scales of the tile's columns, then the weights' one.
+  static constexpr bool kStaged = kBytes && !kRows;
+  static constexpr int kScalePitch = kBN + 4;
+  static constexpr int kScaleBytes = kStaged ? 2 * kScaleBatch * kScalePitch * 4 : 0;
+  static constexpr int kOutWarp = kRows ? 32 * kBN : kOutCols * 64;   // staging of a warp
+  static constexpr int kOutBytes = kEpilogueWarps * kOutWarp;
   static constexpr int kFit = (217 * 1024 - kScaleBytes - kOutBytes) / kStageBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kTmemColumns = kAccums * kBN;
@@ -91,6 +99,8 @@ struct Cfg {
   static_assert(kBN == 32 || kBN == 64 || kBN == 128 || kBN == 256, "tile width");
   static_assert(!kSymmetric || kBN == kTileM, "square tiles");
   static_assert(!kBytes || (!kAMN && !kBMN), "8-bit operands are K-major");
+  static_assert(!kRows || (kBytes && kBN == 256), "rows of tokens: e4m3, two blocks of weights");
+  static_assert(!kStaged || !kTwo, "a CTA's tile has one block of weights");
   static_assert(!kBMN || kBRows % 64 == 0, "whole boxes");
   static_assert(kStages >= 2 && kSmemBytes <= 218 * 1024 + 512, "shared memory beside the table");
 };
@@ -121,6 +131,8 @@ struct Params {
   int tiles_m, tiles_n;       // tiles_n: Ragged::kK and kBatch
   void *c;
   int c_bf16;
+  CUtensorMap tma_c;          // Ragged::kM, where c_tma: C in boxes of 64 rows and 32 columns
+  int c_tma;
   int ldc;
   long long stride_c;         // Ragged::kK and kBatch
   float alpha, beta;
@@ -169,15 +181,16 @@ struct GroupTable {
   int first[kMaxGroups + 1];
 };
 
-// One tile: its matrix, origin, valid columns, and k range.
+// One tile: its matrix, origin, valid columns (and rows, Ragged::kM), k range.
 struct Tile {
-  int group, m0, n0, cols, k0, klen;
+  int group, m0, n0, cols, k0, klen, rows;
 };
 
 template <class G>
 __device__ __forceinline__ int tileCount(const Params &p, const GroupTable &t) {
   if constexpr (G::kSymmetric) return p.tiles_m * (p.tiles_m + 1) / 2 * p.groups;
   if constexpr (G::kRagged == Ragged::kN) return p.tiles_m * t.first[p.groups];
+  if constexpr (G::kRagged == Ragged::kM) return p.tiles_n * t.first[p.groups];
   return p.tiles_m * p.tiles_n * p.groups;
 }
 
@@ -197,9 +210,11 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
     r.cols = min(G::kBN, p.n - r.n0);
     r.k0 = 0;
     r.klen = p.k;
-  } else if constexpr (G::kRagged == Ragged::kN) {
-    const int nt = index / p.tiles_m;
-    r.m0 = (index - nt * p.tiles_m) * G::kTileM;
+  } else if constexpr (G::kRagged == Ragged::kN || G::kRagged == Ragged::kM) {
+    // Tiles of weights vary fastest: the tiles at work at one time share tokens.
+    const int fixed = G::kRagged == Ragged::kN ? p.tiles_m : p.tiles_n;
+    const int nt = index / fixed;
+    const int at = index - nt * fixed;
     int lo = 0, hi = p.groups;   // the last group whose first tile is <= nt
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -207,10 +222,18 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
       else hi = mid;
     }
     r.group = lo;
-    r.n0 = t.offset[lo] + (nt - t.first[lo]) * G::kBN;
-    r.cols = min(G::kBN, t.offset[lo + 1] - r.n0);
     r.k0 = 0;
     r.klen = p.k;
+    if constexpr (G::kRagged == Ragged::kN) {
+      r.m0 = at * G::kTileM;
+      r.n0 = t.offset[lo] + (nt - t.first[lo]) * G::kBN;
+      r.cols = min(G::kBN, t.offset[lo + 1] - r.n0);
+    } else {
+      r.m0 = t.offset[lo] + (nt - t.first[lo]) * G::kTileM;
+      r.rows = t.offset[lo + 1] - r.m0;
+      r.n0 = at * G::kBN;
+      r.cols = min(G::kBN, p.m - r.n0);
+    }
   } else {
     const int per = p.tiles_m * p.tiles_n;
     r.group = index / per;
@@ -233,13 +256,14 @@ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int
 template <class G>
 __device__ __forceinline__ void readGroups(const Params &p, GroupTable *t, int lane) {
   if constexpr (G::kRagged == Ragged::kBatch) return;
-  const int total = G::kRagged == Ragged::kN ? p.n : p.k;
+  const int total = G::kRagged == Ragged::kK ? p.k : p.n;
+  constexpr int kTokens = G::kRagged == Ragged::kM ? G::kTileM : G::kBN;   // of a tile
   if (p.offsets == nullptr) {   // one group
     if (lane == 0) {
       t->offset[0] = 0;
       t->offset[1] = total;
       t->first[0] = 0;
-      t->first[1] = (total + G::kBN - 1) / G::kBN;
+      t->first[1] = (total + kTokens - 1) / kTokens;
     }
     return;
   }
@@ -248,7 +272,7 @@ __device__ __forceinline__ void readGroups(const Params &p, GroupTable *t, int l
     const int g = g0 + lane;
     const int begin = min(max(p.offsets[min(g, p.groups)], 0), total);
     const int end = min(max(p.offsets[min(g + 1, p.groups)], 0), total);
-    const int v = (max(0, end - begin) + G::kBN - 1) / G::kBN;
+    const int v = (max(0, end - begin) + kTokens - 1) / kTokens;
     int scan = v;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -457,6 +481,62 @@ __device__ __forceinline__ void storePair(const Params &p, size_t matrix, bool m
   }
 }
 
+// Four scales, of which `live` exist (zeros for the others).
+__device__ __forceinline__ float4 loadScales(const float *s, int live, bool aligned) {
+  if (aligned && live >= 4) return __ldg(reinterpret_cast<const float4 *>(s));
+  return make_float4(__ldg(s), live > 1 ? __ldg(s + 1) : 0.0F, live > 2 ? __ldg(s + 2) : 0.0F,
+                     live > 3 ? __ldg(s + 3) : 0.0F);
+}
+
+// A warp's 32 tokens (`live` of them in the group) by kCols features from
+// `feature0` (`cols` of them exist), a token per thread: a tile of BF16 leaves
+// through shared memory and TMA (which cuts it at C's last feature), one that
+// ends a group, or FP32, from registers.
+template <int kCols>
+__device__ __forceinline__ void storeTokens(const Params &p, int token0, int live, int feature0,
+                                            int cols, const float2 (&acc)[kCols / 2],
+                                            unsigned char *out, int lane) {
+  if (p.c_tma && live >= 32) {
+    if (lane == 0) bulkWaitRead();   // the tile before has left
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kCols / 8; ++j) {
+      // Eight features, in the box of 64 that holds them: 128-byte rows, 16-byte
+      // pieces exchanged by the row as the map's swizzle has them.
+      uint4 w;
+      w.x = packBf16(acc[4 * j]);
+      w.y = packBf16(acc[4 * j + 1]);
+      w.z = packBf16(acc[4 * j + 2]);
+      w.w = packBf16(acc[4 * j + 3]);
+      *reinterpret_cast<uint4 *>(out + j / 8 * 4096 + lane * 128 + ((j % 8) ^ (lane % 8)) * 16) = w;
+    }
+    fenceProxyAsyncShared();
+    __syncwarp();
+    if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < kCols / 64; ++j)
+        if (j * 64 < cols) tmaStore3d(&p.tma_c, out + j * 4096, feature0 + j * 64, token0, 0);
+      bulkCommit();
+    }
+    return;
+  }
+  if (lane >= live) return;
+  const size_t at = static_cast<size_t>(token0 + lane) * p.ldc + feature0;
+#pragma unroll
+  for (int j = 0; j < kCols / 2; ++j) {
+    if (2 * j >= cols) break;
+    if (p.c_bf16) {
+      __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + at + 2 * j;
+      c[0] = __float2bfloat16(acc[j].x);
+      if (2 * j + 1 < cols) c[1] = __float2bfloat16(acc[j].y);
+    } else {
+      float *c = static_cast<float *>(p.c) + at + 2 * j;
+      c[0] = acc[j].x;
+      if (2 * j + 1 < cols) c[1] = acc[j].y;
+    }
+  }
+}
+
 // The MMA of either form, and its completion signal to this CTA or both.
 template <class G>
 __device__ __forceinline__ void issueMma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
@@ -521,9 +601,9 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
   __shared__ uint32_t tmem_base_slot;
   __shared__ GroupTable table;
   unsigned char *smem = smem_raw + ((1024 - (smemAddr(smem_raw) & 1023)) & 1023);
-  float *scales = reinterpret_cast<float *>(smem + kStages * kStageBytes);
-  unsigned char *out_smem = smem + kStages * kStageBytes + G::kScaleBytes;
-  uint64_t *full = reinterpret_cast<uint64_t *>(out_smem + G::kOutBytes);
+  float *scales = reinterpret_cast<float *>(smem + kStages * kStageBytes + G::kOutBytes);
+  unsigned char *out_smem = smem + kStages * kStageBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(out_smem + G::kOutBytes + G::kScaleBytes);
   uint64_t *empty = full + kStages;
   uint64_t *acc_full = empty + kStages;
   uint64_t *acc_empty = acc_full + kAccums;
@@ -586,8 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       int s = 0, parity = 1;   // the first pass over the ring waits for nothing
       for (int i = worker; i < tiles; i += workers) {
         const Tile t = tileAt<G>(p, table, i);
-        const int za = G::kRagged == Ragged::kK ? 0 : t.group;
-        const int zb = G::kRagged == Ragged::kBatch ? t.group : 0;
+        const int za = G::kRagged == Ragged::kN || G::kRagged == Ragged::kBatch ? t.group : 0;
+        const int zb = G::kRagged == Ragged::kM || G::kRagged == Ragged::kBatch ? t.group : 0;
         const int m0 = t.m0 + rank * kBM;
         const int n0 = t.n0 + (G::kTwo ? rank * (widthOf(t.cols) / 2) : 0);
         for (int kk = 0; kk < t.klen; kk += G::kBK) {
@@ -720,30 +800,113 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
     const int quarter = warp % 4;
     const int col_begin = (warp - kEpilogueWarp0) / 4 * kHalf;
     const int etid = threadIdx.x - 32 * kEpilogueWarp0;
-    unsigned char *out = out_smem + (warp - kEpilogueWarp0) * kOutCols * 64;
+    unsigned char *out = out_smem + (warp - kEpilogueWarp0) * G::kOutWarp;
     // Vectors of eight 16-bit rows: columns aligned to 16 bytes.
     const bool vector = reinterpret_cast<uintptr_t>(p.c) % 16 == 0 && p.ldc % 8 == 0 &&
                         p.stride_c % 8 == 0;
     int b = 0, acc_parity = 0;
-    // Scales of kScaleBatch blocks of one column per thread, one batch ahead;
-    // scale_a * scale_b per (block, column) is staged in shared memory.
-    int scale_batches = 0;
-    float sa_next[kScaleBatch] = {}, sb_next[kScaleBatch] = {};
+    // Scales of kScaleBatch blocks (zeros where there are none), copied into
+    // one of two buffers while the other is in use.
+    int batches = 0;
     auto fetchScales = [&](const Tile &t, int ch) {
-      const int m0 = t.m0 + rank * kBM;
-      if (etid >= t.cols || m0 >= p.m) return;
+      float *dst = scales + (batches & 1) * kScaleBatch * G::kScalePitch;
       const int live = (t.klen + G::kBK - 1) / G::kBK - ch;
-      const float *sb = p.scale_b + static_cast<size_t>(t.n0 + etid) * p.ldsb + ch;
-      const float *sa = p.scale_a + t.group * p.stride_sa + static_cast<size_t>(m0 / 128) * p.ldsa + ch;
-#pragma unroll
-      for (int q = 0; q < kScaleBatch; ++q) {
-        sa_next[q] = q < live ? __ldg(sa + q) : 0.0F;
-        sb_next[q] = q < live ? __ldg(sb + q) : 0.0F;
+      const int c = etid % kBN;
+      const bool in = c < t.cols;
+      const float *sb = p.scale_b + static_cast<size_t>(in ? t.n0 + c : 0) * p.ldsb + ch;
+      for (int q = etid / kBN; q < kScaleBatch; q += kEpilogueThreads / kBN) {
+        const bool there = in && q < live;
+        cpAsync4(dst + q * G::kScalePitch + c, there ? sb + q : p.scale_b, there ? 4 : 0);
       }
+      if (etid < kScaleBatch) {
+        const float *sa = p.scale_a + t.group * p.stride_sa +
+                          static_cast<size_t>(t.m0 / 128) * p.ldsa + ch + etid;
+        const bool there = etid < live;
+        cpAsync4(dst + etid * G::kScalePitch + kBN, there ? sa : p.scale_a, there ? 4 : 0);
+      }
+      cpAsyncCommit();
+      ++batches;
     };
-    if constexpr (G::kBytes) {
+    // The scales of block ch of tile i, the tile of this call's loop.
+    auto scalesOf = [&](const Tile &t, int i, int ch, int chunks) {
+      if (ch % kScaleBatch == 0) {
+        cpAsyncWait<0>();
+        namedBarrier<1, kEpilogueThreads>();   // here for all; the other buffer is free
+        if (ch + kScaleBatch < chunks) fetchScales(t, ch + kScaleBatch);
+        else if (i + workers < tiles) fetchScales(tileAt<G>(p, table, i + workers), 0);
+        else ++batches;
+      }
+      return scales + ((batches & 1) * kScaleBatch + ch % kScaleBatch) * G::kScalePitch;
+    };
+    if constexpr (G::kStaged) {
       if (worker < tiles) fetchScales(tileAt<G>(p, table, worker), 0);
     }
+    if constexpr (G::kRows) {
+      // A row of the tile, one token, per thread. Its scales, four blocks at
+      // a time: those at work, and the next ones on their way.
+      const int row = quarter * 32 + lane;
+      const bool aligned = reinterpret_cast<uintptr_t>(p.scale_a) % 16 == 0 &&
+                           reinterpret_cast<uintptr_t>(p.scale_b) % 16 == 0 && p.ldsa % 4 == 0 &&
+                           p.ldsb % 4 == 0 && p.stride_sa % 4 == 0;
+      auto fetch = [&](const Tile &t, int ch, float4 *sb, float4 *sa) {
+        const int live = (t.klen + G::kBK - 1) / G::kBK - ch;
+        const int token = t.m0 + rank * kBM + row;
+        const int block = (t.n0 + col_begin) / 128;
+        *sb = *sa = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+        if (rank * kBM + row >= t.rows || block * 128 >= p.m || live <= 0) return;
+        *sb = loadScales(p.scale_b + static_cast<size_t>(token) * p.ldsb + ch, live, aligned);
+        *sa = loadScales(p.scale_a + t.group * p.stride_sa + static_cast<size_t>(block) * p.ldsa + ch,
+                         live, aligned);
+      };
+      float4 sb, sa;
+      if (worker < tiles) fetch(tileAt<G>(p, table, worker), 0, &sb, &sa);
+      for (int i = worker; i < tiles; i += workers) {
+        const Tile t = tileAt<G>(p, table, i);
+        const int chunks = (t.klen + G::kBK - 1) / G::kBK;
+        float2 acc[kHalf / 2];
+#pragma unroll
+        for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.0F, 0.0F);
+        float4 scale = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll 1
+        for (int ch = 0; ch < chunks; ++ch) {
+          if (ch % 4 == 0) {
+            scale = make_float4(sb.x * sa.x, sb.y * sa.y, sb.z * sa.z, sb.w * sa.w);
+            if (ch + 4 < chunks) fetch(t, ch + 4, &sb, &sa);
+            else if (i + workers < tiles) fetch(tileAt<G>(p, table, i + workers), 0, &sb, &sa);
+          }
+          const float2 s = make_float2(scale.x, scale.x);
+          scale = make_float4(scale.y, scale.z, scale.w, 0.0F);
+          wait(&acc_full[b], acc_parity);
+          tcgenFenceAfter();
+          const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                 static_cast<uint32_t>(b * kBN + col_begin);
+          uint32_t v[2][16];
+          tmemLoadAsync16(taddr, v[0]);
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 16) {
+            uint32_t(&now)[16] = v[c / 16 % 2];
+            tmemWait16(now);
+            if (c + 16 < kHalf) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              float2 &a = acc[(c + j) / 2];
+              a = __ffma2_rn(make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1])), s, a);
+            }
+          }
+          tcgenFenceBefore();
+          __syncwarp();
+          if (lane == 0) mbarArriveClusterRelaxed(clusterAddr(smemAddr(&acc_empty[b]), 0));
+          b ^= 1;
+          if (b == 0) acc_parity ^= 1;
+        }
+        const int token0 = t.m0 + rank * kBM + quarter * 32;
+        const int live = t.rows - rank * kBM - quarter * 32;
+        const int cols = t.cols - col_begin;
+        if (live > 0 && cols > 0)
+          storeTokens<kHalf>(p, token0, live, t.n0 + col_begin, cols, acc, out, lane);
+      }
+      if (lane == 0) bulkWait();
+    } else
     for (int i = worker; i < tiles; i += workers) {
       const Tile t = tileAt<G>(p, table, i);
       const int m0 = t.m0 + rank * kBM;
@@ -754,25 +917,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       for (int j = 0; j < kBlocks * 4; ++j) acc[j] = make_float2(0.0F, 0.0F);
       for (int ch = 0; ch < chunks; ++ch) {
         const float *sc = nullptr;
-        if constexpr (G::kBytes) {
-          if (ch % kScaleBatch == 0) {
-            // Stage this batch, fetched during the last one, and fetch the next.
-            float *dst = scales + (scale_batches & 1) * kScaleBatch * kBN;
-            if (etid < kBN) {
-#pragma unroll
-              for (int q = 0; q < kScaleBatch; ++q) dst[q * kBN + etid] = sa_next[q] * sb_next[q];
-            }
-            namedBarrier<1, kEpilogueThreads>();
-            ++scale_batches;
-            if (ch + kScaleBatch < chunks) {
-              fetchScales(t, ch + kScaleBatch);
-            } else if (i + workers < tiles) {
-              fetchScales(tileAt<G>(p, table, i + workers), 0);
-            }
-          }
-          sc = scales + ((scale_batches - 1) & 1) * kScaleBatch * kBN +
-               (ch % kScaleBatch) * kBN + col_begin;
-        }
+        if constexpr (G::kBytes) sc = scalesOf(t, i, ch, chunks);
         wait(&acc_full[b], acc_parity);
         tcgenFenceAfter();
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
@@ -782,8 +927,11 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
 #pragma unroll
           for (int i = 0; i < kLoad / 8; ++i) {
             float2 scale = make_float2(0.0F, 0.0F);
-            if constexpr (G::kBytes)
-              scale = *reinterpret_cast<const float2 *>(sc + c + i * 8 + lane % 4 * 2);
+            if constexpr (G::kBytes) {
+              scale = *reinterpret_cast<const float2 *>(sc + col_begin + c + i * 8 + lane % 4 * 2);
+              scale.x *= sc[kBN];
+              scale.y *= sc[kBN];
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int at = r / 2 * (kLoad / 2) + i * 4 + r % 2 * 2;
@@ -822,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
         tcgenFenceBefore();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (G::kTwo) mbarArriveCluster(clusterAddr(smemAddr(&acc_empty[b]), 0));
+          if constexpr (G::kTwo) mbarArriveClusterRelaxed(clusterAddr(smemAddr(&acc_empty[b]), 0));
           else mbarArrive(&acc_empty[b]);
         }
         b ^= 1;

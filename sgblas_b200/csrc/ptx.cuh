@@ -174,6 +174,23 @@ __device__ __forceinline__ void tmaLoad3d(void *dst, const CUtensorMap *map, uin
       : "memory");
 }
 
+// 3-D TMA tile store shared -> global, in this thread's bulk group (the
+// shared memory was written before a fenceProxyAsyncShared of its writers);
+// then the group's end, and the waits for its shared-memory reads and for all
+// of it.
+__device__ __forceinline__ void tmaStore3d(const CUtensorMap *map, const void *src, int x, int y,
+                                           int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   map),
+               "r"(smemAddr(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void bulkCommit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulkWaitRead() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulkWait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 __device__ __forceinline__ void prefetchTensorMap(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -316,8 +333,8 @@ __device__ __forceinline__ void tmemWait16(uint32_t (&v)[16]) {
                : "memory");
 }
 
-// 16 consecutive TMEM columns, as tmemLoad32.
-__device__ __forceinline__ void tmemLoad16(uint32_t taddr, uint32_t (&v)[16]) {
+// 16 consecutive TMEM columns, as tmemLoadAsync32 and tmemLoad32.
+__device__ __forceinline__ void tmemLoadAsync16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
       "%11, %12, %13, %14, %15}, [%16];"
@@ -326,6 +343,9 @@ __device__ __forceinline__ void tmemLoad16(uint32_t taddr, uint32_t (&v)[16]) {
         "=r"(v[14]), "=r"(v[15])
       : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmemLoad16(uint32_t taddr, uint32_t (&v)[16]) {
+  tmemLoadAsync16(taddr, v);
   tmemWait16(v);
 }
 
@@ -428,6 +448,14 @@ __device__ __forceinline__ void storeAsyncCluster4(uint32_t to, uint32_t bar, fl
 // Arrive on an mbarrier in any CTA of the cluster (cluster address).
 __device__ __forceinline__ void mbarArriveCluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+// The same without ordering memory: for an accumulator whose reads have
+// completed (tcgen05.wait::ld) and that publishes nothing. A release at
+// cluster scope waits for the thread's earlier global accesses, 1000 to 2000
+// clocks where a chunk's sums take 400.
+__device__ __forceinline__ void mbarArriveClusterRelaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
                : "memory");
 }
 // TMA 2-D load into this CTA's shared memory whose completion is counted on
