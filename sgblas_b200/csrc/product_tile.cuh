@@ -845,59 +845,72 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       // A row of the tile, one token, per thread. Its scales, four blocks at
       // a time: those at work, and the next ones on their way.
       const int row = quarter * 32 + lane;
+      const uint32_t acc_empty_even = clusterAddr(smemAddr(acc_empty), 0);
       const bool aligned = reinterpret_cast<uintptr_t>(p.scale_a) % 16 == 0 &&
                            reinterpret_cast<uintptr_t>(p.scale_b) % 16 == 0 && p.ldsa % 4 == 0 &&
                            p.ldsb % 4 == 0 && p.stride_sa % 4 == 0;
-      auto fetch = [&](const Tile &t, int ch, float4 *sb, float4 *sa) {
-        const int live = (t.klen + G::kBK - 1) / G::kBK - ch;
-        const int token = t.m0 + rank * kBM + row;
+      // Where a tile's scales begin; NULL for a thread without a token.
+      const float *sb_at = nullptr, *sa_at = nullptr;
+      auto locate = [&](const Tile &t) {
         const int block = (t.n0 + col_begin) / 128;
-        *sb = *sa = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-        if (rank * kBM + row >= t.rows || block * 128 >= p.m || live <= 0) return;
-        *sb = loadScales(p.scale_b + static_cast<size_t>(token) * p.ldsb + ch, live, aligned);
-        *sa = loadScales(p.scale_a + t.group * p.stride_sa + static_cast<size_t>(block) * p.ldsa + ch,
-                         live, aligned);
+        const bool in = rank * kBM + row < t.rows && block * 128 < p.m;
+        sb_at = in ? p.scale_b + static_cast<size_t>(t.m0 + rank * kBM + row) * p.ldsb : nullptr;
+        sa_at = p.scale_a + t.group * p.stride_sa + static_cast<size_t>(block) * p.ldsa;
       };
-      float4 sb, sa;
-      if (worker < tiles) fetch(tileAt<G>(p, table, worker), 0, &sb, &sa);
+      float4 sb = make_float4(0.0F, 0.0F, 0.0F, 0.0F), sa = sb;
+      auto fetch = [&](int ch, int live) {
+        if (sb_at != nullptr && live > 0) {
+          sb = loadScales(sb_at + ch, live, aligned);
+          sa = loadScales(sa_at + ch, live, aligned);
+        }
+      };
+      const int chunks = (p.k + G::kBK - 1) / G::kBK;
+      if (worker < tiles) {
+        locate(tileAt<G>(p, table, worker));
+        fetch(0, chunks);
+      }
       for (int i = worker; i < tiles; i += workers) {
         const Tile t = tileAt<G>(p, table, i);
-        const int chunks = (t.klen + G::kBK - 1) / G::kBK;
         float2 acc[kHalf / 2];
 #pragma unroll
         for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.0F, 0.0F);
-        float4 scale = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
 #pragma unroll 1
-        for (int ch = 0; ch < chunks; ++ch) {
-          if (ch % 4 == 0) {
-            scale = make_float4(sb.x * sa.x, sb.y * sa.y, sb.z * sa.z, sb.w * sa.w);
-            if (ch + 4 < chunks) fetch(t, ch + 4, &sb, &sa);
-            else if (i + workers < tiles) fetch(tileAt<G>(p, table, i + workers), 0, &sb, &sa);
+        for (int ch = 0; ch < chunks; ch += 4) {
+          const float scale[4] = {sb.x * sa.x, sb.y * sa.y, sb.z * sa.z, sb.w * sa.w};
+          if (ch + 4 < chunks) {
+            fetch(ch + 4, chunks - ch - 4);
+          } else if (i + workers < tiles) {
+            locate(tileAt<G>(p, table, i + workers));
+            fetch(0, chunks);
           }
-          const float2 s = make_float2(scale.x, scale.x);
-          scale = make_float4(scale.y, scale.z, scale.w, 0.0F);
-          wait(&acc_full[b], acc_parity);
-          tcgenFenceAfter();
-          const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                 static_cast<uint32_t>(b * kBN + col_begin);
-          uint32_t v[2][16];
-          tmemLoadAsync16(taddr, v[0]);
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 16) {
-            uint32_t(&now)[16] = v[c / 16 % 2];
-            tmemWait16(now);
-            if (c + 16 < kHalf) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
+          for (int q = 0; q < 4; ++q) {
+            if (ch + q >= chunks) break;
+            const float2 s = make_float2(scale[q], scale[q]);
+            wait(&acc_full[b], acc_parity);
+            tcgenFenceAfter();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                   static_cast<uint32_t>(b * kBN + col_begin);
+            uint32_t v[2][16];
+            tmemLoadAsync16(taddr, v[0]);
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              float2 &a = acc[(c + j) / 2];
-              a = __ffma2_rn(make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1])), s, a);
+            for (int c = 0; c < kHalf; c += 16) {
+              uint32_t(&now)[16] = v[c / 16 % 2];
+              tmemWait16(now);
+              if (c + 16 < kHalf) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                float2 &a = acc[(c + j) / 2];
+                a = __ffma2_rn(make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1])), s,
+                               a);
+              }
             }
+            tcgenFenceBefore();
+            __syncwarp();
+            if (lane == 0) mbarArriveClusterRelaxed(acc_empty_even + b * 8);
+            b ^= 1;
+            if (b == 0) acc_parity ^= 1;
           }
-          tcgenFenceBefore();
-          __syncwarp();
-          if (lane == 0) mbarArriveClusterRelaxed(clusterAddr(smemAddr(&acc_empty[b]), 0));
-          b ^= 1;
-          if (b == 0) acc_parity ^= 1;
         }
         const int token0 = t.m0 + rank * kBM + quarter * 32;
         const int live = t.rows - rank * kBM - quarter * 32;
