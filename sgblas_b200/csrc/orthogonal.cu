@@ -129,6 +129,13 @@ cudaError_t launchWith(const void *kernel, dim3 grid, int threads, int smem, cud
 }
 
 // p.m x p.n product of depth p.k over the batch; the epilogue is p.pair.out.
+// Tiles of one matrix.
+template <class G>
+long long pairTiles(int m, int n) {
+  const int tm = (m + G::kTileM - 1) / G::kTileM, tn = (n + G::kBN - 1) / G::kBN;
+  return G::kSymmetric ? t::symmetricTiles<G>(tm, tn) : static_cast<long long>(tm) * tn;
+}
+
 template <class G>
 sgblasStatus_t launchPairTyped(const DeviceInfo &dev, int batch, const PairMatrix &a,
                                const PairMatrix &b, t::Params &p, cudaStream_t stream) {
@@ -141,25 +148,29 @@ sgblasStatus_t launchPairTyped(const DeviceInfo &dev, int batch, const PairMatri
   p.err = dev.err;
   p.tiles_m = (p.m + G::kTileM - 1) / G::kTileM;
   p.tiles_n = (p.n + G::kBN - 1) / G::kBN;
-  const long long tiles = batch * (G::kSymmetric ? p.tiles_m * (p.tiles_m + 1LL) / 2
-                                                 : static_cast<long long>(p.tiles_m) * p.tiles_n);
+  const long long tiles = batch * pairTiles<G>(p.m, p.n);
   if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
   return launchProductKernel<G>(dev, p, tiles, stream);
 }
 
-// Pairs of CTAs where their 256 x 256 tiles are at least half as many as the
-// pairs; 128 x 128 tiles of single CTAs below.
+// The widest tiles of which there are enough for about every worker: pairs of
+// CTAs on 256 rows (a symmetric product's are 128 wide: 2048 x 2048 has 72 of
+// them for 74 pairs, and 36 square ones), else single CTAs on 128.
 template <bool kAMN, bool kBMN, bool kSymmetric>
 sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMatrix &a,
-                                 const PairMatrix &b, t::Params p, cudaStream_t stream) {
+                                 const PairMatrix &b, const t::Params &product,
+                                 cudaStream_t stream) {
   constexpr auto kB = t::Ragged::kBatch;
-  const long long tm = (p.m + 255) / 256, tn = (p.n + 255) / 256;
-  const long long tiles = batch * (kSymmetric ? tm * (tm + 1) / 2 : tm * tn);
-  if (4 * tiles >= dev.sms)
-    return launchPairTyped<t::Cfg<2, kB, 256, kAMN, kBMN, true, 2, kSymmetric>>(dev, batch, a, b, p,
-                                                                                stream);
-  return launchPairTyped<t::Cfg<2, kB, 128, kAMN, kBMN, false, 2, kSymmetric>>(dev, batch, a, b, p,
-                                                                               stream);
+  t::Params p = product;
+  constexpr int kWide = kSymmetric ? 128 : 256;
+  using Two = t::Cfg<2, kB, kWide, kAMN, kBMN, true, false, 2, kSymmetric>;
+  using One = t::Cfg<2, kB, 128, kAMN, kBMN, false, false, 2, kSymmetric>;
+  using Half = t::Cfg<2, kB, 64, kAMN, kBMN, false, false, 2, kSymmetric>;
+  if (4 * batch * pairTiles<Two>(p.m, p.n) >= dev.sms)
+    return launchPairTyped<Two>(dev, batch, a, b, p, stream);
+  if (2 * batch * pairTiles<One>(p.m, p.n) >= dev.sms)
+    return launchPairTyped<One>(dev, batch, a, b, p, stream);
+  return launchPairTyped<Half>(dev, batch, a, b, p, stream);
 }
 
 constexpr size_t align256(size_t v) { return (v + 255) / 256 * 256; }
@@ -239,6 +250,7 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
                                  qargs));
   for (int step = 0; step < steps && st == SGBLAS_STATUS_SUCCESS; ++step) {
     t::Params p = {};
+    p.pair.planes = 2;
     // A = X^T X or X X^T.
     p.m = p.n = s;
     p.k = l;
@@ -266,6 +278,9 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
     p.m = m;
     p.n = n;
     if (step == steps - 1) {
+      // Rounded to BF16 at once: the hi parts' 11 bits add a tenth to that
+      // rounding's error, and take a third of the instructions.
+      p.pair.planes = 1;
       p.pair.out = t::PairOut::kFinal;
       p.c = o;
       p.c_bf16 = 1;

@@ -230,10 +230,19 @@ sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, cons
   if (mean <= 3) return launchThin<t::ThinCfg<kElemBytes, 16, kAMN>>(dev, a, b, p, stream);
   if (mean <= 12) return launchThin<t::ThinCfg<kElemBytes, 32, kAMN>>(dev, a, b, p, stream);
   if (mean <= 40) return launchThin<t::ThinCfg<kElemBytes, 64, kAMN>>(dev, a, b, p, stream);
-  if (mean <= 128)
-    return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false>>(dev, a, b, p, stream);
-  if constexpr (kElemBytes == 1) return launchRows(dev, a, b, p, stream);
-  else return launchTyped<t::Cfg<kElemBytes, kN, 256, kAMN, false, true>>(dev, a, b, p, stream);
+  if (mean <= 128) {
+    if (p.c_bf16)
+      return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, false>>(dev, a, b, p,
+                                                                                 stream);
+    return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, true>>(dev, a, b, p, stream);
+  }
+  if constexpr (kElemBytes == 1) {
+    return launchRows(dev, a, b, p, stream);
+  } else {
+    if (p.c_bf16)
+      return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, false>>(dev, a, b, p, stream);
+    return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, true>>(dev, a, b, p, stream);
+  }
 }
 
 }  // namespace
@@ -271,7 +280,9 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
   else if (ragged == t::Ragged::kN && elem_bytes == 1 && !a_mn && !b_mn)
     st = launchRaggedN<1, false>(dev, a, b, p, stream);
   else if (ragged == t::Ragged::kK && elem_bytes == 2 && a_mn && b_mn)
-    st = launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true>>(dev, a, b, p, stream);
+    st = p.c_bf16
+             ? launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, false>>(dev, a, b, p, stream)
+             : launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, true>>(dev, a, b, p, stream);
   if (used_workspace && !markWorkspaceUse(ctx, stream) && st == SGBLAS_STATUS_SUCCESS)
     return SGBLAS_STATUS_EXECUTION_FAILED;
   return st;

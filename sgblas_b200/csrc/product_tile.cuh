@@ -62,16 +62,19 @@ constexpr int kScaleBatch = 8;      // blocks of 128 whose scales are staged at 
 enum class Ragged { kN, kK, kBatch, kM };
 
 // kPlanes 2: every operand is a pair of fp16 matrices, hi + lo, and a product
-// is hi hi + hi lo + lo hi. kSymmetric: C is symmetric; only tiles on and
-// below the diagonal are computed, and stored twice. kTwo: a pair of CTAs.
+// is hi hi + hi lo + lo hi. kSymmetric: C is symmetric; only tiles that reach
+// the diagonal or lie below it are computed, those below are stored twice.
+// kTwo: a pair of CTAs. kFp32: C is FP32, and a thread holds a row of the
+// tile: a warp's store is then 128 contiguous bytes, whatever C's alignment.
 template <int kElemBytes_, Ragged kRagged_, int kBN_, bool kAMN_, bool kBMN_, bool kTwo_,
-          int kPlanes_ = 1, bool kSymmetric_ = false>
+          bool kFp32_ = false, int kPlanes_ = 1, bool kSymmetric_ = false>
 struct Cfg {
   static constexpr int kElemBytes = kElemBytes_;
   static constexpr Ragged kRagged = kRagged_;
   static constexpr int kBN = kBN_;                     // columns of the tile
   static constexpr bool kAMN = kAMN_, kBMN = kBMN_;
   static constexpr bool kTwo = kTwo_;
+  static constexpr bool kFp32 = kFp32_;
   static constexpr int kPlanes = kPlanes_;
   static constexpr bool kSymmetric = kSymmetric_;
   static constexpr bool kBytes = kElemBytes == 1;
@@ -97,7 +100,7 @@ struct Cfg {
   static constexpr int kSmemBytes =
       kStages * kStageBytes + kScaleBytes + kOutBytes + kBarrierBytes + 1024;
   static_assert(kBN == 32 || kBN == 64 || kBN == 128 || kBN == 256, "tile width");
-  static_assert(!kSymmetric || kBN == kTileM, "square tiles");
+  static_assert(!kSymmetric || kTileM % kBN == 0, "tiles end at the diagonal");
   static_assert(!kBytes || (!kAMN && !kBMN), "8-bit operands are K-major");
   static_assert(!kRows || (kBytes && kBN == 256), "rows of tokens: e4m3, two blocks of weights");
   static_assert(!kStaged || !kTwo, "a CTA's tile has one block of weights");
@@ -121,6 +124,7 @@ struct PairParams {
   __half *hi, *lo;                   // written
   const __half *prev_hi, *prev_lo;   // kPoly reads
   float c0, c1, c2;
+  int planes;   // 2, or 1 to multiply the hi parts alone
 };
 
 struct Params {
@@ -186,9 +190,18 @@ struct Tile {
   int group, m0, n0, cols, k0, klen, rows;
 };
 
+// Tiles of one symmetric matrix: kWays times (tm + 1) in the row of tiles tm,
+// less those past the last column.
+template <class G>
+__host__ __device__ __forceinline__ int symmetricTiles(int tiles_m, int tiles_n) {
+  constexpr int kWays = G::kTileM / G::kBN;
+  const int past = kWays * tiles_m - tiles_n;
+  return kWays * (tiles_m * (tiles_m + 1) / 2) - (past > 0 ? past : 0);
+}
+
 template <class G>
 __device__ __forceinline__ int tileCount(const Params &p, const GroupTable &t) {
-  if constexpr (G::kSymmetric) return p.tiles_m * (p.tiles_m + 1) / 2 * p.groups;
+  if constexpr (G::kSymmetric) return symmetricTiles<G>(p.tiles_m, p.tiles_n) * p.groups;
   if constexpr (G::kRagged == Ragged::kN) return p.tiles_m * t.first[p.groups];
   if constexpr (G::kRagged == Ragged::kM) return p.tiles_n * t.first[p.groups];
   return p.tiles_m * p.tiles_n * p.groups;
@@ -198,15 +211,16 @@ template <class G>
 __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int index) {
   Tile r;
   if constexpr (G::kSymmetric) {
-    const int per = p.tiles_m * (p.tiles_m + 1) / 2;
+    constexpr int kWays = G::kTileM / G::kBN;
+    const int per = symmetricTiles<G>(p.tiles_m, p.tiles_n);
     r.group = index / per;
     const int i = index - r.group * per;
-    // Row of a triangle: the largest tm with tm (tm + 1) / 2 <= i.
-    int tm = static_cast<int>((sqrtf(8.0F * static_cast<float>(i) + 1.0F) - 1.0F) * 0.5F);
-    while (tm * (tm + 1) / 2 > i) --tm;
-    while ((tm + 1) * (tm + 2) / 2 <= i) ++tm;
+    // The row of tiles: the largest tm with kWays tm (tm + 1) / 2 <= i.
+    int tm = static_cast<int>((sqrtf(8.0F / kWays * static_cast<float>(i) + 1.0F) - 1.0F) * 0.5F);
+    while (kWays * (tm * (tm + 1) / 2) > i) --tm;
+    while (kWays * ((tm + 1) * (tm + 2) / 2) <= i) ++tm;
     r.m0 = tm * G::kTileM;
-    r.n0 = (i - tm * (tm + 1) / 2) * G::kBN;
+    r.n0 = (i - kWays * (tm * (tm + 1) / 2)) * G::kBN;
     r.cols = min(G::kBN, p.n - r.n0);
     r.k0 = 0;
     r.klen = p.k;
@@ -384,34 +398,33 @@ __device__ __forceinline__ void storeBf16(const Params &p, __nv_bfloat16 *c, int
   }
 }
 
-// The same in FP32, from registers: a warp's store covers four whole sectors
-// (eight rows) of four columns.
-template <int kBlocks>
+// The same in FP32 (kFp32): acc holds one row's columns, in pairs.
+template <int kCols>
 __device__ __forceinline__ void storeFp32(const Params &p, float *c, int cols, int rows,
-                                          const float2 (&acc)[kBlocks * 4], int lane) {
-  float *at = c + static_cast<long long>(lane % 4 * 2) * p.ldc + lane / 4;
-  const int row = lane / 4, col = lane % 4 * 2;
+                                          const float2 (&acc)[kCols / 2], int lane) {
+  if (lane >= rows) return;
+  c += lane;
+  if (p.beta == 0.0F) {
 #pragma unroll
-  for (int i = 0; i < kBlocks; ++i) {
-    if (i * 8 >= cols) break;
-    const bool in0 = i * 8 + col < cols, in1 = i * 8 + col + 1 < cols;
-    float *next = at + p.ldc;
-    if (p.beta == 0.0F) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool live = r * 8 + row < rows;
-        if (live && in0) at[r * 8] = p.alpha * acc[i * 4 + r].x;
-        if (live && in1) next[r * 8] = p.alpha * acc[i * 4 + r].y;
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool live = r * 8 + row < rows;
-        if (live && in0) at[r * 8] = fmaf(p.beta, at[r * 8], p.alpha * acc[i * 4 + r].x);
-        if (live && in1) next[r * 8] = fmaf(p.beta, next[r * 8], p.alpha * acc[i * 4 + r].y);
-      }
+    for (int j = 0; j < kCols; ++j) {
+      if (j < cols) *c = p.alpha * (j % 2 ? acc[j / 2].y : acc[j / 2].x);
+      c += p.ldc;
     }
-    at += 8LL * p.ldc;
+    return;
+  }
+  // Sixteen elements of C are read together.
+#pragma unroll
+  for (int j0 = 0; j0 < kCols; j0 += 16) {
+    float old[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j0 + j < cols) old[j] = c[static_cast<long long>(j) * p.ldc];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j0 + j < cols)
+        c[static_cast<long long>(j) * p.ldc] =
+            fmaf(p.beta, old[j], p.alpha * ((j % 2) ? acc[(j0 + j) / 2].y : acc[(j0 + j) / 2].x));
+    c += 16LL * p.ldc;
   }
 }
 
@@ -562,6 +575,7 @@ __device__ __forceinline__ void loadStage(const Params &p, unsigned char *stage,
                                           int m0, int n0, int k0, int za, int zb) {
 #pragma unroll
   for (int plane = 0; plane < G::kPlanes; ++plane) {
+    if (G::kPlanes == 2 && plane == p.pair.planes) break;
     unsigned char *sa = stage + plane * G::kABytes;
     unsigned char *sb = stage + G::kPlanes * G::kABytes + plane * G::kBBytes;
     const CUtensorMap *map_a = plane == 0 ? &p.tma_a : &p.pair.tma_a_lo;
@@ -674,11 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
           wait(&empty[s], parity);
           unsigned char *stage = smem + s * kStageBytes;
           const bool cut = G::kRagged == Ragged::kK && t.klen - kk < G::kBK;
+          const uint32_t bytes =
+              G::kPlanes == 2 && p.pair.planes == 1 ? kStageBytes / 2 : kStageBytes;
           if (!G::kTwo || cut) {
-            mbarArriveExpectTx(&full[s], kStageBytes);
+            mbarArriveExpectTx(&full[s], bytes);
             loadStage<G, false>(p, stage, &full[s], m0, n0, t.k0 + kk, za, zb);
           } else {
-            if (rank == 0) mbarArriveExpectTx(&full[s], 2 * kStageBytes);
+            if (rank == 0) mbarArriveExpectTx(&full[s], 2 * bytes);
             loadStage<G, G::kTwo>(p, stage, &full[s], m0, n0, t.k0 + kk, za, zb);
           }
           if (++s == kStages) {
@@ -746,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
             for (int j = 0; j < G::kBK / G::kMmaK; ++j) {
               if (j < steps) {
                 issueMma<G>(d_tmem, ad, bd, idesc, !first || j > 0);
-                if constexpr (G::kPlanes == 2) {
+                if (G::kPlanes == 2 && p.pair.planes == 2) {
                   issueMma<G>(d_tmem, ad, bd + G::kBBytes / 16, idesc, true);
                   issueMma<G>(d_tmem, ad + G::kABytes / 16, bd, idesc, true);
                 }
@@ -935,6 +951,29 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
         tcgenFenceAfter();
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                                static_cast<uint32_t>(b * kBN + col_begin);
+        if constexpr (G::kFp32) {
+          uint32_t v[2][16];
+          tmemLoadAsync16(taddr, v[0]);
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 16) {
+            uint32_t(&now)[16] = v[c / 16 % 2];
+            tmemWait16(now);
+            if (c + 16 < kHalf) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float2 x = make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1]));
+              float2 &a = acc[(c + j) / 2];
+              if constexpr (G::kBytes) {
+                float2 scale = *reinterpret_cast<const float2 *>(sc + col_begin + c + j);
+                scale.x *= sc[kBN];
+                scale.y *= sc[kBN];
+                a = __ffma2_rn(x, scale, a);
+              } else {
+                a = __fadd2_rn(a, x);
+              }
+            }
+          }
+        } else {
         // v: rows 0-15 of kLoad columns from c, then rows 16-31.
         auto accumulate = [&](int c, const uint32_t (&v)[kLoad]) {
 #pragma unroll
@@ -980,6 +1019,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
             accumulate(c, now);
           }
         }
+        }
         tcgenFenceBefore();
         __syncwarp();
         if (lane == 0) {
@@ -996,13 +1036,13 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       if (row0 < p.m && cols > 0) {
         const size_t at = matrix + static_cast<size_t>(col0) * p.ldc + row0;
         if constexpr (G::kPlanes == 2)
-          storePair<kBlocks, G::kSymmetric>(p, matrix, G::kSymmetric && t.m0 != t.n0, row0, col0,
+          storePair<kBlocks, G::kSymmetric>(p, matrix, G::kSymmetric && t.n0 + kBN <= t.m0, row0, col0,
                                             cols, acc, out, lane, vector);
-        else if (p.c_bf16)
+        else if constexpr (G::kFp32)
+          storeFp32<kHalf>(p, static_cast<float *>(p.c) + at, cols, p.m - row0, acc, lane);
+        else
           storeBf16<kBlocks>(p, static_cast<__nv_bfloat16 *>(p.c) + at, cols, p.m - row0, acc, out,
                              lane, vector);
-        else
-          storeFp32<kBlocks>(p, static_cast<float *>(p.c) + at, cols, p.m - row0, acc, lane);
       }
     }
   }
