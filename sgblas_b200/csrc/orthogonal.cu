@@ -31,11 +31,10 @@ namespace {
 namespace t = kern::prod;
 
 constexpr int kNormThreads = 256;
-constexpr int kMaxPartials = 256;   // partial sums of squares per matrix
+constexpr int kMaxPartials = 1024;   // partial sums of squares per matrix
 
 struct NormParams {
   const void *g;
-  int bf16;
   int m, n, ldg;
   long long stride_g;
   int partials;        // per matrix
@@ -46,11 +45,21 @@ struct NormParams {
   long long stride_x;
 };
 
-__device__ __forceinline__ float loadG(const NormParams &p, long long matrix, int row, int col) {
-  const long long at = matrix * p.stride_g + static_cast<long long>(col) * p.ldg + row;
-  return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.g)[at])
-                : static_cast<const float *>(p.g)[at];
-}
+// Values of one column a thread reads at once: 16 bytes where G is aligned.
+template <typename T, bool kVector>
+struct Run {
+  static constexpr int kCount = kVector ? 16 / static_cast<int>(sizeof(T)) : 1;
+  alignas(16) T v[kCount];
+  // From row `row` of a column of `rows`; zeros past its end.
+  __device__ __forceinline__ void load(const T *column, int row, int rows) {
+    if (kVector && row + kCount <= rows) {
+      *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(column + row));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kCount; ++j) v[j] = row + j < rows ? column[row + j] : static_cast<T>(0.0F);
+    }
+  }
+};
 
 // Sum over the block, the same in every thread; the order is fixed.
 __device__ __forceinline__ float blockSum(float v) {
@@ -66,34 +75,67 @@ __device__ __forceinline__ float blockSum(float v) {
 }
 
 // sums[matrix][i] = sum of squares of the columns i, i + partials, ...
+// Memory-bound, as is splitKernel.
+template <typename T, bool kVector>
 __global__ void __launch_bounds__(kNormThreads) squaresKernel(const NormParams p) {
+  using R = Run<T, kVector>;
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   float s = 0.0F;
-  for (int col = blockIdx.x; col < p.n; col += p.partials)
-    for (int row = threadIdx.x; row < p.m; row += kNormThreads) {
-      const float v = loadG(p, blockIdx.y, row, col);
-      s = fmaf(v, v, s);
+  for (int col = blockIdx.x; col < p.n; col += p.partials) {
+    const T *column = static_cast<const T *>(p.g) + blockIdx.y * p.stride_g +
+                      static_cast<long long>(col) * p.ldg;
+#pragma unroll 4
+    for (int row = threadIdx.x * R::kCount; row < p.m; row += kNormThreads * R::kCount) {
+      R r;
+      r.load(column, row, p.m);
+#pragma unroll
+      for (int j = 0; j < R::kCount; ++j) {
+        const float v = static_cast<float>(r.v[j]);
+        s = fmaf(v, v, s);
+      }
     }
+  }
   s = blockSum(s);
   if (threadIdx.x == 0) p.sums[static_cast<size_t>(blockIdx.y) * p.partials + blockIdx.x] = s;
 }
 
 // X = G / (norm + eps) as pairs.
+template <typename T, bool kVector>
 __global__ void __launch_bounds__(kNormThreads) splitKernel(const NormParams p) {
+  using R = Run<T, kVector>;
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const float *sums = p.sums + static_cast<size_t>(blockIdx.y) * p.partials;
-  const float norm =
-      sqrtf(blockSum(static_cast<int>(threadIdx.x) < p.partials ? sums[threadIdx.x] : 0.0F));
-  const float divisor = norm + p.eps;
-  for (int col = blockIdx.x; col < p.n; col += gridDim.x)
-    for (int row = threadIdx.x; row < p.m; row += kNormThreads) {
-      const float v = loadG(p, blockIdx.y, row, col) / divisor * t::kPairScale;
-      const size_t at = blockIdx.y * static_cast<size_t>(p.stride_x) +
-                        static_cast<size_t>(col) * p.ldx + row;
-      t::splitPair(v, &p.hi[at], &p.lo[at]);
+  float part = 0.0F;
+  for (int i = threadIdx.x; i < p.partials; i += kNormThreads) part += sums[i];
+  const float factor = t::kPairScale / (sqrtf(blockSum(part)) + p.eps);
+  for (int col = blockIdx.x; col < p.n; col += gridDim.x) {
+    const T *column = static_cast<const T *>(p.g) + blockIdx.y * p.stride_g +
+                      static_cast<long long>(col) * p.ldg;
+    const size_t to = blockIdx.y * static_cast<size_t>(p.stride_x) +
+                      static_cast<size_t>(col) * p.ldx;
+#pragma unroll 2
+    for (int row = threadIdx.x * R::kCount; row < p.m; row += kNormThreads * R::kCount) {
+      R r;
+      r.load(column, row, p.m);
+      // Columns of X are padded to 64 rows: whole vectors may be written.
+      alignas(16) __half hi[R::kCount], lo[R::kCount];
+#pragma unroll
+      for (int j = 0; j < R::kCount; ++j)
+        t::splitPair(static_cast<float>(r.v[j]) * factor, &hi[j], &lo[j]);
+      if constexpr (R::kCount == 8) {
+        *reinterpret_cast<uint4 *>(p.hi + to + row) = *reinterpret_cast<const uint4 *>(hi);
+        *reinterpret_cast<uint4 *>(p.lo + to + row) = *reinterpret_cast<const uint4 *>(lo);
+      } else if constexpr (R::kCount == 4) {
+        *reinterpret_cast<uint2 *>(p.hi + to + row) = *reinterpret_cast<const uint2 *>(hi);
+        *reinterpret_cast<uint2 *>(p.lo + to + row) = *reinterpret_cast<const uint2 *>(lo);
+      } else {
+        p.hi[to + row] = hi[0];
+        p.lo[to + row] = lo[0];
+      }
     }
+  }
 }
 
 // One pair matrix of the workspace: `batch` matrices of dim0 x dim1.
@@ -163,14 +205,26 @@ sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMat
   constexpr auto kB = t::Ragged::kBatch;
   t::Params p = product;
   constexpr int kWide = kSymmetric ? 128 : 256;
-  using Two = t::Cfg<2, kB, kWide, kAMN, kBMN, true, false, 2, kSymmetric>;
-  using One = t::Cfg<2, kB, 128, kAMN, kBMN, false, false, 2, kSymmetric>;
-  using Half = t::Cfg<2, kB, 64, kAMN, kBMN, false, false, 2, kSymmetric>;
+  using Two = t::Cfg<2, kB, kWide, kAMN, kBMN, true, true, 2, kSymmetric>;
+  using One = t::Cfg<2, kB, 128, kAMN, kBMN, false, true, 2, kSymmetric>;
+  using Half = t::Cfg<2, kB, 64, kAMN, kBMN, false, true, 2, kSymmetric>;
   if (4 * batch * pairTiles<Two>(p.m, p.n) >= dev.sms)
     return launchPairTyped<Two>(dev, batch, a, b, p, stream);
   if (2 * batch * pairTiles<One>(p.m, p.n) >= dev.sms)
     return launchPairTyped<One>(dev, batch, a, b, p, stream);
   return launchPairTyped<Half>(dev, batch, a, b, p, stream);
+}
+
+// The sums of squares, then the scaled pairs.
+template <typename T, bool kVector>
+sgblasStatus_t launchNorm(NormParams q, int batch, cudaStream_t stream) {
+  void *args[] = {&q};
+  const dim3 grid(static_cast<unsigned>(q.partials), static_cast<unsigned>(batch));
+  const cudaError_t e = launchWith(reinterpret_cast<const void *>(squaresKernel<T, kVector>), grid,
+                                   kNormThreads, 0, stream, args);
+  if (e != cudaSuccess) return launchStatus(e);
+  return launchStatus(launchWith(reinterpret_cast<const void *>(splitKernel<T, kVector>), grid,
+                                 kNormThreads, 0, stream, args));
 }
 
 constexpr size_t align256(size_t v) { return (v + 255) / 256 * 256; }
@@ -203,7 +257,8 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
   const bool tall = m >= n;
   const int s = std::min(m, n), l = std::max(m, n);
   const long long ldx = (m + 63LL) / 64 * 64, lds = (s + 63LL) / 64 * 64;
-  const int partials = std::min(n, kMaxPartials);
+  // About eight blocks per SM over the batch.
+  const int partials = std::min({n, kMaxPartials, std::max(1, 8 * dev.sms / batch)});
   const size_t sum_bytes = align256(static_cast<size_t>(batch) * partials * sizeof(float));
   const size_t x_bytes = static_cast<size_t>(ldx) * n * batch * sizeof(__half);   // 128-byte units
   const size_t s_bytes = static_cast<size_t>(lds) * s * batch * sizeof(__half);
@@ -229,7 +284,6 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
 
   NormParams q = {};
   q.g = g;
-  q.bf16 = gtype == SGBLAS_TYPE_BF16;
   q.m = m;
   q.n = n;
   q.ldg = ldg;
@@ -241,13 +295,15 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
   q.lo = x.lo;
   q.ldx = static_cast<int>(ldx);
   q.stride_x = x.stride;
-  void *qargs[] = {&q};
-  st = launchStatus(launchWith(reinterpret_cast<const void *>(squaresKernel),
-                               dim3(partials, batch), kNormThreads, 0, stream, qargs));
-  if (st == SGBLAS_STATUS_SUCCESS)
-    st = launchStatus(launchWith(reinterpret_cast<const void *>(splitKernel),
-                                 dim3(std::min(n, 4 * dev.sms), batch), kNormThreads, 0, stream,
-                                 qargs));
+  const int gsize = gtype == SGBLAS_TYPE_BF16 ? 2 : 4;
+  const bool vector = aligned16(g) && static_cast<long long>(ldg) * gsize % 16 == 0 &&
+                      q.stride_g * gsize % 16 == 0;
+  if (gtype == SGBLAS_TYPE_BF16)
+    st = vector ? launchNorm<__nv_bfloat16, true>(q, batch, stream)
+                : launchNorm<__nv_bfloat16, false>(q, batch, stream);
+  else
+    st = vector ? launchNorm<float, true>(q, batch, stream)
+                : launchNorm<float, false>(q, batch, stream);
   for (int step = 0; step < steps && st == SGBLAS_STATUS_SUCCESS; ++step) {
     t::Params p = {};
     p.pair.planes = 2;

@@ -64,8 +64,9 @@ enum class Ragged { kN, kK, kBatch, kM };
 // kPlanes 2: every operand is a pair of fp16 matrices, hi + lo, and a product
 // is hi hi + hi lo + lo hi. kSymmetric: C is symmetric; only tiles that reach
 // the diagonal or lie below it are computed, those below are stored twice.
-// kTwo: a pair of CTAs. kFp32: C is FP32, and a thread holds a row of the
-// tile: a warp's store is then 128 contiguous bytes, whatever C's alignment.
+// kTwo: a pair of CTAs. kFp32: what leaves the registers is FP32 (C, or pairs'
+// sums), and a thread holds a row of the tile: a warp's store is then 128
+// contiguous bytes, whatever C's alignment.
 template <int kElemBytes_, Ragged kRagged_, int kBN_, bool kAMN_, bool kBMN_, bool kTwo_,
           bool kFp32_ = false, int kPlanes_ = 1, bool kSymmetric_ = false>
 struct Cfg {
@@ -103,6 +104,7 @@ struct Cfg {
   static_assert(!kSymmetric || kTileM % kBN == 0, "tiles end at the diagonal");
   static_assert(!kBytes || (!kAMN && !kBMN), "8-bit operands are K-major");
   static_assert(!kRows || (kBytes && kBN == 256), "rows of tokens: e4m3, two blocks of weights");
+  static_assert(kPlanes == 1 || kFp32, "pairs leave from FP32 sums");
   static_assert(!kStaged || !kTwo, "a CTA's tile has one block of weights");
   static_assert(!kBMN || kBRows % 64 == 0, "whole boxes");
   static_assert(kStages >= 2 && kSmemBytes <= 218 * 1024 + 512, "shared memory beside the table");
@@ -428,70 +430,117 @@ __device__ __forceinline__ void storeFp32(const Params &p, float *c, int cols, i
   }
 }
 
-// A pair product's result (PairOut). `at` is this warp's first element in
-// hi, lo, prev (or c); row0 and col0 are its place in the matrix. The
-// polynomial reads A across (A is symmetric, and two columns of a row lie
-// together); the mirrored tile is written the same way. Rows of the pair
-// matrices are padded to 64 elements, so whole pairs and vectors may reach
-// past the last row or column into padding that nothing reads.
-template <int kBlocks, bool kSymmetric>
-__device__ __forceinline__ void storePair(const Params &p, size_t matrix, bool mirror, int row0,
-                                          int col0, int cols, const float2 (&acc)[kBlocks * 4],
-                                          unsigned char *out, int lane, bool vector) {
-  const size_t at = matrix + static_cast<size_t>(col0) * p.ldc + row0;
+// A pair product's result (PairOut) leaves kPairCols columns at a time: FP32
+// sums to shared memory, then flushPair, in a loop that is not unrolled over
+// the warp's columns (unrolled, it ran from a cold instruction cache: 11 to
+// 14 us of a 2048 x 2048 symmetric product's 45).
+constexpr int kPairCols = 16;
+
+// Word of (column, row) in a warp's staging block: groups of four rows are
+// rotated by the column, so that a row's columns, a column's rows and the
+// eight-row vectors of eight columns all spread over the banks.
+__device__ __forceinline__ int pairSlot(int col, int row) {
+  return col * 32 + ((row / 4 + col + col / 8) % 8) * 4 + row % 4;
+}
+
+// Writes the staged columns (`cols` of them exist) at row0, col0 of the
+// matrix: hi and lo of each value in vectors of eight rows, and (mirror) of
+// eight columns across the diagonal. The polynomial reads A the same way. Rows
+// of the pair matrices are padded to 64 elements, so vectors may reach past
+// the last row or column into padding that nothing reads.
+__device__ __forceinline__ void flushPair(const Params &p, size_t matrix, bool mirror, int row0,
+                                       int col0, int cols, uint32_t *out, int lane, bool vector) {
   const int rows = p.m - row0;
-  if (p.pair.out == PairOut::kFinal) {
-    storeBf16<kBlocks>(p, static_cast<__nv_bfloat16 *>(p.c) + at, cols, rows, acc, out, lane,
-                       vector);
-    return;
-  }
-  constexpr int kPass = kOutCols / 2 / 8;   // half the staging area each for hi and lo
-  unsigned char *out_lo = out + kOutCols / 2 * 64;
-  const bool poly = kSymmetric && p.pair.out == PairOut::kPoly;
+  // The polynomial's reads of A, together.
+  uint4 prev[kPairCols / 8][2];
+  if (p.pair.out == PairOut::kPoly) {
 #pragma unroll
-  for (int i0 = 0; i0 < kBlocks; i0 += kPass) {
-    if (i0 * 8 >= cols) break;
-#pragma unroll
-    for (int i = 0; i < kPass; ++i) {
-      const int col = (i0 + i) * 8 + lane % 4 * 2;
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = r * 8 + lane / 4;
-        const bool live = row < rows && col < cols;
-        const size_t across = matrix + static_cast<size_t>(row0 + row) * p.ldc + col0 + col;
-        float2 v = acc[(i0 + i) * 4 + r];
-        v.x *= 1.0F / kPairScale;
-        v.y *= 1.0F / kPairScale;
-        if (poly) {
-          float2 h = make_float2(0.0F, 0.0F), l = h;
-          if (live) {
-            h = __half22float2(*reinterpret_cast<const __half2 *>(p.pair.prev_hi + across));
-            l = __half22float2(*reinterpret_cast<const __half2 *>(p.pair.prev_lo + across));
-          }
-          v.x = fmaf(p.pair.c1, h.x + l.x, v.x * p.pair.c2);
-          v.y = fmaf(p.pair.c1, h.y + l.y, v.y * p.pair.c2);
-          if (col0 + col == row0 + row) v.x = fmaf(p.pair.c0, kPairScale, v.x);
-          if (col0 + col + 1 == row0 + row) v.y = fmaf(p.pair.c0, kPairScale, v.y);
-        }
-        const __half2 h2 = __float22half2_rn(v);
-        const float2 hf = __half22float2(h2);
-        const __half2 l2 = __float22half2_rn(make_float2(v.x - hf.x, v.y - hf.y));
-        hi[r] = *reinterpret_cast<const uint32_t *>(&h2);
-        lo[r] = *reinterpret_cast<const uint32_t *>(&l2);
-        if (mirror && live) {
-          *reinterpret_cast<uint32_t *>(p.pair.hi + across) = hi[r];
-          *reinterpret_cast<uint32_t *>(p.pair.lo + across) = lo[r];
-        }
+    for (int pass = 0; pass < kPairCols / 8; ++pass) {
+      const int col = pass * 8 + lane / 4, row = lane % 4 * 8;
+      const size_t at = matrix + static_cast<size_t>(col0 + col) * p.ldc + row0 + row;
+      const bool live = col < cols && row < rows;
+      prev[pass][0] = prev[pass][1] = make_uint4(0, 0, 0, 0);
+      if (live) {
+        prev[pass][0] = *reinterpret_cast<const uint4 *>(p.pair.prev_hi + at);
+        prev[pass][1] = *reinterpret_cast<const uint4 *>(p.pair.prev_lo + at);
       }
-      stageBlock(out, i, lane, hi);
-      stageBlock(out_lo, i, lane, lo);
     }
-    const size_t to = at + static_cast<size_t>(i0) * 8 * p.ldc;
-    const int left = min(cols - i0 * 8, kPass * 8);
-    copyOut(out, reinterpret_cast<uint16_t *>(p.pair.hi + to), p.ldc, left, rows, lane, true);
-    copyOut(out_lo, reinterpret_cast<uint16_t *>(p.pair.lo + to), p.ldc, left, rows, lane, true);
   }
+  __syncwarp();
+#pragma unroll
+  for (int pass = 0; pass < kPairCols / 8; ++pass) {
+    const int col = pass * 8 + lane / 4, row = lane % 4 * 8;
+    const bool live = col < cols && row < rows;
+    uint4 *slot[2] = {reinterpret_cast<uint4 *>(out + pairSlot(col, row)),
+                      reinterpret_cast<uint4 *>(out + pairSlot(col, row + 4))};
+    const size_t at = matrix + static_cast<size_t>(col0 + col) * p.ldc + row0 + row;
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 w = *slot[h];
+      v[4 * h] = __uint_as_float(w.x);
+      v[4 * h + 1] = __uint_as_float(w.y);
+      v[4 * h + 2] = __uint_as_float(w.z);
+      v[4 * h + 3] = __uint_as_float(w.w);
+    }
+    if (p.pair.out == PairOut::kFinal) {
+      __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + at;
+      alignas(16) __nv_bfloat16 r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = __float2bfloat16(v[j] * p.alpha);
+      if (live && vector && row + 8 <= rows) {
+        *reinterpret_cast<uint4 *>(c) = *reinterpret_cast<const uint4 *>(r);
+      } else if (live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (row + j < rows) c[j] = r[j];
+      }
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= 1.0F / kPairScale;
+    if (p.pair.out == PairOut::kPoly) {
+      const __half *ph = reinterpret_cast<const __half *>(&prev[pass][0]);
+      const __half *pl = reinterpret_cast<const __half *>(&prev[pass][1]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = fmaf(p.pair.c1, __half2float(ph[j]) + __half2float(pl[j]), v[j] * p.pair.c2);
+        if (row0 + row + j == col0 + col) v[j] = fmaf(p.pair.c0, kPairScale, v[j]);
+      }
+    }
+    alignas(16) __half hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) splitPair(v[j], &hi[j], &lo[j]);
+    const uint4 h = *reinterpret_cast<const uint4 *>(hi), l = *reinterpret_cast<const uint4 *>(lo);
+    if (live) {
+      *reinterpret_cast<uint4 *>(p.pair.hi + at) = h;
+      *reinterpret_cast<uint4 *>(p.pair.lo + at) = l;
+    }
+    if (mirror) {   // the pairs take the sums' places
+      *slot[0] = make_uint4(__byte_perm(h.x, l.x, 0x5410), __byte_perm(h.x, l.x, 0x7632),
+                            __byte_perm(h.y, l.y, 0x5410), __byte_perm(h.y, l.y, 0x7632));
+      *slot[1] = make_uint4(__byte_perm(h.z, l.z, 0x5410), __byte_perm(h.z, l.z, 0x7632),
+                            __byte_perm(h.w, l.w, 0x5410), __byte_perm(h.w, l.w, 0x7632));
+    }
+  }
+  __syncwarp();
+  if (!mirror) return;
+#pragma unroll
+  for (int pass = 0; pass < kPairCols / 8; ++pass) {
+    const int row = pass * 16 + lane / 2, col = lane % 2 * 8;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = out[pairSlot(col + j, row)];
+    if (row >= rows || col >= cols) continue;
+    const size_t at = matrix + static_cast<size_t>(row0 + row) * p.ldc + col0 + col;
+    *reinterpret_cast<uint4 *>(p.pair.hi + at) =
+        make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410),
+                   __byte_perm(w[4], w[5], 0x5410), __byte_perm(w[6], w[7], 0x5410));
+    *reinterpret_cast<uint4 *>(p.pair.lo + at) =
+        make_uint4(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632),
+                   __byte_perm(w[4], w[5], 0x7632), __byte_perm(w[6], w[7], 0x7632));
+  }
+  __syncwarp();
 }
 
 // Four scales, of which `live` exist (zeros for the others).
@@ -1035,10 +1084,22 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       const int col0 = t.n0 + col_begin, cols = t.cols - col_begin;
       if (row0 < p.m && cols > 0) {
         const size_t at = matrix + static_cast<size_t>(col0) * p.ldc + row0;
-        if constexpr (G::kPlanes == 2)
-          storePair<kBlocks, G::kSymmetric>(p, matrix, G::kSymmetric && t.n0 + kBN <= t.m0, row0, col0,
-                                            cols, acc, out, lane, vector);
-        else if constexpr (G::kFp32)
+        if constexpr (G::kPlanes == 2) {
+          uint32_t *words = reinterpret_cast<uint32_t *>(out);
+          const bool mirror = G::kSymmetric && t.n0 + kBN <= t.m0;
+#pragma unroll 1
+          for (int c = 0; c < min(cols, kHalf); c += kPairCols) {
+#pragma unroll
+            for (int k = 0; k < kHalf; k += kPairCols) {
+              if (k != c) continue;
+#pragma unroll
+              for (int j = 0; j < kPairCols; ++j)
+                words[pairSlot(j, lane)] =
+                    __float_as_uint(j % 2 ? acc[(k + j) / 2].y : acc[(k + j) / 2].x);
+            }
+            flushPair(p, matrix, mirror, row0, col0 + c, cols - c, words, lane, vector);
+          }
+        } else if constexpr (G::kFp32)
           storeFp32<kHalf>(p, static_cast<float *>(p.c) + at, cols, p.m - row0, acc, lane);
         else
           storeBf16<kBlocks>(p, static_cast<__nv_bfloat16 *>(p.c) + at, cols, p.m - row0, acc, out,
