@@ -47,7 +47,7 @@ extern "C" sgblasStatus_t sgblasGroupedGemmN(sgblasHandle_t handle, sgblasOperat
   p.c = c;
   p.c_bf16 = ctype == SGBLAS_TYPE_BF16;
   p.ldc = ldc;
-  p.alpha = *alpha;
+  p.alpha = product ? *alpha : 0.0F;
   p.beta = *beta;
   p.format = t::kFormatBf16;
   NarrowOperand oa, ob;
@@ -94,7 +94,7 @@ extern "C" sgblasStatus_t sgblasGroupedGemmK(sgblasHandle_t handle, int m, int n
   p.c_bf16 = ctype == SGBLAS_TYPE_BF16;
   p.ldc = ldc;
   p.stride_c = stride_c;
-  p.alpha = *alpha;
+  p.alpha = product ? *alpha : 0.0F;
   p.beta = *beta;
   p.format = t::kFormatBf16;
   NarrowOperand oa, ob;

@@ -125,6 +125,20 @@ sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const 
           ? static_cast<long long>(p.tiles_m) * (p.n / G::kBN + std::min<long long>(p.groups, p.n))
           : static_cast<long long>(p.tiles_m) * p.tiles_n * p.groups;
   if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  constexpr unsigned kSize = G::kFp32 ? 4 : 2;
+  const int matrices = G::kRagged == t::Ragged::kN ? 1 : p.groups;
+  const unsigned long long column = static_cast<unsigned long long>(p.ldc) * kSize;
+  const long long matrix = matrices == 1 ? static_cast<long long>(column * p.n)
+                                         : p.stride_c * static_cast<long long>(kSize);
+  p.c_tma = p.beta == 0.0F && aligned16(p.c) && column % 16 == 0 && matrix > 0 &&
+            matrix % 16 == 0 && matrix < (1LL << 40) && column < (1ULL << 40);
+  if (p.c_tma &&
+      !encodeTyped3d(&p.tma_c,
+                     G::kFp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                     p.c, p.m, p.n, matrices, column, static_cast<unsigned long long>(matrix), 32,
+                     t::kOutCols,
+                     G::kFp32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
   return launchProductKernel<G>(dev, p, tiles, stream);
 }
 
@@ -214,7 +228,7 @@ sgblasStatus_t launchRows(const DeviceInfo &dev, const NarrowOperand &a, const N
   p.c_tma = p.c_bf16 && aligned16(p.c) && p.ldc % 8 == 0;
   if (p.c_tma) {
     const unsigned long long column = static_cast<unsigned long long>(p.ldc) * 2;
-    if (!encodeTyped3d(&p.tma_c, CU_TENSOR_MAP_DATA_TYPE_UINT16, p.c, p.m, p.n, 1, column,
+    if (!encodeTyped3d(&p.tma_c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.c, p.m, p.n, 1, column,
                        column * p.n, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
       return SGBLAS_STATUS_EXECUTION_FAILED;
   }

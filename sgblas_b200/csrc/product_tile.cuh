@@ -50,7 +50,8 @@ constexpr int kThreads = 384;
 constexpr int kEpilogueWarp0 = 4;
 constexpr int kEpilogueWarps = 8;
 constexpr int kEpilogueThreads = 32 * kEpilogueWarps;
-constexpr int kOutCols = 32;         // columns a warp passes through shared memory at once
+constexpr int kOutCols = 16;         // columns in one of a warp's two staging buffers
+constexpr int kPairCols = 16;        // columns a warp of a pair product stages
 constexpr int kMaxGroups = 1024;
 constexpr int kScaleBatch = 8;      // blocks of 128 whose scales are staged at once
 
@@ -92,7 +93,11 @@ struct Cfg {
   static constexpr bool kStaged = kBytes && !kRows;
   static constexpr int kScalePitch = kBN + 4;
   static constexpr int kScaleBytes = kStaged ? 2 * kScaleBatch * kScalePitch * 4 : 0;
-  static constexpr int kOutWarp = kRows ? 32 * kBN : kOutCols * 64;   // staging of a warp
+  // Staging of a warp: 32 rows by 128 columns of BF16, the FP32 sums of
+  // kPairCols columns, or two buffers of kOutCols columns.
+  static constexpr int kOutWarp = kRows          ? 32 * kBN
+                                  : kPlanes == 2 ? kPairCols * 32 * 4
+                                                 : 2 * kOutCols * 32 * (kFp32 ? 4 : 2);
   static constexpr int kOutBytes = kEpilogueWarps * kOutWarp;
   static constexpr int kFit = (217 * 1024 - kScaleBytes - kOutBytes) / kStageBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
@@ -137,8 +142,8 @@ struct Params {
   int tiles_m, tiles_n;       // tiles_n: Ragged::kK and kBatch
   void *c;
   int c_bf16;
-  CUtensorMap tma_c;          // Ragged::kM, where c_tma: C in boxes of 64 rows and 32 columns
-  int c_tma;
+  CUtensorMap tma_c;          // where c_tma: C in boxes of 32 rows (Ragged::kM: 64) and 16 (32) columns
+  int c_tma;                  // C is aligned for TMA, and beta is 0
   int ldc;
   long long stride_c;         // Ragged::kK and kBatch
   float alpha, beta;
@@ -323,29 +328,40 @@ __device__ __forceinline__ void splitPair(float v, __half *hi, __half *lo) {
   *lo = __float2half_rn(v - __half2float(*hi));
 }
 
-// A warp's share of a tile in registers: 32 rows by 8 * kBlocks columns, as
-// tmemFragments gives them. acc[4 * i + r] holds columns 8 i + 2 (t % 4) + {0, 1}
+// Where a warp's share of a tile goes: its first element in C, that element's
+// row, column and matrix, and how many rows and columns of it exist. Columns
+// past the tile's last are another group's (kN) unless `clip` says that C ends
+// there.
+struct Place {
+  size_t at;
+  int row, col, matrix, rows, cols;
+  bool clip, vector;
+};
+
+// A warp's share in registers is 32 rows by 8 * kBlocks columns, as
+// tmemFragments gives them: acc[4 * i + r] holds columns 8 i + 2 (t % 4) + {0, 1}
 // of row 8 r + t / 4.
 //
-// 16-bit results pass through shared memory, 32 columns at a time: stmatrix
-// transposes each 8 x 8 block, so that a column's 32 rows (64 bytes) lie
-// together and leave in vectors. The 16-byte pieces of a column are rotated by
-// the column's pair, which spreads eight columns over all banks.
+// 16-bit results pass through shared memory, 16 columns at a time in two
+// buffers: stmatrix transposes each 8 x 8 block, so that a column's 32 rows (64
+// bytes) lie together. TMA takes them from there while the next columns are
+// staged (a group's last columns, and a C that TMA cannot write, leave by
+// copyOut). The 16-byte pieces of a column are exchanged by the column's pair,
+// as the 64-byte swizzle has them, which spreads eight columns over all banks.
 __device__ __forceinline__ uint32_t outSlot(int col, int piece) {
   return static_cast<uint32_t>(col * 64 + ((piece ^ (col / 2 % 4)) * 16));
 }
 
-// Block i of the columns (8 of them) into the staging area.
+// Block i of the columns (8 of them) into the staging buffer.
 __device__ __forceinline__ void stageBlock(unsigned char *out, int block, int lane,
                                            const uint32_t (&w)[4]) {
   storeMatrixTrans4(smemAddr(out) + outSlot(block * 8 + lane % 8, lane / 8), w[0], w[1], w[2], w[3]);
 }
 
-// kOutCols staged columns (of which `cols` exist) to c: vectors of eight rows
-// where the address allows, else a row per lane.
+// The staged columns (`cols` of them exist) to c: vectors of eight rows where
+// the address allows, else a row per lane.
 __device__ __forceinline__ void copyOut(const unsigned char *out, uint16_t *c, long long ldc,
                                         int cols, int rows, int lane, bool vector) {
-  __syncwarp();
   if (vector && rows >= 32) {
 #pragma unroll
     for (int i = 0; i < kOutCols / 8; ++i) {
@@ -370,15 +386,22 @@ __device__ __forceinline__ uint32_t packBf16(float2 v) {
 
 // C = alpha * acc + beta * C in BF16.
 template <int kBlocks>
-__device__ __forceinline__ void storeBf16(const Params &p, __nv_bfloat16 *c, int cols, int rows,
+__device__ __forceinline__ void storeBf16(const Params &p, const Place &to,
                                           const float2 (&acc)[kBlocks * 4], unsigned char *out,
-                                          int lane, bool vector) {
-  constexpr int kPass = kBlocks < kOutCols / 8 ? kBlocks : kOutCols / 8;
+                                          int lane) {
+  static_assert(kBlocks % 2 == 0, "whole buffers");
+  __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + to.at;
 #pragma unroll
-  for (int i0 = 0; i0 < kBlocks; i0 += kPass) {
-    if (i0 * 8 >= cols) break;
+  for (int i0 = 0; i0 < kBlocks; i0 += 2) {
+    if (i0 * 8 >= to.cols) break;
+    unsigned char *buffer = out + i0 / 2 % 2 * (kOutCols * 64);
+    const bool tma = p.c_tma && (to.clip || i0 * 8 + kOutCols <= to.cols);
+    if (p.c_tma) {
+      if (lane == 0) bulkWaitRead<1>();   // the buffer's last columns have left
+      __syncwarp();
+    }
 #pragma unroll
-    for (int i = 0; i < kPass; ++i) {
+    for (int i = 0; i < 2; ++i) {
       uint32_t w[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -388,45 +411,73 @@ __device__ __forceinline__ void storeBf16(const Params &p, __nv_bfloat16 *c, int
         if (p.beta != 0.0F) {
           const int row = r * 8 + lane / 4, col = (i0 + i) * 8 + lane % 4 * 2;
           const __nv_bfloat16 *at = c + static_cast<long long>(col) * p.ldc + row;
-          if (row < rows && col < cols) v.x = fmaf(p.beta, __bfloat162float(at[0]), v.x);
-          if (row < rows && col + 1 < cols) v.y = fmaf(p.beta, __bfloat162float(at[p.ldc]), v.y);
+          if (row < to.rows && col < to.cols) v.x = fmaf(p.beta, __bfloat162float(at[0]), v.x);
+          if (row < to.rows && col + 1 < to.cols)
+            v.y = fmaf(p.beta, __bfloat162float(at[p.ldc]), v.y);
         }
         w[r] = packBf16(v);
       }
-      stageBlock(out, i, lane, w);
+      stageBlock(buffer, i, lane, w);
     }
-    copyOut(out, reinterpret_cast<uint16_t *>(c) + static_cast<long long>(i0) * 8 * p.ldc, p.ldc,
-            min(cols - i0 * 8, kPass * 8), rows, lane, vector);
+    if (tma) {
+      fenceProxyAsyncShared();
+      __syncwarp();
+      if (lane == 0) tmaStore3d(&p.tma_c, buffer, to.row, to.col + i0 * 8, to.matrix);
+    } else {
+      __syncwarp();
+      copyOut(buffer, reinterpret_cast<uint16_t *>(c) + static_cast<long long>(i0) * 8 * p.ldc,
+              p.ldc, to.cols - i0 * 8, to.rows, lane, to.vector);
+    }
+    if (p.c_tma && lane == 0) bulkCommit();
   }
 }
 
-// The same in FP32 (kFp32): acc holds one row's columns, in pairs.
+// The same in FP32 (kFp32): acc holds one row's columns, in pairs, and a
+// column's 32 rows are 128 bytes.
 template <int kCols>
-__device__ __forceinline__ void storeFp32(const Params &p, float *c, int cols, int rows,
-                                          const float2 (&acc)[kCols / 2], int lane) {
-  if (lane >= rows) return;
-  c += lane;
-  if (p.beta == 0.0F) {
+__device__ __forceinline__ void storeFp32(const Params &p, const Place &to,
+                                          const float2 (&acc)[kCols / 2], unsigned char *out,
+                                          int lane) {
+  auto value = [&](int j) { return p.alpha * (j % 2 ? acc[j / 2].y : acc[j / 2].x); };
+  float *c = static_cast<float *>(p.c) + to.at + lane;
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) {
-      if (j < cols) *c = p.alpha * (j % 2 ? acc[j / 2].y : acc[j / 2].x);
-      c += p.ldc;
+  for (int j0 = 0; j0 < kCols; j0 += kOutCols) {
+    if (j0 >= to.cols) break;
+    if (p.c_tma) {
+      float *buffer = reinterpret_cast<float *>(out) + j0 / kOutCols % 2 * (kOutCols * 32);
+      if (lane == 0) bulkWaitRead<1>();
+      __syncwarp();
+      if (to.clip || j0 + kOutCols <= to.cols) {
+#pragma unroll
+        for (int j = 0; j < kOutCols; ++j) buffer[j * 32 + lane] = value(j0 + j);
+        fenceProxyAsyncShared();
+        __syncwarp();
+        if (lane == 0) {
+          tmaStore3d(&p.tma_c, buffer, to.row, to.col + j0, to.matrix);
+          bulkCommit();
+        }
+        c += static_cast<long long>(kOutCols) * p.ldc;
+        continue;
+      }
+      if (lane == 0) bulkCommit();
     }
-    return;
-  }
-  // Sixteen elements of C are read together.
+    if (lane < to.rows) {
+      float old[kOutCols];
+      if (p.beta != 0.0F) {   // read together
 #pragma unroll
-  for (int j0 = 0; j0 < kCols; j0 += 16) {
-    float old[16];
+        for (int j = 0; j < kOutCols; ++j)
+          if (j0 + j < to.cols) old[j] = c[static_cast<long long>(j) * p.ldc];
+      }
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j0 + j < cols) old[j] = c[static_cast<long long>(j) * p.ldc];
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j0 + j < cols)
-        c[static_cast<long long>(j) * p.ldc] =
-            fmaf(p.beta, old[j], p.alpha * ((j % 2) ? acc[(j0 + j) / 2].y : acc[(j0 + j) / 2].x));
-    c += 16LL * p.ldc;
+      for (int j = 0; j < kOutCols; ++j) {
+        if (j0 + j < to.cols) {
+          float v = value(j0 + j);
+          if (p.beta != 0.0F) v = fmaf(p.beta, old[j], v);
+          c[static_cast<long long>(j) * p.ldc] = v;
+        }
+      }
+    }
+    c += static_cast<long long>(kOutCols) * p.ldc;
   }
 }
 
@@ -434,7 +485,6 @@ __device__ __forceinline__ void storeFp32(const Params &p, float *c, int cols, i
 // sums to shared memory, then flushPair, in a loop that is not unrolled over
 // the warp's columns (unrolled, it ran from a cold instruction cache: 11 to
 // 14 us of a 2048 x 2048 symmetric product's 45).
-constexpr int kPairCols = 16;
 
 // Word of (column, row) in a warp's staging block: groups of four rows are
 // rotated by the column, so that a row's columns, a column's rows and the
@@ -551,16 +601,17 @@ __device__ __forceinline__ float4 loadScales(const float *s, int live, bool alig
 }
 
 // A warp's 32 tokens (`live` of them in the group) by kCols features from
-// `feature0` (`cols` of them exist), a token per thread: a tile of BF16 leaves
-// through shared memory and TMA (which cuts it at C's last feature), one that
-// ends a group, or FP32, from registers.
+// `feature0` (`cols` of them exist), a token per thread, through shared
+// memory. A whole tile of BF16 leaves by TMA (which cuts it at C's last
+// feature); one that ends a group, or another C, row by row.
 template <int kCols>
 __device__ __forceinline__ void storeTokens(const Params &p, int token0, int live, int feature0,
                                             int cols, const float2 (&acc)[kCols / 2],
                                             unsigned char *out, int lane) {
-  if (p.c_tma && live >= 32) {
-    if (lane == 0) bulkWaitRead();   // the tile before has left
-    __syncwarp();
+  if (lane == 0) bulkWaitRead<0>();   // the tile before has left
+  __syncwarp();
+  const size_t at = static_cast<size_t>(token0) * p.ldc + feature0;
+  if (p.c_bf16) {
 #pragma unroll
     for (int j = 0; j < kCols / 8; ++j) {
       // Eight features, in the box of 64 that holds them: 128-byte rows, 16-byte
@@ -572,30 +623,62 @@ __device__ __forceinline__ void storeTokens(const Params &p, int token0, int liv
       w.w = packBf16(acc[4 * j + 3]);
       *reinterpret_cast<uint4 *>(out + j / 8 * 4096 + lane * 128 + ((j % 8) ^ (lane % 8)) * 16) = w;
     }
-    fenceProxyAsyncShared();
-    __syncwarp();
-    if (lane == 0) {
+    if (p.c_tma && live >= 32) {
+      fenceProxyAsyncShared();
+      __syncwarp();
+      if (lane == 0) {
 #pragma unroll
-      for (int j = 0; j < kCols / 64; ++j)
-        if (j * 64 < cols) tmaStore3d(&p.tma_c, out + j * 4096, feature0 + j * 64, token0, 0);
-      bulkCommit();
+        for (int j = 0; j < kCols / 64; ++j)
+          if (j * 64 < cols) tmaStore3d(&p.tma_c, out + j * 4096, feature0 + j * 64, token0, 0);
+        bulkCommit();
+      }
+      return;
     }
+    __syncwarp();
+    __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + at;
+    const int f = 2 * lane;   // two features of each box
+#pragma unroll 2
+    for (int r = 0; r < min(live, 32); ++r) {
+      const bool pairs = reinterpret_cast<uintptr_t>(c) % 4 == 0;
+#pragma unroll
+      for (int j = 0; j < kCols / 64; ++j) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(
+            out + j * 4096 + r * 128 + ((lane / 4) ^ (r % 8)) * 16 + lane % 4 * 4);
+        const int first = j * 64 + f;
+        if (pairs && first + 1 < cols) {
+          *reinterpret_cast<uint32_t *>(c + first) = w;
+        } else {
+          const auto *h = reinterpret_cast<const __nv_bfloat16 *>(&w);
+          if (first < cols) c[first] = h[0];
+          if (first + 1 < cols) c[first + 1] = h[1];
+        }
+      }
+      c += p.ldc;
+    }
+    __syncwarp();
     return;
   }
-  if (lane >= live) return;
-  const size_t at = static_cast<size_t>(token0 + lane) * p.ldc + feature0;
+  // FP32: 64 features at a time, 256-byte rows with their pieces exchanged by the row.
 #pragma unroll
-  for (int j = 0; j < kCols / 2; ++j) {
-    if (2 * j >= cols) break;
-    if (p.c_bf16) {
-      __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + at + 2 * j;
-      c[0] = __float2bfloat16(acc[j].x);
-      if (2 * j + 1 < cols) c[1] = __float2bfloat16(acc[j].y);
-    } else {
-      float *c = static_cast<float *>(p.c) + at + 2 * j;
-      c[0] = acc[j].x;
-      if (2 * j + 1 < cols) c[1] = acc[j].y;
+  for (int f0 = 0; f0 < kCols; f0 += 64) {
+    if (f0 >= cols) break;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      *reinterpret_cast<float4 *>(out + lane * 256 + (j ^ (lane % 16)) * 16) =
+          make_float4(acc[f0 / 2 + 2 * j].x, acc[f0 / 2 + 2 * j].y, acc[f0 / 2 + 2 * j + 1].x,
+                      acc[f0 / 2 + 2 * j + 1].y);
+    __syncwarp();
+    float *c = static_cast<float *>(p.c) + at + f0 + lane;
+#pragma unroll 2
+    for (int r = 0; r < min(live, 32); ++r) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (f0 + h * 32 + lane < cols)
+          c[h * 32] = *reinterpret_cast<const float *>(
+              out + r * 256 + ((lane / 4 + h * 8) ^ (r % 16)) * 16 + lane % 4 * 4);
+      c += p.ldc;
     }
+    __syncwarp();
   }
 }
 
@@ -983,7 +1066,6 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
         if (live > 0 && cols > 0)
           storeTokens<kHalf>(p, token0, live, t.n0 + col_begin, cols, acc, out, lane);
       }
-      if (lane == 0) bulkWait();
     } else
     for (int i = worker; i < tiles; i += workers) {
       const Tile t = tileAt<G>(p, table, i);
@@ -1083,7 +1165,6 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       const int row0 = m0 + quarter * 32;
       const int col0 = t.n0 + col_begin, cols = t.cols - col_begin;
       if (row0 < p.m && cols > 0) {
-        const size_t at = matrix + static_cast<size_t>(col0) * p.ldc + row0;
         if constexpr (G::kPlanes == 2) {
           uint32_t *words = reinterpret_cast<uint32_t *>(out);
           const bool mirror = G::kSymmetric && t.n0 + kBN <= t.m0;
@@ -1099,13 +1180,22 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
             }
             flushPair(p, matrix, mirror, row0, col0 + c, cols - c, words, lane, vector);
           }
-        } else if constexpr (G::kFp32)
-          storeFp32<kHalf>(p, static_cast<float *>(p.c) + at, cols, p.m - row0, acc, lane);
-        else
-          storeBf16<kBlocks>(p, static_cast<__nv_bfloat16 *>(p.c) + at, cols, p.m - row0, acc, out,
-                             lane, vector);
+        } else {
+          Place to;
+          to.at = matrix + static_cast<size_t>(col0) * p.ldc + row0;
+          to.row = row0;
+          to.col = col0;
+          to.matrix = G::kRagged == Ragged::kN ? 0 : t.group;
+          to.rows = p.m - row0;
+          to.cols = cols;
+          to.clip = G::kRagged != Ragged::kN;
+          to.vector = vector;
+          if constexpr (G::kFp32) storeFp32<kHalf>(p, to, acc, out, lane);
+          else storeBf16<kBlocks>(p, to, acc, out, lane);
+        }
       }
     }
+    if (lane == 0) bulkWait();   // every store has been made
   }
 
   tcgenFenceBefore();

@@ -186,8 +186,9 @@ __device__ __forceinline__ void tmaStore3d(const CUtensorMap *map, const void *s
                : "memory");
 }
 __device__ __forceinline__ void bulkCommit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int kLeft>   // all but the last kLeft groups
 __device__ __forceinline__ void bulkWaitRead() {
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
 }
 __device__ __forceinline__ void bulkWait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
