@@ -130,7 +130,7 @@ sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const 
   const unsigned long long column = static_cast<unsigned long long>(p.ldc) * kSize;
   const long long matrix = matrices == 1 ? static_cast<long long>(column * p.n)
                                          : p.stride_c * static_cast<long long>(kSize);
-  p.c_tma = p.beta == 0.0F && aligned16(p.c) && column % 16 == 0 && matrix > 0 &&
+  p.c_tma = p.beta == 0.0F && (p.c_bf16 != 0) == (kSize == 2) && aligned16(p.c) && column % 16 == 0 && matrix > 0 &&
             matrix % 16 == 0 && matrix < (1LL << 40) && column < (1ULL << 40);
   if (p.c_tma &&
       !encodeTyped3d(&p.tma_c,
@@ -241,11 +241,12 @@ sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, cons
                              t::Params &p, cudaStream_t stream) {
   constexpr auto kN = t::Ragged::kN;
   const long long mean = p.n / std::max(p.groups, 1);
+  const bool plain = p.c_bf16 && p.beta == 0.0F;   // else rows of FP32 sums
   if (mean <= 3) return launchThin<t::ThinCfg<kElemBytes, 16, kAMN>>(dev, a, b, p, stream);
   if (mean <= 12) return launchThin<t::ThinCfg<kElemBytes, 32, kAMN>>(dev, a, b, p, stream);
   if (mean <= 40) return launchThin<t::ThinCfg<kElemBytes, 64, kAMN>>(dev, a, b, p, stream);
   if (mean <= 128) {
-    if (p.c_bf16)
+    if (plain)
       return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, false>>(dev, a, b, p,
                                                                                  stream);
     return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, true>>(dev, a, b, p, stream);
@@ -253,7 +254,7 @@ sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, cons
   if constexpr (kElemBytes == 1) {
     return launchRows(dev, a, b, p, stream);
   } else {
-    if (p.c_bf16)
+    if (plain)
       return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, false>>(dev, a, b, p, stream);
     return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, true>>(dev, a, b, p, stream);
   }
@@ -294,7 +295,7 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
   else if (ragged == t::Ragged::kN && elem_bytes == 1 && !a_mn && !b_mn)
     st = launchRaggedN<1, false>(dev, a, b, p, stream);
   else if (ragged == t::Ragged::kK && elem_bytes == 2 && a_mn && b_mn)
-    st = p.c_bf16
+    st = p.c_bf16 && p.beta == 0.0F
              ? launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, false>>(dev, a, b, p, stream)
              : launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, true>>(dev, a, b, p, stream);
   if (used_workspace && !markWorkspaceUse(ctx, stream) && st == SGBLAS_STATUS_SUCCESS)

@@ -65,9 +65,9 @@ enum class Ragged { kN, kK, kBatch, kM };
 // kPlanes 2: every operand is a pair of fp16 matrices, hi + lo, and a product
 // is hi hi + hi lo + lo hi. kSymmetric: C is symmetric; only tiles that reach
 // the diagonal or lie below it are computed, those below are stored twice.
-// kTwo: a pair of CTAs. kFp32: what leaves the registers is FP32 (C, or pairs'
-// sums), and a thread holds a row of the tile: a warp's store is then 128
-// contiguous bytes, whatever C's alignment.
+// kTwo: a pair of CTAs. kFp32: C is FP32 or BF16 with a beta, or a pair's
+// sums are staged, and a thread holds a row of the tile: a warp's store is then
+// 32 contiguous rows, whatever C's alignment.
 template <int kElemBytes_, Ragged kRagged_, int kBN_, bool kAMN_, bool kBMN_, bool kTwo_,
           bool kFp32_ = false, int kPlanes_ = 1, bool kSymmetric_ = false>
 struct Cfg {
@@ -384,13 +384,14 @@ __device__ __forceinline__ uint32_t packBf16(float2 v) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// C = alpha * acc + beta * C in BF16.
+// C = alpha * acc in BF16 (beta is 0 here: its reads of C, even unused, would
+// double the code that every tile runs through).
 template <int kBlocks>
 __device__ __forceinline__ void storeBf16(const Params &p, const Place &to,
                                           const float2 (&acc)[kBlocks * 4], unsigned char *out,
                                           int lane) {
   static_assert(kBlocks % 2 == 0, "whole buffers");
-  __nv_bfloat16 *c = static_cast<__nv_bfloat16 *>(p.c) + to.at;
+  uint16_t *c = static_cast<uint16_t *>(p.c) + to.at;
 #pragma unroll
   for (int i0 = 0; i0 < kBlocks; i0 += 2) {
     if (i0 * 8 >= to.cols) break;
@@ -405,17 +406,8 @@ __device__ __forceinline__ void storeBf16(const Params &p, const Place &to,
       uint32_t w[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float2 v = acc[(i0 + i) * 4 + r];
-        v.x *= p.alpha;
-        v.y *= p.alpha;
-        if (p.beta != 0.0F) {
-          const int row = r * 8 + lane / 4, col = (i0 + i) * 8 + lane % 4 * 2;
-          const __nv_bfloat16 *at = c + static_cast<long long>(col) * p.ldc + row;
-          if (row < to.rows && col < to.cols) v.x = fmaf(p.beta, __bfloat162float(at[0]), v.x);
-          if (row < to.rows && col + 1 < to.cols)
-            v.y = fmaf(p.beta, __bfloat162float(at[p.ldc]), v.y);
-        }
-        w[r] = packBf16(v);
+        const float2 v = acc[(i0 + i) * 4 + r];
+        w[r] = packBf16(make_float2(v.x * p.alpha, v.y * p.alpha));
       }
       stageBlock(buffer, i, lane, w);
     }
@@ -425,60 +417,80 @@ __device__ __forceinline__ void storeBf16(const Params &p, const Place &to,
       if (lane == 0) tmaStore3d(&p.tma_c, buffer, to.row, to.col + i0 * 8, to.matrix);
     } else {
       __syncwarp();
-      copyOut(buffer, reinterpret_cast<uint16_t *>(c) + static_cast<long long>(i0) * 8 * p.ldc,
-              p.ldc, to.cols - i0 * 8, to.rows, lane, to.vector);
+      copyOut(buffer, c, p.ldc, to.cols - i0 * 8, to.rows, lane, to.vector);
     }
     if (p.c_tma && lane == 0) bulkCommit();
+    c += static_cast<long long>(kOutCols) * p.ldc;
   }
 }
 
-// The same in FP32 (kFp32): acc holds one row's columns, in pairs, and a
-// column's 32 rows are 128 bytes.
+// C = alpha * acc + beta * C from rows (kFp32): FP32, or BF16 with beta, whose
+// columns' rows are read and written 32 at a time.
+template <typename T>
+__device__ __forceinline__ void updateColumns(const Params &p, T *c, int cols, const float *sums,
+                                              int lane) {
+#pragma unroll 4
+  for (int j = 0; j < cols; ++j) {
+    float v = p.alpha * sums[j * 32 + lane];
+    if (p.beta != 0.0F) v = fmaf(p.beta, static_cast<float>(*c), v);
+    *c = static_cast<T>(v);
+    c += p.ldc;
+  }
+}
+
+// A kFp32 warp's share: acc holds one row's columns, in pairs. FP32 without
+// beta leaves 16 columns at a time, by TMA from two buffers (a column's 32 rows
+// are 128 bytes there) or, where TMA cannot write them, a column per store.
+// The rest is rare and compact.
 template <int kCols>
 __device__ __forceinline__ void storeFp32(const Params &p, const Place &to,
                                           const float2 (&acc)[kCols / 2], unsigned char *out,
                                           int lane) {
-  auto value = [&](int j) { return p.alpha * (j % 2 ? acc[j / 2].y : acc[j / 2].x); };
-  float *c = static_cast<float *>(p.c) + to.at + lane;
+  auto sum = [&](int j) { return j % 2 ? acc[j / 2].y : acc[j / 2].x; };
+  float *buffers = reinterpret_cast<float *>(out);
+  if (p.beta == 0.0F && !p.c_bf16) {
+    float *c = static_cast<float *>(p.c) + to.at + lane;
 #pragma unroll
-  for (int j0 = 0; j0 < kCols; j0 += kOutCols) {
-    if (j0 >= to.cols) break;
-    if (p.c_tma) {
-      float *buffer = reinterpret_cast<float *>(out) + j0 / kOutCols % 2 * (kOutCols * 32);
-      if (lane == 0) bulkWaitRead<1>();
-      __syncwarp();
-      if (to.clip || j0 + kOutCols <= to.cols) {
+    for (int j0 = 0; j0 < kCols; j0 += kOutCols) {
+      if (j0 >= to.cols) break;
+      float *buffer = buffers + j0 / kOutCols % 2 * (kOutCols * 32);
+      if (p.c_tma) {
+        if (lane == 0) bulkWaitRead<1>();   // the buffer's last columns have left
+        __syncwarp();
+      }
+      if (p.c_tma && (to.clip || j0 + kOutCols <= to.cols)) {
 #pragma unroll
-        for (int j = 0; j < kOutCols; ++j) buffer[j * 32 + lane] = value(j0 + j);
+        for (int j = 0; j < kOutCols; ++j) buffer[j * 32 + lane] = p.alpha * sum(j0 + j);
         fenceProxyAsyncShared();
         __syncwarp();
-        if (lane == 0) {
-          tmaStore3d(&p.tma_c, buffer, to.row, to.col + j0, to.matrix);
-          bulkCommit();
-        }
-        c += static_cast<long long>(kOutCols) * p.ldc;
-        continue;
-      }
-      if (lane == 0) bulkCommit();
-    }
-    if (lane < to.rows) {
-      float old[kOutCols];
-      if (p.beta != 0.0F) {   // read together
+        if (lane == 0) tmaStore3d(&p.tma_c, buffer, to.row, to.col + j0, to.matrix);
+      } else if (lane < to.rows) {
 #pragma unroll
         for (int j = 0; j < kOutCols; ++j)
-          if (j0 + j < to.cols) old[j] = c[static_cast<long long>(j) * p.ldc];
+          if (j0 + j < to.cols) c[static_cast<long long>(j) * p.ldc] = p.alpha * sum(j0 + j);
       }
-#pragma unroll
-      for (int j = 0; j < kOutCols; ++j) {
-        if (j0 + j < to.cols) {
-          float v = value(j0 + j);
-          if (p.beta != 0.0F) v = fmaf(p.beta, old[j], v);
-          c[static_cast<long long>(j) * p.ldc] = v;
-        }
-      }
+      if (p.c_tma && lane == 0) bulkCommit();
+      c += static_cast<long long>(kOutCols) * p.ldc;
     }
-    c += static_cast<long long>(kOutCols) * p.ldc;
+    return;
   }
+#pragma unroll 1
+  for (int j0 = 0; j0 < min(to.cols, kCols); j0 += kOutCols) {
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kCols; k += kOutCols) {
+      if (k != j0) continue;
+#pragma unroll
+      for (int j = 0; j < kOutCols; ++j) buffers[j * 32 + lane] = sum(k + j);
+    }
+    if (lane < to.rows) {
+      const size_t at = to.at + static_cast<size_t>(j0) * p.ldc + lane;
+      const int cols = min(to.cols - j0, kOutCols);
+      if (p.c_bf16) updateColumns(p, static_cast<__nv_bfloat16 *>(p.c) + at, cols, buffers, lane);
+      else updateColumns(p, static_cast<float *>(p.c) + at, cols, buffers, lane);
+    }
+  }
+  __syncwarp();
 }
 
 // A pair product's result (PairOut) leaves kPairCols columns at a time: FP32
