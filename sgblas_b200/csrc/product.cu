@@ -135,9 +135,9 @@ sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const 
   if (p.c_tma &&
       !encodeTyped3d(&p.tma_c,
                      G::kFp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                     p.c, p.m, p.n, matrices, column, static_cast<unsigned long long>(matrix), 32,
-                     t::kOutCols,
-                     G::kFp32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B))
+                     p.c, p.m, p.n, matrices, column, static_cast<unsigned long long>(matrix),
+                     G::kFp32 ? 32 : 64, t::kOutCols,
+                     G::kFp32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
     return SGBLAS_STATUS_EXECUTION_FAILED;
   return launchProductKernel<G>(dev, p, tiles, stream);
 }

@@ -142,7 +142,7 @@ struct Params {
   int tiles_m, tiles_n;       // tiles_n: Ragged::kK and kBatch
   void *c;
   int c_bf16;
-  CUtensorMap tma_c;          // where c_tma: C in boxes of 32 rows (Ragged::kM: 64) and 16 (32) columns
+  CUtensorMap tma_c;          // where c_tma: C in boxes of 64 rows (FP32: 32) and 16 columns (kM: 32)
   int c_tma;                  // C is aligned for TMA, and beta is 0
   int ldc;
   long long stride_c;         // Ragged::kK and kBatch
@@ -343,40 +343,48 @@ struct Place {
 // of row 8 r + t / 4.
 //
 // 16-bit results pass through shared memory, 16 columns at a time in two
-// buffers: stmatrix transposes each 8 x 8 block, so that a column's 32 rows (64
-// bytes) lie together. TMA takes them from there while the next columns are
-// staged (a group's last columns, and a C that TMA cannot write, leave by
-// copyOut). The 16-byte pieces of a column are exchanged by the column's pair,
-// as the 64-byte swizzle has them, which spreads eight columns over all banks.
+// buffers that two warps share: stmatrix transposes each 8 x 8 block, so that a
+// column's 64 rows (128 bytes) lie together. TMA takes them from there while
+// the next columns are staged (a group's last columns, and a C that TMA cannot
+// write, leave by copyOut). TMA stores about one row of a box per four clocks,
+// whatever its length: 64-byte rows of single warps left at 4.7 TB/s. The
+// 16-byte pieces of a column are exchanged by the column, as the 128-byte
+// swizzle has them, which spreads eight columns over all banks.
 __device__ __forceinline__ uint32_t outSlot(int col, int piece) {
-  return static_cast<uint32_t>(col * 64 + ((piece ^ (col / 2 % 4)) * 16));
+  return static_cast<uint32_t>(col * 128 + ((piece ^ (col % 8)) * 16));
 }
 
-// Block i of the columns (8 of them) into the staging buffer.
-__device__ __forceinline__ void stageBlock(unsigned char *out, int block, int lane,
+// Block i of the columns (8 of them), the upper or lower 32 rows, into the
+// staging buffer.
+__device__ __forceinline__ void stageBlock(unsigned char *out, int block, int lower, int lane,
                                            const uint32_t (&w)[4]) {
-  storeMatrixTrans4(smemAddr(out) + outSlot(block * 8 + lane % 8, lane / 8), w[0], w[1], w[2], w[3]);
+  storeMatrixTrans4(smemAddr(out) + outSlot(block * 8 + lane % 8, lower * 4 + lane / 8), w[0], w[1],
+                    w[2], w[3]);
 }
 
-// The staged columns (`cols` of them exist) to c: vectors of eight rows where
-// the address allows, else a row per lane.
-__device__ __forceinline__ void copyOut(const unsigned char *out, uint16_t *c, long long ldc,
-                                        int cols, int rows, int lane, bool vector) {
+// A warp's rows of the staged columns (`cols` of them exist) to c: vectors of
+// eight rows where the address allows, else a row per lane.
+__device__ __forceinline__ void copyOut(const unsigned char *out, int lower, uint16_t *c,
+                                        long long ldc, int cols, int rows, int lane, bool vector) {
   if (vector && rows >= 32) {
 #pragma unroll
     for (int i = 0; i < kOutCols / 8; ++i) {
       const int col = i * 8 + lane / 4;
       if (col < cols)
         *reinterpret_cast<uint4 *>(c + col * ldc + lane % 4 * 8) =
-            *reinterpret_cast<const uint4 *>(out + outSlot(col, lane % 4));
+            *reinterpret_cast<const uint4 *>(out + outSlot(col, lower * 4 + lane % 4));
     }
   } else if (lane < rows) {
 #pragma unroll 4
     for (int col = 0; col < min(cols, kOutCols); ++col)
-      c[col * ldc + lane] =
-          *reinterpret_cast<const uint16_t *>(out + outSlot(col, lane / 8) + lane % 8 * 2);
+      c[col * ldc + lane] = *reinterpret_cast<const uint16_t *>(
+          out + outSlot(col, lower * 4 + lane / 8) + lane % 8 * 2);
   }
-  __syncwarp();
+}
+
+// The two warps that share staging buffers (`pair` 0 to 3).
+__device__ __forceinline__ void pairBarrier(int pair) {
+  asm volatile("bar.sync %0, 64;" ::"r"(2 + pair) : "memory");
 }
 
 __device__ __forceinline__ uint32_t packBf16(float2 v) {
@@ -385,22 +393,21 @@ __device__ __forceinline__ uint32_t packBf16(float2 v) {
 }
 
 // C = alpha * acc in BF16 (beta is 0 here: its reads of C, even unused, would
-// double the code that every tile runs through).
+// double the code that every tile runs through). Both warps of a pair call
+// it; one of them may have no rows.
 template <int kBlocks>
 __device__ __forceinline__ void storeBf16(const Params &p, const Place &to,
                                           const float2 (&acc)[kBlocks * 4], unsigned char *out,
-                                          int lane) {
+                                          int pair, int lower, int lane) {
   static_assert(kBlocks % 2 == 0, "whole buffers");
   uint16_t *c = static_cast<uint16_t *>(p.c) + to.at;
+  const bool issues = lower == 0 && lane == 0;
 #pragma unroll
   for (int i0 = 0; i0 < kBlocks; i0 += 2) {
     if (i0 * 8 >= to.cols) break;
-    unsigned char *buffer = out + i0 / 2 % 2 * (kOutCols * 64);
-    const bool tma = p.c_tma && (to.clip || i0 * 8 + kOutCols <= to.cols);
-    if (p.c_tma) {
-      if (lane == 0) bulkWaitRead<1>();   // the buffer's last columns have left
-      __syncwarp();
-    }
+    unsigned char *buffer = out + i0 / 2 % 2 * (kOutCols * 128);
+    if (issues) bulkWaitRead<1>();   // the buffer's last columns have left
+    pairBarrier(pair);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       uint32_t w[4];
@@ -409,17 +416,17 @@ __device__ __forceinline__ void storeBf16(const Params &p, const Place &to,
         const float2 v = acc[(i0 + i) * 4 + r];
         w[r] = packBf16(make_float2(v.x * p.alpha, v.y * p.alpha));
       }
-      stageBlock(buffer, i, lane, w);
+      stageBlock(buffer, i, lower, lane, w);
     }
-    if (tma) {
+    if (p.c_tma && (to.clip || i0 * 8 + kOutCols <= to.cols)) {
       fenceProxyAsyncShared();
-      __syncwarp();
-      if (lane == 0) tmaStore3d(&p.tma_c, buffer, to.row, to.col + i0 * 8, to.matrix);
+      pairBarrier(pair);
+      if (issues) tmaStore3d(&p.tma_c, buffer, to.row, to.col + i0 * 8, to.matrix);
     } else {
       __syncwarp();
-      copyOut(buffer, c, p.ldc, to.cols - i0 * 8, to.rows, lane, to.vector);
+      copyOut(buffer, lower, c, p.ldc, to.cols - i0 * 8, to.rows, lane, to.vector);
     }
-    if (p.c_tma && lane == 0) bulkCommit();
+    if (issues) bulkCommit();
     c += static_cast<long long>(kOutCols) * p.ldc;
   }
 }
@@ -960,6 +967,8 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
     const int quarter = warp % 4;
     const int col_begin = (warp - kEpilogueWarp0) / 4 * kHalf;
     const int etid = threadIdx.x - 32 * kEpilogueWarp0;
+    // Warps that hold neighbouring rows of the same columns share staging.
+    const int lower = quarter % 2, pair = (warp - kEpilogueWarp0) / 2;
     unsigned char *out = out_smem + (warp - kEpilogueWarp0) * G::kOutWarp;
     // Vectors of eight 16-bit rows: columns aligned to 16 bytes.
     const bool vector = reinterpret_cast<uintptr_t>(p.c) % 16 == 0 && p.ldc % 8 == 0 &&
@@ -1176,7 +1185,8 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
           G::kRagged == Ragged::kN ? 0 : static_cast<size_t>(t.group * p.stride_c);
       const int row0 = m0 + quarter * 32;
       const int col0 = t.n0 + col_begin, cols = t.cols - col_begin;
-      if (row0 < p.m && cols > 0) {
+      constexpr bool kShared = G::kPlanes == 1 && !G::kFp32;
+      if (row0 - (kShared ? lower * 32 : 0) < p.m && cols > 0) {
         if constexpr (G::kPlanes == 2) {
           uint32_t *words = reinterpret_cast<uint32_t *>(out);
           const bool mirror = G::kSymmetric && t.n0 + kBN <= t.m0;
@@ -1203,7 +1213,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
           to.clip = G::kRagged != Ragged::kN;
           to.vector = vector;
           if constexpr (G::kFp32) storeFp32<kHalf>(p, to, acc, out, lane);
-          else storeBf16<kBlocks>(p, to, acc, out, lane);
+          else storeBf16<kBlocks>(p, to, acc, out - lower * G::kOutWarp, pair, lower, lane);
         }
       }
     }
