@@ -235,28 +235,36 @@ sgblasStatus_t launchRows(const DeviceInfo &dev, const NarrowOperand &a, const N
   return launchProductKernel<G>(dev, p, tiles, stream);
 }
 
-// Tile width by the tokens a group has on average.
+// Width (columns of tokens) of the tiles of a product ragged along n: 16, 32
+// or 64 for the thin kernel, 128 for single CTAs, 256 for pairs.
+int chooseWidth(const DeviceInfo &dev, const t::Params &p, int elem_bytes) {
+  const long long mean = p.n / std::max(p.groups, 1);
+  return mean <= 3 ? 16 : mean <= 12 ? 32 : mean <= 40 ? 64 : mean <= 128 ? 128 : 256;
+}
+
 template <int kElemBytes, bool kAMN>
 sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
                              t::Params &p, cudaStream_t stream) {
   constexpr auto kN = t::Ragged::kN;
-  const long long mean = p.n / std::max(p.groups, 1);
   const bool plain = p.c_bf16 && p.beta == 0.0F;   // else rows of FP32 sums
-  if (mean <= 3) return launchThin<t::ThinCfg<kElemBytes, 16, kAMN>>(dev, a, b, p, stream);
-  if (mean <= 12) return launchThin<t::ThinCfg<kElemBytes, 32, kAMN>>(dev, a, b, p, stream);
-  if (mean <= 40) return launchThin<t::ThinCfg<kElemBytes, 64, kAMN>>(dev, a, b, p, stream);
-  if (mean <= 128) {
-    if (plain)
-      return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, false>>(dev, a, b, p,
-                                                                                 stream);
-    return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, true>>(dev, a, b, p, stream);
-  }
-  if constexpr (kElemBytes == 1) {
-    return launchRows(dev, a, b, p, stream);
-  } else {
-    if (plain)
-      return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, false>>(dev, a, b, p, stream);
-    return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, true>>(dev, a, b, p, stream);
+  switch (chooseWidth(dev, p, kElemBytes)) {
+    case 16: return launchThin<t::ThinCfg<kElemBytes, 16, kAMN>>(dev, a, b, p, stream);
+    case 32: return launchThin<t::ThinCfg<kElemBytes, 32, kAMN>>(dev, a, b, p, stream);
+    case 64: return launchThin<t::ThinCfg<kElemBytes, 64, kAMN>>(dev, a, b, p, stream);
+    case 128:
+      if (plain)
+        return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, false>>(dev, a, b, p,
+                                                                                   stream);
+      return launchTyped<t::Cfg<kElemBytes, kN, 128, kAMN, false, false, true>>(dev, a, b, p,
+                                                                                stream);
+    default:
+      if constexpr (kElemBytes == 1) {
+        return launchRows(dev, a, b, p, stream);
+      } else {
+        if (plain)
+          return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, false>>(dev, a, b, p, stream);
+        return launchTyped<t::Cfg<2, kN, 256, kAMN, false, true, true>>(dev, a, b, p, stream);
+      }
   }
 }
 
