@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 
 namespace sgblas::detail {
 
@@ -236,10 +237,40 @@ sgblasStatus_t launchRows(const DeviceInfo &dev, const NarrowOperand &a, const N
 }
 
 // Width (columns of tokens) of the tiles of a product ragged along n: 16, 32
-// or 64 for the thin kernel, 128 for single CTAs, 256 for pairs.
+// or 64 for the thin kernel, 128 for single CTAs, 256 for pairs. The host
+// knows the number of tokens, not how they fall to the groups: a group is
+// taken to end in half a tile.
+//
+// Thin tiles, whose k several CTAs may share, pay while a group has few tokens
+// (8 x 2048 x 2048 BF16, 2 tokens each: 13.3 us against 19.0 in 128 columns; 6:
+// 14.4 and 14.2), longer where 128-wide tiles would leave half the SMs idle over
+// a long k (2 x 4096 x 4096, 12 tokens: 16.3 and 18.1; 48: 18.7 and 19.0), and
+// longest where they would leave three quarters (4096 x 4096 e4m3, 48 tokens:
+// 10.0 and 13.1; 160: 22.6 and 15.3).
+//
+// Of the wide ones, pairs have the faster clock per product, single CTAs the
+// finer waves: a wave of 256-wide pair tiles takes about 1.35 times one of
+// 128-wide tiles (e4m3: 1.45) for four times the work of a worker (8 x 2048 x
+// 2048 BF16, 160 tokens each: pairs 18.9 us in one wave, singles 21.5 in two;
+// 2 x 1024 x 1024, 700 tokens: pairs 10.0 us, singles 7.4, both in one wave).
 int chooseWidth(const DeviceInfo &dev, const t::Params &p, int elem_bytes) {
-  const long long mean = p.n / std::max(p.groups, 1);
-  return mean <= 3 ? 16 : mean <= 12 ? 32 : mean <= 40 ? 64 : mean <= 128 ? 128 : 256;
+  const int active = std::min(p.groups, p.n);
+  const double mean = static_cast<double>(p.n) / std::max(p.groups, 1);
+  auto tiles = [&](int rows, int width) {
+    const double columns = p.groups == 1
+                               ? static_cast<double>((p.n - 1) / width + 1)
+                               : std::max<double>(active, static_cast<double>(p.n) / width + 0.5 * active);
+    return columns * ((p.m - 1) / rows + 1);
+  };
+  const int iters = (p.k * elem_bytes - 1) / t::kRowBytes + 1;   // slices of k
+  const double single = tiles(t::kBM, 128);
+  if (mean <= 6) return 16;
+  const bool thin = mean <= 8 || (mean <= 16 && 2 * single <= dev.sms && iters >= 32) ||
+                    (mean <= 64 && 4 * single <= dev.sms && iters >= 16);
+  if (thin) return mean <= 16 ? 32 : 64;
+  const double waves = std::ceil(single / dev.sms);
+  const double pair_waves = std::ceil(tiles(2 * t::kBM, 256) / (dev.sms / 2));
+  return pair_waves * (elem_bytes == 1 ? 1.45 : 1.35) < waves ? 256 : 128;
 }
 
 template <int kElemBytes, bool kAMN>
