@@ -162,8 +162,14 @@ def _ptr(x) -> int | None:
     return x.data_ptr()
 
 
+_SCALARS = {v: ctypes.byref(ctypes.c_float(v)) for v in (0.0, 1.0)}   # read, never written
+
+
 def _fp(v):
-    return None if v is None else ctypes.byref(ctypes.c_float(v))
+    if v is None:
+        return None
+    known = _SCALARS.get(v)
+    return ctypes.byref(ctypes.c_float(v)) if known is None else known
 
 
 class Handle:

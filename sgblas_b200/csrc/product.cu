@@ -31,28 +31,45 @@ sgblasStatus_t currentDevice(DeviceInfo *info) {
 
 namespace {
 
-// Copies rows of `dim0` elements to rows a multiple of 16 bytes apart, so
-// that TMA can read them; eight elements per thread, whose writes are whole
-// vectors. The elements beyond dim0 up to the padded row are not read by TMA.
-template <typename T>
-__global__ void __launch_bounds__(256) copyRowsKernel(const T *__restrict__ src, int dim0,
-                                                      long long rows_per_matrix, long long ld,
-                                                      long long stride, T *__restrict__ dst,
-                                                      long long ldp, long long rows) {
-  constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+// Copies rows of `bytes` bytes, at any address, to rows a multiple of 16 bytes
+// apart, so that TMA can read them: a warp per row, kCopyWords loads per lane
+// in flight, aligned words of the source, each joined with its neighbour's
+// first bytes. Bytes of the last word beyond the row are not read by TMA. Words
+// are read whole, so up to three bytes beside a row are, inside the row's first
+// and last aligned word. Memory-bound.
+constexpr int kCopyWords = 8;
+__global__ void __launch_bounds__(256) copyRowsKernel(const unsigned char *__restrict__ src,
+                                                      long long bytes, long long rows_per_matrix,
+                                                      long long ld, long long stride,
+                                                      unsigned char *__restrict__ dst, long long ldp,
+                                                      long long rows) {
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
-  const long long per_row = (dim0 + kVec - 1) / kVec;
-  const long long total = rows * per_row;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const long long row = i / per_row;
-    const int x = static_cast<int>(i - row * per_row) * kVec;
-    const long long matrix = row / rows_per_matrix;
-    const T *sp = src + matrix * stride + (row - matrix * rows_per_matrix) * ld + x;
-    alignas(16) T v[kVec];
+  const int lane = threadIdx.x % 32;
+  const int words = static_cast<int>((bytes + 3) / 4);
+  for (long long row = blockIdx.x * 8LL + threadIdx.x / 32; row < rows; row += gridDim.x * 8LL) {
+    const long long matrix = rows_per_matrix == rows ? 0 : row / rows_per_matrix;
+    const auto from = reinterpret_cast<uintptr_t>(src) +
+                      static_cast<uintptr_t>(matrix * stride + (row - matrix * rows_per_matrix) * ld);
+    const auto *aligned = reinterpret_cast<const uint32_t *>(from & ~uintptr_t{3});
+    const unsigned shift = static_cast<unsigned>(from & 3) * 8;
+    const int last = static_cast<int>((static_cast<long long>(from & 3) + bytes - 1) / 4);
+    auto *to = reinterpret_cast<uint32_t *>(dst + row * ldp);
+    for (int word0 = lane; word0 - lane < words; word0 += 32 * kCopyWords) {
+      uint32_t v[kCopyWords], edge = 0;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) v[j] = x + j < dim0 ? sp[j] : T{0};
-    *reinterpret_cast<uint4 *>(dst + row * ldp + x) = *reinterpret_cast<const uint4 *>(v);
+      for (int u = 0; u < kCopyWords; ++u)
+        v[u] = word0 + u * 32 <= last ? __ldg(aligned + word0 + u * 32) : 0;
+      // After the last lane's word comes the first lane's next one, and after
+      // its last word the one that follows this run.
+      if (lane == 0 && word0 + kCopyWords * 32 <= last) edge = __ldg(aligned + word0 + kCopyWords * 32);
+#pragma unroll
+      for (int u = 0; u < kCopyWords; ++u) {
+        const uint32_t mine = lane == 0 ? (u + 1 < kCopyWords ? v[u + 1 < kCopyWords ? u + 1 : u] : edge) : v[u];
+        const uint32_t next = __shfl_sync(0xffffffffu, mine, (lane + 1) % 32);
+        if (word0 + u * 32 < words) to[word0 + u * 32] = __funnelshift_r(v[u], next, shift);
+      }
+    }
   }
 }
 
@@ -75,9 +92,9 @@ sgblasStatus_t copyOperand(NarrowOperand *o, int elem_bytes, void *dst, int sms,
                            cudaStream_t stream) {
   const long long ldp = copyLd(*o, elem_bytes);
   const long long rows = static_cast<long long>(o->dim1) * o->count;
-  const long long vectors = rows * ((o->dim0 * elem_bytes + 15LL) / 16);
+  const long long bytes = static_cast<long long>(o->dim0) * elem_bytes;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>((vectors + 255) / 256, 8LL * sms)));
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>((rows + 7) / 8, 8LL * sms)));
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {};
@@ -85,15 +102,10 @@ sgblasStatus_t copyOperand(NarrowOperand *o, int elem_bytes, void *dst, int sms,
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e =
-      elem_bytes == 2
-          ? cudaLaunchKernelEx(&cfg, copyRowsKernel<uint16_t>,
-                               static_cast<const uint16_t *>(o->ptr), o->dim0,
-                               static_cast<long long>(o->dim1), o->ld, o->stride,
-                               static_cast<uint16_t *>(dst), ldp, rows)
-          : cudaLaunchKernelEx(&cfg, copyRowsKernel<uint8_t>, static_cast<const uint8_t *>(o->ptr),
-                               o->dim0, static_cast<long long>(o->dim1), o->ld, o->stride,
-                               static_cast<uint8_t *>(dst), ldp, rows);
+  const cudaError_t e = cudaLaunchKernelEx(
+      &cfg, copyRowsKernel, static_cast<const unsigned char *>(o->ptr), bytes,
+      static_cast<long long>(o->dim1), o->ld * elem_bytes, o->stride * elem_bytes,
+      static_cast<unsigned char *>(dst), ldp * elem_bytes, rows);
   o->ptr = dst;
   o->ld = ldp;
   o->stride = ldp * o->dim1;
