@@ -312,7 +312,7 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
     p.k = l;
     p.ldc = static_cast<int>(lds);
     p.stride_c = gram.stride;
-    p.pair.out = t::PairOut::kGram;
+    p.pair.out = t::PairOut::kSum;
     p.pair.hi = gram.hi;
     p.pair.lo = gram.lo;
     st = tall ? launchPairProduct<false, false, true>(dev, batch, x, x, p, stream)
@@ -344,7 +344,7 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
       p.stride_c = batch > 1 ? stride_o : 0;
       p.alpha = scale / (t::kPairScale * t::kPairScale);
     } else {
-      p.pair.out = t::PairOut::kUpdate;
+      p.pair.out = t::PairOut::kSum;
       p.pair.hi = next.hi;
       p.pair.lo = next.lo;
       p.ldc = static_cast<int>(ldx);

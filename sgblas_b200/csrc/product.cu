@@ -254,8 +254,8 @@ sgblasStatus_t launchRows(const DeviceInfo &dev, const NarrowOperand &a, const N
 // taken to end in half a tile.
 //
 // Thin tiles, whose k several CTAs may share, pay while a group has few tokens
-// (8 x 2048 x 2048 BF16, 2 tokens each: 13.3 us against 19.0 in 128 columns; 6:
-// 14.4 and 14.2), longer where 128-wide tiles would leave half the SMs idle over
+// (8 x 2048 x 2048 BF16, 2 tokens each: 13.3 us against 19.0 in 128 columns; 12:
+// 14.8 and 14.4; 32 x 2048 x 2048 e4m3, 12: 28.4 and 29.5), longer where 128-wide tiles would leave half the SMs idle over
 // a long k (2 x 4096 x 4096, 12 tokens: 16.3 and 18.1; 48: 18.7 and 19.0), and
 // longest where they would leave three quarters (4096 x 4096 e4m3, 48 tokens:
 // 10.0 and 13.1; 160: 22.6 and 15.3).
@@ -277,7 +277,7 @@ int chooseWidth(const DeviceInfo &dev, const t::Params &p, int elem_bytes) {
   const int iters = (p.k * elem_bytes - 1) / t::kRowBytes + 1;   // slices of k
   const double single = tiles(t::kBM, 128);
   if (mean <= 6) return 16;
-  const bool thin = mean <= 8 || (mean <= 16 && 2 * single <= dev.sms && iters >= 32) ||
+  const bool thin = mean <= 12 || (mean <= 16 && 2 * single <= dev.sms && iters >= 32) ||
                     (mean <= 64 && 4 * single <= dev.sms && iters >= 16);
   if (thin) return mean <= 16 ? 32 : 64;
   const double waves = std::ceil(single / dev.sms);

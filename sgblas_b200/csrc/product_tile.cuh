@@ -105,7 +105,7 @@ struct Cfg {
   static constexpr int kBarrierBytes = 8 * (3 * kStages + 2 * kAccums);
   static constexpr int kSmemBytes =
       kStages * kStageBytes + kScaleBytes + kOutBytes + kBarrierBytes + 1024;
-  static_assert(kBN == 32 || kBN == 64 || kBN == 128 || kBN == 256, "tile width");
+  static_assert(kBN == 64 || kBN == 128 || kBN == 256, "tile width");
   static_assert(!kSymmetric || kTileM % kBN == 0, "tiles end at the diagonal");
   static_assert(!kBytes || (!kAMN && !kBMN), "8-bit operands are K-major");
   static_assert(!kRows || (kBytes && kBN == 256), "rows of tokens: e4m3, two blocks of weights");
@@ -116,13 +116,12 @@ struct Cfg {
 };
 
 // What the epilogue of a pair product writes (values v of the sum):
-//   kGram    hi + lo of v * 2^-12
+//   kSum     hi + lo of v * 2^-12
 //   kPoly    hi + lo of c2 v 2^-12 + c1 A + c0 2^12 I, A the pair at prev
-//   kUpdate  hi + lo of v * 2^-12
 //   kFinal   bf16 of v * alpha
 // Pairs hold 2^12 times their value: fp16 then keeps 22 bits of every value
 // above 2^-16 and an absolute 2^-37 below, and reaches 15.99.
-enum class PairOut { kGram, kPoly, kUpdate, kFinal };
+enum class PairOut { kSum, kPoly, kFinal };
 constexpr float kPairScale = 4096.0F;
 
 struct PairParams {
@@ -328,6 +327,92 @@ __device__ __forceinline__ void splitPair(float v, __half *hi, __half *lo) {
   *lo = __float2half_rn(v - __half2float(*hi));
 }
 
+// ---- a chunk's sums from TMEM, added to the registers -----------------------
+// In each the next load is in flight while one is added. Columns past the
+// tile's width hold what an earlier tile left; they are not written.
+
+// acc[j] += row of kCols columns, a row per lane, times one scale.
+template <int kCols>
+__device__ __forceinline__ void addScaledRow(uint32_t taddr, float2 (&acc)[kCols / 2], float2 scale) {
+  uint32_t v[2][16];
+  tmemLoadAsync16(taddr, v[0]);
+#pragma unroll
+  for (int c = 0; c < kCols; c += 16) {
+    uint32_t(&now)[16] = v[c / 16 % 2];
+    tmemWait16(now);
+    if (c + 16 < kCols) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      float2 &a = acc[(c + j) / 2];
+      a = __ffma2_rn(make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1])), scale, a);
+    }
+  }
+}
+
+// The same, each column times its own scale (kScaled) or none.
+template <int kCols, bool kScaled>
+__device__ __forceinline__ void addRows(uint32_t taddr, float2 (&acc)[kCols / 2],
+                                        const float *scales, float weight) {
+  uint32_t v[2][16];
+  tmemLoadAsync16(taddr, v[0]);
+#pragma unroll
+  for (int c = 0; c < kCols; c += 16) {
+    uint32_t(&now)[16] = v[c / 16 % 2];
+    tmemWait16(now);
+    if (c + 16 < kCols) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float2 x = make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1]));
+      float2 &a = acc[(c + j) / 2];
+      if constexpr (kScaled) {
+        const float2 s = *reinterpret_cast<const float2 *>(scales + c + j);
+        a = __ffma2_rn(x, make_float2(s.x * weight, s.y * weight), a);
+      } else {
+        a = __fadd2_rn(a, x);
+      }
+    }
+  }
+}
+
+// The same into fragments: acc[4 * i + r] holds columns 8 i + 2 (t % 4) + {0, 1}
+// of row 8 r + t / 4 for lane t.
+template <int kCols, bool kScaled>
+__device__ __forceinline__ void addFragments(uint32_t taddr, float2 (&acc)[kCols / 2],
+                                             const float *scales, float weight, int lane) {
+  constexpr uint32_t kLower = 16u << 16;   // the quarter's lanes 16-31
+  uint32_t v[2][32];                       // rows 0-15 of 32 columns, then rows 16-31
+  tmemFragments(taddr, v[0], 0);
+  tmemFragments(taddr + kLower, v[0], 16);
+#pragma unroll
+  for (int c = 0; c < kCols; c += 32) {
+    uint32_t(&now)[32] = v[c / 32 % 2];
+    uint32_t(&next)[32] = v[(c / 32 + 1) % 2];
+    tmemWait32(now);
+    if (c + 32 < kCols) {
+      tmemFragments(taddr + c + 32, next, 0);
+      tmemFragments(taddr + kLower + c + 32, next, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 scale = make_float2(0.0F, 0.0F);
+      if constexpr (kScaled) {
+        const float2 s = *reinterpret_cast<const float2 *>(scales + c + i * 8 + lane % 4 * 2);
+        scale = make_float2(s.x * weight, s.y * weight);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = r / 2 * 16 + i * 4 + r % 2 * 2;
+        const float2 x = make_float2(__uint_as_float(now[at]), __uint_as_float(now[at + 1]));
+        float2 &a = acc[(c / 8 + i) * 4 + r];
+        if constexpr (kScaled) a = __ffma2_rn(x, scale, a);
+        else a = __fadd2_rn(a, x);
+      }
+    }
+  }
+}
+
+// ---- from registers to C -----------------------------------------------------
+
 // Where a warp's share of a tile goes: its first element in C, that element's
 // row, column and matrix, and how many rows and columns of it exist. Columns
 // past the tile's last are another group's (kN) unless `clip` says that C ends
@@ -338,11 +423,7 @@ struct Place {
   bool clip, vector;
 };
 
-// A warp's share in registers is 32 rows by 8 * kBlocks columns, as
-// tmemFragments gives them: acc[4 * i + r] holds columns 8 i + 2 (t % 4) + {0, 1}
-// of row 8 r + t / 4.
-//
-// 16-bit results pass through shared memory, 16 columns at a time in two
+// 16-bit results (fragments) pass through shared memory, 16 columns at a time in two
 // buffers that two warps share: stmatrix transposes each 8 x 8 block, so that a
 // column's 64 rows (128 bytes) lie together. TMA takes them from there while
 // the next columns are staged (a group's last columns, and a C that TMA cannot
@@ -963,7 +1044,6 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
     regAlloc<216>();
     constexpr int kHalf = kBN / 2;                     // columns of this warp
     constexpr int kBlocks = kHalf / 8;
-    constexpr int kLoad = kHalf < 32 ? kHalf : 32;     // columns of one TMEM load
     const int quarter = warp % 4;
     const int col_begin = (warp - kEpilogueWarp0) / 4 * kHalf;
     const int etid = threadIdx.x - 32 * kEpilogueWarp0;
@@ -1060,20 +1140,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
             tcgenFenceAfter();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                                    static_cast<uint32_t>(b * kBN + col_begin);
-            uint32_t v[2][16];
-            tmemLoadAsync16(taddr, v[0]);
-#pragma unroll
-            for (int c = 0; c < kHalf; c += 16) {
-              uint32_t(&now)[16] = v[c / 16 % 2];
-              tmemWait16(now);
-              if (c + 16 < kHalf) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
-#pragma unroll
-              for (int j = 0; j < 16; j += 2) {
-                float2 &a = acc[(c + j) / 2];
-                a = __ffma2_rn(make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1])), s,
-                               a);
-              }
-            }
+            addScaledRow<kHalf>(taddr, acc, s);
             tcgenFenceBefore();
             __syncwarp();
             if (lane == 0) mbarArriveClusterRelaxed(acc_empty_even + b * 8);
@@ -1103,75 +1170,13 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
         tcgenFenceAfter();
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                                static_cast<uint32_t>(b * kBN + col_begin);
-        if constexpr (G::kFp32) {
-          uint32_t v[2][16];
-          tmemLoadAsync16(taddr, v[0]);
-#pragma unroll
-          for (int c = 0; c < kHalf; c += 16) {
-            uint32_t(&now)[16] = v[c / 16 % 2];
-            tmemWait16(now);
-            if (c + 16 < kHalf) tmemLoadAsync16(taddr + c + 16, v[(c / 16 + 1) % 2]);
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              const float2 x = make_float2(__uint_as_float(now[j]), __uint_as_float(now[j + 1]));
-              float2 &a = acc[(c + j) / 2];
-              if constexpr (G::kBytes) {
-                float2 scale = *reinterpret_cast<const float2 *>(sc + col_begin + c + j);
-                scale.x *= sc[kBN];
-                scale.y *= sc[kBN];
-                a = __ffma2_rn(x, scale, a);
-              } else {
-                a = __fadd2_rn(a, x);
-              }
-            }
-          }
-        } else {
-        // v: rows 0-15 of kLoad columns from c, then rows 16-31.
-        auto accumulate = [&](int c, const uint32_t (&v)[kLoad]) {
-#pragma unroll
-          for (int i = 0; i < kLoad / 8; ++i) {
-            float2 scale = make_float2(0.0F, 0.0F);
-            if constexpr (G::kBytes) {
-              scale = *reinterpret_cast<const float2 *>(sc + col_begin + c + i * 8 + lane % 4 * 2);
-              scale.x *= sc[kBN];
-              scale.y *= sc[kBN];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int at = r / 2 * (kLoad / 2) + i * 4 + r % 2 * 2;
-              const float2 x = make_float2(__uint_as_float(v[at]), __uint_as_float(v[at + 1]));
-              float2 &a = acc[(c / 8 + i) * 4 + r];
-              if constexpr (G::kBytes) a = __ffma2_rn(x, scale, a);
-              else a = __fadd2_rn(a, x);
-            }
-          }
-        };
-        // The next load is in flight while one is added. Columns past the
-        // tile's width hold what an earlier tile left; they are not written.
-        constexpr uint32_t kLower = 16u << 16;   // the quarter's lanes 16-31
-        if constexpr (kLoad == 16) {
-          uint32_t v[16];
-          tmemFragments<16>(taddr, v, 0);
-          tmemFragments<16>(taddr + kLower, v, 8);
-          tmemWait16(v);
-          accumulate(0, v);
-        } else {
-          uint32_t v[2][32];
-          tmemFragments<32>(taddr, v[0], 0);
-          tmemFragments<32>(taddr + kLower, v[0], 16);
-#pragma unroll
-          for (int c = 0; c < kHalf; c += 32) {
-            uint32_t(&now)[32] = v[c / 32 % 2];
-            uint32_t(&next)[32] = v[(c / 32 + 1) % 2];
-            tmemWait32(now);
-            if (c + 32 < kHalf) {
-              tmemFragments<32>(taddr + c + 32, next, 0);
-              tmemFragments<32>(taddr + kLower + c + 32, next, 16);
-            }
-            accumulate(c, now);
-          }
+        float weight = 0.0F;
+        if constexpr (G::kStaged) {
+          weight = sc[kBN];
+          sc += col_begin;
         }
-        }
+        if constexpr (G::kFp32) addRows<kHalf, G::kStaged>(taddr, acc, sc, weight);
+        else addFragments<kHalf, G::kStaged>(taddr, acc, sc, weight, lane);
         tcgenFenceBefore();
         __syncwarp();
         if (lane == 0) {

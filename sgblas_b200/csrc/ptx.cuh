@@ -350,32 +350,22 @@ __device__ __forceinline__ void tmemLoad16(uint32_t taddr, uint32_t (&v)[16]) {
   tmemWait16(v);
 }
 
-// Sixteen TMEM lanes (from the one in taddr) by 16 or 32 consecutive
-// columns as fragments: for the 8 columns from 8 i, lane t of the warp gets
-// columns 8 i + 2 (t % 4) + {0, 1} of row t / 4 in v[at + 4 i + {0, 1}] and of
-// row t / 4 + 8 in v[at + 4 i + {2, 3}]. Usable after tmemWait.
-template <int kColumns, int kRegs>
-__device__ __forceinline__ void tmemFragments(uint32_t taddr, uint32_t (&v)[kRegs], int at) {
-  static_assert(kColumns == 16 || kColumns == 32, "fragment width");
-  if constexpr (kColumns == 16) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-        : "=r"(v[at + 0]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]),
-          "=r"(v[at + 5]), "=r"(v[at + 6]), "=r"(v[at + 7])
-        : "r"(taddr)
-        : "memory");
-  } else {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[at + 0]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]),
-          "=r"(v[at + 5]), "=r"(v[at + 6]), "=r"(v[at + 7]), "=r"(v[at + 8]), "=r"(v[at + 9]),
-          "=r"(v[at + 10]), "=r"(v[at + 11]), "=r"(v[at + 12]), "=r"(v[at + 13]), "=r"(v[at + 14]),
-          "=r"(v[at + 15])
-        : "r"(taddr)
-        : "memory");
-  }
+// Sixteen TMEM lanes (from the one in taddr) by 32 consecutive columns as
+// fragments: for the 8 columns from 8 i, lane t of the warp gets columns 8 i +
+// 2 (t % 4) + {0, 1} of row t / 4 in v[at + 4 i + {0, 1}] and of row t / 4 + 8 in
+// v[at + 4 i + {2, 3}]. Usable after tmemWait32.
+__device__ __forceinline__ void tmemFragments(uint32_t taddr, uint32_t (&v)[32], int at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[at + 0]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]),
+        "=r"(v[at + 5]), "=r"(v[at + 6]), "=r"(v[at + 7]), "=r"(v[at + 8]), "=r"(v[at + 9]),
+        "=r"(v[at + 10]), "=r"(v[at + 11]), "=r"(v[at + 12]), "=r"(v[at + 13]), "=r"(v[at + 14]),
+        "=r"(v[at + 15])
+      : "r"(taddr)
+      : "memory");
 }
+
 // Four 8 x 8 matrices of 16-bit values to shared memory, transposed: lane t
 // holds elements (t / 4, 2 (t % 4) + {0, 1}) of each; lane 8 i + j gives the
 // address (16 bytes) where column j of matrix i goes.
