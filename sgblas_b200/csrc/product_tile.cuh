@@ -864,7 +864,12 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
     if (p.k > 0) {
       prefetchTensorMap(&p.tma_a);
       prefetchTensorMap(&p.tma_b);
+      if constexpr (G::kPlanes == 2) {
+        prefetchTensorMap(&p.pair.tma_a_lo);
+        prefetchTensorMap(&p.pair.tma_b_lo);
+      }
     }
+    if (p.c_tma) prefetchTensorMap(&p.tma_c);
     for (int s = 0; s < kStages; ++s) {
       mbarInit(&full[s], 1);
       mbarInit(&empty[s], 1);
