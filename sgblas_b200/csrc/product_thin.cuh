@@ -5,11 +5,18 @@
 // C(:, group) is cut into 128-row by kBN-column tiles as in product_tile.cuh;
 // a tile is computed by a cluster of `split` CTAs, each over its share of the
 // k slices. The partial tiles meet in distributed shared memory: each CTA
-// receives 128 / split rows from the others, adds them in rank order and
-// writes them, so
-// there is no workspace, no atomic, and no order that varies. Splitting k
-// gives SMs to a call with few tiles, and evens out the last wave of one
-// with many.
+// receives 128 / split rows from the others (asynchronous stores counted on a
+// barrier: no release has to wait for them), adds them in rank order and
+// writes them. There is no workspace, no atomic, and no order that varies.
+// Splitting k gives SMs to a call with few tiles, and evens out the last wave
+// of one with many.
+//
+// Memory-bound where the weights come from HBM: 32 experts of 2048 x 4096
+// BF16 (537 MB), 192 tokens, 80 to 84 us, 6.4 to 6.7 TB/s; of 2048 x 2048 e4m3
+// (134 MB), 384 tokens, 28 us, 4.8 TB/s (3.5 waves of tiles in four). The
+// smallest calls are a chain of latencies (8 tokens, 8 experts of 1024 x 1024:
+// 5.5 us, of which the offsets 0.6, the first slice 1.0, the stream 2.2, the
+// hand-over and C 1.5).
 //
 // Warp roles (8 warps): warp 0 TMA producer, warp 1 MMA issuer, warp 2 TMEM,
 // warps 4-7 epilogue (a row of the tile per thread). Chunks of k and e4m3
