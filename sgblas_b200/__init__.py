@@ -155,11 +155,12 @@ def _check(where: str, status: int) -> None:
 
 def _ptr(x) -> int | None:
     """Device pointer of a torch tensor, or an integer address, or None."""
-    if x is None:
-        return None
-    if isinstance(x, int):
-        return x
-    return x.data_ptr()
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        if x is None or isinstance(x, int):
+            return x
+        raise
 
 
 _SCALARS = {v: ctypes.byref(ctypes.c_float(v)) for v in (0.0, 1.0)}   # read, never written
@@ -262,7 +263,9 @@ class Handle:
                                       ctype, ldc)
 
     def grouped_gemm_n(self, *args) -> None:
-        _check("sgblasGroupedGemmN", self.grouped_gemm_n_status(*args))
+        status = self.grouped_gemm_n_status(*args)
+        if status:
+            raise SgblasError("sgblasGroupedGemmN", status)
 
     def grouped_gemm_k_status(self, m, n, k, groups, offsets, alpha, a, lda, b, ldb, beta, c, ctype,
                               ldc, stride_c) -> int:
@@ -271,7 +274,9 @@ class Handle:
                                       lda, _ptr(b), ldb, _fp(beta), _ptr(c), ctype, ldc, stride_c)
 
     def grouped_gemm_k(self, *args) -> None:
-        _check("sgblasGroupedGemmK", self.grouped_gemm_k_status(*args))
+        status = self.grouped_gemm_k_status(*args)
+        if status:
+            raise SgblasError("sgblasGroupedGemmK", status)
 
     def quantize_fp8_status(self, k, n, block_n, x, xtype, ldx, q, ldq, scale, ldscale, batch=1,
                             stride_x=0, stride_q=0, stride_scale=0) -> int:
@@ -289,7 +294,9 @@ class Handle:
                                  _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
 
     def gemm_fp8(self, *args) -> None:
-        _check("sgblasGemmFp8", self.gemm_fp8_status(*args))
+        status = self.gemm_fp8_status(*args)
+        if status:
+            raise SgblasError("sgblasGemmFp8", status)
 
     def grouped_gemm_fp8_status(self, m, n, k, groups, offsets, a, lda, stride_a, scale_a, ldsa,
                                 stride_sa, b, ldb, scale_b, ldsb, c, ctype, ldc) -> int:
@@ -299,7 +306,9 @@ class Handle:
                                         _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
 
     def grouped_gemm_fp8(self, *args) -> None:
-        _check("sgblasGroupedGemmFp8", self.grouped_gemm_fp8_status(*args))
+        status = self.grouped_gemm_fp8_status(*args)
+        if status:
+            raise SgblasError("sgblasGroupedGemmFp8", status)
 
     def orthogonalize_status(self, m, n, batch, steps, coefficients, eps, scale, g, gtype, ldg,
                              stride_g, o, ldo, stride_o) -> int:
