@@ -12,12 +12,14 @@
 // last product's operands alone rounded to 11 bits, 2e-4 to 8e-4, under BF16's
 // own 1.7e-3.)
 //
-// Measured: 4096 x 2048 FP32, five steps, 760 to 800 us, where the three-fold
-// products take 420 us of the tensor core's time at its full clock (the pipe is
-// busy 48 to 64 % of a product's cycles: one or two tiles per worker leave the
-// first loads and the last stores uncovered). 8 x 256 x 512 BF16, 107 to 116 us:
-// 17 launches, each a chain of latencies (the first slice 1.4 us, the stream 2 to
-// 4, the stores 1).
+// Where it pays, two steps share a Gram product and an update (pairsSteps).
+//
+// Measured: 4096 x 2048 FP32, five steps, 690 us (790 with every step apart),
+// where the three-fold products take 345 us of the tensor core's time at its full
+// clock (the pipe is busy 48 to 64 % of a product's cycles: one or two tiles per
+// worker leave the first loads and the last stores uncovered). 8 x 256 x 512 BF16,
+// 107 to 116 us: 17 launches, each a chain of latencies (the first slice 1.4 us,
+// the stream 2 to 4, the stores 1).
 //
 // X stays in G's orientation. m >= n: A = X^T X (both operands contiguous
 // along k), X P (X contiguous along m). m < n: A = X X^T (both contiguous along
@@ -33,6 +35,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <utility>
 
 namespace sgblas::detail {
@@ -237,6 +240,37 @@ sgblasStatus_t launchNorm(NormParams q, int batch, cudaStream_t stream) {
                                  kNormThreads, 0, stream, args));
 }
 
+// Whether two steps share one Gram matrix and one update of X:
+//
+//   A, P = P(A), A' = P A P, P' = P(A'), X <- X (P P')
+//
+// All are polynomials of A, so symmetric and at half their tiles: five
+// s x s products for one more Gram product and update of X, 3 l s^2 + 5 s^3
+// multiplications for 6 l s^2 + 2 s^3.
+//
+// An error d in A is one of P P' too, through its derivative (212 at a zero
+// singular value for the usual coefficients): 2^-22 of the largest entry stays
+// below 6e-5 there. Over all five steps that derivative is 1.5e7: hence two at a
+// time. The product has to fit the pairs' range (15.99), as c0^2 = 11.9 does.
+//
+// It has one launch more (7 for 6, about 7 us), which long sums (the Gram
+// product's tiles are few and 7 ns deep per row) or much saved work must repay.
+// FP32 or BF16, five steps, apart and paired: 4096 x 2048 792 and 690 us,
+// 4 x 1024 x 4096 963 and 768, 1024 x 2560 286 and 262, 400 x 4000 243 and 209,
+// 128 x 2048 (2) 131 and 114, 64 x 1024 89 and 82; at the rule's edges 512 x 2048
+// 169 and 170, 1536 x 2304 384 and 383; kept apart: 2048 x 2048 492 and 513,
+// 1024 x 1152 182 and 203, 8 x 256 x 512 107 and 118, 128 x 512 77 and 79.
+bool pairsSteps(int l, int s, int batch, const float *c) {
+  const double saved = 9.0 * batch * (l - s) * s * s;   // operations, three products each
+  if (!(l >= 768 && l / 4 >= s) && saved < 1.2e10) return false;
+  for (int i = 0; i <= 48; ++i) {   // squared singular values of 0 to 1.5
+    const float a = static_cast<float>(i) / 32.0F, p = c[0] + a * (c[1] + a * c[2]),
+                b = a * p * p;
+    if (!(std::fabs(p * (c[0] + b * (c[1] + b * c[2]))) < 15.0F)) return false;
+  }
+  return true;
+}
+
 constexpr size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace
@@ -272,7 +306,9 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
   const size_t sum_bytes = align256(static_cast<size_t>(batch) * partials * sizeof(float));
   const size_t x_bytes = static_cast<size_t>(ldx) * n * batch * sizeof(__half);   // 128-byte units
   const size_t s_bytes = static_cast<size_t>(lds) * s * batch * sizeof(__half);
-  if (!ensureWorkspace(handle, kCounterRegionBytes + sum_bytes + 4 * x_bytes + 4 * s_bytes,
+  const bool paired = steps > 2 && pairsSteps(l, s, batch, coefficients);
+  const size_t s_matrices = paired ? 6 : 4;
+  if (!ensureWorkspace(handle, kCounterRegionBytes + sum_bytes + 4 * x_bytes + s_matrices * s_bytes,
                        dev.device, stream))
     return SGBLAS_STATUS_NOT_SUPPORTED;
   auto *base = static_cast<unsigned char *>(handle->workspace) + kCounterRegionBytes;
@@ -291,6 +327,7 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
   };
   PairMatrix x = take(m, n, ldx, x_bytes), next = take(m, n, ldx, x_bytes);
   PairMatrix gram = take(s, s, lds, s_bytes), poly = take(s, s, lds, s_bytes);
+  const PairMatrix other = paired ? take(s, s, lds, s_bytes) : PairMatrix{};
 
   NormParams q = {};
   q.g = g;
@@ -314,6 +351,27 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
   else
     st = vector ? launchNorm<float, true>(q, batch, stream)
                 : launchNorm<float, false>(q, batch, stream);
+  // A symmetric s x s product of matrices that commute, if all went well so far.
+  auto square = [&](const PairMatrix &a, const PairMatrix &b, const PairMatrix &out,
+                    t::PairOut what) {
+    if (st != SGBLAS_STATUS_SUCCESS) return;
+    t::Params p = {};
+    p.pair.planes = 2;
+    p.m = p.n = p.k = s;
+    p.ldc = static_cast<int>(lds);
+    p.stride_c = out.stride;
+    p.pair.out = what;
+    p.pair.hi = out.hi;
+    p.pair.lo = out.lo;
+    if (what == t::PairOut::kPoly) {
+      p.pair.prev_hi = a.hi;
+      p.pair.prev_lo = a.lo;
+      p.pair.c0 = coefficients[0];
+      p.pair.c1 = coefficients[1];
+      p.pair.c2 = coefficients[2];
+    }
+    st = launchPairProduct<false, false, true>(dev, batch, a, b, p, stream);
+  };
   for (int step = 0; step < steps && st == SGBLAS_STATUS_SUCCESS; ++step) {
     t::Params p = {};
     p.pair.planes = 2;
@@ -327,22 +385,21 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
     p.pair.lo = gram.lo;
     st = tall ? launchPairProduct<false, false, true>(dev, batch, x, x, p, stream)
               : launchPairProduct<true, true, true>(dev, batch, x, x, p, stream);
-    if (st != SGBLAS_STATUS_SUCCESS) break;
-    // P = c0 I + c1 A + c2 A A.
-    p.k = s;
-    p.pair.out = t::PairOut::kPoly;
-    p.pair.hi = poly.hi;
-    p.pair.lo = poly.lo;
-    p.pair.prev_hi = gram.hi;
-    p.pair.prev_lo = gram.lo;
-    p.pair.c0 = coefficients[0];
-    p.pair.c1 = coefficients[1];
-    p.pair.c2 = coefficients[2];
-    st = launchPairProduct<false, false, true>(dev, batch, gram, gram, p, stream);
-    if (st != SGBLAS_STATUS_SUCCESS) break;
+    square(gram, gram, poly, t::PairOut::kPoly);
+    PairMatrix by = poly;
+    if (paired && step + 2 < steps) {
+      // The next step's A = P A P and P, and the two polynomials' product.
+      square(poly, gram, other, t::PairOut::kSum);
+      square(other, poly, gram, t::PairOut::kSum);
+      square(gram, gram, other, t::PairOut::kPoly);
+      square(poly, other, gram, t::PairOut::kSum);
+      by = gram;
+      ++step;
+    }
     // X P or P X; the last one is the result.
     p.m = m;
     p.n = n;
+    p.k = s;
     if (step == steps - 1) {
       // Rounded to BF16 at once: the hi parts' 11 bits add a tenth to that
       // rounding's error, and take a third of the instructions.
@@ -354,14 +411,14 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
       p.stride_c = batch > 1 ? stride_o : 0;
       p.alpha = scale / (t::kPairScale * t::kPairScale);
     } else {
-      p.pair.out = t::PairOut::kSum;
       p.pair.hi = next.hi;
       p.pair.lo = next.lo;
       p.ldc = static_cast<int>(ldx);
       p.stride_c = next.stride;
     }
-    st = tall ? launchPairProduct<true, false, false>(dev, batch, x, poly, p, stream)
-              : launchPairProduct<false, false, false>(dev, batch, poly, x, p, stream);
+    if (st != SGBLAS_STATUS_SUCCESS) break;
+    st = tall ? launchPairProduct<true, false, false>(dev, batch, x, by, p, stream)
+              : launchPairProduct<false, false, false>(dev, batch, by, x, p, stream);
     std::swap(x, next);
   }
   if (!markWorkspaceUse(handle, stream) && st == SGBLAS_STATUS_SUCCESS)

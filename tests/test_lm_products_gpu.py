@@ -416,6 +416,54 @@ def test_orthogonalize(cuda, handle, rows, cols, batch, type_, steps, scale, pad
         assert rel <= 2.0 ** -9 + 2.0 ** -10, (i, rel)
 
 
+@pytest.mark.parametrize("spectrum", ["equal", "decay", "one strong"])
+@pytest.mark.parametrize("diagonal", [False, True])
+@pytest.mark.parametrize("rows,cols,steps", [(64, 1024, 5), (1030, 129, 6), (1000, 200, 4),
+                                             (1024, 2560, 5), (64, 96, 5)])
+def test_orthogonalize_spectra(cuda, handle, rows, cols, steps, diagonal, spectrum):
+    """Long matrices take two steps per Gram product; (64, 96) and the last steps
+    do not. The bound: BF16's rounding, half a unit of 2^-8 at most and 2^-8 /
+    sqrt(3) over a binade in the mean (1.4 times the test above for entries at a
+    binade's low end, as a diagonal's few may be), and the last product's
+    operands as there: 2^-8 holds them, and a lost digit of the small singular
+    values does not fit in it."""
+    torch = cuda
+    gen = generator(torch, rows + cols)
+    k = min(rows, cols)
+    kinds = {"equal": torch.ones(k), "decay": torch.logspace(0, -4, k),
+             "one strong": torch.cat([torch.ones(1), torch.full((k - 1,), 1e-3)])}
+    values = kinds[spectrum].to("cuda", torch.float64)
+    if diagonal:
+        g = torch.zeros(rows, cols, device="cuda", dtype=torch.float64)
+        g[range(k), range(k)] = values
+    else:
+        u, v = (torch.linalg.qr(torch.randn(d, k, generator=gen, device="cuda",
+                                            dtype=torch.float64))[0] for d in (rows, cols))
+        g = (u * values) @ v.T
+    g = g.float().contiguous()
+    o = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    handle.orthogonalize(cols, rows, 1, steps, ABC, 1e-7, 1.0, g, FP32, cols, 0, o, cols, 0)
+    want = newton_schulz(g, steps, ABC, 1e-7, 1.0)
+    assert sg.get_device_errors() == 0
+    assert ((o.double() - want).norm() / want.norm()).item() <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("abc", [(1.5, -0.5, 0.0), (4.0, -7.0, 3.3), (-2.0, 1.5, 0.0)])
+def test_orthogonalize_coefficients(cuda, handle, abc):
+    """4 * 4 is outside the pairs' range, so those steps go one by one. The
+    bound: BF16's 2^-8, and 2^-11 of each operand of the last product by norms."""
+    torch = cuda
+    g = torch.randn(100, 1500, generator=generator(torch, 9), device="cuda")
+    o = torch.empty(100, 1500, device="cuda", dtype=torch.bfloat16)
+    handle.orthogonalize(1500, 100, 1, 3, abc, 0.0, 1.0, g, FP32, 1500, 0, o, 1500, 0)
+    want, x = (newton_schulz(g, k, abc, 0.0, 1.0) for k in (3, 2))
+    a = x @ x.T
+    p = abc[0] * torch.eye(100, device="cuda", dtype=torch.float64) + abc[1] * a + abc[2] * a @ a
+    operands = p.norm() * torch.linalg.matrix_norm(x, 2) + torch.linalg.matrix_norm(p, 2) * x.norm()
+    assert sg.get_device_errors() == 0
+    assert (o.double() - want).norm() <= 2.0 ** -8 * want.norm() + 2.0 ** -11 * operands
+
+
 def test_orthogonalize_zero_and_nan(cuda, handle):
     torch = cuda
     g = torch.zeros(2, 100, 70, device="cuda")
