@@ -18,7 +18,7 @@
 // where the three-fold products take 345 us of the tensor core's time at its full
 // clock (the pipe is busy 48 to 64 % of a product's cycles: one or two tiles per
 // worker leave the first loads and the last stores uncovered). 8 x 256 x 512 BF16,
-// 107 to 116 us: 17 launches, each a chain of latencies (the first slice 1.4 us,
+// 93 us: 17 launches, each a chain of latencies (the first slice 1.4 us,
 // the stream 2 to 4, the stores 1).
 //
 // X stays in G's orientation. m >= n: A = X^T X (both operands contiguous
@@ -210,7 +210,12 @@ sgblasStatus_t launchPairTyped(const DeviceInfo &dev, int batch, const PairMatri
 
 // The widest tiles of which there are enough for about every worker: pairs of
 // CTAs on 256 rows (a symmetric product's are 128 wide: 2048 x 2048 has 72 of
-// them for 74 pairs, and 36 square ones), else single CTAs on 128.
+// them for 74 pairs, and 36 square ones), else single CTAs on 128. Where even
+// those of 32 columns are one wave at most, they are taken for their shorter
+// epilogues (an instruction takes 41 clocks, one of 64 columns 48): 64 and 32
+// columns, five steps: 8 x 256 x 512 107 and 93 us, 1024 x 1024 177 and 156,
+// 64 x 64 54 and 45; past one wave, 16 x 200 x 300 112 and 121. (B contiguous
+// along n comes in boxes of 64.)
 template <bool kAMN, bool kBMN, bool kSymmetric>
 sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMatrix &a,
                                  const PairMatrix &b, const t::Params &product,
@@ -225,6 +230,11 @@ sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMat
     return launchPairTyped<Two>(dev, batch, a, b, p, stream);
   if (2 * batch * pairTiles<One>(p.m, p.n) >= dev.sms)
     return launchPairTyped<One>(dev, batch, a, b, p, stream);
+  if constexpr (!kBMN) {
+    using Quarter = t::Cfg<2, kB, 32, kAMN, kBMN, false, true, 2, kSymmetric>;
+    if (batch * pairTiles<Quarter>(p.m, p.n) <= dev.sms)
+      return launchPairTyped<Quarter>(dev, batch, a, b, p, stream);
+  }
   return launchPairTyped<Half>(dev, batch, a, b, p, stream);
 }
 
@@ -259,7 +269,8 @@ sgblasStatus_t launchNorm(NormParams q, int batch, cudaStream_t stream) {
 // 4 x 1024 x 4096 963 and 768, 1024 x 2560 286 and 262, 400 x 4000 243 and 209,
 // 128 x 2048 (2) 131 and 114, 64 x 1024 89 and 82; at the rule's edges 512 x 2048
 // 169 and 170, 1536 x 2304 384 and 383; kept apart: 2048 x 2048 492 and 513,
-// 1024 x 1152 182 and 203, 8 x 256 x 512 107 and 118, 128 x 512 77 and 79.
+// 1024 x 1152 182 and 203, 8 x 256 x 512 107 and 118, 128 x 512 77 and 79 (all
+// before the tiles of 32 columns).
 bool pairsSteps(int l, int s, int batch, const float *c) {
   const double saved = 9.0 * batch * (l - s) * s * s;   // operations, three products each
   if (!(l >= 768 && l / 4 >= s) && saved < 1.2e10) return false;

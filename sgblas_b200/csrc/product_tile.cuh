@@ -116,7 +116,7 @@ struct Cfg {
   static constexpr int kBarrierBytes = 8 * (3 * kStages + 2 * kAccums);
   static constexpr int kSmemBytes =
       kStages * kStageBytes + kScaleBytes + kOutBytes + kBarrierBytes + 1024;
-  static_assert(kBN == 64 || kBN == 128 || kBN == 256, "tile width");
+  static_assert((kBN == 32 && kPlanes == 2) || kBN == 64 || kBN == 128 || kBN == 256, "tile width");
   static_assert(!kSymmetric || kTileM % kBN == 0, "tiles end at the diagonal");
   static_assert(!kBytes || (!kAMN && !kBMN), "8-bit operands are K-major");
   static_assert(!kRows || (kBytes && kBN == 256), "rows of tokens: e4m3, two blocks of weights");
