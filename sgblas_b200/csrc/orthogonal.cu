@@ -18,7 +18,7 @@
 // where the three-fold products take 345 us of the tensor core's time at its full
 // clock (the pipe is busy 48 to 64 % of a product's cycles: one or two tiles per
 // worker leave the first loads and the last stores uncovered). 8 x 256 x 512 BF16,
-// 93 us: 17 launches, each a chain of latencies (the first slice 1.4 us,
+// 87 us: 17 launches, each a chain of latencies (the first slice 1.4 us,
 // the stream 2 to 4, the stores 1).
 //
 // X stays in G's orientation. m >= n: A = X^T X (both operands contiguous

@@ -112,7 +112,12 @@ struct Cfg {
   static constexpr int kOutBytes = kEpilogueWarps * kOutWarp;
   static constexpr int kFit = (217 * 1024 - kScaleBytes - kOutBytes) / kStageBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
-  static constexpr int kTmemColumns = kAccums * kBN;
+  // Narrow pairs: one instruction multiplies A's hi by B's hi and lo, which lie
+  // one after the other, into columns of their own (tiles of 32: 48 + 41 clocks
+  // for three of 41).
+  static constexpr bool kJoined = kPlanes == 2 && !kTwo && kBN <= 64;
+  static constexpr int kAccColumns = kJoined ? 2 * kBN : kBN;
+  static constexpr int kTmemColumns = kAccums * kAccColumns;
   static constexpr int kBarrierBytes = 8 * (3 * kStages + 2 * kAccums);
   static constexpr int kSmemBytes =
       kStages * kStageBytes + kScaleBytes + kOutBytes + kBarrierBytes + 1024;
@@ -604,29 +609,33 @@ __device__ __forceinline__ int pairSlot(int col, int row) {
   return col * 32 + ((row / 4 + col + col / 8) % 8) * 4 + row % 4;
 }
 
+// A's hi and lo at the places that a lane of flushPair writes, for the polynomial.
+struct PairColumns {
+  uint4 v[kPairCols / 8][2];
+};
+__device__ __forceinline__ void readPair(const Params &p, size_t matrix, int row0, int col0,
+                                         int cols, int lane, PairColumns *prev) {
+#pragma unroll
+  for (int pass = 0; pass < kPairCols / 8; ++pass) {
+    const int col = pass * 8 + lane / 4, row = lane % 4 * 8;
+    const size_t at = matrix + static_cast<size_t>(col0 + col) * p.ldc + row0 + row;
+    prev->v[pass][0] = prev->v[pass][1] = make_uint4(0, 0, 0, 0);
+    if (col < cols && row < p.m - row0) {
+      prev->v[pass][0] = *reinterpret_cast<const uint4 *>(p.pair.prev_hi + at);
+      prev->v[pass][1] = *reinterpret_cast<const uint4 *>(p.pair.prev_lo + at);
+    }
+  }
+}
+
 // Writes the staged columns (`cols` of them exist) at row0, col0 of the
 // matrix: hi and lo of each value in vectors of eight rows, and (mirror) of
 // eight columns across the diagonal. The polynomial reads A the same way. Rows
 // of the pair matrices are padded to 64 elements, so vectors may reach past
 // the last row or column into padding that nothing reads.
 __device__ __forceinline__ void flushPair(const Params &p, size_t matrix, bool mirror, int row0,
-                                       int col0, int cols, uint32_t *out, int lane, bool vector) {
+                                          int col0, int cols, const PairColumns &prev,
+                                          uint32_t *out, int lane, bool vector) {
   const int rows = p.m - row0;
-  // The polynomial's reads of A, together.
-  uint4 prev[kPairCols / 8][2];
-  if (p.pair.out == PairOut::kPoly) {
-#pragma unroll
-    for (int pass = 0; pass < kPairCols / 8; ++pass) {
-      const int col = pass * 8 + lane / 4, row = lane % 4 * 8;
-      const size_t at = matrix + static_cast<size_t>(col0 + col) * p.ldc + row0 + row;
-      const bool live = col < cols && row < rows;
-      prev[pass][0] = prev[pass][1] = make_uint4(0, 0, 0, 0);
-      if (live) {
-        prev[pass][0] = *reinterpret_cast<const uint4 *>(p.pair.prev_hi + at);
-        prev[pass][1] = *reinterpret_cast<const uint4 *>(p.pair.prev_lo + at);
-      }
-    }
-  }
   __syncwarp();
 #pragma unroll
   for (int pass = 0; pass < kPairCols / 8; ++pass) {
@@ -661,8 +670,8 @@ __device__ __forceinline__ void flushPair(const Params &p, size_t matrix, bool m
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= 1.0F / kPairScale;
     if (p.pair.out == PairOut::kPoly) {
-      const __half *ph = reinterpret_cast<const __half *>(&prev[pass][0]);
-      const __half *pl = reinterpret_cast<const __half *>(&prev[pass][1]);
+      const __half *ph = reinterpret_cast<const __half *>(&prev.v[pass][0]);
+      const __half *pl = reinterpret_cast<const __half *>(&prev.v[pass][1]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = fmaf(p.pair.c1, __half2float(ph[j]) + __half2float(pl[j]), v[j] * p.pair.c2);
@@ -972,6 +981,8 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       for (int i = worker; i < tiles; i += workers) {
         const Tile t = tileAt<G>(p, table, i);
         const uint32_t idesc = instrDesc<G>(p.format, widthOf(t.cols));
+        const uint32_t idesc_hi =
+            G::kJoined && p.pair.planes == 2 ? instrDesc<G>(p.format, 2 * kBN) : idesc;
         const int iters = (t.klen + G::kBK - 1) / G::kBK;
         int in_chunk = 0;
         for (int kb = 0; kb < iters; ++kb) {
@@ -998,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
           }
           if (leader) {
             tcgenFenceAfter();
-            const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * kBN);
+            const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * G::kAccColumns);
             // Descriptors count 16 bytes. K-major: the next instruction's k
             // are 32 bytes further along each row; MN-major: 16 rows of 128
             // bytes further.
@@ -1009,9 +1020,10 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
 #pragma unroll
             for (int j = 0; j < G::kBK / G::kMmaK; ++j) {
               if (j < steps) {
-                issueMma<G>(d_tmem, ad, bd, idesc, !first || j > 0);
+                issueMma<G>(d_tmem, ad, bd, idesc_hi, !first || j > 0);
                 if (G::kPlanes == 2 && p.pair.planes == 2) {
-                  issueMma<G>(d_tmem, ad, bd + G::kBBytes / 16, idesc, true);
+                  if constexpr (!G::kJoined)
+                    issueMma<G>(d_tmem, ad, bd + G::kBBytes / 16, idesc, true);
                   issueMma<G>(d_tmem, ad + G::kABytes / 16, bd, idesc, true);
                 }
               }
@@ -1176,6 +1188,15 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
       const int m0 = t.m0 + rank * kBM;
       const int iters = (t.klen + G::kBK - 1) / G::kBK;
       const int chunks = iters > 0 ? (iters - 1) / p.chunk_iters + 1 : 0;
+      // The polynomial's A, while the products are made (wider tiles have no
+      // registers for it): 16 x 100 x 200 65 -> 63 us, 512 x 512 90 -> 88.
+      constexpr bool kEarly = G::kPlanes == 2 && kHalf == kPairCols;
+      [[maybe_unused]] PairColumns prev;
+      if constexpr (kEarly) {
+        if (p.pair.out == PairOut::kPoly)
+          readPair(p, static_cast<size_t>(t.group * p.stride_c), m0 + quarter * 32,
+                   t.n0 + col_begin, t.cols - col_begin, lane, &prev);
+      }
       float2 acc[kBlocks * 4];
 #pragma unroll
       for (int j = 0; j < kBlocks * 4; ++j) acc[j] = make_float2(0.0F, 0.0F);
@@ -1185,11 +1206,14 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
         wait(&acc_full[b], acc_parity);
         tcgenFenceAfter();
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                               static_cast<uint32_t>(b * kBN + col_begin);
+                               static_cast<uint32_t>(b * G::kAccColumns + col_begin);
         float weight = 0.0F;
         if constexpr (G::kStaged) {
           weight = sc[kBN];
           sc += col_begin;
+        }
+        if constexpr (G::kJoined) {
+          if (p.pair.planes == 2) addRows<kHalf, false>(taddr + kBN, acc, nullptr, 0.0F);
         }
         if constexpr (G::kFp32) addRows<kHalf, G::kStaged>(taddr, acc, sc, weight);
         else addFragments<kHalf, G::kStaged>(taddr, acc, sc, weight, lane);
@@ -1221,7 +1245,11 @@ __global__ void __launch_bounds__(kThreads, 1) productKernel(const __grid_consta
                 words[pairSlot(j, lane)] =
                     __float_as_uint(j % 2 ? acc[(k + j) / 2].y : acc[(k + j) / 2].x);
             }
-            flushPair(p, matrix, mirror, row0, col0 + c, cols - c, words, lane, vector);
+            if constexpr (!kEarly) {
+              if (p.pair.out == PairOut::kPoly)
+                readPair(p, matrix, row0, col0 + c, cols - c, lane, &prev);
+            }
+            flushPair(p, matrix, mirror, row0, col0 + c, cols - c, prev, words, lane, vector);
           }
         } else {
           Place to;
