@@ -263,17 +263,17 @@ sgblasStatus_t launchNorm(NormParams q, int batch, cudaStream_t stream) {
 // below 6e-5 there. Over all five steps that derivative is 1.5e7: hence two at a
 // time. The product has to fit the pairs' range (15.99), as c0^2 = 11.9 does.
 //
-// It has one launch more (7 for 6, about 7 us), which long sums (the Gram
-// product's tiles are few and 7 ns deep per row) or much saved work must repay.
-// FP32 or BF16, five steps, apart and paired: 4096 x 2048 792 and 690 us,
-// 4 x 1024 x 4096 963 and 768, 1024 x 2560 286 and 262, 400 x 4000 243 and 209,
-// 128 x 2048 (2) 131 and 114, 64 x 1024 89 and 82; at the rule's edges 512 x 2048
-// 169 and 170, 1536 x 2304 384 and 383; kept apart: 2048 x 2048 492 and 513,
-// 1024 x 1152 182 and 203, 8 x 256 x 512 107 and 118, 128 x 512 77 and 79 (all
-// before the tiles of 32 columns).
+// It has one launch more (7 for 6), which much saved work, or a Gram product of
+// few and long tiles (7 ns per row), must repay. Five steps, apart and paired:
+// 4096 x 2048 792 and 690 us, 4 x 1024 x 4096 963 and 768, 1024 x 2560 242 and
+// 213, 2000 x 600 203 and 175, 128 x 2048 (2) 100 and 88, 64 x 1024 68 and 64; at
+// the rule's edges 1536 x 2304 378 and 377, 384 x 1536 108 and 109, 128 x 768 68
+// and 68; kept apart: 4 x 512 x 1024 147 and 151, 256 x 1024 87 and 89, 16 x 64 x
+// 512 61 and 63 (but also 16 x 128 x 640, 99 and 89).
 bool pairsSteps(int l, int s, int batch, const float *c) {
   const double saved = 9.0 * batch * (l - s) * s * s;   // operations, three products each
-  if (!(l >= 768 && l / 4 >= s) && saved < 1.2e10) return false;
+  const bool pays = saved >= 1e10 || (l >= 2.5 * s && saved >= 1.5e9) || (l >= 768 && l >= 5.0 * s);
+  if (!pays) return false;
   for (int i = 0; i <= 48; ++i) {   // squared singular values of 0 to 1.5
     const float a = static_cast<float>(i) / 32.0F, p = c[0] + a * (c[1] + a * c[2]),
                 b = a * p * p;
