@@ -36,19 +36,23 @@ namespace {
 // in flight, aligned words of the source, each joined with its neighbour's
 // first bytes. Bytes of the last word beyond the row are not read by TMA. Words
 // are read whole, so up to three bytes beside a row are, inside the row's first
-// and last aligned word. Memory-bound.
+// and last aligned word. With offsets, matrices of groups without columns are
+// left out (nothing reads their copies): 1 token of 9 x 2368 x 1177, 24.5 -> 8.5 us
+// with the product. Memory-bound.
 constexpr int kCopyWords = 8;
 __global__ void __launch_bounds__(256) copyRowsKernel(const unsigned char *__restrict__ src,
                                                       long long bytes, long long rows_per_matrix,
                                                       long long ld, long long stride,
                                                       unsigned char *__restrict__ dst, long long ldp,
-                                                      long long rows) {
+                                                      long long rows,
+                                                      const int *__restrict__ offsets) {
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const int lane = threadIdx.x % 32;
   const int words = static_cast<int>((bytes + 3) / 4);
   for (long long row = blockIdx.x * 8LL + threadIdx.x / 32; row < rows; row += gridDim.x * 8LL) {
     const long long matrix = rows_per_matrix == rows ? 0 : row / rows_per_matrix;
+    if (offsets != nullptr && __ldg(offsets + matrix + 1) <= __ldg(offsets + matrix)) continue;
     const auto from = reinterpret_cast<uintptr_t>(src) +
                       static_cast<uintptr_t>(matrix * stride + (row - matrix * rows_per_matrix) * ld);
     const auto *aligned = reinterpret_cast<const uint32_t *>(from & ~uintptr_t{3});
@@ -87,9 +91,10 @@ size_t copyBytes(const NarrowOperand &o, int elem_bytes) {
   return static_cast<size_t>(copyLd(o, elem_bytes)) * elem_bytes * o.dim1 * o.count;
 }
 
-// Copies the operand to dst and points it there.
+// Copies the operand to dst and points it there; with offsets only the matrices
+// of groups that have columns.
 sgblasStatus_t copyOperand(NarrowOperand *o, int elem_bytes, void *dst, int sms,
-                           cudaStream_t stream) {
+                           const int *offsets, cudaStream_t stream) {
   const long long ldp = copyLd(*o, elem_bytes);
   const long long rows = static_cast<long long>(o->dim1) * o->count;
   const long long bytes = static_cast<long long>(o->dim0) * elem_bytes;
@@ -105,7 +110,7 @@ sgblasStatus_t copyOperand(NarrowOperand *o, int elem_bytes, void *dst, int sms,
   const cudaError_t e = cudaLaunchKernelEx(
       &cfg, copyRowsKernel, static_cast<const unsigned char *>(o->ptr), bytes,
       static_cast<long long>(o->dim1), o->ld * elem_bytes, o->stride * elem_bytes,
-      static_cast<unsigned char *>(dst), ldp * elem_bytes, rows);
+      static_cast<unsigned char *>(dst), ldp * elem_bytes, rows, offsets);
   o->ptr = dst;
   o->ld = ldp;
   o->stride = ldp * o->dim1;
@@ -332,9 +337,10 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
       used_workspace = true;
       auto *base = static_cast<unsigned char *>(ctx->workspace) + kCounterRegionBytes;
       sgblasStatus_t st = SGBLAS_STATUS_SUCCESS;
-      if (copy_a) st = copyOperand(&a, elem_bytes, base, dev.sms, stream);
+      const int *reached = ragged == t::Ragged::kN ? p.offsets : nullptr;
+      if (copy_a) st = copyOperand(&a, elem_bytes, base, dev.sms, reached, stream);
       if (copy_b && st == SGBLAS_STATUS_SUCCESS)
-        st = copyOperand(&b, elem_bytes, base + bytes_a, dev.sms, stream);
+        st = copyOperand(&b, elem_bytes, base + bytes_a, dev.sms, nullptr, stream);
       if (st != SGBLAS_STATUS_SUCCESS) return st;
     }
   }
