@@ -460,7 +460,9 @@ __device__ __forceinline__ void stageBlock(unsigned char *out, int block, int lo
 }
 
 // A warp's rows of the staged columns (`cols` of them exist) to c: vectors of
-// eight rows where the address allows, else a row per lane.
+// eight rows where the address allows, else a row per lane, eight columns at a
+// time (24 gradients of 1000 x 1537 68.8 -> 63.4 us against a rolled loop; 28.7 at
+// 1536 by TMA).
 __device__ __forceinline__ void copyOut(const unsigned char *out, int lower, uint16_t *c,
                                         long long ldc, int cols, int rows, int lane, bool vector) {
   if (vector && rows >= 32) {
@@ -472,10 +474,20 @@ __device__ __forceinline__ void copyOut(const unsigned char *out, int lower, uin
             *reinterpret_cast<const uint4 *>(out + outSlot(col, lower * 4 + lane % 4));
     }
   } else if (lane < rows) {
-#pragma unroll 4
-    for (int col = 0; col < min(cols, kOutCols); ++col)
-      c[col * ldc + lane] = *reinterpret_cast<const uint16_t *>(
-          out + outSlot(col, lower * 4 + lane / 8) + lane % 8 * 2);
+    c += lane;
+#pragma unroll
+    for (int col0 = 0; col0 < kOutCols; col0 += 8) {
+      uint16_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = *reinterpret_cast<const uint16_t *>(
+            out + outSlot(col0 + j, lower * 4 + lane / 8) + lane % 8 * 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (col0 + j < cols) *c = v[j];
+        c += ldc;
+      }
+    }
   }
 }
 
