@@ -208,14 +208,30 @@ sgblasStatus_t launchPairTyped(const DeviceInfo &dev, int batch, const PairMatri
   return launchProductKernel<G>(dev, p, tiles, stream);
 }
 
-// The widest tiles of which there are enough for about every worker: pairs of
-// CTAs on 256 rows (a symmetric product's are 128 wide: 2048 x 2048 has 72 of
-// them for 74 pairs, and 36 square ones), else single CTAs on 128. Where even
-// those of 32 columns are one wave at most, they are taken for their shorter
-// epilogues (an instruction takes 41 clocks, one of 64 columns 48): 64 and 32
-// columns, five steps: 8 x 256 x 512 107 and 93 us, 1024 x 1024 177 and 156,
-// 64 x 64 54 and 45; past one wave, 16 x 200 x 300 112 and 121. (B contiguous
-// along n comes in boxes of 64.)
+// Clocks of a product on tiles G, less what all kinds share: whole waves, each
+// of the longer of a tile's slices and its epilogue, which overlap the next tile's.
+// `slice` is what 64 of k take; 16 columns of a warp take 1500 in the epilogue.
+template <class G>
+long long pairClocks(const DeviceInfo &dev, int batch, const t::Params &p, int slice) {
+  const long long workers = G::kTwo ? dev.sms / 2 : dev.sms;
+  const long long waves = (batch * pairTiles<G>(p.m, p.n) + workers - 1) / workers;
+  const long long stream = (p.k + 63LL) / 64 * slice / (p.pair.planes == 1 ? 3 : 1);
+  const long long epilogue = 1500 * (G::kBN / 32);
+  return stream + (waves - 1) * std::max(stream, epilogue) + epilogue;
+}
+
+// The tiles that take the fewest clocks: pairs of CTAs on 256 x 256 (a symmetric
+// product's are 128 wide, for 2048 x 2048 has 72 of them for 74 pairs, and 36
+// square ones), single CTAs on 128 x 128, 64 or 32 (B contiguous along n comes in
+// boxes of 64). Wide tiles load less per product, narrow ones fill the last wave
+// and have short epilogues. The clocks of a slice are fitted to 23 shapes run with
+// each kind of tile alone (64 x 64 to 2304 x 1536, batches of 1 to 16; the times
+// come out within 6 %); they are those of the loads more than of the
+// instructions (1536, 768, 768, 448 and 356). Against the widest tiles that about
+// every worker had one of, five steps: 16 x 640 x 320 262 -> 198 us, 4 x 1024 x
+// 1024 380 -> 324, 1300 x 1300 278 -> 227, 15 x 512 x 384 213 -> 191, 1024 x 1024
+// and 64 x 64 the same; at worst 4 x 512 x 640 136 -> 138. Tiles of 32 for those
+// of 64, 8 x 256 x 512: 107 and 93.
 template <bool kAMN, bool kBMN, bool kSymmetric>
 sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMatrix &a,
                                  const PairMatrix &b, const t::Params &product,
@@ -226,16 +242,18 @@ sgblasStatus_t launchPairProduct(const DeviceInfo &dev, int batch, const PairMat
   using Two = t::Cfg<2, kB, kWide, kAMN, kBMN, true, true, 2, kSymmetric>;
   using One = t::Cfg<2, kB, 128, kAMN, kBMN, false, true, 2, kSymmetric>;
   using Half = t::Cfg<2, kB, 64, kAMN, kBMN, false, true, 2, kSymmetric>;
-  if (4 * batch * pairTiles<Two>(p.m, p.n) >= dev.sms)
-    return launchPairTyped<Two>(dev, batch, a, b, p, stream);
-  if (2 * batch * pairTiles<One>(p.m, p.n) >= dev.sms)
-    return launchPairTyped<One>(dev, batch, a, b, p, stream);
+  const long long two = pairClocks<Two>(dev, batch, p, kSymmetric ? 1180 : 1870),
+                  one = pairClocks<One>(dev, batch, p, 1300),
+                  half = pairClocks<Half>(dev, batch, p, 880);
+  long long least = std::min({two, one, half});
   if constexpr (!kBMN) {
     using Quarter = t::Cfg<2, kB, 32, kAMN, kBMN, false, true, 2, kSymmetric>;
-    if (batch * pairTiles<Quarter>(p.m, p.n) <= dev.sms)
+    if (pairClocks<Quarter>(dev, batch, p, 690) <= least)
       return launchPairTyped<Quarter>(dev, batch, a, b, p, stream);
   }
-  return launchPairTyped<Half>(dev, batch, a, b, p, stream);
+  if (half == least) return launchPairTyped<Half>(dev, batch, a, b, p, stream);
+  if (one == least) return launchPairTyped<One>(dev, batch, a, b, p, stream);
+  return launchPairTyped<Two>(dev, batch, a, b, p, stream);
 }
 
 // The sums of squares, then the scaled pairs.
@@ -265,7 +283,7 @@ sgblasStatus_t launchNorm(NormParams q, int batch, cudaStream_t stream) {
 //
 // It has one launch more (7 for 6), which much saved work, or a Gram product of
 // few and long tiles (7 ns per row), must repay. Five steps, apart and paired:
-// 4096 x 2048 792 and 690 us, 4 x 1024 x 4096 963 and 768, 1024 x 2560 242 and
+// 4096 x 2048 792 and 690 us, 4 x 1024 x 4096 842 and 644, 1024 x 2560 242 and
 // 213, 2000 x 600 203 and 175, 128 x 2048 (2) 100 and 88, 64 x 1024 68 and 64; at
 // the rule's edges 1536 x 2304 378 and 377, 384 x 1536 108 and 109, 128 x 768 68
 // and 68; kept apart: 4 x 512 x 1024 147 and 151, 256 x 1024 87 and 89, 16 x 64 x
