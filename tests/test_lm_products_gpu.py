@@ -556,3 +556,27 @@ def test_offsets_past_32_bits(cuda, handle):
     ok, worst = close(w[-1], want, dy.double().abs().T @ x.double().abs(), chain_bound(n, BF16), True)
     assert ok, worst
     assert not w[:-1].any()
+
+
+def test_unaligned_weights_of_empty_groups(cuda, handle):
+    """Weights that TMA cannot read are copied for groups with tokens only: what an
+    earlier call left in the others' copies (NaN here) reaches nothing. Products
+    of small integers are exact."""
+    torch = cuda
+    groups, m, k, n = 4, 70, 77, 40
+    gen = generator(torch, 12)
+    w = torch.randint(-3, 4, (groups, m, k), generator=gen, device="cuda").to(torch.bfloat16)
+    x = torch.randint(-3, 4, (n, k), generator=gen, device="cuda").to(torch.bfloat16)
+    every = torch.tensor([0, 10, 20, 30, 40], dtype=torch.int32, device="cuda")
+    y = torch.empty(n, m, device="cuda")
+    handle.grouped_gemm_n(sg.SGBLAS_OP_T, m, n, k, groups, every, 1.0, torch.full_like(w, float("nan")),
+                          k, m * k, x, k, 0.0, y, FP32, m)
+    assert torch.isnan(y).all()
+    for offsets in ([0, 0, 40, 40, 40], [0, 0, 13, 13, 40], [0, 40, 40, 40, 40], [0, 0, 0, 0, 40]):
+        o = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+        y.fill_(float("nan"))
+        handle.grouped_gemm_n(sg.SGBLAS_OP_T, m, n, k, groups, o, 1.0, w, k, m * k, x, k, 0.0, y, FP32, m)
+        for g in range(groups):
+            a, b = offsets[g], offsets[g + 1]
+            assert torch.equal(y[a:b], x[a:b].float() @ w[g].float().T)
+    assert sg.get_device_errors() == 0
