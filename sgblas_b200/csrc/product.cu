@@ -128,6 +128,15 @@ bool encodeOperand(CUtensorMap *map, const NarrowOperand &o, int elem_bytes, boo
                        mn ? 64u : static_cast<unsigned>(rows), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Whether TMA can write C: addresses and strides of whole 16-byte units (matrices
+// `matrix` bytes apart), and such columns too, for it writes a column to the end
+// of its last unit: rows beyond C, which are not C's.
+bool tmaWritable(const t::Params &p, int size, long long matrix) {
+  const long long column = static_cast<long long>(p.ldc) * size;
+  return aligned16(p.c) && column % 16 == 0 && static_cast<long long>(p.m) * size % 16 == 0 &&
+         matrix > 0 && matrix % 16 == 0 && matrix < (1LL << 40);
+}
+
 template <class G>
 sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
                            t::Params &p, cudaStream_t stream) {
@@ -148,8 +157,7 @@ sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const 
   const unsigned long long column = static_cast<unsigned long long>(p.ldc) * kSize;
   const long long matrix = matrices == 1 ? static_cast<long long>(column * p.n)
                                          : p.stride_c * static_cast<long long>(kSize);
-  p.c_tma = p.beta == 0.0F && (p.c_bf16 != 0) == (kSize == 2) && aligned16(p.c) && column % 16 == 0 && matrix > 0 &&
-            matrix % 16 == 0 && matrix < (1LL << 40) && column < (1ULL << 40);
+  p.c_tma = p.beta == 0.0F && (p.c_bf16 != 0) == (kSize == 2) && tmaWritable(p, kSize, matrix);
   if (p.c_tma &&
       !encodeTyped3d(&p.tma_c,
                      G::kFp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
@@ -243,13 +251,11 @@ sgblasStatus_t launchRows(const DeviceInfo &dev, const NarrowOperand &a, const N
   const long long tiles = static_cast<long long>(p.tiles_n) *
                           (p.n / G::kTileM + std::min<long long>(p.groups, p.n));
   if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
-  p.c_tma = p.c_bf16 && aligned16(p.c) && p.ldc % 8 == 0;
-  if (p.c_tma) {
-    const unsigned long long column = static_cast<unsigned long long>(p.ldc) * 2;
-    if (!encodeTyped3d(&p.tma_c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.c, p.m, p.n, 1, column,
-                       column * p.n, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
-      return SGBLAS_STATUS_EXECUTION_FAILED;
-  }
+  const long long column = static_cast<long long>(p.ldc) * 2;
+  p.c_tma = p.c_bf16 && tmaWritable(p, 2, column * p.n);
+  if (p.c_tma && !encodeTyped3d(&p.tma_c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.c, p.m, p.n, 1, column,
+                                column * p.n, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
   return launchProductKernel<G>(dev, p, tiles, stream);
 }
 

@@ -158,7 +158,7 @@ struct Params {
   void *c;
   int c_bf16;
   CUtensorMap tma_c;          // where c_tma: C in boxes of 64 rows (FP32: 32) and 16 columns (kM: 32)
-  int c_tma;                  // C is aligned for TMA, and beta is 0
+  int c_tma;                  // TMA can write C (tmaWritable), and beta is 0
   int ldc;
   long long stride_c;         // Ragged::kK and kBatch
   float alpha, beta;

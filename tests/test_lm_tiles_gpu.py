@@ -105,3 +105,38 @@ def test_odd_pieces_of_gradients(cuda, handle, most, ctype):
         handle.grouped_gemm_k(m, n, k, groups, offsets, 1.0, a, m, b, n, 0.0, c, ctype, m, n * m)
         assert torch.equal(c.view(groups, n, m), want)
     assert guards_ok(cbuf) and sg.get_device_errors() == 0
+
+
+@pytest.mark.parametrize("m", [1985, 1990, 1991, 1993, 1996, 1999, 2000])
+@pytest.mark.parametrize("ctype", [FP32, BF16])
+def test_rows_beyond_a_result_stay(cuda, handle, ctype, m):
+    """Results written into the first m of 2000 rows, which may belong to
+    anything: TMA writes whole units of 16 bytes."""
+    torch = cuda
+    gen = generator(torch, 25 + m)
+    n, k, ldc = 4096, 64, 2000
+    type_ = dtype_of(torch, ctype)
+    x, w = whole(torch, gen, n, k), whole(torch, gen, 1, m, k)
+    tokens = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    few = torch.tensor([0, 112], dtype=torch.int32, device="cuda")
+    ones = torch.ones(n, device="cuda")
+    q, wq = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
+    b = whole(torch, gen, k, 512)
+    a = whole(torch, gen, k, ldc)   # m of its columns
+    depth = torch.tensor([0, k], dtype=torch.int32, device="cuda")
+
+    def check(rows, call, want):
+        buf, c = output(torch, rows * ldc, type_)
+        before = c.clone().view(rows, ldc)
+        call(c)
+        before[:, :m] = want.to(type_)
+        assert torch.equal(c.view(rows, ldc), before) and guards_ok(buf)
+
+    for rows, offsets in ((n, tokens), (112, few)):   # pairs of CTAs, single ones
+        want = by_group(torch, x[:rows], w, [0, rows])
+        check(rows, lambda c: handle.grouped_gemm_n(OP_T, m, rows, k, 1, offsets, 1.0, w, k, 0, x, k, 0.0,
+                                                    c, ctype, ldc), want)
+        check(rows, lambda c: handle.gemm_fp8(m, rows, k, wq, k, ones, 1, q, k, ones, 1, c, ctype, ldc),
+              want)
+    check(512, lambda c: handle.grouped_gemm_k(m, 512, k, 1, depth, 1.0, a, ldc, b, 512, 0.0, c, ctype, ldc,
+                                               0), b.double().T @ a[:, :m].double())
