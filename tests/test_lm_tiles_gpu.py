@@ -1,13 +1,13 @@
-"""The wide kernels of the language-model products where a worker takes several
+"""Every kernel of the language-model products, most where a worker takes several
 tiles one after the other: ring, accumulators, scales and staging buffers go
-from tile to tile. Operands are small whole numbers, so every sum is exact in
-FP32 and a result is equal to the definition's, rounded once.
+from tile to tile. Operands of the products are small whole numbers, so every
+sum is exact in FP32 and a result is equal to the definition's, rounded once.
 """
 import pytest
 
 import sgblas_b200 as sg
-from tests.lm_cases import ODD_PIECES
-from tests.test_lm_products_gpu import dtype_of, generator, guards_ok, output
+from tests.lm_cases import GRADIENTS, ODD_PIECES, ORTHOGONAL, RAGGED
+from tests.test_lm_products_gpu import ABC, dtype_of, generator, guards_ok, newton_schulz, output
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +140,114 @@ def test_rows_beyond_a_result_stay(cuda, handle, ctype, m):
               want)
     check(512, lambda c: handle.grouped_gemm_k(m, 512, k, 1, depth, 1.0, a, ldc, b, 512, 0.0, c, ctype, ldc,
                                                0), b.double().T @ a[:, :m].double())
+
+
+# ---- every kernel --------------------------------------------------------------------
+
+@pytest.mark.parametrize("case", RAGGED, ids=lambda c: c["name"])
+@pytest.mark.parametrize("ctype,beta,pad", [(BF16, 0.0, 0), (BF16, 0.0, 8), (FP32, 0.0, 0), (FP32, 0.0, 3),
+                                            (BF16, 1.0, 0), (FP32, 0.5, 1)])
+@pytest.mark.parametrize("trans", [OP_T, OP_N])
+def test_ragged_products(cuda, handle, trans, ctype, beta, pad, case):
+    """alpha A B + beta C with tokens before and after all groups, which stay as they are."""
+    torch = cuda
+    lengths, m, k = case["lengths"], case["m"], case["k"]
+    gen = generator(torch, 31 + k)
+    ends, groups, alpha = ends_of(lengths, head=1), len(lengths), -2.0
+    n = ends[-1] + 2
+    x, w = whole(torch, gen, n, k), whole(torch, gen, groups, m, k)
+    x[0], x[-1] = float("nan"), float("inf")
+    stored = w if trans == OP_T else w.mT.contiguous()
+    lda = k if trans == OP_T else m
+    offsets = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    type_, ldc = dtype_of(torch, ctype), m + pad
+    cbuf, c = output(torch, n * ldc, type_)
+    c0 = whole(torch, gen, n, ldc).to(type_)
+    c.copy_(c0.reshape(-1))
+    want = c0.clone()
+    inside = slice(1, ends[-1])
+    want[inside, :m] = (alpha * by_group(torch, x, w, ends)[inside] +
+                        beta * c0[inside, :m].double()).to(type_)
+    handle.grouped_gemm_n(trans, m, n, k, groups, offsets, alpha, stored, lda, m * k, x, k, beta, c,
+                          ctype, ldc)
+    assert torch.equal(c.view(n, ldc), want)
+    assert guards_ok(cbuf) and sg.get_device_errors() == 0
+
+
+@pytest.mark.parametrize("case", RAGGED, ids=lambda c: c["name"])
+@pytest.mark.parametrize("ctype,pad", [(BF16, 0), (BF16, 8), (BF16, 1), (FP32, 0), (FP32, 3)])
+def test_ragged_products_fp8(cuda, handle, ctype, pad, case):
+    """Scales are powers of two within 2^-2 .. 2^2, so the blocks' sums are exact too."""
+    torch = cuda
+    lengths, m, k = case["lengths"], case["m"], case["k"]
+    gen = generator(torch, 41 + k)
+    ends, groups = ends_of(lengths), len(lengths)
+    n = ends[-1] + (groups > 1)
+    kb, mb = -(-k // 128), -(-m // 128)
+    lds, ldc = kb + pad, m + pad
+    x, w = whole(torch, gen, n, k), whole(torch, gen, groups, m, k)
+    power = lambda *s: 2.0 ** torch.randint(-2, 3, s, generator=gen, device="cuda").float()  # noqa: E731
+    xs, ws = power(n, lds), power(groups, mb, lds)
+    spread = lambda v: v[..., :kb].repeat_interleave(128, -1)[..., :k]  # noqa: E731
+    want = by_group(torch, x.float() * spread(xs),
+                    w.float() * spread(ws).repeat_interleave(128, 1)[:, :m], ends)
+    type_ = dtype_of(torch, ctype)
+    q, wq = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
+    cbuf, c = output(torch, n * ldc, type_)
+    c0 = c.clone().view(n, ldc)
+    if groups == 1:
+        handle.gemm_fp8(m, n, k, wq, k, ws, lds, q, k, xs, lds, c, ctype, ldc)
+    else:
+        offsets = torch.tensor(ends, dtype=torch.int32, device="cuda")
+        handle.grouped_gemm_fp8(m, n, k, groups, offsets, wq, k, m * k, ws, lds, mb * lds, q, k, xs, lds,
+                                c, ctype, ldc)
+    c0[:ends[-1], :m] = want[:ends[-1]].to(type_)
+    assert torch.equal(c.view(n, ldc), c0)
+    assert guards_ok(cbuf) and sg.get_device_errors() == 0
+
+
+@pytest.mark.parametrize("m,n", GRADIENTS)
+@pytest.mark.parametrize("ctype,beta,pad", [(FP32, 0.0, 0), (FP32, 1.0, 0), (FP32, 0.0, 1), (BF16, 0.0, 0),
+                                            (BF16, 0.0, 8), (BF16, 0.5, 0)])
+def test_ragged_gradients(cuda, handle, ctype, beta, pad, m, n):
+    """Twelve groups, cut slices of every kind, four tiles per pair of CTAs."""
+    torch = cuda
+    gen = generator(torch, 51 + m)
+    lengths = [1, 63, 64, 65, 0, 127, 129, 200, 31, 500, 17, 300]
+    ends, groups, alpha = ends_of(lengths, head=1), len(lengths), -2.0
+    k = ends[-1] + 1
+    a, b = whole(torch, gen, k, m), whole(torch, gen, k, n)
+    a[0], b[-1] = float("nan"), float("inf")
+    offsets = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    type_, ldc = dtype_of(torch, ctype), m + pad
+    cbuf, c = output(torch, groups * n * ldc, type_)
+    c0 = whole(torch, gen, groups, n, ldc).to(type_)
+    c.copy_(c0.reshape(-1))
+    want = c0.clone()
+    for g, (lo, hi) in enumerate(zip(ends, ends[1:])):
+        want[g, :, :m] = (alpha * (b[lo:hi].double().T @ a[lo:hi].double()) +
+                          beta * c0[g, :, :m].double()).to(type_)
+    handle.grouped_gemm_k(m, n, k, groups, offsets, alpha, a, m, b, n, beta, c, ctype, ldc, n * ldc)
+    assert torch.equal(c.view(groups, n, ldc), want)
+    assert guards_ok(cbuf) and sg.get_device_errors() == 0
+
+
+@pytest.mark.parametrize("rows,cols,batch", ORTHOGONAL)
+def test_orthogonalize(cuda, handle, rows, cols, batch):
+    """The bound of the test of the same name for smaller matrices, with the same
+    inputs: BF16's rounding, and the last product's operands of 11 bits."""
+    torch = cuda
+    gen = generator(torch, rows)
+    rank = min(rows, cols) // 8
+    g = 1e-3 * (torch.randn(batch, rows, rank, generator=gen, device="cuda") @
+                torch.randn(batch, rank, cols, generator=gen, device="cuda") +
+                0.3 * torch.randn(batch, rows, cols, generator=gen, device="cuda"))
+    buf, o = output(torch, batch * rows * cols, torch.bfloat16)
+    handle.orthogonalize(cols, rows, batch, 5, ABC, 1e-7, 1.0, g, FP32, cols, rows * cols, o, cols,
+                         rows * cols)
+    got = o.view(batch, rows, cols).double()
+    for i in range(batch):
+        want = newton_schulz(g[i], 5, ABC, 1e-7, 1.0)
+        rel = ((got[i] - want).norm() / want.norm()).item()
+        assert rel <= 2.0 ** -9 + 2.0 ** -10, (i, rel)
+    assert guards_ok(buf) and sg.get_device_errors() == 0
