@@ -169,7 +169,8 @@ _SCALARS = {v: ctypes.byref(ctypes.c_float(v)) for v in (0.0, 1.0)}   # read, ne
 def _fp(v):
     if v is None:
         return None
-    known = _SCALARS.get(v)
+    # Anything else that converts to a float is taken too (0-d arrays have no hash).
+    known = _SCALARS.get(v) if type(v) is float else None
     return ctypes.byref(ctypes.c_float(v)) if known is None else known
 
 
