@@ -51,7 +51,7 @@ struct NormParams {
   int m, n, ldg;
   long long stride_g;
   int partials;        // per matrix
-  float *sums;         // [batch][partials]
+  double *sums;        // [batch][partials]
   float eps;
   __half *hi, *lo;     // written by splitKernel
   int ldx;
@@ -75,26 +75,27 @@ struct Run {
 };
 
 // Sum over the block, the same in every thread; the order is fixed.
-__device__ __forceinline__ float blockSum(float v) {
-  __shared__ float part[kNormThreads / 32];
+__device__ __forceinline__ double blockSum(double v) {
+  __shared__ double part[kNormThreads / 32];
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
   __syncthreads();
-  float s = 0.0F;
+  double s = 0.0;
 #pragma unroll
   for (int w = 0; w < kNormThreads / 32; ++w) s += part[w];
   return s;
 }
 
-// sums[matrix][i] = sum of squares of the columns i, i + partials, ...
-// Memory-bound, as is splitKernel.
+// sums[matrix][i] = sum of squares of the columns i, i + partials, ... In 64 bits:
+// the squares of FP32 values leave FP32's range above 2^64 and below 2^-64, and
+// G may be of any magnitude. Memory-bound, as is splitKernel.
 template <typename T, bool kVector>
 __global__ void __launch_bounds__(kNormThreads) squaresKernel(const NormParams p) {
   using R = Run<T, kVector>;
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
-  float s = 0.0F;
+  double s = 0.0;
   for (int col = blockIdx.x; col < p.n; col += p.partials) {
     const T *column = static_cast<const T *>(p.g) + blockIdx.y * p.stride_g +
                       static_cast<long long>(col) * p.ldg;
@@ -104,8 +105,8 @@ __global__ void __launch_bounds__(kNormThreads) squaresKernel(const NormParams p
       r.load(column, row, p.m);
 #pragma unroll
       for (int j = 0; j < R::kCount; ++j) {
-        const float v = static_cast<float>(r.v[j]);
-        s = fmaf(v, v, s);
+        const double v = static_cast<float>(r.v[j]);
+        s = fma(v, v, s);
       }
     }
   }
@@ -113,16 +114,20 @@ __global__ void __launch_bounds__(kNormThreads) squaresKernel(const NormParams p
   if (threadIdx.x == 0) p.sums[static_cast<size_t>(blockIdx.y) * p.partials + blockIdx.x] = s;
 }
 
-// X = G / (norm + eps) as pairs.
+// X = G / (norm + eps) as pairs. The factor can leave FP32's range too, so where
+// it is beyond 2^-100 .. 2^100 a power of two of it is applied first: exactly, but
+// for values so far below the norm that a pair holds nothing of them.
 template <typename T, bool kVector>
 __global__ void __launch_bounds__(kNormThreads) splitKernel(const NormParams p) {
   using R = Run<T, kVector>;
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
-  const float *sums = p.sums + static_cast<size_t>(blockIdx.y) * p.partials;
-  float part = 0.0F;
+  const double *sums = p.sums + static_cast<size_t>(blockIdx.y) * p.partials;
+  double part = 0.0;
   for (int i = threadIdx.x; i < p.partials; i += kNormThreads) part += sums[i];
-  const float factor = t::kPairScale / (sqrtf(blockSum(part)) + p.eps);
+  const double whole = t::kPairScale / (sqrt(blockSum(part)) + p.eps);
+  const float power = whole > 0x1p100 ? 0x1p80F : whole < 0x1p-100 ? 0x1p-80F : 1.0F;
+  const float factor = static_cast<float>(whole / power);
   for (int col = blockIdx.x; col < p.n; col += gridDim.x) {
     const T *column = static_cast<const T *>(p.g) + blockIdx.y * p.stride_g +
                       static_cast<long long>(col) * p.ldg;
@@ -136,7 +141,7 @@ __global__ void __launch_bounds__(kNormThreads) splitKernel(const NormParams p) 
       alignas(16) __half hi[R::kCount], lo[R::kCount];
 #pragma unroll
       for (int j = 0; j < R::kCount; ++j)
-        t::splitPair(static_cast<float>(r.v[j]) * factor, &hi[j], &lo[j]);
+        t::splitPair(static_cast<float>(r.v[j]) * power * factor, &hi[j], &lo[j]);
       if constexpr (R::kCount == 8) {
         *reinterpret_cast<uint4 *>(p.hi + to + row) = *reinterpret_cast<const uint4 *>(hi);
         *reinterpret_cast<uint4 *>(p.lo + to + row) = *reinterpret_cast<const uint4 *>(lo);
@@ -332,7 +337,7 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
   const long long ldx = (m + 63LL) / 64 * 64, lds = (s + 63LL) / 64 * 64;
   // About eight blocks per SM over the batch.
   const int partials = std::min({n, kMaxPartials, std::max(1, 8 * dev.sms / batch)});
-  const size_t sum_bytes = align256(static_cast<size_t>(batch) * partials * sizeof(float));
+  const size_t sum_bytes = align256(static_cast<size_t>(batch) * partials * sizeof(double));
   const size_t x_bytes = static_cast<size_t>(ldx) * n * batch * sizeof(__half);   // 128-byte units
   const size_t s_bytes = static_cast<size_t>(lds) * s * batch * sizeof(__half);
   const bool paired = steps > 2 && pairsSteps(l, s, batch, coefficients);
@@ -341,7 +346,7 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
                        dev.device, stream))
     return SGBLAS_STATUS_NOT_SUPPORTED;
   auto *base = static_cast<unsigned char *>(handle->workspace) + kCounterRegionBytes;
-  auto *sums = reinterpret_cast<float *>(base);
+  auto *sums = reinterpret_cast<double *>(base);
   base += sum_bytes;
   auto take = [&](int dim0, int dim1, long long ld, size_t bytes) {
     PairMatrix x;

@@ -251,3 +251,29 @@ def test_orthogonalize(cuda, handle, rows, cols, batch):
         rel = ((got[i] - want).norm() / want.norm()).item()
         assert rel <= 2.0 ** -9 + 2.0 ** -10, (i, rel)
     assert guards_ok(buf) and sg.get_device_errors() == 0
+
+
+@pytest.mark.parametrize("type_", ["float32", "bfloat16"])
+@pytest.mark.parametrize("exponent", [-149, -140, -100, -70, 60, 70, 100, 124])
+def test_orthogonalize_any_magnitude(cuda, handle, exponent, type_):
+    """G scaled by a power of two gives, without an eps, what G gives: the squares
+    of its values lie outside FP32's range. Below 2^-126 G itself is coarser, and in
+    BF16 nothing below 2^-134, so the definition takes what it holds (0 / 0 of
+    nothing). The bound is that of test_orthogonalize."""
+    torch = cuda
+    g = torch.randn(1, 200, 300, generator=generator(torch, 61), device="cuda", dtype=torch.float64)
+    g = (g * 2.0 ** exponent).to(getattr(torch, type_)).repeat(2, 1, 1)
+    g[1] = 0.0
+    o = torch.empty(2, 200, 300, dtype=torch.bfloat16, device="cuda")
+    code = BF16 if type_ == "bfloat16" else FP32
+    for eps in (0.0, 2.0 ** (exponent - 2) if exponent > 0 else 1e-7):
+        handle.orthogonalize(300, 200, 2, 5, ABC, eps, 1.0, g, code, 300, 60000, o, 300, 60000)
+        want = newton_schulz(g[0], 5, ABC, torch.tensor(eps, dtype=torch.float32).item(), 1.0)
+        if torch.isnan(want).all():
+            assert not g.any() and torch.isnan(o).all()
+        elif eps == 0.0 or exponent > 0:
+            assert ((o[0].double() - want).norm() / want.norm()).item() <= 2.0 ** -9 + 2.0 ** -10
+        else:   # next to eps there is little left of G: an absolute 2^-37 per value of X, times 485
+            assert ((o[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -27).all()
+        assert (o[1] == 0).all() if eps > 0.0 else torch.isnan(o[1]).all()
+    assert sg.get_device_errors() == 0
