@@ -44,9 +44,9 @@ typedef enum sgblasDataType_t {
  * k x m), with transa = N the gradient of its tokens.
  *
  * Products are exact, sums are FP32. The tensor core's adder truncates, so
- * for an FP32 C at most 512 of k are chained there and the chains are added
- * with rounding to nearest (a BF16 C, whose own rounding is far coarser, chains
- * all of k); the result is rounded once to ctype. Scalars as for sgblasSgemm:
+ * at most 512 of k are chained there for an FP32 C, and 4096 for a BF16 C, whose
+ * own rounding is far coarser; the chains are added with rounding to nearest,
+ * and the result is rounded once to ctype. Scalars as for sgblasSgemm:
  * *beta == 0 writes C without reading it; *alpha == 0 or k == 0 does not read
  * A and B. Any alignment and leading dimension: an operand TMA cannot read (a
  * base not 16-byte aligned, lda, ldb or stride_a not a multiple of 8) is

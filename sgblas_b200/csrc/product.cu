@@ -329,9 +329,13 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
                             bool b_mn, t::Params p) {
   const auto stream = static_cast<cudaStream_t>(ctx->stream);
   p.err = dev.err;
-  // Chains of one block of 128 (e4m3) or 512 of k; a BF16 result of BF16
-  // operands is rounded at 2^-9, a thousand times a whole chain's error.
-  p.chunk_iters = elem_bytes == 1 ? 1 : p.c_bf16 ? INT_MAX : 8;
+  // Chains of one block of 128 (e4m3), of 512 of k, or, for a BF16 result of BF16
+  // operands, of 4096: its own rounding is up to 2^-8, a chain of 4096 positive
+  // products comes out 8e-6 too small (6e-5 at most: 256 instructions, 2^-22
+  // each). The whole of k in one chain, which may be an expert's tokens, would
+  // not do: sums of 2^17 came out 8e-4 too small, of 2^20 6.6e-3 (2e-5 in chains
+  // of 4096, at the same speed: 2048 x 2048 x 16384 96 us).
+  p.chunk_iters = elem_bytes == 1 ? 1 : p.c_bf16 ? 64 : 8;
   bool used_workspace = false;
   if (p.k > 0) {
     const bool copy_a = !tmaReadable(a, elem_bytes), copy_b = !tmaReadable(b, elem_bytes);

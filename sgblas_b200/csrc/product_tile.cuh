@@ -20,8 +20,8 @@
 //
 // Sums. The tensor core's FP32 adder truncates: the relative error of a chain
 // grows with its length (measured 3e-7 after 32 instructions, 3e-6 after 512).
-// So the k range is cut into chunks (128 to 512 of k; none for a BF16 result of
-// BF16 operands, whose rounding is a thousand times larger). The issuer
+// So the k range is cut into chunks (128 to 512 of k; 4096 for a BF16 result of
+// BF16 operands, whose own rounding is a hundred times such a chain's). The issuer
 // alternates between the two accumulators, and the epilogue adds each chunk to
 // the registers with rounding to nearest. For e4m3 the chunk is one block of
 // 128, and the same addition applies the block's scales.

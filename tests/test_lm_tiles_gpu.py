@@ -277,3 +277,32 @@ def test_orthogonalize_any_magnitude(cuda, handle, exponent, type_):
             assert ((o[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -27).all()
         assert (o[1] == 0).all() if eps > 0.0 else torch.isnan(o[1]).all()
     assert sg.get_device_errors() == 0
+
+
+@pytest.mark.parametrize("trans", [None, OP_T, OP_N])
+def test_long_sums_are_not_biased(cuda, handle, trans):
+    """Positive products, so that every truncation of a chain goes the same way,
+    and a BF16 result: the mean over 16384 of them shows what its own rounding
+    (up to 2^-8, without bias: 1.7e-3 / 128 in the mean, five times that allowed)
+    hides. A chain of 4096 of k is off by 256 instructions' 2^-22 at most; its 256
+    pieces are added with rounding to nearest, 2^-24 each at most.
+    """
+    torch = cuda
+    gen = generator(torch, 71)
+    k, m = 1 << 20, 128
+    # Each row and column of the result of its own size, so their roundings differ.
+    a, b = ((torch.rand(k, m, generator=gen, device="cuda").add_(0.5) *
+             torch.exp2(torch.rand(m, generator=gen, device="cuda"))).to(torch.bfloat16)
+            for _ in range(2))
+    c = torch.empty(m, m, dtype=torch.bfloat16, device="cuda")
+    offsets = torch.tensor([0, k if trans is None else m], dtype=torch.int32, device="cuda")
+    if trans is None:      # a weight gradient of 2^20 tokens
+        handle.grouped_gemm_k(m, m, k, 1, offsets, 1.0, a, m, b, m, 0.0, c, BF16, m, 0)
+    else:
+        tokens = b.T.contiguous()
+        w, lda = (a.T.contiguous(), k) if trans == OP_T else (a, m)
+        handle.grouped_gemm_n(trans, m, m, k, 1, offsets, 1.0, w, lda, 0, tokens, k, 0.0, c, BF16, m)
+    want = b.double().T @ a.double()
+    bias = ((c.double() - want) / want).mean().abs().item()
+    assert bias <= 5 * 1.7e-3 / 128 + 256 * 2.0 ** -22 + 256 * 2.0 ** -24, bias
+    assert sg.get_device_errors() == 0
