@@ -322,6 +322,22 @@ sgblasStatus_t launchRaggedN(const DeviceInfo &dev, const NarrowOperand &a, cons
   }
 }
 
+sgblasStatus_t launchKind(const DeviceInfo &dev, int elem_bytes, t::Ragged ragged,
+                          const NarrowOperand &a, bool a_mn, const NarrowOperand &b, bool b_mn,
+                          t::Params &p, cudaStream_t stream) {
+  if (ragged == t::Ragged::kN && elem_bytes == 2 && a_mn && !b_mn)
+    return launchRaggedN<2, true>(dev, a, b, p, stream);
+  if (ragged == t::Ragged::kN && elem_bytes == 2 && !a_mn && !b_mn)
+    return launchRaggedN<2, false>(dev, a, b, p, stream);
+  if (ragged == t::Ragged::kN && elem_bytes == 1 && !a_mn && !b_mn)
+    return launchRaggedN<1, false>(dev, a, b, p, stream);
+  if (ragged == t::Ragged::kK && elem_bytes == 2 && a_mn && b_mn)
+    return p.c_bf16 && p.beta == 0.0F
+               ? launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, false>>(dev, a, b, p, stream)
+               : launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, true>>(dev, a, b, p, stream);
+  return SGBLAS_STATUS_INTERNAL_ERROR;
+}
+
 }  // namespace
 
 sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_bytes,
@@ -336,6 +352,7 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
   // not do: sums of 2^17 came out 8e-4 too small, of 2^20 6.6e-3 (2e-5 in chains
   // of 4096, at the same speed: 2048 x 2048 x 16384 96 us).
   p.chunk_iters = elem_bytes == 1 ? 1 : p.c_bf16 ? 64 : 8;
+  sgblasStatus_t st = SGBLAS_STATUS_SUCCESS;
   bool used_workspace = false;
   if (p.k > 0) {
     const bool copy_a = !tmaReadable(a, elem_bytes), copy_b = !tmaReadable(b, elem_bytes);
@@ -346,25 +363,15 @@ sgblasStatus_t launchNarrow(sgblasContext *ctx, const DeviceInfo &dev, int elem_
         return SGBLAS_STATUS_NOT_SUPPORTED;
       used_workspace = true;
       auto *base = static_cast<unsigned char *>(ctx->workspace) + kCounterRegionBytes;
-      sgblasStatus_t st = SGBLAS_STATUS_SUCCESS;
       const int *reached = ragged == t::Ragged::kN ? p.offsets : nullptr;
       if (copy_a) st = copyOperand(&a, elem_bytes, base, dev.sms, reached, stream);
       if (copy_b && st == SGBLAS_STATUS_SUCCESS)
         st = copyOperand(&b, elem_bytes, base + bytes_a, dev.sms, nullptr, stream);
-      if (st != SGBLAS_STATUS_SUCCESS) return st;
     }
   }
-  sgblasStatus_t st = SGBLAS_STATUS_INTERNAL_ERROR;
-  if (ragged == t::Ragged::kN && elem_bytes == 2 && a_mn && !b_mn)
-    st = launchRaggedN<2, true>(dev, a, b, p, stream);
-  else if (ragged == t::Ragged::kN && elem_bytes == 2 && !a_mn && !b_mn)
-    st = launchRaggedN<2, false>(dev, a, b, p, stream);
-  else if (ragged == t::Ragged::kN && elem_bytes == 1 && !a_mn && !b_mn)
-    st = launchRaggedN<1, false>(dev, a, b, p, stream);
-  else if (ragged == t::Ragged::kK && elem_bytes == 2 && a_mn && b_mn)
-    st = p.c_bf16 && p.beta == 0.0F
-             ? launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, false>>(dev, a, b, p, stream)
-             : launchTyped<t::Cfg<2, t::Ragged::kK, 256, true, true, true, true>>(dev, a, b, p, stream);
+  if (st == SGBLAS_STATUS_SUCCESS)
+    st = launchKind(dev, elem_bytes, ragged, a, a_mn, b, b_mn, p, stream);
+  // Failed or not: a copy may be on its way, and later users wait for it.
   if (used_workspace && !markWorkspaceUse(ctx, stream) && st == SGBLAS_STATUS_SUCCESS)
     return SGBLAS_STATUS_EXECUTION_FAILED;
   return st;

@@ -439,6 +439,7 @@ sgblasStatus_t launchProduct(sgblasContext *ctx, sgblasOperation_t ta, sgblasOpe
   const bool pack_a = single && (!(aligned16(a) && lda % 4 == 0) || (tA && worthCopy(n, m)));
   const bool pack_b = single && (!(aligned16(b) && ldb % 4 == 0) || (!tB && worthCopy(m, n)));
   bool packed = false;
+  sgblasStatus_t st = SGBLAS_STATUS_SUCCESS;
   if (pack_a || pack_b) {
     const int sms = smCount(device);
     if (sms <= 0) return SGBLAS_STATUS_EXECUTION_FAILED;
@@ -450,43 +451,43 @@ sgblasStatus_t launchProduct(sgblasContext *ctx, sgblasOperation_t ta, sgblasOpe
     const size_t off_b = roundUp(off_a + bytes_a, kPackAlign);
     const size_t bytes_b = pack_b ? static_cast<size_t>(ldp_b) * k * sizeof(float) : 0;
     if (ldp_a >= m && ldp_b >= n && ensureWorkspace(ctx, off_b + bytes_b, device, stream)) {
+      packed = true;
       auto *ws = static_cast<unsigned char *>(ctx->workspace);
       if (pack_a) {
         auto *dst = reinterpret_cast<float *>(ws + off_a);
-        const sgblasStatus_t st = launchPack(a, lda, tA, m, k, dst, ldp_a, sms, stream);
-        if (st != SGBLAS_STATUS_SUCCESS) return st;
+        st = launchPack(a, lda, tA, m, k, dst, ldp_a, sms, stream);
         p.a = dst;
         p.lda = ldp_a;
         tA = false;
       }
-      if (pack_b) {
+      if (pack_b && st == SGBLAS_STATUS_SUCCESS) {
         auto *dst = reinterpret_cast<float *>(ws + off_b);
-        const sgblasStatus_t st = launchPack(b, ldb, !tB, n, k, dst, ldp_b, sms, stream);
-        if (st != SGBLAS_STATUS_SUCCESS) return st;
+        st = launchPack(b, ldb, !tB, n, k, dst, ldp_b, sms, stream);
         p.b = dst;
         p.ldb = ldp_b;
         tB = true;
       }
-      packed = true;
     }
   }
-  sgblasStatus_t st;
   // TF32 for one matrix or a strided batch whose matrices TMA can all read
   // (positive strides, multiples of 4 floats); otherwise FP32, which is
   // more accurate than TF32 mode asks.
   auto tf32Stride = [](long long stride) {
     return stride > 0 && stride % 4 == 0 && stride < (1LL << 38);
   };
-  if (ctx->math_mode == SGBLAS_MATH_TF32 && batch.a_ptrs == nullptr &&
-      tf32Eligible(p.a, p.lda, p.b, p.ldb) &&
-      (batch.count == 1 || (tf32Stride(batch.stride_a) && tf32Stride(batch.stride_b)))) {
+  if (st != SGBLAS_STATUS_SUCCESS) {
+    // A copy failed: no product.
+  } else if (ctx->math_mode == SGBLAS_MATH_TF32 && batch.a_ptrs == nullptr &&
+             tf32Eligible(p.a, p.lda, p.b, p.ldb) &&
+             (batch.count == 1 || (tf32Stride(batch.stride_a) && tf32Stride(batch.stride_b)))) {
     st = launchTf32(tA, tB, p, scratch, device, stream);
   } else if (!tA && !tB) st = launchMode<false, false>(p, scratch, device, stream);
   else if (!tA && tB) st = launchMode<false, true>(p, scratch, device, stream);
   else if (tA && !tB) st = launchMode<true, false>(p, scratch, device, stream);
   else st = launchMode<true, true>(p, scratch, device, stream);
-  // The product read the packed operands: later users of the workspace wait.
-  if (st == SGBLAS_STATUS_SUCCESS && packed && !markWorkspaceUse(ctx, stream))
+  // The product reads the packed operands, and after a failure a copy may still
+  // write them: later users of the workspace wait.
+  if (packed && !markWorkspaceUse(ctx, stream) && st == SGBLAS_STATUS_SUCCESS)
     return SGBLAS_STATUS_EXECUTION_FAILED;
   return st;
 }
