@@ -12,6 +12,14 @@
 
 #include <cstddef>
 
+// A workspace that a captured call uses: its graph may be replayed for as long
+// as the handle exists, so the memory stays when the handle takes a larger one.
+struct sgblasRetained {
+  void *workspace;
+  int device;
+  sgblasRetained *next;
+};
+
 struct sgblasContext {
   sgblasStream_t stream = nullptr;
   sgblasMathMode_t math_mode = SGBLAS_MATH_FP32;
@@ -24,6 +32,8 @@ struct sgblasContext {
   std::size_t workspace_bytes = 0;
   int workspace_device = -1;
   void *workspace_event = nullptr;
+  bool workspace_captured = false;   // a call inside a stream capture used it
+  sgblasRetained *retained = nullptr;
   // Epoch of the last launch that used the workspace's arrival counters
   // (each such launch takes the next one; see kern::arriveCounter).
   unsigned workspace_epoch = 0;

@@ -20,6 +20,7 @@
 #include <atomic>
 #include <climits>
 #include <cstdint>
+#include <new>
 
 namespace sgblas::detail {
 
@@ -236,9 +237,37 @@ bool capturing(cudaStream_t stream) {
   return status != cudaStreamCaptureStatusNone;
 }
 
-}  // namespace
+void forgetWorkspace(sgblasContext *ctx) {
+  ctx->workspace = nullptr;
+  ctx->workspace_bytes = 0;
+  ctx->workspace_device = -1;
+  ctx->workspace_event = nullptr;
+  ctx->workspace_captured = false;
+}
 
-namespace {
+// Keeps a workspace that graphs use until the handle is destroyed (should there
+// be no memory for the note of it, for good). Its event is released once it
+// completes.
+void retainWorkspace(sgblasContext *ctx) {
+  auto *kept = new (std::nothrow)
+      sgblasRetained{ctx->workspace, ctx->workspace_device, ctx->retained};
+  if (kept != nullptr) ctx->retained = kept;
+  if (ctx->workspace_event != nullptr)
+    (void)cudaEventDestroy(static_cast<cudaEvent_t>(ctx->workspace_event));
+  forgetWorkspace(ctx);
+}
+
+// Frees memory that lives on `device`, after the work using it.
+void freeOn(int device, void *memory, void *event) {
+  int current = -1;
+  const bool restore = cudaGetDevice(&current) == cudaSuccess;
+  if (cudaSetDevice(device) == cudaSuccess) {
+    (void)cudaFree(memory);  // synchronizes with the launches using it
+    if (event != nullptr) (void)cudaEventDestroy(static_cast<cudaEvent_t>(event));
+  }
+  if (restore) (void)cudaSetDevice(current);
+  (void)cudaGetLastError();
+}
 
 // The handle moved to another device: its workspace is freed on the device
 // it lives on, stream-ordered after its last user there (the legacy stream
@@ -256,10 +285,7 @@ bool retireOnOwnDevice(sgblasContext *ctx) {
                   cudaFreeAsync(ctx->workspace, cudaStreamLegacy) == cudaSuccess;
   if (ok) {
     if (ev != nullptr) (void)cudaEventDestroy(ev);   // released once it completes
-    ctx->workspace = nullptr;
-    ctx->workspace_bytes = 0;
-    ctx->workspace_device = -1;
-    ctx->workspace_event = nullptr;
+    forgetWorkspace(ctx);
   }
   (void)cudaGetLastError();
   (void)cudaSetDevice(current);
@@ -278,26 +304,27 @@ bool ensureWorkspace(sgblasContext *ctx, size_t need, int device, cudaStream_t s
       (void)cudaGetLastError();
       return false;
     }
+    if (in_capture) ctx->workspace_captured = true;
     return true;
   }
   if (in_capture) return false;   // the caller falls back to a path without it
-  if (ctx->workspace != nullptr && ctx->workspace_device == device) {
+  if (ctx->workspace != nullptr && ctx->workspace_captured) {
+    retainWorkspace(ctx);
+  } else if (ctx->workspace != nullptr && ctx->workspace_device == device) {
     // Growing: free the old buffer stream-ordered after its last user, so the
     // call does not block the host.
     const auto ev = static_cast<cudaEvent_t>(ctx->workspace_event);
     const bool ordered = ev == nullptr || cudaStreamWaitEvent(stream, ev, 0) == cudaSuccess;
     if (!ordered || cudaFreeAsync(ctx->workspace, stream) != cudaSuccess) {
       (void)cudaGetLastError();
-      releaseWorkspace(ctx);
-    } else {
-      if (ev != nullptr) (void)cudaEventDestroy(ev);  // released once it completes
-      ctx->workspace = nullptr;
-      ctx->workspace_bytes = 0;
-      ctx->workspace_device = -1;
-      ctx->workspace_event = nullptr;
+      freeOn(ctx->workspace_device, ctx->workspace, ctx->workspace_event);
+    } else if (ev != nullptr) {
+      (void)cudaEventDestroy(ev);  // released once it completes
     }
+    forgetWorkspace(ctx);
   } else if (ctx->workspace != nullptr && !retireOnOwnDevice(ctx)) {
-    releaseWorkspace(ctx);
+    freeOn(ctx->workspace_device, ctx->workspace, ctx->workspace_event);
+    forgetWorkspace(ctx);
   }
   if (cudaSetDevice(device) != cudaSuccess) {
     (void)cudaGetLastError();
@@ -496,19 +523,14 @@ sgblasStatus_t launchProduct(sgblasContext *ctx, sgblasOperation_t ta, sgblasOpe
 
 void releaseWorkspace(sgblasContext *context) {
   if (context->workspace != nullptr) {
-    int current = -1;
-    const bool restore = cudaGetDevice(&current) == cudaSuccess;
-    if (cudaSetDevice(context->workspace_device) == cudaSuccess) {
-      (void)cudaFree(context->workspace);  // synchronizes with the launches using it
-      if (context->workspace_event != nullptr)
-        (void)cudaEventDestroy(static_cast<cudaEvent_t>(context->workspace_event));
-    }
-    context->workspace_event = nullptr;
-    if (restore) (void)cudaSetDevice(current);
-    (void)cudaGetLastError();
-    context->workspace = nullptr;
-    context->workspace_bytes = 0;
-    context->workspace_device = -1;
+    freeOn(context->workspace_device, context->workspace, context->workspace_event);
+    forgetWorkspace(context);
+  }
+  while (context->retained != nullptr) {
+    sgblasRetained *kept = context->retained;
+    context->retained = kept->next;
+    freeOn(kept->device, kept->workspace, nullptr);
+    delete kept;
   }
 }
 

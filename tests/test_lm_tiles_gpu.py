@@ -306,3 +306,35 @@ def test_long_sums_are_not_biased(cuda, handle, trans):
     bias = ((c.double() - want) / want).mean().abs().item()
     assert bias <= 5 * 1.7e-3 / 128 + 256 * 2.0 ** -22 + 256 * 2.0 ** -24, bias
     assert sg.get_device_errors() == 0
+
+
+def test_a_graph_outlives_a_larger_call(cuda, lib):
+    """A captured call keeps the workspace it was captured with."""
+    torch = cuda
+    gen = generator(torch, 81)
+    m, k, n = 301, 77, 200
+    x, w = whole(torch, gen, n, k), whole(torch, gen, 1, m, k)
+    large = torch.full((1, 5001, 5001), float("nan"), dtype=torch.bfloat16, device="cuda")
+    offsets = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    y, z = torch.empty(n, m, device="cuda"), torch.empty(5001, 5001, device="cuda")
+    end = torch.tensor([0, 5001], dtype=torch.int32, device="cuda")
+    with lib.Handle() as h:
+        call = lambda: h.grouped_gemm_n(OP_T, m, n, k, 1, offsets, 1.0, w, k, 0, x, k, 0.0, y, FP32, m)  # noqa: E731
+        call()
+        stream = torch.cuda.Stream()
+        h.set_stream(stream)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call()
+        for _ in range(2):
+            h.grouped_gemm_n(OP_T, 5001, 5001, 5001, 1, end, 1.0, large, 5001, 0, large, 5001, 0.0, z, FP32,
+                             5001)
+            torch.cuda.synchronize()
+            y.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, (x.double() @ w[0].double().T).float())
+        del graph
+    assert sg.get_device_errors() == 0

@@ -50,3 +50,36 @@ def test_copies_before_a_failed_launch_are_uses(log, call, at):
         assert call(h) == sg.SGBLAS_STATUS_EXECUTION_FAILED
         assert len(log.launches()) == at - 1
         assert log.lines()[-1] == "record"
+
+
+def addresses(log, what):
+    return [line.split()[1] for line in log.lines() if line.startswith(what + " ")]
+
+
+def larger(h):
+    return h.grouped_gemm_n_status(sg.SGBLAS_OP_T, 4001, 4001, 4001, 4, FAKE, 1.0, FAKE, 4001, 4001 * 4001,
+                                   FAKE, 4001, 0.0, FAKE, FP32, 4001)
+
+
+def orthogonalize(h):
+    return h.orthogonalize_status(64, 64, 1, 5, (3.4445, -4.7750, 2.0315), 1e-7, 1.0, FAKE, FP32, 64, 0, FAKE,
+                                  64, 0)
+
+
+@pytest.mark.parametrize("call", [grouped_n, sgemm, orthogonalize])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_workspace_in_a_graph_stays(log, captured, call):
+    """A graph may be replayed after a larger call: the workspace it uses is not
+    freed before the handle is destroyed. Without a capture it is."""
+    with sg.Handle() as h:
+        assert call(h) == 0
+        first = addresses(log, "malloc")
+        assert len(first) == 1
+        if captured:
+            log.dll.fakeCapture(1)
+            assert call(h) == 0
+            log.dll.fakeCapture(0)
+        assert larger(h) == 0
+        assert len(addresses(log, "malloc")) == 2
+        assert addresses(log, "free") == ([] if captured else first)
+    assert sorted(addresses(log, "free")) == sorted(addresses(log, "malloc"))
