@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
       const int boxes = (t.cols + kThinBox - 1) / kThinBox;
       for (int kb = kb0; kb < kb1; ++kb) {
         wait(&empty[s], parity);
+        if (!ok) continue;
         unsigned char *sa = smem + s * kStageBytes;
         mbarArriveExpectTx(&full[s], G::kABytes + static_cast<uint32_t>(boxes * kThinBox * kRowBytes));
         if constexpr (G::kAMN) {
@@ -173,6 +174,16 @@ __global__ void __launch_bounds__(kThinThreads, 1)
           s = 0;
           parity ^= 1;
         }
+      }
+    }
+    // The last copies have landed and been read (productKernel).
+#pragma unroll 1
+    for (int j = 0; j < kStages; ++j) {
+      wait(&full[s], parity);
+      wait(&empty[s], parity);
+      if (++s == kStages) {
+        s = 0;
+        parity ^= 1;
       }
     }
   } else if (warp == 1 && electOne()) {
