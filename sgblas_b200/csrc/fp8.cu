@@ -198,8 +198,6 @@ cudaError_t launchQuantize(const QuantParams &p, int block_n, unsigned grid, cud
                       : cudaLaunchKernelEx(&cfg, quantizeBlocksKernel<T, kVector>, p);
 }
 
-bool isType(sgblasDataType_t type) { return type == SGBLAS_TYPE_FP32 || type == SGBLAS_TYPE_BF16; }
-
 sgblasStatus_t gemmFp8(sgblasHandle_t handle, int m, int n, int k, int groups, const int *offsets,
                        bool grouped, const void *a, int lda, long long stride_a,
                        const float *scale_a, int ldsa, long long stride_sa, const void *b, int ldb,

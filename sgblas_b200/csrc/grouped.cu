@@ -9,8 +9,6 @@ namespace {
 
 namespace t = kern::prod;
 
-bool isType(sgblasDataType_t type) { return type == SGBLAS_TYPE_FP32 || type == SGBLAS_TYPE_BF16; }
-
 }  // namespace
 }  // namespace sgblas::detail
 

@@ -188,7 +188,6 @@ cudaError_t launchWith(const void *kernel, dim3 grid, int threads, int smem, cud
   return cudaLaunchKernelExC(&cfg, kernel, args);
 }
 
-// p.m x p.n product of depth p.k over the batch; the epilogue is p.pair.out.
 // Tiles of one matrix.
 template <class G>
 long long pairTiles(int m, int n) {
@@ -196,6 +195,7 @@ long long pairTiles(int m, int n) {
   return G::kSymmetric ? t::symmetricTiles<G>(tm, tn) : static_cast<long long>(tm) * tn;
 }
 
+// p.m x p.n product of depth p.k over the batch; the epilogue is p.pair.out.
 template <class G>
 sgblasStatus_t launchPairTyped(const DeviceInfo &dev, int batch, const PairMatrix &a,
                                const PairMatrix &b, t::Params &p, cudaStream_t stream) {
@@ -317,9 +317,8 @@ extern "C" sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int 
                                               long long stride_o) {
   using namespace sgblas::detail;
   if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
-  if (m < 0 || n < 0 || batch < 0 || steps < 1 || steps > 32 ||
-      (gtype != SGBLAS_TYPE_FP32 && gtype != SGBLAS_TYPE_BF16) || ldg < std::max(1, m) ||
-      ldo < std::max(1, m))
+  if (m < 0 || n < 0 || batch < 0 || steps < 1 || steps > 32 || !isType(gtype) ||
+      ldg < std::max(1, m) || ldo < std::max(1, m))
     return SGBLAS_STATUS_INVALID_VALUE;
   if (m == 0 || n == 0 || batch == 0) return SGBLAS_STATUS_SUCCESS;
   if (coefficients == nullptr || g == nullptr || o == nullptr || !(eps >= 0.0F))

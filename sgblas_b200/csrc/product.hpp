@@ -18,6 +18,10 @@
 
 namespace sgblas::detail {
 
+inline bool isType(sgblasDataType_t type) {
+  return type == SGBLAS_TYPE_FP32 || type == SGBLAS_TYPE_BF16;
+}
+
 // An operand as it lies in memory: `count` matrices of `dim1` rows of `dim0`
 // contiguous elements, rows `ld` and matrices `stride` elements apart.
 struct NarrowOperand {
