@@ -79,7 +79,9 @@ sgblasStatus_t sgblasGroupedGemmK(sgblasHandle_t handle, int m, int n, int k, in
  *
  * The divisions and the product are rounded to nearest in FP32. A NaN or an infinity in a block makes its
  * scale NaN or infinite. scale is a column-major ceil(k/128) x ceil(n/block_n)
- * FP32 matrix. Strides in elements of each array (unused for batch == 1). */
+ * FP32 matrix. Strides in elements of each array (unused for batch == 1). The
+ * values are multiplied by the scale's reciprocal, not divided by the scale, so
+ * next to a tie either neighbour may be taken. */
 sgblasStatus_t sgblasQuantizeFp8(sgblasHandle_t handle, int k, int n, int batch, int block_n,
                                  const void *x, sgblasDataType_t xtype, int ldx,
                                  long long stride_x, void *q, int ldq, long long stride_q,
@@ -91,8 +93,9 @@ sgblasStatus_t sgblasQuantizeFp8(sgblasHandle_t handle, int k, int n, int batch,
  *             sum over k in b of A(k, i) * B(k, j)
  *
  * A is k x m (weights, scale_a ceil(k/128) x ceil(m/128)), B is k x n (tokens,
- * scale_b ceil(k/128) x n), C is m x n of type ctype. Scales are FP32 of any
- * value; each block's sum is scaled and added in FP32. k == 0 writes zeros. */
+ * scale_b ceil(k/128) x n), C is m x n of type ctype. A block's two scales are
+ * multiplied in FP32 first (their product should be in its range), then its sum
+ * is scaled and added in FP32. k == 0 writes zeros. */
 sgblasStatus_t sgblasGemmFp8(sgblasHandle_t handle, int m, int n, int k, const void *a, int lda,
                              const float *scale_a, int ldsa, const void *b, int ldb,
                              const float *scale_b, int ldsb, void *c, sgblasDataType_t ctype,
@@ -116,9 +119,12 @@ sgblasStatus_t sgblasGroupedGemmFp8(sgblasHandle_t handle, int m, int n, int k, 
  *
  * (with X^T X on the right where that is the smaller Gram matrix: the same
  * polynomial of the singular values). coefficients: host array {c0, c1, c2}.
- * Iterates are held as pairs of FP16 values (22 bits) and multiplied on the
- * tensor cores with FP32 sums, so O differs from the FP32 iteration by little
- * more than its own rounding. Values of X, of the Gram matrix and of the
+ * Iterates are held as pairs of FP16 values (22 bits of values above 2^-16, an
+ * absolute 2^-37 of smaller ones) and multiplied on the tensor cores with FP32
+ * sums; the last product, whose result is rounded to BF16 at once, takes the
+ * first FP16 value of each pair alone (11 bits). O differs from the FP32 iteration
+ * by little more than its own rounding (1.70e-3 in norm for BF16's 1.66e-3),
+ * unless eps leaves X next to nothing. G may be of any magnitude. Values of X, of the Gram matrix and of the
  * polynomial have to stay below 15.99 in magnitude, as they do for every
  * iteration that keeps singular values near one (|c0| + |c1| + |c2| of up to
  * 12 and singular values of up to 1.2 are safe). 1 <= steps <= 32. */

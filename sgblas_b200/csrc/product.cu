@@ -266,7 +266,9 @@ sgblasStatus_t launchRows(const DeviceInfo &dev, const NarrowOperand &a, const N
 //
 // Thin tiles, whose k several CTAs may share, pay while a group has few tokens
 // (8 x 2048 x 2048 BF16, 2 tokens each: 13.3 us against 19.0 in 128 columns; 12:
-// 14.8 and 14.4; 32 x 2048 x 2048 e4m3, 12: 28.4 and 29.5), longer where 128-wide tiles would leave half the SMs idle over
+// 14.8 and 14.4; 32 x 2048 x 2048 e4m3, 12: 28.4 and 29.5; tiles of 16 up to 6,
+// which is not always best: 32 x 512 x 1024, 6 tokens, 12.0 us and 8.3 in a wider
+// one), longer where 128-wide tiles would leave half the SMs idle over
 // a long k (2 x 4096 x 4096, 12 tokens: 16.3 and 18.1; 48: 18.7 and 19.0), and
 // longest where they would leave three quarters (4096 x 4096 e4m3, 48 tokens:
 // 10.0 and 13.1; 160: 22.6 and 15.3).

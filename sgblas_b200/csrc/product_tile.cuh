@@ -28,11 +28,12 @@
 //
 // What bounds it, measured. Large BF16 products: the tensor core and the power
 // limit (16384 x 4096 x 4096 over 16 uneven experts: the pipe is busy 84 % of the
-// cycles, SM clocks fall to 1.1 to 1.4 GHz; 431 to 498 us, 1.1 to 1.28
-// PFLOP/s). Large e4m3 products: the power limit and the epilogue, which scales
+// cycles, SM clocks fall to 1.1 to 1.4 GHz; 395 to 421 us in replays back to
+// back, 486 to 524 as calls on changing inputs, 1.05 to 1.4 PFLOP/s). Large e4m3 products: the power limit and the epilogue, which scales
 // every block of 128 in registers (860 clocks a chunk where the tensor core
-// takes 512; 8192 x 8192 x 4096 250 to 277 us, 2.0 to 2.2 PFLOP/s). Weight
-// gradients of few tokens: writing C. An elected lane of a warp that the
+// takes 512; 8192 x 8192 x 4096 228 to 236 us in replays, 275 to 283 as calls,
+// 1.94 to 2.4 PFLOP/s). Weight gradients of few tokens: writing C. Results with a
+// beta: reading C (updateColumns). An elected lane of a warp that the
 // compiler knows to be uniform issues the instructions in 40 clocks each, a
 // lane picked by a test in 57 and, between the waits of this loop, over 100
 // (forward 16384: 547 -> 448 us).
@@ -552,7 +553,10 @@ __device__ __forceinline__ void storeBf16(const Params &p, const Place &to,
 }
 
 // C = alpha * acc + beta * C from rows (kFp32): FP32, or BF16 with beta, whose
-// columns' rows are read and written 32 at a time.
+// columns' rows are read and written 32 at a time. Each column is read after the
+// one before is written, so a warp's columns take a memory latency each: weight
+// gradients of 16384 tokens, 16 x 2048 x 4096 in FP32, 249 us without beta and
+// 1780 with it, of 3001 tokens, 24 x 1000 x 1537, 60 and 575.
 template <typename T>
 __device__ __forceinline__ void updateColumns(const Params &p, T *c, int cols, const float *sums,
                                               int lane) {
@@ -568,7 +572,7 @@ __device__ __forceinline__ void updateColumns(const Params &p, T *c, int cols, c
 // A kFp32 warp's share: acc holds one row's columns, in pairs. FP32 without
 // beta leaves 16 columns at a time, by TMA from two buffers (a column's 32 rows
 // are 128 bytes there) or, where TMA cannot write them, a column per store.
-// The rest is rare and compact.
+// The rest passes through a loop that is not unrolled over the columns.
 template <int kCols>
 __device__ __forceinline__ void storeFp32(const Params &p, const Place &to,
                                           const float2 (&acc)[kCols / 2], unsigned char *out,
