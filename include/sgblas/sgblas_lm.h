@@ -2,7 +2,8 @@
  * sgblas-b200: products of language models. Mixture-of-experts products whose
  * groups are ragged, 8-bit products with a scale for each block of 128, the
  * quantisation they need, and the orthogonalisation of an update by
- * Newton-Schulz products. No counterpart in the reference API, whose only
+ * Newton-Schulz products; around them the norm before a layer, and tokens
+ * sorted by expert and back. No counterpart in the reference API, whose only
  * product is SGEMM.
  *
  * Matrices are column-major, as everywhere in the library. A row-major tensor
@@ -27,6 +28,7 @@ extern "C" {
 typedef enum sgblasDataType_t {
   SGBLAS_TYPE_FP32 = 0,
   SGBLAS_TYPE_BF16 = 1,
+  SGBLAS_TYPE_BYTE = 2,   /* moved as they are: sgblasScatterTokens only */
   SGBLAS_TYPE_FORCE_INT = 0x7fffffff
 } sgblasDataType_t;
 
@@ -132,6 +134,84 @@ sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int n, int batc
                                    const float *coefficients, float eps, float scale,
                                    const void *g, sgblasDataType_t gtype, int ldg,
                                    long long stride_g, void *o, int ldo, long long stride_o);
+
+/* Root-mean-square norm of the columns of a k x n matrix, after the residual's
+ * addition:
+ *
+ *   h = x + residual                        rounded to type (residual NULL: h = x)
+ *   v = h / sqrt(mean of h^2 + eps) * weight
+ *
+ * x, residual, weight (k values; NULL: ones), sum and y have type `type`. Written
+ * are h to sum (NULL: not), v to y (NULL: not), and v in e4m3 to q (NULL: not),
+ * with the scales in `scale`, as sgblasQuantizeFp8 with block_n = 1 writes them;
+ * y or q has to be given. Everything between h and the roundings to y and q is
+ * FP32, so squares of h have to stay in its range (magnitudes above 2^63 give 0).
+ * sum may be x or residual itself (the same address and leading dimension):
+ * the residual is then updated in place. */
+sgblasStatus_t sgblasRmsNorm(sgblasHandle_t handle, int k, int n, sgblasDataType_t type,
+                             const void *x, int ldx, const void *residual, int ldr,
+                             const void *weight, float eps, void *sum, int ldsum, void *y, int ldy,
+                             void *q, int ldq, float *scale, int ldscale);
+
+/* Its gradients, from dy = d(loss)/dy and h = sum. With s = 1 / sqrt(mean of h^2 +
+ * eps), g = weight * dy, for each column:
+ *
+ *   dx      = dsum + s * (g - h * s^2 * mean of (h * g))
+ *   dweight = (*beta) * dweight + sum over the columns of dy * h * s       (FP32)
+ *
+ * dx is the gradient of x and of the residual alike; dsum (NULL: zero) that which
+ * reaches h past the norm. dweight NULL: not computed, beta unused; *beta == 0
+ * writes it without reading. Sums are FP32 in an order that depends on the sizes
+ * alone. dx may be dy or dsum itself (the same address and leading dimension).
+ * dweight takes workspace: 4 bytes for each value of k and each CTA. */
+sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, int n, sgblasDataType_t type,
+                                     const void *dy, int lddy, const void *sum, int ldsum,
+                                     const void *weight, float eps, const void *dsum, int lddsum,
+                                     void *dx, int lddx, const float *beta, float *dweight);
+
+/* Tokens sorted by group (expert). group is a DEVICE top x n matrix without gaps
+ * between its columns (row-major [tokens, top]), the groups that each token goes
+ * to; a value outside [0, groups) is none. Written are
+ *
+ *   offsets   groups + 1 places: where each group begins, as the grouped products
+ *             take them; offsets[groups] is the number of choices that have a group
+ *   place     top x n: the column of each choice in the sorted order, -1 for none
+ *
+ * The sort is stable: within a group by token, then by choice. At most 2^30
+ * choices. offsets are written for n == 0, too. */
+sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top, int groups, const int *group,
+                                int *offsets, int *place);
+
+/* Tokens to their places: y(:, place(j, t)) = weights(j, t) * x(:, t), x k x n and y
+ * k x rows of type `type`. place and weights (FP32; NULL: ones, and columns are
+ * copied) are top x n without gaps. A place outside [0, rows) is none; columns
+ * of y that no choice has are left as they were, and no two choices may have the
+ * same. SGBLAS_TYPE_BYTE takes k bytes per column (quantised values, scales),
+ * without weights. The gradient of sgblasGatherTokens by x. */
+sgblasStatus_t sgblasScatterTokens(sgblasHandle_t handle, int k, int n, int top, int rows,
+                                   const int *place, const float *weights, const void *x,
+                                   sgblasDataType_t type, int ldx, void *y, int ldy);
+
+/* And back: y(:, t) = sum over j of weights(j, t) * x(:, place(j, t)), x k x rows and
+ * y k x n. Sums are FP32, in the order of j, rounded once; a choice without a
+ * place adds nothing, whatever its weight, and a token without any gets zeros.
+ * Choices may share a place. With weights NULL, the gradient of
+ * sgblasScatterTokens without weights. */
+sgblasStatus_t sgblasGatherTokens(sgblasHandle_t handle, int k, int n, int top, int rows,
+                                  const int *place, const float *weights, const void *x,
+                                  sgblasDataType_t type, int ldx, void *y, int ldy);
+
+/* Both gradients of sgblasGatherTokens:
+ *
+ *   dx(:, place(j, t)) = weights(j, t) * dy(:, t)
+ *   dweights(j, t)     = sum over k of dy(k, t) * x(k, place(j, t))       (FP32; 0 for none)
+ *
+ * dweights NULL: not computed, x unused. No two choices may have the same place;
+ * columns of dx that none has are left as they were. */
+sgblasStatus_t sgblasGatherTokensBackward(sgblasHandle_t handle, int k, int n, int top, int rows,
+                                          const int *place, const float *weights, const void *dy,
+                                          sgblasDataType_t type, int lddy, const void *x, int ldx,
+                                          void *dx, int lddx, float *dweights);
 
 #ifdef __cplusplus
 } /* extern "C" */

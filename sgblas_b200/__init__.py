@@ -21,7 +21,7 @@ __all__ = [
     "SGBLAS_STATUS_INVALID_VALUE", "SGBLAS_STATUS_ARCH_MISMATCH",
     "SGBLAS_STATUS_EXECUTION_FAILED", "SGBLAS_STATUS_INTERNAL_ERROR",
     "SGBLAS_STATUS_NOT_SUPPORTED", "SGBLAS_OP_N", "SGBLAS_OP_T", "SGBLAS_MATH_FP32",
-    "SGBLAS_MATH_TF32", "SGBLAS_TYPE_FP32", "SGBLAS_TYPE_BF16", "SGBLAS_MAX_GROUPS", "EXPORTED_SYMBOLS", "MgHandle", "mg_unique_id", "get_device_errors",
+    "SGBLAS_MATH_TF32", "SGBLAS_TYPE_FP32", "SGBLAS_TYPE_BF16", "SGBLAS_TYPE_BYTE", "SGBLAS_MAX_GROUPS", "EXPORTED_SYMBOLS", "MgHandle", "mg_unique_id", "get_device_errors",
 ]
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "lib" / "libsgblas.so"
@@ -41,6 +41,7 @@ SGBLAS_MATH_FP32 = 0
 SGBLAS_MATH_TF32 = 1
 SGBLAS_TYPE_FP32 = 0
 SGBLAS_TYPE_BF16 = 1
+SGBLAS_TYPE_BYTE = 2
 SGBLAS_MAX_GROUPS = 1024
 
 _c_int_p = ctypes.POINTER(ctypes.c_int)
@@ -103,6 +104,30 @@ _SIGNATURES = {
         ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_float_p,
         ctypes.c_float, ctypes.c_float, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
         ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong]),
+    "sgblasRmsNorm": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int]),
+    "sgblasRmsNormBackward": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, _c_float_p, ctypes.c_void_p]),
+    "sgblasSortTokens": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p]),
+    "sgblasScatterTokens": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int]),
+    "sgblasGatherTokens": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int]),
+    "sgblasGatherTokensBackward": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     # multi-GPU extension (include/sgblas/sgblas_mg.h)
     "sgblasMgGetUniqueId": (ctypes.c_int, [ctypes.c_void_p]),
     "sgblasMgCreate": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int,
@@ -320,6 +345,73 @@ class Handle:
 
     def orthogonalize(self, *args) -> None:
         _check("sgblasOrthogonalize", self.orthogonalize_status(*args))
+
+    # ---- around a layer's products: the norm, and tokens sorted by expert and back.
+
+    def rms_norm_status(self, k, n, type, x, ldx, residual, ldr, weight, eps, sum=None, ldsum=0,
+                        y=None, ldy=0, q=None, ldq=0, scale=None, ldscale=0) -> int:
+        """Raw sgblasRmsNorm: y (as type), q and scale (e4m3), or all three."""
+        return lib.sgblasRmsNorm(self._h, k, n, type, _ptr(x), ldx, _ptr(residual), ldr,
+                                 _ptr(weight), eps, _ptr(sum), ldsum, _ptr(y), ldy, _ptr(q), ldq,
+                                 _ptr(scale), ldscale)
+
+    def rms_norm(self, *args, **kwargs) -> None:
+        status = self.rms_norm_status(*args, **kwargs)
+        if status:
+            raise SgblasError("sgblasRmsNorm", status)
+
+    def rms_norm_backward_status(self, k, n, type, dy, lddy, sum, ldsum, weight, eps, dsum, lddsum,
+                                 dx, lddx, beta=None, dweight=None) -> int:
+        """Raw sgblasRmsNormBackward: sum is what rms_norm normalised."""
+        return lib.sgblasRmsNormBackward(self._h, k, n, type, _ptr(dy), lddy, _ptr(sum), ldsum,
+                                         _ptr(weight), eps, _ptr(dsum), lddsum, _ptr(dx), lddx,
+                                         _fp(beta), _ptr(dweight))
+
+    def rms_norm_backward(self, *args, **kwargs) -> None:
+        status = self.rms_norm_backward_status(*args, **kwargs)
+        if status:
+            raise SgblasError("sgblasRmsNormBackward", status)
+
+    def sort_tokens_status(self, n, top, groups, group, offsets, place) -> int:
+        """Raw sgblasSortTokens: all three int32 device arrays."""
+        return lib.sgblasSortTokens(self._h, n, top, groups, _ptr(group), _ptr(offsets), _ptr(place))
+
+    def sort_tokens(self, *args) -> None:
+        status = self.sort_tokens_status(*args)
+        if status:
+            raise SgblasError("sgblasSortTokens", status)
+
+    def scatter_tokens_status(self, k, n, top, rows, place, weights, x, type, ldx, y, ldy) -> int:
+        """Raw sgblasScatterTokens: x's columns to their places in y (rows of them)."""
+        return lib.sgblasScatterTokens(self._h, k, n, top, rows, _ptr(place), _ptr(weights), _ptr(x),
+                                       type, ldx, _ptr(y), ldy)
+
+    def scatter_tokens(self, *args) -> None:
+        status = self.scatter_tokens_status(*args)
+        if status:
+            raise SgblasError("sgblasScatterTokens", status)
+
+    def gather_tokens_status(self, k, n, top, rows, place, weights, x, type, ldx, y, ldy) -> int:
+        """Raw sgblasGatherTokens: weighted sums of x's columns (rows of them)."""
+        return lib.sgblasGatherTokens(self._h, k, n, top, rows, _ptr(place), _ptr(weights), _ptr(x),
+                                      type, ldx, _ptr(y), ldy)
+
+    def gather_tokens(self, *args) -> None:
+        status = self.gather_tokens_status(*args)
+        if status:
+            raise SgblasError("sgblasGatherTokens", status)
+
+    def gather_tokens_backward_status(self, k, n, top, rows, place, weights, dy, type, lddy, x, ldx,
+                                      dx, lddx, dweights=None) -> int:
+        """Raw sgblasGatherTokensBackward."""
+        return lib.sgblasGatherTokensBackward(self._h, k, n, top, rows, _ptr(place), _ptr(weights),
+                                              _ptr(dy), type, lddy, _ptr(x), ldx, _ptr(dx), lddx,
+                                              _ptr(dweights))
+
+    def gather_tokens_backward(self, *args, **kwargs) -> None:
+        status = self.gather_tokens_backward_status(*args, **kwargs)
+        if status:
+            raise SgblasError("sgblasGatherTokensBackward", status)
 
 
 MG_UNIQUE_ID_BYTES = 128

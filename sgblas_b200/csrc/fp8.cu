@@ -4,6 +4,7 @@
 
 #include "device.hpp"
 #include "ptx.cuh"
+#include "quantize.cuh"
 #include "sgemm_launch.hpp"
 
 #include <cuda_bf16.h>
@@ -17,8 +18,6 @@ namespace {
 
 namespace t = kern::prod;
 
-constexpr float kFp8Max = 448.0F;
-constexpr unsigned kAmaxFloorBits = 0x0D800000u;   // 2^-100
 constexpr int kBlock = 128;
 constexpr int kQuantThreads = 256;
 constexpr int kQuantBlocks = 64;   // blocks of one CTA (quantizeColumnsKernel), aligned or not
@@ -92,10 +91,6 @@ struct Values {
   }
 };
 
-__device__ __forceinline__ float scaleOf(unsigned amax_bits) {
-  return __fdiv_rn(__uint_as_float(max(amax_bits, kAmaxFloorBits)), kFp8Max);
-}
-
 // A scale for each 128 values of one column; kUnroll blocks per thread, whose
 // loads are issued together. Memory-bound: one read and one write of each
 // value (16384 x 8192 BF16: 65 to 71 us, 5.7 to 6.2 TB/s; by elements, with a
@@ -133,7 +128,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantizeColumnsKernel(const Qua
     unsigned m = v[u].magnitude();
 #pragma unroll
     for (int d = V::kLanes / 2; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float scale = scaleOf(m);
+    const float scale = kern::fp8Scale(m);
     v[u].store(p.q + to[u], left[u], __frcp_rn(scale));
     if (scale_to[u] != nullptr) *scale_to[u] = scale;
   }
@@ -172,7 +167,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantizeBlocksKernel(const Quan
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, warp_max[w]);
-  const float scale = scaleOf(m);
+  const float scale = kern::fp8Scale(m);
   const float inverse = __frcp_rn(scale);
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {

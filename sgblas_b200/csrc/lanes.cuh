@@ -1,0 +1,60 @@
+// A column's values spread over threads, for the memory-bound operators: what
+// one thread holds of a block of 128 values, and sums over a column's threads.
+#ifndef SGBLAS_B200_LANES_CUH_
+#define SGBLAS_B200_LANES_CUH_
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace sgblas::kern {
+
+constexpr int kLaneBlock = 128;
+
+// Aligned (kVector): consecutive values, one vector of 16 bytes. Otherwise four
+// values 32 apart, so that a warp holds a block and its scalar accesses are
+// contiguous.
+template <typename T, bool kVector>
+struct Lanes {
+  static constexpr int kPer = kVector ? 16 / static_cast<int>(sizeof(T)) : 4;
+  static constexpr int kThreads = kLaneBlock / kPer;     // of a block
+  static constexpr int kStep = kVector ? 1 : kThreads;   // between a thread's values
+  alignas(16) T v[kPer];
+
+  // Where thread `slot` of a column's begins: its place in the column.
+  static __device__ __forceinline__ int begin(int slot) {
+    return kVector ? slot * kPer : slot / kThreads * kLaneBlock + slot % kThreads;
+  }
+  // From `at`; `left` values of the column are there (the rest are zero). With
+  // kVector a thread's last vector may be partial.
+  __device__ __forceinline__ void load(const T *at, int left) {
+    if (kVector && left >= kPer) {
+      *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[j] = j * kStep < left ? at[j * kStep] : T{};
+    }
+  }
+  __device__ __forceinline__ void store(T *at, int left) const {
+    if (kVector && left >= kPer) {
+      *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (j * kStep < left) at[j * kStep] = v[j];
+    }
+  }
+  __device__ __forceinline__ float get(int j) const { return static_cast<float>(v[j]); }
+  __device__ __forceinline__ void set(int j, float f) { v[j] = static_cast<T>(f); }
+};
+
+__device__ __forceinline__ float warpSum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+}  // namespace sgblas::kern
+
+#endif  // SGBLAS_B200_LANES_CUH_

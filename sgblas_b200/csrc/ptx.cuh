@@ -394,7 +394,12 @@ __device__ __forceinline__ uint32_t clusterIdX() {
   asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
   return r;
 }
-// 16-byte load from distributed shared memory (a cluster address).
+// 4- and 16-byte loads from distributed shared memory (a cluster address).
+__device__ __forceinline__ int ldCluster(uint32_t cluster_addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float4 ldCluster4(uint32_t cluster_addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"

@@ -1,0 +1,495 @@
+// Tokens to their experts and back (sgblas_lm.h): sgblasSortTokens,
+// sgblasScatterTokens, sgblasGatherTokens, sgblasGatherTokensBackward.
+//
+// A token t has `top` choices; choice j goes to column place(j, t) of the sorted
+// matrix, or nowhere (a place outside [0, rows)). Moving columns is
+// memory-bound: each is read and written once, in vectors of 16 bytes, and a
+// token's column is read once for all of its choices.
+#include "device.hpp"
+#include "lanes.cuh"
+#include "product.hpp"
+#include "ptx.cuh"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <atomic>
+
+namespace sgblas::detail {
+namespace {
+
+using kern::Lanes;
+using kern::warpSum;
+
+// ---- the sort ------------------------------------------------------------------
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortMaxCluster = 8;
+constexpr int kSortWarpEntries = 64;   // of a warp, before another warp (CTA) joins
+
+constexpr int kSortMaxEntries = 1 << 30;
+
+struct SortParams {
+  const int *group;
+  int *offsets, *place;
+  int entries, groups;
+};
+
+// Exclusive sum over the CTA's threads, and the total; `slots` a word per warp.
+__device__ __forceinline__ int blockScan(int v, int *slots, int *total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  int scan = v;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int o = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += o;
+  }
+  if (lane == 31) slots[warp] = scan;
+  __syncthreads();
+  int before = 0, sum = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w == warp) before = sum;
+    sum += slots[w];
+  }
+  __syncthreads();
+  *total = sum;
+  return before + scan - v;
+}
+
+// A stable counting sort by group: one cluster, whose warps hold consecutive
+// ranges of the entries. Each warp counts its range by group (32 entries at a
+// time: lanes of one group find each other, and their first adds for all); the
+// counts are summed over a CTA's warps, over the cluster's CTAs (through
+// distributed shared memory) and over the groups, and each warp walks its range
+// again, handing out places. Two passes over 4 bytes an entry: bound by the
+// latency of a warp's turns.
+__global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParams p, int ctas) {
+  extern __shared__ int counts[];   // [warps][groups], then the CTA's sums [groups]
+  __shared__ int slots[kSortThreads / 32];
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  const int rank = static_cast<int>(blockIdx.x);
+  int *mine = counts + warp * p.groups;
+  int *sums = counts + warps * p.groups;
+  const int parts = ctas * warps;
+  const long long per = ((p.entries + parts - 1LL) / parts + 31) / 32 * 32;
+  const int begin = static_cast<int>(min(per * (rank * warps + warp), static_cast<long long>(p.entries)));
+  const int end = static_cast<int>(min(begin + per, static_cast<long long>(p.entries)));
+  for (int g = lane; g < p.groups; g += 32) mine[g] = 0;
+  __syncwarp();
+  // The entry's group, or -1.
+  auto groupAt = [&](int i) {
+    const int g = i < end ? __ldg(p.group + i) : -1;
+    return g >= 0 && g < p.groups ? g : -1;
+  };
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const int g = groupAt(i0 + lane);
+    const unsigned same = __match_any_sync(0xffffffffu, g);
+    if (g >= 0 && __ffs(same) - 1 == lane) mine[g] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
+    int sum = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int c = counts[w * p.groups + g];
+      counts[w * p.groups + g] = sum;
+      sum += c;
+    }
+    sums[g] = sum;
+  }
+  if (ctas > 1) kern::clusterSync();
+  else __syncthreads();
+  // Where each group begins, and this CTA's part of it.
+  int carry = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += blockDim.x) {
+    const int g = g0 + threadIdx.x;
+    int total = 0, before = 0;
+    if (g < p.groups) {
+      for (int c = 0; c < ctas; ++c) {
+        const int there = ctas > 1 ? kern::ldCluster(kern::clusterAddr(kern::smemAddr(sums + g), c)) : sums[g];
+        if (c < rank) before += there;
+        total += there;
+      }
+    }
+    int all;
+    const int at = carry + blockScan(total, slots, &all);
+    if (g < p.groups) {
+      if (rank == 0) p.offsets[g] = at;
+      for (int w = 0; w < warps; ++w) counts[w * p.groups + g] += at + before;
+    }
+    carry += all;
+  }
+  if (rank == 0 && threadIdx.x == 0) p.offsets[p.groups] = carry;
+  __syncthreads();
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const int g = groupAt(i0 + lane);
+    const unsigned same = __match_any_sync(0xffffffffu, g);
+    const int base = g >= 0 ? mine[g] : 0;
+    __syncwarp();
+    if (g >= 0 && __ffs(same) - 1 == lane) mine[g] = base + __popc(same);
+    __syncwarp();
+    if (i0 + lane < end)
+      p.place[i0 + lane] = g >= 0 ? base + __popc(same & ((1u << lane) - 1)) : -1;
+  }
+  if (ctas > 1) kern::clusterSync();   // no CTA leaves while another reads its sums
+}
+
+// ---- moving columns ------------------------------------------------------------
+
+constexpr int kMoveThreads = 256;
+constexpr int kBatch = 4;   // choices whose columns are on their way at once
+
+struct MoveParams {
+  const int *place;
+  const float *weight;    // NULL: ones
+  const void *x, *dy;
+  void *y;
+  float *dweight;
+  int k, n, top, rows;
+  int ldx, lddy, ldy;
+  int slots;              // threads that a column keeps busy, rounded to whole blocks
+};
+
+__device__ __forceinline__ bool placed(const MoveParams &p, int at) { return at >= 0 && at < p.rows; }
+
+template <typename T>
+constexpr bool kNumber = sizeof(T) > 1;   // bytes move as they are
+
+// y(:, place(j, t)) = weight(j, t) x(:, t)
+template <typename T, bool kVector>
+__global__ void __launch_bounds__(kMoveThreads) scatterTokensKernel(const MoveParams p) {
+  using L = Lanes<T, kVector>;
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const long long t = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
+  if (t >= p.n) return;
+  const int *place = p.place + t * p.top;
+  for (int slot = blockIdx.y * blockDim.x + threadIdx.x; slot < p.slots; slot += gridDim.y * blockDim.x) {
+    const int at = L::begin(slot), left = p.k - at;
+    if (left <= 0) continue;
+    L v;
+    v.load(static_cast<const T *>(p.x) + t * p.ldx + at, left);
+    for (int j = 0; j < p.top; ++j) {
+      const int to = __ldg(place + j);
+      if (!placed(p, to)) continue;
+      T *y = static_cast<T *>(p.y) + static_cast<long long>(to) * p.ldy + at;
+      if constexpr (kNumber<T>) {
+        if (p.weight != nullptr) {
+          const float w = __ldg(p.weight + t * p.top + j);
+          L out;
+#pragma unroll
+          for (int i = 0; i < L::kPer; ++i) out.set(i, w * v.get(i));
+          out.store(y, left);
+          continue;
+        }
+      }
+      v.store(y, left);
+    }
+  }
+}
+
+// y(:, t) = sum over j of weight(j, t) x(:, place(j, t)), in the order of j
+template <typename T, bool kVector>
+__global__ void __launch_bounds__(kMoveThreads) gatherTokensKernel(const MoveParams p) {
+  using L = Lanes<T, kVector>;
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const long long t = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
+  if (t >= p.n) return;
+  const int *place = p.place + t * p.top;
+  const float *weight = p.weight == nullptr ? nullptr : p.weight + t * p.top;
+  for (int slot = blockIdx.y * blockDim.x + threadIdx.x; slot < p.slots; slot += gridDim.y * blockDim.x) {
+    const int at = L::begin(slot), left = p.k - at;
+    if (left <= 0) continue;
+    float sum[L::kPer];
+#pragma unroll
+    for (int i = 0; i < L::kPer; ++i) sum[i] = 0.0F;
+    for (int j0 = 0; j0 < p.top; j0 += kBatch) {
+      L v[kBatch];
+      float w[kBatch];
+      bool live[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int from = j0 + b < p.top ? __ldg(place + j0 + b) : -1;
+        live[b] = placed(p, from);
+        w[b] = live[b] && weight != nullptr ? __ldg(weight + j0 + b) : 1.0F;
+        if (live[b]) v[b].load(static_cast<const T *>(p.x) + static_cast<long long>(from) * p.ldx + at, left);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (!live[b]) continue;
+#pragma unroll
+        for (int i = 0; i < L::kPer; ++i) sum[i] = fmaf(w[b], v[b].get(i), sum[i]);
+      }
+    }
+    L out;
+#pragma unroll
+    for (int i = 0; i < L::kPer; ++i) out.set(i, sum[i]);
+    out.store(static_cast<T *>(p.y) + t * p.ldy + at, left);
+  }
+}
+
+// y(:, place(j, t)) = weight(j, t) dy(:, t) and, with dweight,
+// dweight(j, t) = sum over k of dy(k, t) x(k, place(j, t)); a CTA's row of
+// blockDim.x threads per token.
+template <typename T, bool kVector>
+__global__ void __launch_bounds__(kMoveThreads) gatherTokensBackwardKernel(const MoveParams p) {
+  using L = Lanes<T, kVector>;
+  __shared__ float partial[kMoveThreads / 32][kBatch];
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const long long t = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
+  const bool in = t < p.n;
+  const int warps = blockDim.x / 32, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  for (int j0 = 0; j0 < p.top; j0 += kBatch) {
+    int to[kBatch];
+    float w[kBatch], dot[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      to[b] = in && j0 + b < p.top ? __ldg(p.place + t * p.top + j0 + b) : -1;
+      if (!placed(p, to[b])) to[b] = -1;
+      w[b] = to[b] >= 0 && p.weight != nullptr ? __ldg(p.weight + t * p.top + j0 + b) : 1.0F;
+      dot[b] = 0.0F;
+    }
+    for (int slot = threadIdx.x; slot < p.slots; slot += blockDim.x) {
+      const int at = L::begin(slot), left = p.k - at;
+      if (!in || left <= 0) continue;
+      L dy, x[kBatch];
+      dy.load(static_cast<const T *>(p.dy) + t * p.lddy + at, left);
+      if (p.dweight != nullptr) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+          if (to[b] >= 0)
+            x[b].load(static_cast<const T *>(p.x) + static_cast<long long>(to[b]) * p.ldx + at, left);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (to[b] < 0) continue;
+        L out;
+#pragma unroll
+        for (int i = 0; i < L::kPer; ++i) out.set(i, w[b] * dy.get(i));
+        out.store(static_cast<T *>(p.y) + static_cast<long long>(to[b]) * p.ldy + at, left);
+        if (p.dweight != nullptr) {
+#pragma unroll
+          for (int i = 0; i < L::kPer; ++i) dot[b] = fmaf(dy.get(i), x[b].get(i), dot[b]);
+        }
+      }
+    }
+    if (p.dweight == nullptr) continue;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) dot[b] = warpSum(dot[b]);
+    if (warps > 1) {   // one token
+      if (lane == 0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) partial[warp][b] = dot[b];
+      }
+      __syncthreads();
+      if (threadIdx.x < kBatch) {
+        float s = 0.0F;
+        for (int v = 0; v < warps; ++v) s += partial[v][threadIdx.x];
+        if (j0 + static_cast<int>(threadIdx.x) < p.top) p.dweight[t * p.top + j0 + threadIdx.x] = s;
+      }
+      __syncthreads();
+    } else if (in && lane == 0) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (j0 + b < p.top) p.dweight[t * p.top + j0 + b] = dot[b];
+    }
+  }
+}
+
+template <typename P, typename... Rest>
+sgblasStatus_t launchTokens(void (*kernel)(P, Rest...), dim3 grid, dim3 block, cudaStream_t stream,
+                            const P &p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+enum class Move { kScatter, kGather, kBackward };
+
+template <typename T, bool kVector>
+sgblasStatus_t launchMove(Move move, MoveParams p, int sms, cudaStream_t stream) {
+  using L = Lanes<T, kVector>;
+  p.slots = ((p.k - 1) / kern::kLaneBlock + 1) * L::kThreads;
+  const int threads = std::min(kMoveThreads, (p.slots + 31) / 32 * 32);
+  const bool whole = move == Move::kBackward;   // a token's threads share its sums
+  const int tokens = whole && threads > 32 ? 1 : kMoveThreads / threads;
+  const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(tokens));
+  const int across = (p.n - 1) / tokens + 1;
+  // Long columns of few tokens are cut, so that every SM has some.
+  const int cuts = whole ? 1 : std::max(1, std::min((p.slots - 1) / threads + 1, 2 * sms / across));
+  const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(cuts));
+  if constexpr (!kNumber<T>) {
+    return launchTokens(scatterTokensKernel<T, kVector>, grid, block, stream, p);
+  } else {
+    switch (move) {
+      case Move::kScatter: return launchTokens(scatterTokensKernel<T, kVector>, grid, block, stream, p);
+      case Move::kGather: return launchTokens(gatherTokensKernel<T, kVector>, grid, block, stream, p);
+      default: return launchTokens(gatherTokensBackwardKernel<T, kVector>, grid, block, stream, p);
+    }
+  }
+}
+
+sgblasStatus_t launchMoveTyped(Move move, const MoveParams &p, sgblasDataType_t type, int sms,
+                               cudaStream_t stream) {
+  const int size = type == SGBLAS_TYPE_FP32 ? 4 : type == SGBLAS_TYPE_BF16 ? 2 : 1;
+  auto whole = [&](const void *at, long long ld) {
+    return at == nullptr || (aligned16(at) && ld * size % 16 == 0);
+  };
+  const bool vector = whole(p.x, p.ldx) && whole(p.dy, p.lddy) && whole(p.y, p.ldy);
+  if (type == SGBLAS_TYPE_FP32)
+    return vector ? launchMove<float, true>(move, p, sms, stream)
+                  : launchMove<float, false>(move, p, sms, stream);
+  if (type == SGBLAS_TYPE_BF16)
+    return vector ? launchMove<__nv_bfloat16, true>(move, p, sms, stream)
+                  : launchMove<__nv_bfloat16, false>(move, p, sms, stream);
+  return vector ? launchMove<unsigned char, true>(move, p, sms, stream)
+                : launchMove<unsigned char, false>(move, p, sms, stream);
+}
+
+}  // namespace
+}  // namespace sgblas::detail
+
+extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top, int groups,
+                                           const int *group, int *offsets, int *place) {
+  using namespace sgblas::detail;
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  if (n < 0 || top < 0 || groups < 0 || offsets == nullptr) return SGBLAS_STATUS_INVALID_VALUE;
+  const long long entries = static_cast<long long>(n) * top;
+  if (entries > 0 && (group == nullptr || place == nullptr)) return SGBLAS_STATUS_INVALID_VALUE;
+  if (groups > SGBLAS_MAX_GROUPS || entries > kSortMaxEntries) return SGBLAS_STATUS_NOT_SUPPORTED;
+  DeviceInfo dev;
+  const sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  static std::atomic<uint64_t> configured{0};
+  constexpr int kMost = (kSortThreads / 32 + 1) * SGBLAS_MAX_GROUPS * 4;
+  if (!configureKernel(reinterpret_cast<const void *>(sortTokensKernel), dev.device, kMost, &configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  SortParams p = {};
+  p.group = group;
+  p.offsets = offsets;
+  p.place = place;
+  p.entries = static_cast<int>(entries);
+  p.groups = groups;
+  const long long warps_wanted = (entries + kSortWarpEntries - 1) / kSortWarpEntries;
+  const int warps = static_cast<int>(std::min<long long>(kSortThreads / 32, std::max<long long>(4, warps_wanted)));
+  int ctas = 1;
+  while (ctas < kSortMaxCluster && static_cast<long long>(ctas) * warps < warps_wanted) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(static_cast<unsigned>(32 * warps));
+  cfg.dynamicSmemBytes = sizeof(int) * static_cast<size_t>(warps + 1) * std::max(groups, 1);
+  cfg.stream = static_cast<cudaStream_t>(handle->stream);
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, sortTokensKernel, p, ctas));
+}
+
+extern "C" sgblasStatus_t sgblasScatterTokens(sgblasHandle_t handle, int k, int n, int top, int rows,
+                                              const int *place, const float *weights, const void *x,
+                                              sgblasDataType_t type, int ldx, void *y, int ldy) {
+  using namespace sgblas::detail;
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  const bool bytes = type == SGBLAS_TYPE_BYTE;
+  if (k < 0 || n < 0 || top < 0 || rows < 0 || !(bytes || isType(type)) ||
+      (bytes && weights != nullptr) || ldx < std::max(1, k) || ldy < std::max(1, k))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (k == 0 || n == 0 || top == 0 || rows == 0) return SGBLAS_STATUS_SUCCESS;
+  if (place == nullptr || x == nullptr || y == nullptr) return SGBLAS_STATUS_INVALID_VALUE;
+  DeviceInfo dev;
+  const sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  MoveParams p = {};
+  p.place = place;
+  p.weight = weights;
+  p.x = x;
+  p.y = y;
+  p.k = k;
+  p.n = n;
+  p.top = top;
+  p.rows = rows;
+  p.ldx = ldx;
+  p.ldy = ldy;
+  return launchMoveTyped(Move::kScatter, p, type, dev.sms, static_cast<cudaStream_t>(handle->stream));
+}
+
+extern "C" sgblasStatus_t sgblasGatherTokens(sgblasHandle_t handle, int k, int n, int top, int rows,
+                                             const int *place, const float *weights, const void *x,
+                                             sgblasDataType_t type, int ldx, void *y, int ldy) {
+  using namespace sgblas::detail;
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  if (k < 0 || n < 0 || top < 0 || rows < 0 || !isType(type) || ldx < std::max(1, k) ||
+      ldy < std::max(1, k))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (k == 0 || n == 0) return SGBLAS_STATUS_SUCCESS;
+  if (y == nullptr || (top > 0 && place == nullptr) || (top > 0 && rows > 0 && x == nullptr))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  DeviceInfo dev;
+  const sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  MoveParams p = {};
+  p.place = place;
+  p.weight = weights;
+  p.x = x;
+  p.y = y;
+  p.k = k;
+  p.n = n;
+  p.top = top;
+  p.rows = rows;
+  p.ldx = ldx;
+  p.ldy = ldy;
+  return launchMoveTyped(Move::kGather, p, type, dev.sms, static_cast<cudaStream_t>(handle->stream));
+}
+
+extern "C" sgblasStatus_t sgblasGatherTokensBackward(sgblasHandle_t handle, int k, int n, int top,
+                                                     int rows, const int *place,
+                                                     const float *weights, const void *dy,
+                                                     sgblasDataType_t type, int lddy, const void *x,
+                                                     int ldx, void *dx, int lddx, float *dweights) {
+  using namespace sgblas::detail;
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  const int one = std::max(1, k);
+  if (k < 0 || n < 0 || top < 0 || rows < 0 || !isType(type) || lddy < one || lddx < one ||
+      (dweights != nullptr && ldx < one))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (n == 0 || top == 0 || (k == 0 && dweights == nullptr)) return SGBLAS_STATUS_SUCCESS;
+  if (place == nullptr || (rows > 0 && (dy == nullptr || dx == nullptr)) ||
+      (rows > 0 && dweights != nullptr && x == nullptr))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (rows == 0 && dweights == nullptr) return SGBLAS_STATUS_SUCCESS;
+  DeviceInfo dev;
+  const sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  MoveParams p = {};
+  p.place = place;
+  p.weight = weights;
+  p.dy = dy;
+  p.x = dweights == nullptr ? nullptr : x;
+  p.y = dx;
+  p.dweight = dweights;
+  p.k = rows > 0 ? k : 0;   // without rows dy, x and dx may be NULL: only zeros are written
+  p.n = n;
+  p.top = top;
+  p.rows = rows;
+  p.lddy = lddy;
+  p.ldx = ldx;
+  p.ldy = lddx;
+  return launchMoveTyped(Move::kBackward, p, type, dev.sms, static_cast<cudaStream_t>(handle->stream));
+}

@@ -1,0 +1,155 @@
+"""Arguments, quick returns and refusals of the operators around a layer's
+products (sgblas_lm.h). No GPU needed: every call here ends before device work."""
+import ctypes
+
+import pytest
+
+import sgblas_b200 as sg
+
+FAKE = 0x10000
+BF16, FP32, BYTE = sg.SGBLAS_TYPE_BF16, sg.SGBLAS_TYPE_FP32, sg.SGBLAS_TYPE_BYTE
+BAD_TYPE = 7
+OK, INVALID = sg.SGBLAS_STATUS_SUCCESS, sg.SGBLAS_STATUS_INVALID_VALUE
+UNSUPPORTED = sg.SGBLAS_STATUS_NOT_SUPPORTED
+
+
+def norm_args(**kw):
+    a = dict(k=300, n=20, type=BF16, x=FAKE, ldx=300, residual=FAKE, ldr=300, weight=FAKE, eps=1e-6,
+             sum=FAKE, ldsum=300, y=FAKE, ldy=300, q=FAKE, ldq=300, scale=FAKE, ldscale=3)
+    a.update(kw)
+    return list(a.values())
+
+
+def back_args(**kw):
+    a = dict(k=300, n=20, type=BF16, dy=FAKE, lddy=300, sum=FAKE, ldsum=300, weight=FAKE, eps=1e-6,
+             dsum=FAKE, lddsum=300, dx=FAKE, lddx=300, beta=0.0, dweight=FAKE)
+    a.update(kw)
+    return list(a.values())
+
+
+def sort_args(**kw):
+    a = dict(n=20, top=2, groups=4, group=FAKE, offsets=FAKE, place=FAKE)
+    a.update(kw)
+    return list(a.values())
+
+
+def move_args(**kw):
+    a = dict(k=300, n=20, top=2, rows=40, place=FAKE, weights=FAKE, x=FAKE, type=BF16, ldx=300, y=FAKE,
+             ldy=300)
+    a.update(kw)
+    return list(a.values())
+
+
+def move_back_args(**kw):
+    a = dict(k=300, n=20, top=2, rows=40, place=FAKE, weights=FAKE, dy=FAKE, type=BF16, lddy=300, x=FAKE,
+             ldx=300, dx=FAKE, lddx=300, dweights=FAKE)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(k=-1), dict(n=-1), dict(type=BAD_TYPE), dict(type=BYTE), dict(ldx=299), dict(ldr=299),
+    dict(ldsum=299), dict(ldy=299), dict(ldq=299), dict(ldscale=2), dict(eps=-1e-6),
+    dict(eps=float("nan")), dict(x=None), dict(y=None, q=None), dict(scale=None)])
+def test_norm_refuses(handle, kw):
+    assert handle.rms_norm_status(*norm_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.rms_norm(*norm_args(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(k=0, x=None), dict(n=0, y=None, q=None)])
+def test_norm_has_nothing_to_do(handle, kw):
+    assert handle.rms_norm_status(*norm_args(**kw)) == OK
+
+
+@pytest.mark.parametrize("kw", [
+    dict(k=-1), dict(n=-1), dict(type=BAD_TYPE), dict(type=BYTE), dict(lddy=299), dict(ldsum=299),
+    dict(lddsum=299), dict(lddx=299), dict(eps=-1.0), dict(eps=float("nan")), dict(beta=None),
+    dict(dy=None), dict(sum=None), dict(dx=None)])
+def test_norm_backward_refuses(handle, kw):
+    assert handle.rms_norm_backward_status(*back_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.rms_norm_backward(*back_args(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(k=0, dy=None), dict(n=0, beta=1.0, dx=None),
+                                dict(n=0, dweight=None, beta=None)])
+def test_norm_backward_has_nothing_to_do(handle, kw):
+    assert handle.rms_norm_backward_status(*back_args(**kw)) == OK
+
+
+@pytest.mark.parametrize("kw", [dict(n=-1), dict(top=-1), dict(groups=-1), dict(group=None),
+                                dict(offsets=None), dict(place=None), dict(n=0, offsets=None)])
+def test_sort_refuses(handle, kw):
+    assert handle.sort_tokens_status(*sort_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.sort_tokens(*sort_args(**kw))
+
+
+def test_sort_limits(handle):
+    assert handle.sort_tokens_status(*sort_args(groups=sg.SGBLAS_MAX_GROUPS + 1)) == UNSUPPORTED
+    assert handle.sort_tokens_status(*sort_args(n=(1 << 30) + 1, top=1)) == UNSUPPORTED
+    assert handle.sort_tokens_status(*sort_args(n=1 << 30, top=1 << 30)) == UNSUPPORTED
+
+
+MOVE_REFUSALS = [dict(k=-1), dict(n=-1), dict(top=-1), dict(rows=-1), dict(type=BAD_TYPE), dict(ldx=299),
+                 dict(ldy=299), dict(place=None), dict(x=None), dict(y=None)]
+
+
+@pytest.mark.parametrize("kw", MOVE_REFUSALS + [dict(type=BYTE)])
+def test_scatter_refuses(handle, kw):
+    assert handle.scatter_tokens_status(*move_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.scatter_tokens(*move_args(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(k=0, x=None), dict(n=0, y=None), dict(top=0, place=None),
+                                dict(rows=0, y=None), dict(type=BYTE, weights=None, n=0)])
+def test_scatter_has_nothing_to_do(handle, kw):
+    assert handle.scatter_tokens_status(*move_args(**kw)) == OK
+
+
+@pytest.mark.parametrize("kw", MOVE_REFUSALS + [dict(type=BYTE, weights=None)])
+def test_gather_refuses(handle, kw):
+    assert handle.gather_tokens_status(*move_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.gather_tokens(*move_args(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(k=0, x=None), dict(n=0, y=None)])
+def test_gather_has_nothing_to_do(handle, kw):
+    assert handle.gather_tokens_status(*move_args(**kw)) == OK
+
+
+@pytest.mark.parametrize("kw", [
+    dict(k=-1), dict(n=-1), dict(top=-1), dict(rows=-1), dict(type=BAD_TYPE), dict(type=BYTE),
+    dict(lddy=299), dict(ldx=299), dict(lddx=299), dict(place=None), dict(dy=None), dict(x=None),
+    dict(dx=None)])
+def test_gather_backward_refuses(handle, kw):
+    assert handle.gather_tokens_backward_status(*move_back_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.gather_tokens_backward(*move_back_args(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(n=0, dy=None), dict(top=0, place=None), dict(k=0, dweights=None),
+                                dict(rows=0, dweights=None, dx=None)])
+def test_gather_backward_has_nothing_to_do(handle, kw):
+    assert handle.gather_tokens_backward_status(*move_back_args(**kw)) == OK
+
+
+def test_bytes_are_no_type_of_products(handle):
+    assert handle.quantize_fp8_status(300, 20, 1, FAKE, BYTE, 300, FAKE, 300, FAKE, 3) == INVALID
+    assert handle.gemm_fp8_status(64, 32, 300, FAKE, 300, FAKE, 3, FAKE, 300, FAKE, 3, FAKE, BYTE,
+                                  64) == INVALID
+
+
+def test_null_handle():
+    none = ctypes.c_void_p(None)
+    zero = ctypes.byref(ctypes.c_float(0.0))
+    back = back_args()
+    back[13] = zero
+    for name, args in (("sgblasRmsNorm", norm_args()), ("sgblasRmsNormBackward", back),
+                       ("sgblasSortTokens", sort_args()), ("sgblasScatterTokens", move_args()),
+                       ("sgblasGatherTokens", move_args()),
+                       ("sgblasGatherTokensBackward", move_back_args())):
+        assert getattr(sg.lib, name)(none, *args) == sg.SGBLAS_STATUS_NOT_INITIALIZED
