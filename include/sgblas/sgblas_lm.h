@@ -1,7 +1,7 @@
 /*
  * sgblas-b200: products of language models. Mixture-of-experts products whose
- * groups are ragged, 8-bit products with a scale for each block of 128, the
- * quantisation they need, and the orthogonalisation of an update by
+ * groups are ragged, 8-bit products with a scale for each block of 128 and 4-bit
+ * ones with a power of two for each 32, the quantisation they need, and the orthogonalisation of an update by
  * Newton-Schulz products; around them the norm before a layer, and tokens
  * sorted by expert and back. No counterpart in the reference API, whose only
  * product is SGEMM.
@@ -110,6 +110,49 @@ sgblasStatus_t sgblasGroupedGemmFp8(sgblasHandle_t handle, int m, int n, int k, 
                                     long long stride_a, const float *scale_a, int ldsa,
                                     long long stride_sa, const void *b, int ldb,
                                     const float *scale_b, int ldsb, void *c,
+                                    sgblasDataType_t ctype, int ldc);
+
+/* Quantises `batch` column-major k x n matrices of type xtype to 4 bits, in the OCP
+ * microscaling format MXFP4: e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), and for
+ * each block of 32 along k a power of two, as a byte (e8m0: 2^(byte - 127)):
+ *
+ *   byte = max(exponent byte of the block's largest magnitude in FP32 - 2, 0)
+ *   q    = the e2m1 value nearest to x * 2^(127 - byte), ties to even, at most 6
+ *
+ * which is exact but for q's own rounding. A NaN or an infinity in a block makes its
+ * byte 255, e8m0's NaN. Two values share a byte of q, the first in its low half;
+ * a column is ceil(k/2) bytes (the last half of an odd k is zero) and ldq and stride_q
+ * count bytes. scale is a column-major ceil(k/32) x n matrix of bytes. Strides are
+ * unused for batch == 1. */
+sgblasStatus_t sgblasQuantizeFp4(sgblasHandle_t handle, int k, int n, int batch, const void *x,
+                                 sgblasDataType_t xtype, int ldx, long long stride_x, void *q,
+                                 int ldq, long long stride_q, void *scale, int ldscale,
+                                 long long stride_scale);
+
+/* C = A^T * B with operands as sgblasQuantizeFp4 leaves them:
+ *
+ *   C(i, j) = sum over blocks b of 32 of k: 2^(sa(b, i) - 127) * 2^(sb(b, j) - 127) *
+ *             sum over k in b of A(k, i) * B(k, j)
+ *
+ * A is k x m (weights, scale_a ceil(k/32) x m), B is k x n (tokens, scale_b ceil(k/32) x
+ * n), C is m x n of type ctype; lda and ldb count bytes. Products and scales are
+ * exact, sums are FP32, chained in the tensor core over at most 512 of k for an
+ * FP32 C and 4096 for a BF16 C, as in sgblasGroupedGemmN; a block's two scales together
+ * should be in FP32's range. With an odd k, the last half byte of every column has to
+ * be zero. k == 0 writes zeros. Any alignment: operands and scales whose base is not
+ * 16-byte aligned, or whose leading dimension (or stride) is not a multiple of 16
+ * bytes, are first copied into the handle's workspace. */
+sgblasStatus_t sgblasGemmFp4(sgblasHandle_t handle, int m, int n, int k, const void *a, int lda,
+                             const void *scale_a, int ldsa, const void *b, int ldb,
+                             const void *scale_b, int ldsb, void *c, sgblasDataType_t ctype,
+                             int ldc);
+
+/* The same grouped along n, as sgblasGroupedGemmFp8: group g uses A_g at a + g *
+ * stride_a and its scales at scale_a + g * stride_sa (bytes). */
+sgblasStatus_t sgblasGroupedGemmFp4(sgblasHandle_t handle, int m, int n, int k, int groups,
+                                    const int *offsets, const void *a, int lda, long long stride_a,
+                                    const void *scale_a, int ldsa, long long stride_sa,
+                                    const void *b, int ldb, const void *scale_b, int ldsb, void *c,
                                     sgblasDataType_t ctype, int ldc);
 
 /* Orthogonalises a batch of m x n matrices G (type gtype) by Newton-Schulz

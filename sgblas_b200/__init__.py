@@ -100,6 +100,19 @@ _SIGNATURES = {
         ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int,
         ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
         ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
+    "sgblasQuantizeFp4": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong]),
+    "sgblasGemmFp4": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
+    "sgblasGroupedGemmFp4": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
     "sgblasOrthogonalize": (ctypes.c_int, [
         ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_float_p,
         ctypes.c_float, ctypes.c_float, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
@@ -335,6 +348,40 @@ class Handle:
         status = self.grouped_gemm_fp8_status(*args)
         if status:
             raise SgblasError("sgblasGroupedGemmFp8", status)
+
+    def quantize_fp4_status(self, k, n, x, xtype, ldx, q, ldq, scale, ldscale, batch=1, stride_x=0,
+                            stride_q=0, stride_scale=0) -> int:
+        """Raw sgblasQuantizeFp4 of one k x n matrix, or of a strided batch (q's ld in bytes)."""
+        return lib.sgblasQuantizeFp4(self._h, k, n, batch, _ptr(x), xtype, ldx, stride_x, _ptr(q),
+                                     ldq, stride_q, _ptr(scale), ldscale, stride_scale)
+
+    def quantize_fp4(self, *args, **kwargs) -> None:
+        status = self.quantize_fp4_status(*args, **kwargs)
+        if status:
+            raise SgblasError("sgblasQuantizeFp4", status)
+
+    def gemm_fp4_status(self, m, n, k, a, lda, scale_a, ldsa, b, ldb, scale_b, ldsb, c, ctype,
+                        ldc) -> int:
+        """Raw sgblasGemmFp4: C = A^T B with e2m1 operands and a power of two for each 32 of k."""
+        return lib.sgblasGemmFp4(self._h, m, n, k, _ptr(a), lda, _ptr(scale_a), ldsa, _ptr(b), ldb,
+                                 _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
+
+    def gemm_fp4(self, *args) -> None:
+        status = self.gemm_fp4_status(*args)
+        if status:
+            raise SgblasError("sgblasGemmFp4", status)
+
+    def grouped_gemm_fp4_status(self, m, n, k, groups, offsets, a, lda, stride_a, scale_a, ldsa,
+                                stride_sa, b, ldb, scale_b, ldsb, c, ctype, ldc) -> int:
+        """Raw sgblasGroupedGemmFp4."""
+        return lib.sgblasGroupedGemmFp4(self._h, m, n, k, groups, _ptr(offsets), _ptr(a), lda,
+                                        stride_a, _ptr(scale_a), ldsa, stride_sa, _ptr(b), ldb,
+                                        _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
+
+    def grouped_gemm_fp4(self, *args) -> None:
+        status = self.grouped_gemm_fp4_status(*args)
+        if status:
+            raise SgblasError("sgblasGroupedGemmFp4", status)
 
     def orthogonalize_status(self, m, n, batch, steps, coefficients, eps, scale, g, gtype, ldg,
                              stride_g, o, ldo, stride_o) -> int:

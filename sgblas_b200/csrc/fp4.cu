@@ -1,0 +1,450 @@
+// 4-bit products with a power of two for each 32 of k (MXFP4), and the
+// quantisation to that form (sgblas_lm.h).
+#include "product_fp4.cuh"
+
+#include "device.hpp"
+#include "product.hpp"
+#include "ptx.cuh"
+#include "sgemm_launch.hpp"
+
+#include <cuda_bf16.h>
+#include <cuda_fp4.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+
+namespace sgblas::detail {
+namespace {
+
+namespace t = kern::prod;
+
+constexpr int kBlock = 32;
+constexpr int kQuantThreads = 256;
+
+struct QuantParams {
+  const void *x;
+  unsigned char *q, *scale;
+  int k, n, kblocks, ldx, ldq, ldscale;
+  long long stride_x, stride_q, stride_scale;
+  unsigned blocks;   // of the whole batch
+};
+
+// The scale byte of a block whose largest magnitude has these bits: its exponent
+// less 2, that of the largest e2m1 value (4 <= 6 < 8), so that magnitudes from 6 to 8
+// times the power of two are cut to 6; 255 (NaN) where a value is none or infinite.
+__device__ __forceinline__ unsigned scaleByte(unsigned amax_bits) {
+  const unsigned exponent = amax_bits >> 23;
+  return exponent == 255 ? 255u : max(exponent, 2u) - 2u;
+}
+// 2^(127 - byte), exact: byte is 0 to 252 for numbers.
+__device__ __forceinline__ float inverseOf(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
+
+__device__ __forceinline__ unsigned pairOf(float lo, float hi) {
+  return __nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest);
+}
+
+template <typename T>
+__device__ __forceinline__ unsigned magnitude(T v) {
+  return __float_as_uint(static_cast<float>(v)) & 0x7FFFFFFFu;
+}
+
+// Two threads to a block of 32, 16 consecutive values each, kUnroll blocks per
+// thread whose loads are issued together. Memory-bound.
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads) quantizeFp4Kernel(const QuantParams p) {
+  constexpr int kPer = 16, kUnroll = 2, kVectors = kPer * static_cast<int>(sizeof(T)) / 16;
+  constexpr int kAtOnce = kQuantThreads / 2;
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const int part = threadIdx.x % 2;
+  const unsigned first = blockIdx.x * static_cast<unsigned>(kUnroll * kAtOnce) + threadIdx.x / 2;
+  alignas(16) T v[kUnroll][kPer];
+  int left[kUnroll];
+  unsigned char *q_to[kUnroll], *scale_to[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const unsigned block = first + u * kAtOnce;
+    const bool in = block < p.blocks;
+    const unsigned column = in ? block / static_cast<unsigned>(p.kblocks) : 0;
+    const int kb = in ? static_cast<int>(block - column * p.kblocks) : 0;
+    const unsigned matrix = column / static_cast<unsigned>(p.n);
+    const long long col = column - matrix * static_cast<unsigned>(p.n);
+    const int k0 = kb * kBlock + part * kPer;
+    left[u] = in ? p.k - k0 : 0;
+    const T *x = static_cast<const T *>(p.x) + matrix * p.stride_x + col * p.ldx + k0;
+    if (left[u] >= kPer) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j)
+        reinterpret_cast<uint4 *>(v[u])[j] = __ldg(reinterpret_cast<const uint4 *>(x) + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[u][j] = j < left[u] ? x[j] : static_cast<T>(0.0F);
+    }
+    q_to[u] = p.q + matrix * p.stride_q + col * p.ldq + k0 / 2;
+    scale_to[u] = in && part == 0 ? p.scale + matrix * p.stride_scale + col * p.ldscale + kb : nullptr;
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) m = max(m, magnitude(v[u][j]));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    const unsigned byte = scaleByte(m);
+    const float inverse = inverseOf(byte);
+    alignas(8) unsigned char b[kPer / 2];
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2)
+      b[j / 2] = static_cast<unsigned char>(pairOf(static_cast<float>(v[u][j]) * inverse,
+                                                   static_cast<float>(v[u][j + 1]) * inverse));
+    if (left[u] >= kPer) {
+      *reinterpret_cast<uint2 *>(q_to[u]) = *reinterpret_cast<const uint2 *>(b);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer / 2; ++j)
+        if (2 * j < left[u]) q_to[u][j] = b[j];
+    }
+    if (scale_to[u] != nullptr) *scale_to[u] = static_cast<unsigned char>(byte);
+  }
+}
+
+// Any alignment: a warp to a block, a value per lane, kUnroll blocks per warp.
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads) quantizeFp4ScalarKernel(const QuantParams p) {
+  constexpr int kUnroll = 8, kAtOnce = kQuantThreads / 32;
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const int lane = threadIdx.x % 32;
+  const unsigned first = blockIdx.x * static_cast<unsigned>(kUnroll * kAtOnce) + threadIdx.x / 32;
+  float v[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const unsigned block = first + u * kAtOnce;
+    v[u] = 0.0F;
+    if (block >= p.blocks) continue;
+    const unsigned column = block / static_cast<unsigned>(p.kblocks);
+    const unsigned matrix = column / static_cast<unsigned>(p.n);
+    const int at = static_cast<int>(block - column * p.kblocks) * kBlock + lane;
+    if (at < p.k)
+      v[u] = static_cast<float>(static_cast<const T *>(p.x)[matrix * p.stride_x +
+                                                            static_cast<long long>(column - matrix * p.n) * p.ldx + at]);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const unsigned block = first + u * kAtOnce;
+    const unsigned byte = scaleByte(__reduce_max_sync(0xffffffffu, magnitude(v[u])));
+    const float scaled = v[u] * inverseOf(byte);
+    const float next = __shfl_down_sync(0xffffffffu, scaled, 1);
+    if (block >= p.blocks) continue;
+    const unsigned column = block / static_cast<unsigned>(p.kblocks);
+    const unsigned matrix = column / static_cast<unsigned>(p.n);
+    const long long col = column - matrix * static_cast<unsigned>(p.n);
+    const int kb = static_cast<int>(block - column * p.kblocks), at = kb * kBlock + lane;
+    if (lane % 2 == 0 && at < p.k)
+      p.q[matrix * p.stride_q + col * p.ldq + at / 2] = static_cast<unsigned char>(pairOf(scaled, next));
+    if (lane == 0)
+      p.scale[matrix * p.stride_scale + col * p.ldscale + kb] = static_cast<unsigned char>(byte);
+  }
+}
+
+sgblasStatus_t launchQuantize(void (*kernel)(QuantParams), const QuantParams &p, unsigned per_cta,
+                              cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.blocks - 1) / per_cta + 1);
+  cfg.blockDim = dim3(kQuantThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+// ---- products --------------------------------------------------------------------
+
+template <class G>
+sgblasStatus_t launchTile(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+                          t::Fp4Params &f, cudaStream_t stream) {
+  t::Params &p = f.p;
+  if (p.k > 0 && (!encodeOperand(&p.tma_a, a, 1, false, t::kBM) ||
+                  !encodeOperand(&p.tma_b, b, 1, false, G::kBRows)))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  p.tiles_m = (p.m - 1) / G::kTileM + 1;
+  const long long tiles = static_cast<long long>(p.tiles_m) *
+                          (p.n / G::kBN + std::min<long long>(p.groups, p.n));
+  if (tiles > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  constexpr int kSize = G::kFp32 ? 4 : 2;
+  const long long column = static_cast<long long>(p.ldc) * kSize;
+  p.c_tma = tmaWritable(p, kSize, column * p.n);
+  if (p.c_tma &&
+      !encodeTyped3d(&p.tma_c,
+                     G::kFp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                     p.c, p.m, p.n, 1, column, column * p.n, G::kFp32 ? 32 : 64, t::kOutCols,
+                     G::kFp32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  auto kernel = t::fp4TileKernel<G>;
+  static std::atomic<uint64_t> configured{0};
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes, &configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  constexpr int kCtas = G::kTwo ? 2 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::min<long long>(tiles, dev.sms / kCtas)));
+  cfg.blockDim = dim3(t::kThreads);
+  cfg.dynamicSmemBytes = G::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kCtas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = G::kTwo ? 2 : 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, f));
+}
+
+// Clusters of `split` CTAs per 128 x kBN tile, chosen as launchThin (product.cu) does.
+template <class G>
+sgblasStatus_t launchThin(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+                          t::Fp4Params &f, cudaStream_t stream) {
+  t::Params &p = f.p;
+  if (p.k > 0 && (!encodeOperand(&p.tma_a, a, 1, false, t::kBM) ||
+                  !encodeOperand(&p.tma_b, b, 1, false, t::kThinBox)))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  p.tiles_m = (p.m - 1) / t::kBM + 1;
+  const long long most =
+      static_cast<long long>(p.tiles_m) * (p.n / G::kBN + std::min<long long>(p.groups, p.n));
+  if (most > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;
+  const long long tiles = static_cast<long long>(p.tiles_m) *
+                          std::max<long long>(std::min(p.groups, p.n), p.n / G::kBN);
+  auto kernel = t::fp4ThinKernel<G>;
+  static std::atomic<uint64_t> configured{0};
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, G::kSmemBytes, &configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(t::kThinThreads);
+  cfg.dynamicSmemBytes = G::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  static std::atomic<int> resident[kMaxDevices][4];   // clusters of 2^i CTAs
+  const int iters = (p.k + t::kRowBytes - 1) / t::kRowBytes;
+  int split = 1, grid = 0;
+  double best = 1e30;
+  for (int i = 0, s = 1; s <= t::kMaxSplit; ++i, s *= 2) {
+    if (s > 1 && iters < 2 * s) break;
+    int clusters = s == 1 ? dev.sms : resident[dev.device][i].load(std::memory_order_relaxed);
+    if (clusters == 0) {
+      attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+      cfg.gridDim = dim3(static_cast<unsigned>(s));
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        clusters = 0;
+      }
+      if (clusters <= 0) clusters = -1;
+      resident[dev.device][i].store(clusters, std::memory_order_relaxed);
+    }
+    if (clusters < 0) break;
+    if (s > 1 && tiles > clusters && iters < 32 * s) continue;
+    const double run = static_cast<double>((tiles + clusters - 1) / clusters) / s;
+    if (run < 0.97 * best) {
+      best = run;
+      split = s;
+      grid = static_cast<int>(std::min<long long>(most, clusters));
+    }
+  }
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  cfg.gridDim = dim3(static_cast<unsigned>(split * grid));
+  cfg.attrs = split > 1 ? attr : attr + 1;   // without a split there is no cluster to launch
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, f, split));
+}
+
+// Width (columns of tokens) of the tiles: 16, 32 or 64 for the thin kernel, 128 for
+// single CTAs, 192 for pairs.
+int chooseWidth(const DeviceInfo &dev, const t::Params &p) {
+  const int active = std::min(p.groups, p.n);
+  const double mean = static_cast<double>(p.n) / std::max(p.groups, 1);
+  auto tiles = [&](int rows, int width) {
+    const double columns = p.groups == 1
+                               ? static_cast<double>((p.n - 1) / width + 1)
+                               : std::max<double>(active, static_cast<double>(p.n) / width + 0.5 * active);
+    return columns * ((p.m - 1) / rows + 1);
+  };
+  if (mean <= 6) return 16;
+  const double single = tiles(t::kBM, 128);
+  if (mean <= 12 || (mean <= 64 && 4 * single <= dev.sms)) return mean <= 16 ? 32 : 64;
+  const double waves = std::ceil(single / dev.sms);
+  const double pair_waves = std::ceil(tiles(2 * t::kBM, 192) / (dev.sms / 2));
+  return pair_waves * 1.35 < waves ? 192 : 128;
+}
+
+sgblasStatus_t launchFp4(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+                         t::Fp4Params &f, cudaStream_t stream) {
+  const bool fp32 = !f.p.c_bf16;
+  switch (chooseWidth(dev, f.p)) {
+    case 16: return launchThin<t::Fp4ThinCfg<16>>(dev, a, b, f, stream);
+    case 32: return launchThin<t::Fp4ThinCfg<32>>(dev, a, b, f, stream);
+    case 64: return launchThin<t::Fp4ThinCfg<64>>(dev, a, b, f, stream);
+    case 128:
+      return fp32 ? launchTile<t::Fp4Cfg<128, false, true>>(dev, a, b, f, stream)
+                  : launchTile<t::Fp4Cfg<128, false, false>>(dev, a, b, f, stream);
+    default:
+      return fp32 ? launchTile<t::Fp4Cfg<192, true, true>>(dev, a, b, f, stream)
+                  : launchTile<t::Fp4Cfg<192, true, false>>(dev, a, b, f, stream);
+  }
+}
+
+sgblasStatus_t gemmFp4(sgblasHandle_t handle, int m, int n, int k, int groups, const int *offsets,
+                       bool grouped, const void *a, int lda, long long stride_a, const void *scale_a,
+                       int ldsa, long long stride_sa, const void *b, int ldb, const void *scale_b,
+                       int ldsb, void *c, sgblasDataType_t ctype, int ldc) {
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  const int bytes = k > 0 ? (k - 1) / 2 + 1 : 0, blocks = k > 0 ? (k - 1) / kBlock + 1 : 0;
+  if (m < 0 || n < 0 || k < 0 || groups < 0 || !isType(ctype) || lda < std::max(1, bytes) ||
+      ldb < std::max(1, bytes) || ldc < std::max(1, m) || ldsa < std::max(1, blocks) ||
+      ldsb < std::max(1, blocks))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (m == 0 || n == 0 || groups == 0) return SGBLAS_STATUS_SUCCESS;
+  if (c == nullptr || (grouped && offsets == nullptr) ||
+      (k > 0 && (a == nullptr || b == nullptr || scale_a == nullptr || scale_b == nullptr)))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (groups > SGBLAS_MAX_GROUPS) return SGBLAS_STATUS_NOT_SUPPORTED;
+  DeviceInfo dev;
+  sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  t::Fp4Params f = {};
+  t::Params &p = f.p;
+  p.offsets = offsets;
+  p.groups = groups;
+  p.m = m;
+  p.n = n;
+  p.k = bytes;
+  p.c = c;
+  p.c_bf16 = ctype == SGBLAS_TYPE_BF16;
+  p.ldc = ldc;
+  p.alpha = 1.0F;
+  p.err = dev.err;
+  // Chains of 512 of k for an FP32 result, of 4096 for a BF16 one (launchNarrow).
+  p.chunk_iters = p.c_bf16 ? 16 : 2;
+  // Operands, then their scales, whose rows the kernels read 16 bytes at a time.
+  NarrowOperand op[4];
+  const void *ptr[4] = {a, b, scale_a, scale_b};
+  const int width[4] = {bytes, bytes, blocks, blocks};
+  const int ld[4] = {lda, ldb, ldsa, ldsb};
+  for (int i = 0; i < 4; ++i) {
+    op[i].ptr = ptr[i];
+    op[i].dim0 = width[i];
+    op[i].dim1 = i % 2 == 0 ? m : n;
+    op[i].ld = ld[i];
+    op[i].count = i % 2 == 0 ? groups : 1;
+    op[i].stride = i == 0 ? stride_a : i == 2 ? stride_sa : 0;
+  }
+  const auto stream = static_cast<cudaStream_t>(handle->stream);
+  bool used_workspace = false;
+  if (k > 0) {
+    size_t size[4], all = 0;
+    for (int i = 0; i < 4; ++i) {
+      size[i] = tmaReadable(op[i], 1) ? 0 : copyBytes(op[i], 1);
+      all += size[i];
+    }
+    if (all > 0) {
+      if (!ensureWorkspace(handle, kCounterRegionBytes + all, dev.device, stream))
+        return SGBLAS_STATUS_NOT_SUPPORTED;
+      used_workspace = true;
+      auto *to = static_cast<unsigned char *>(handle->workspace) + kCounterRegionBytes;
+      for (int i = 0; i < 4 && st == SGBLAS_STATUS_SUCCESS; ++i) {
+        if (size[i] == 0) continue;
+        st = copyOperand(&op[i], 1, to, dev.sms, i % 2 == 0 ? offsets : nullptr, stream);
+        to += size[i];
+      }
+    }
+  }
+  f.scale_a = static_cast<const unsigned char *>(op[2].ptr);
+  f.scale_b = static_cast<const unsigned char *>(op[3].ptr);
+  f.ldsa = static_cast<int>(op[2].ld);
+  f.ldsb = static_cast<int>(op[3].ld);
+  f.stride_sa = op[2].count == 1 ? 0 : op[2].stride;
+  f.blocks = blocks;
+  if (st == SGBLAS_STATUS_SUCCESS) st = launchFp4(dev, op[0], op[1], f, stream);
+  // Failed or not: a copy may be on its way, and later users wait for it.
+  if (used_workspace && !markWorkspaceUse(handle, stream) && st == SGBLAS_STATUS_SUCCESS)
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  return st;
+}
+
+}  // namespace
+}  // namespace sgblas::detail
+
+extern "C" sgblasStatus_t sgblasQuantizeFp4(sgblasHandle_t handle, int k, int n, int batch,
+                                            const void *x, sgblasDataType_t xtype, int ldx,
+                                            long long stride_x, void *q, int ldq, long long stride_q,
+                                            void *scale, int ldscale, long long stride_scale) {
+  using namespace sgblas::detail;
+  if (handle == nullptr) return SGBLAS_STATUS_NOT_INITIALIZED;
+  const int bytes = k > 0 ? (k - 1) / 2 + 1 : 0, kblocks = k > 0 ? (k - 1) / kBlock + 1 : 0;
+  if (k < 0 || n < 0 || batch < 0 || !isType(xtype) || ldx < std::max(1, k) ||
+      ldq < std::max(1, bytes) || ldscale < std::max(1, kblocks))
+    return SGBLAS_STATUS_INVALID_VALUE;
+  if (k == 0 || n == 0 || batch == 0) return SGBLAS_STATUS_SUCCESS;
+  if (x == nullptr || q == nullptr || scale == nullptr) return SGBLAS_STATUS_INVALID_VALUE;
+  const double blocks = static_cast<double>(n) * kblocks * batch;
+  if (blocks > INT_MAX) return SGBLAS_STATUS_NOT_SUPPORTED;   // 64 Gi values
+  DeviceInfo dev;
+  const sgblasStatus_t st = currentDevice(&dev);
+  if (st != SGBLAS_STATUS_SUCCESS) return st;
+  QuantParams p = {};
+  p.x = x;
+  p.q = static_cast<unsigned char *>(q);
+  p.scale = static_cast<unsigned char *>(scale);
+  p.k = k;
+  p.n = n;
+  p.kblocks = kblocks;
+  p.ldx = ldx;
+  p.ldq = ldq;
+  p.ldscale = ldscale;
+  if (batch > 1) {
+    p.stride_x = stride_x;
+    p.stride_q = stride_q;
+    p.stride_scale = stride_scale;
+  }
+  p.blocks = static_cast<unsigned>(blocks);
+  const auto stream = static_cast<cudaStream_t>(handle->stream);
+  // Whole vectors where 16 values start on 16 bytes of x and on 8 of q.
+  const int size = xtype == SGBLAS_TYPE_BF16 ? 2 : 4;
+  const bool vector = aligned16(x) && ldx * static_cast<long long>(size) % 16 == 0 &&
+                      p.stride_x * size % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 &&
+                      ldq % 8 == 0 && p.stride_q % 8 == 0;
+  if (xtype == SGBLAS_TYPE_BF16)
+    return vector ? launchQuantize(quantizeFp4Kernel<__nv_bfloat16>, p, kQuantThreads, stream)
+                  : launchQuantize(quantizeFp4ScalarKernel<__nv_bfloat16>, p, kQuantThreads / 4, stream);
+  return vector ? launchQuantize(quantizeFp4Kernel<float>, p, kQuantThreads, stream)
+                : launchQuantize(quantizeFp4ScalarKernel<float>, p, kQuantThreads / 4, stream);
+}
+
+extern "C" sgblasStatus_t sgblasGemmFp4(sgblasHandle_t handle, int m, int n, int k, const void *a,
+                                        int lda, const void *scale_a, int ldsa, const void *b, int ldb,
+                                        const void *scale_b, int ldsb, void *c, sgblasDataType_t ctype,
+                                        int ldc) {
+  return sgblas::detail::gemmFp4(handle, m, n, k, 1, nullptr, false, a, lda, 0, scale_a, ldsa, 0, b, ldb,
+                                 scale_b, ldsb, c, ctype, ldc);
+}
+
+extern "C" sgblasStatus_t sgblasGroupedGemmFp4(sgblasHandle_t handle, int m, int n, int k, int groups,
+                                               const int *offsets, const void *a, int lda,
+                                               long long stride_a, const void *scale_a, int ldsa,
+                                               long long stride_sa, const void *b, int ldb,
+                                               const void *scale_b, int ldsb, void *c,
+                                               sgblasDataType_t ctype, int ldc) {
+  return sgblas::detail::gemmFp4(handle, m, n, k, groups, offsets, true, a, lda, stride_a, scale_a, ldsa,
+                                 stride_sa, b, ldb, scale_b, ldsb, c, ctype, ldc);
+}

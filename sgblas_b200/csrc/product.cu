@@ -77,12 +77,14 @@ __global__ void __launch_bounds__(256) copyRowsKernel(const unsigned char *__res
   }
 }
 
+}  // namespace
+
 bool tmaReadable(const NarrowOperand &o, int elem_bytes) {
   return aligned16(o.ptr) && o.ld * elem_bytes % 16 == 0 &&
          (o.count == 1 || (o.stride * elem_bytes % 16 == 0 && o.stride > 0));
 }
 
-long long copyLd(const NarrowOperand &o, int elem_bytes) {
+static long long copyLd(const NarrowOperand &o, int elem_bytes) {
   const int unit = 128 / elem_bytes;   // whole 128-byte lines
   return (o.dim0 + unit - 1LL) / unit * unit;
 }
@@ -91,8 +93,6 @@ size_t copyBytes(const NarrowOperand &o, int elem_bytes) {
   return static_cast<size_t>(copyLd(o, elem_bytes)) * elem_bytes * o.dim1 * o.count;
 }
 
-// Copies the operand to dst and points it there; with offsets only the matrices
-// of groups that have columns.
 sgblasStatus_t copyOperand(NarrowOperand *o, int elem_bytes, void *dst, int sms,
                            const int *offsets, cudaStream_t stream) {
   const long long ldp = copyLd(*o, elem_bytes);
@@ -128,14 +128,13 @@ bool encodeOperand(CUtensorMap *map, const NarrowOperand &o, int elem_bytes, boo
                        mn ? 64u : static_cast<unsigned>(rows), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Whether TMA can write C: addresses and strides of whole 16-byte units (matrices
-// `matrix` bytes apart), and such columns too, for it writes a column to the end
-// of its last unit: rows beyond C, which are not C's.
 bool tmaWritable(const t::Params &p, int size, long long matrix) {
   const long long column = static_cast<long long>(p.ldc) * size;
   return aligned16(p.c) && column % 16 == 0 && static_cast<long long>(p.m) * size % 16 == 0 &&
          matrix > 0 && matrix % 16 == 0 && matrix < (1LL << 40);
 }
+
+namespace {
 
 template <class G>
 sgblasStatus_t launchTyped(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,

@@ -69,6 +69,20 @@ sgblasStatus_t launchProductKernel(const DeviceInfo &dev, const kern::prod::Para
   return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
+// Whether TMA can read the operand as it lies.
+bool tmaReadable(const NarrowOperand &o, int elem_bytes);
+// Otherwise its copy's size, and the copy: to dst, where `o` then points; with offsets
+// only the matrices of groups that have columns.
+size_t copyBytes(const NarrowOperand &o, int elem_bytes);
+sgblasStatus_t copyOperand(NarrowOperand *o, int elem_bytes, void *dst, int sms, const int *offsets,
+                           cudaStream_t stream);
+// Tensor map of the operand in boxes of 128 bytes by `rows` (K-major) or 64 rows.
+bool encodeOperand(CUtensorMap *map, const NarrowOperand &o, int elem_bytes, bool mn, int rows);
+// Whether TMA can write C: addresses and strides of whole 16-byte units (matrices
+// `matrix` bytes apart), and such columns too, for it writes a column to the end
+// of its last unit: rows beyond C, which are not C's.
+bool tmaWritable(const kern::prod::Params &p, int size, long long matrix);
+
 // Launches a product of `elem_bytes` operands (1: e4m3, 2: 16-bit). `mn`
 // operands are contiguous along m (or n) instead of k. p carries the sizes,
 // C, the scalars, scales, offsets and type bits; the maps and tile counts are

@@ -1,0 +1,688 @@
+// Products of 4-bit operands (e2m1 values, a power of two for each 32 of k, as
+// the OCP microscaling format MXFP4 has them): C = A^T B per group, FP32 sums.
+//
+// The tiles, roles and ragged groups are those of product_tile.cuh (many tokens)
+// and product_thin.cuh (few); operands are rows of bytes, two values each, and a
+// k slice of 128 bytes is 256 of k. What differs is the scales: the tensor core
+// applies them itself (kind::mxf4), from tensor memory, where each instruction (64
+// of k) takes two for every row of A and of B.
+//
+// Scales' way. In global memory they lie as bytes, contiguous along k, a row per
+// column of A or B. A warp of its own (kScaleWarp) copies 16 of a row at once (two
+// slices) into shared memory by cp.async, each lane the rows lane + 32 i, several
+// chunks ahead; it then writes a slice's, four per row and 128 of k, as the 512-byte
+// blocks that tcgen05.cp takes: 32 rows (lanes) of four words, word i for row
+// lane + 32 i. The issuer copies the blocks to TMEM before the slice's four
+// instructions. (Gathering them directly from global memory into the blocks would
+// take a 4-byte access per row and 128 of k, twice what the L1 cache can look up.)
+// A stage of the ring holds a slice of A, of B and of the blocks; its TMEM columns
+// are the stage's, too, so one barrier frees all of it.
+#ifndef SGBLAS_B200_PRODUCT_FP4_CUH_
+#define SGBLAS_B200_PRODUCT_FP4_CUH_
+
+#include "product_thin.cuh"
+#include "product_tile.cuh"
+
+namespace sgblas::kern::prod {
+
+constexpr int kScaleBlock = 512;     // bytes: four scales of each of 128 rows
+constexpr int kScaleWarp = 3;
+constexpr int kRawChunks = 4;        // chunks of 16 scales per row: one at work, the others on their way
+constexpr int kSliceScales = 8;      // of a row in a slice
+
+struct Fp4Params {
+  Params p;                          // k in bytes
+  const unsigned char *scale_a, *scale_b;
+  int ldsa, ldsb, blocks;            // blocks of 32 along k
+  long long stride_sa;
+};
+
+// Shared layout of both forms: kBN columns of the tile, all of whose scales each
+// CTA has.
+template <int kBN_, bool kTwo_, bool kThin_>
+struct Fp4Shape {
+  static constexpr Ragged kRagged = Ragged::kN;
+  static constexpr int kElemBytes = 1;
+  static constexpr int kBN = kBN_;
+  static constexpr bool kTwo = kTwo_, kSymmetric = false;
+  static constexpr int kTileM = kTwo ? 2 * kBM : kBM;
+  static constexpr int kBRows = kTwo ? kBN / 2 : kBN;
+  static constexpr int kNStep = kTwo ? 32 : 16;
+  static constexpr int kABytes = kBM * kRowBytes;
+  static constexpr int kBBytes = kBRows * kRowBytes;
+  static constexpr int kBBlocks = (kBN + 127) / 128;   // of scales of B, per 128 of k
+  static constexpr int kScaleBytes = 2 * (1 + kBBlocks) * kScaleBlock;
+  static constexpr int kScaleColumns = kScaleBytes / 128;   // of TMEM
+  static constexpr int kStageBytes = kABytes + kBBytes + kScaleBytes;
+  static constexpr int kRawRows = kBM + kBN;
+  static constexpr int kRawBytes = kRawChunks * kRawRows * 16;
+  static constexpr int kAccums = kThin_ ? (kBN == 64 ? 4 : 8) : 2;
+  static constexpr int kScaleColumn0 = kAccums * kBN;
+  static constexpr int kFitColumns = (512 - kScaleColumn0) / kScaleColumns;
+  static constexpr int kTmemColumns = 512;
+  static_assert(kBN % 16 == 0 && kBN <= 256, "the instruction's N");
+  static_assert(!kTwo || kBN % 32 == 0, "halves of whole swizzle groups");
+};
+
+template <int kBN_, bool kTwo_, bool kFp32_>
+struct Fp4Cfg : Fp4Shape<kBN_, kTwo_, false> {
+  using S = Fp4Shape<kBN_, kTwo_, false>;
+  static constexpr bool kFp32 = kFp32_;
+  static constexpr int kOutWarp = 2 * kOutCols * 32 * (kFp32 ? 4 : 2);
+  static constexpr int kOutBytes = kEpilogueWarps * kOutWarp;
+  static constexpr int kFit = (217 * 1024 - kOutBytes - S::kRawBytes) / S::kStageBytes;
+  static constexpr int kLess = kFit < S::kFitColumns ? kFit : S::kFitColumns;
+  static constexpr int kStages = kLess > 8 ? 8 : kLess;
+  static constexpr int kBarrierBytes = 8 * (2 * kStages + 2 * S::kAccums);
+  static constexpr int kSmemBytes =
+      kStages * S::kStageBytes + kOutBytes + S::kRawBytes + kBarrierBytes + 1024;
+  static_assert(kStages >= 3 && kSmemBytes <= 218 * 1024 + 512, "shared memory beside the table");
+  static_assert(S::kBN / 2 % 32 == 0, "an epilogue warp's columns");
+};
+
+template <int kBN_>
+struct Fp4ThinCfg : Fp4Shape<kBN_, false, true> {
+  using S = Fp4Shape<kBN_, false, true>;
+  static constexpr int kPartPitch = S::kBN + 4;
+  static constexpr int kPartBytes = kPartPitch * kBM * 4;
+  static constexpr int kFit = (kThinSmem - kPartBytes - S::kRawBytes) / S::kStageBytes;
+  static constexpr int kStages = kFit < S::kFitColumns ? kFit : S::kFitColumns;
+  static constexpr int kBarrierBytes = 8 * (2 * kStages + 2 * S::kAccums + 2);
+  static constexpr int kSmemBytes =
+      kStages * S::kStageBytes + kPartBytes + S::kRawBytes + kBarrierBytes + 1024;
+  static_assert(S::kBN == 16 || S::kBN == 32 || S::kBN == 64, "tile width");
+  static_assert(kSmemBytes <= 218 * 1024, "shared memory beside the table");
+};
+
+// Instruction descriptor: e2m1 operands, e8m0 scales; `half` of a word of four
+// scales (bits 4-5 and 29-30: the first byte's number).
+template <class G>
+__device__ __forceinline__ uint32_t fp4InstrDesc(int n, int half) {
+  return (static_cast<uint32_t>(2 * half) << 4) | (1u << 7) | (1u << 10) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(G::kTileM >> 4) << 24) | (static_cast<uint32_t>(2 * half) << 29);
+}
+
+// Descriptor of a block of scales: 16-byte rows without swizzle, groups of eight
+// rows 128 bytes apart.
+__device__ __forceinline__ uint64_t scaleDesc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(8) << 16) |
+         (static_cast<uint64_t>(8) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+
+// The role of kScaleWarp: the scales of every slice [kb0, kb1) of this worker's tiles into
+// the ring's stages. `ready(s)` announces stage s.
+template <class G, int kStages, class Wait, class Ready>
+__device__ __forceinline__ void stageScales(const Fp4Params &f, const GroupTable &table, int tiles,
+                                            int worker, int workers, int rank, int kb0, int kb1,
+                                            unsigned char *ring, unsigned char *raw, int lane,
+                                            Wait wait, Ready ready) {
+  const Params &p = f.p;
+  const int chunk0 = kb0 / 2, chunk1 = (kb1 + 1) / 2;
+  if (kb0 >= kb1) return;
+  // What is fetched next, chunks ahead of what is at work.
+  int fetch_tile = worker, fetch_chunk = chunk0, fetched = 0;
+  const unsigned char *at_a = nullptr, *at_b = nullptr;
+  int rows_a = 0, rows_b = 0;
+  auto fetch = [&]() {
+    if (fetch_tile < tiles) {
+      if (fetch_chunk == chunk0) {
+        const Tile t = tileAt<G>(p, table, fetch_tile);
+        const int m0 = t.m0 + rank * kBM;
+        rows_a = p.m - m0;
+        rows_b = t.cols;
+        at_a = f.scale_a + t.group * f.stride_sa + static_cast<long long>(m0 + lane) * f.ldsa;
+        at_b = f.scale_b + static_cast<long long>(t.n0 + lane) * f.ldsb;
+      }
+      unsigned char *to = raw + (fetched % kRawChunks) * (G::kRawRows * 16) + lane * 16;
+      const uint32_t bytes = static_cast<uint32_t>(min(16, f.blocks - fetch_chunk * 16));
+#pragma unroll
+      for (int i = 0; i < kBM / 32; ++i) {
+        const bool in = lane + 32 * i < rows_a;
+        cpAsyncN<16>(to + i * 512, in ? at_a + static_cast<long long>(32 * i) * f.ldsa + fetch_chunk * 16 : f.scale_a,
+                     in ? bytes : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < (G::kBN + 31) / 32; ++i) {
+        if (G::kBN % 32 != 0 && lane >= G::kBN) break;
+        const bool in = lane + 32 * i < rows_b;
+        cpAsyncN<16>(to + (kBM / 32 + i) * 512,
+                     in ? at_b + static_cast<long long>(32 * i) * f.ldsb + fetch_chunk * 16 : f.scale_b,
+                     in ? bytes : 0);
+      }
+      if (++fetch_chunk == chunk1) {
+        fetch_chunk = chunk0;
+        fetch_tile += workers;
+      }
+    }
+    cpAsyncCommit();
+    ++fetched;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kRawChunks - 1; ++i) fetch();
+  int s = 0, parity = 1, done = 0;
+  for (int i = worker; i < tiles; i += workers) {
+#pragma unroll 1
+    for (int c = chunk0; c < chunk1; ++c) {
+      fetch();   // into the chunk that this lane read last
+      cpAsyncWait<kRawChunks - 1>();
+      const unsigned char *from = raw + (done % kRawChunks) * (G::kRawRows * 16) + lane * 16;
+      ++done;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const int kb = 2 * c + half;
+        if (kb < kb0 || kb >= kb1) continue;
+        wait(s, parity);
+        unsigned char *to = ring + s * G::kStageBytes + G::kABytes + G::kBBytes + lane * 16;
+        // Blocks: A's of the first and second 128 of k, then B's likewise.
+#pragma unroll
+        for (int b = 0; b < 1 + G::kBBlocks; ++b) {
+          uint2 w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row0 = (b * 4 + r) * 32;   // of the raw rows
+            w[r] = make_uint2(0, 0);
+            if (row0 < G::kRawRows && (row0 + 32 <= G::kRawRows || lane < G::kRawRows - row0))
+              w[r] = *reinterpret_cast<const uint2 *>(from + row0 * 16 + half * kSliceScales);
+          }
+          const int first = b == 0 ? 0 : 2 + (b - 1), next = b == 0 ? 1 : G::kBBlocks;
+          *reinterpret_cast<uint4 *>(to + first * kScaleBlock) = make_uint4(w[0].x, w[1].x, w[2].x, w[3].x);
+          *reinterpret_cast<uint4 *>(to + (first + next) * kScaleBlock) =
+              make_uint4(w[0].y, w[1].y, w[2].y, w[3].y);
+        }
+        fenceProxyAsyncShared();
+        __syncwarp();
+        ready(s);
+        if (++s == kStages) {
+          s = 0;
+          parity ^= 1;
+        }
+      }
+    }
+  }
+}
+
+// One slice: its scales to TMEM, then its instructions (one thread).
+template <class G>
+__device__ __forceinline__ void issueSlice(uint32_t tmem_base, uint32_t d_tmem, uint32_t stage_addr,
+                                           uint64_t desc_a, uint64_t desc_b, int s, int n,
+                                           bool accumulate) {
+  const uint32_t sf = tmem_base + G::kScaleColumn0 + static_cast<uint32_t>(s * G::kScaleColumns);
+  const uint64_t from =
+      scaleDesc(stage_addr + static_cast<uint32_t>(s * G::kStageBytes + G::kABytes + G::kBBytes));
+#pragma unroll
+  for (int b = 0; b < 2 * (1 + G::kBBlocks); ++b)
+    tmemCopyScales<G::kTwo>(sf + 4 * b, from + b * (kScaleBlock / 16));
+  uint64_t ad = desc_a + static_cast<uint64_t>(s) * (G::kStageBytes / 16);
+  uint64_t bd = desc_b + static_cast<uint64_t>(s) * (G::kStageBytes / 16);
+  const uint32_t idesc[2] = {fp4InstrDesc<G>(n, 0), fp4InstrDesc<G>(n, 1)};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    mmaFp4<G::kTwo>(d_tmem, ad, bd, idesc[j % 2], sf + j / 2 * 4, sf + 8 + j / 2 * (4 * G::kBBlocks),
+                    accumulate || j > 0);
+    ad += 2;   // 32 bytes
+    bd += 2;
+  }
+}
+
+// Many tokens: as productKernel.
+//   full[s]   stage s has its operands (TMA) and the scales of each CTA (kScaleWarp)
+template <class G>
+__global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_constant__ Fp4Params f) {
+  constexpr int kBN = G::kBN;
+  constexpr int kStages = G::kStages;
+  constexpr int kStageBytes = G::kStageBytes;
+  const Params &p = f.p;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ GroupTable table;
+  unsigned char *smem = smem_raw + ((1024 - (smemAddr(smem_raw) & 1023)) & 1023);
+  unsigned char *out_smem = smem + kStages * kStageBytes;
+  unsigned char *raw = out_smem + G::kOutBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(raw + G::kRawBytes);
+  uint64_t *empty = full + kStages;
+  uint64_t *acc_full = empty + kStages;
+  uint64_t *acc_empty = acc_full + kAccums;
+
+  const int warp = uniformWarp(), lane = threadIdx.x % 32;
+  const int rank = G::kTwo ? static_cast<int>(blockIdx.x & 1) : 0;
+  const int worker = G::kTwo ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int workers = G::kTwo ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  if (threadIdx.x == 0) {
+    if (p.k > 0) {
+      prefetchTensorMap(&p.tma_a);
+      prefetchTensorMap(&p.tma_b);
+    }
+    if (p.c_tma) prefetchTensorMap(&p.tma_c);
+    for (int s = 0; s < kStages; ++s) {
+      mbarInit(&full[s], G::kTwo ? 3 : 2);
+      mbarInit(&empty[s], 1);
+    }
+    for (int b = 0; b < kAccums; ++b) {
+      mbarInit(&acc_full[b], 1);
+      mbarInit(&acc_empty[b], (G::kTwo ? 2 : 1) * kEpilogueWarps);
+    }
+    fenceBarrierInit();
+  }
+  if (warp == 2) {
+    if constexpr (G::kTwo) {
+      tmemAllocPair(&tmem_base_slot, G::kTmemColumns);
+      tmemRelinquishPair();
+    } else {
+      tmemAlloc(&tmem_base_slot, G::kTmemColumns);
+      tmemRelinquish();
+    }
+  }
+  tcgenFenceBefore();
+  __syncthreads();
+  if constexpr (G::kTwo) clusterSync();   // both CTAs' barriers and TMEM exist
+  tcgenFenceAfter();
+  allowDependentLaunch();
+  gridDependencyWait();
+  if (warp == 0) readGroups<G>(p, &table, lane);
+  __syncthreads();
+  const uint32_t tmem_base = tmem_base_slot;
+  const int tiles = tileCount<G>(p, table);
+  const int iters = (p.k + kRowBytes - 1) / kRowBytes;
+
+  bool ok = true;
+  auto wait = [&](uint64_t *bar, int parity) {
+    if (ok) ok = mbarWait(bar, static_cast<uint32_t>(parity), p.err);
+  };
+  auto widthOf = [](int cols) { return (cols + G::kNStep - 1) / G::kNStep * G::kNStep; };
+
+  if (warp < kEpilogueWarp0) {
+    regDealloc<72>();
+    if (warp == 0 && electOne()) {
+      // ---------------- TMA producer ----------------
+      int s = 0, parity = 1;
+      for (int i = worker; i < tiles; i += workers) {
+        const Tile t = tileAt<G>(p, table, i);
+        const int m0 = t.m0 + rank * kBM;
+        const int n0 = t.n0 + (G::kTwo ? rank * (widthOf(t.cols) / 2) : 0);
+        for (int kb = 0; kb < iters; ++kb) {
+          wait(&empty[s], parity);
+          if (!ok) continue;
+          unsigned char *stage = smem + s * kStageBytes;
+          constexpr uint32_t kBytes = G::kABytes + G::kBBytes;
+          if constexpr (G::kTwo) {
+            if (rank == 0) mbarArriveExpectTx(&full[s], 2 * kBytes);
+            const uint32_t bar = clusterAddr(smemAddr(&full[s]), 0);
+            tmaLoad3dPair(stage, &p.tma_a, bar, kb * kRowBytes, m0, t.group);
+            tmaLoad3dPair(stage + G::kABytes, &p.tma_b, bar, kb * kRowBytes, n0, 0);
+          } else {
+            mbarArriveExpectTx(&full[s], kBytes);
+            tmaLoad3d(stage, &p.tma_a, &full[s], kb * kRowBytes, m0, t.group);
+            tmaLoad3d(stage + G::kABytes, &p.tma_b, &full[s], kb * kRowBytes, n0, 0);
+          }
+          if (++s == kStages) {
+            s = 0;
+            parity ^= 1;
+          }
+        }
+      }
+      // The last copies have landed and been read (productKernel).
+#pragma unroll 1
+      for (int j = 0; j < kStages; ++j) {
+        if (rank == 0) wait(&full[s], parity);
+        wait(&empty[s], parity);
+        if (++s == kStages) {
+          s = 0;
+          parity ^= 1;
+        }
+      }
+    } else if (warp == kScaleWarp) {
+      // ---------------- scales ----------------
+      stageScales<G, kStages>(
+          f, table, tiles, worker, workers, rank, 0, iters, smem, raw, lane,
+          [&](int s, int parity) { wait(&empty[s], parity); },
+          [&](int s) {
+            if (lane != 0) return;
+            if constexpr (G::kTwo) mbarArriveCluster(clusterAddr(smemAddr(&full[s]), 0));
+            else mbarArrive(&full[s]);
+          });
+      cpAsyncWait<0>();
+    } else if (warp == 1 && rank == 0) {
+      // ---------------- MMA issuer ----------------
+      const bool leader = electOne();
+      int s = 0, parity = 0;
+      int b = 0, acc_parity = 1;
+      const uint64_t desc_a = smemDesc<false>(smemAddr(smem));
+      const uint64_t desc_b = smemDesc<false>(smemAddr(smem) + G::kABytes);
+      for (int i = worker; i < tiles; i += workers) {
+        const Tile t = tileAt<G>(p, table, i);
+        const int n = widthOf(t.cols);
+        int in_chunk = 0;
+        for (int kb = 0; kb < iters; ++kb) {
+          const bool first = in_chunk == 0;
+          const bool last = ++in_chunk == p.chunk_iters || kb == iters - 1;
+          if (last) in_chunk = 0;
+          if (first) wait(&acc_empty[b], acc_parity);
+          if constexpr (G::kTwo) {
+            if (ok) ok = mbarWaitCluster(&full[s], static_cast<uint32_t>(parity), p.err);
+          } else {
+            wait(&full[s], parity);
+          }
+          if (leader) {
+            tcgenFenceAfter();
+            issueSlice<G>(tmem_base, tmem_base + static_cast<uint32_t>(b * kBN), smemAddr(smem), desc_a,
+                          desc_b, s, n, !first);
+            if constexpr (G::kTwo) {
+              mmaCommitBoth(&empty[s]);
+              if (last) mmaCommitBoth(&acc_full[b]);
+            } else {
+              mmaCommit(&empty[s]);
+              if (last) mmaCommit(&acc_full[b]);
+            }
+          }
+          __syncwarp();
+          if (last) {
+            b ^= 1;
+            if (b == 0) acc_parity ^= 1;
+          }
+          if (++s == kStages) {
+            s = 0;
+            parity ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    regAlloc<216>();
+    constexpr int kHalf = kBN / 2;
+    constexpr int kBlocks = kHalf / 8;
+    const int quarter = warp % 4;
+    const int col_begin = (warp - kEpilogueWarp0) / 4 * kHalf;
+    const int lower = quarter % 2, pair = (warp - kEpilogueWarp0) / 2;
+    unsigned char *out = out_smem + (warp - kEpilogueWarp0) * G::kOutWarp;
+    const bool vector = reinterpret_cast<uintptr_t>(p.c) % 16 == 0 && p.ldc % 8 == 0;
+    const int chunks = iters > 0 ? (iters - 1) / p.chunk_iters + 1 : 0;
+    int b = 0, acc_parity = 0;
+    for (int i = worker; i < tiles; i += workers) {
+      const Tile t = tileAt<G>(p, table, i);
+      float2 acc[kBlocks * 4];
+#pragma unroll
+      for (int j = 0; j < kBlocks * 4; ++j) acc[j] = make_float2(0.0F, 0.0F);
+      for (int ch = 0; ch < chunks; ++ch) {
+        wait(&acc_full[b], acc_parity);
+        tcgenFenceAfter();
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                               static_cast<uint32_t>(b * kBN + col_begin);
+        if constexpr (G::kFp32) addRows<kHalf, false>(taddr, acc, nullptr, 0.0F);
+        else addFragments<kHalf, false>(taddr, acc, nullptr, 0.0F, lane);
+        tcgenFenceBefore();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (G::kTwo) mbarArriveClusterRelaxed(clusterAddr(smemAddr(&acc_empty[b]), 0));
+          else mbarArrive(&acc_empty[b]);
+        }
+        b ^= 1;
+        if (b == 0) acc_parity ^= 1;
+      }
+      const int row0 = t.m0 + rank * kBM + quarter * 32;
+      const int cols = t.cols - col_begin;
+      if (row0 - (G::kFp32 ? 0 : lower * 32) < p.m && cols > 0) {
+        Place to;
+        to.row = row0;
+        to.col = t.n0 + col_begin;
+        to.at = static_cast<size_t>(to.col) * p.ldc + row0;
+        to.matrix = 0;
+        to.rows = p.m - row0;
+        to.cols = cols;
+        to.clip = false;
+        to.vector = vector;
+        if constexpr (G::kFp32) storeFp32<kHalf>(p, to, acc, out, lane);
+        else storeBf16<kBlocks>(p, to, acc, out - lower * G::kOutWarp, pair, lower, lane);
+      }
+    }
+    if (lane == 0) bulkWait();   // every store has been made
+  }
+
+  tcgenFenceBefore();
+  __syncthreads();
+  if constexpr (G::kTwo) clusterSync();   // neither CTA leaves while the pair still works
+  if (warp == 2) {
+    tcgenFenceAfter();
+    if constexpr (G::kTwo) tmemDeallocPair(tmem_base, G::kTmemColumns);
+    else tmemDealloc(tmem_base, G::kTmemColumns);
+  }
+}
+
+// Few tokens: as thinProductKernel, clusters of `split` CTAs that share k.
+template <class G>
+__global__ void __launch_bounds__(kThinThreads, 1)
+    fp4ThinKernel(const __grid_constant__ Fp4Params f, int split) {
+  constexpr int kBN = G::kBN;
+  constexpr int kStages = G::kStages;
+  constexpr int kStageBytes = G::kStageBytes;
+  constexpr int kPitch = G::kPartPitch;
+  const Params &p = f.p;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ GroupTable table;
+  unsigned char *smem = smem_raw + ((1024 - (smemAddr(smem_raw) & 1023)) & 1023);
+  float *part = reinterpret_cast<float *>(smem + kStages * kStageBytes);
+  unsigned char *raw = smem + kStages * kStageBytes + G::kPartBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(raw + G::kRawBytes);
+  uint64_t *empty = full + kStages;
+  uint64_t *acc_full = empty + kStages;
+  uint64_t *acc_empty = acc_full + G::kAccums;
+  uint64_t *part_full = acc_empty + G::kAccums;
+  uint64_t *part_free = part_full + 1;
+
+  const int warp = uniformWarp(), lane = threadIdx.x % 32;
+  const int rank = static_cast<int>(blockIdx.x) % split;
+  const int worker = static_cast<int>(blockIdx.x) / split;
+  const int workers = static_cast<int>(gridDim.x) / split;
+  if (threadIdx.x == 0) {
+    if (p.k > 0) {
+      prefetchTensorMap(&p.tma_a);
+      prefetchTensorMap(&p.tma_b);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbarInit(&full[s], 2);
+      mbarInit(&empty[s], 1);
+    }
+    for (int b = 0; b < G::kAccums; ++b) {
+      mbarInit(&acc_full[b], 1);
+      mbarInit(&acc_empty[b], kThinEpilogue / 32);
+    }
+    mbarInit(part_full, 1);
+    mbarInit(part_free, static_cast<uint32_t>(split));
+    fenceBarrierInit();
+  }
+  if (warp == 2) {
+    tmemAlloc(&tmem_base_slot, G::kTmemColumns);
+    tmemRelinquish();
+  }
+  tcgenFenceBefore();
+  __syncthreads();
+  if (split > 1) clusterSync();   // the cluster's barriers exist
+  tcgenFenceAfter();
+  allowDependentLaunch();
+  gridDependencyWait();
+  if (warp == 0) readGroups<G>(p, &table, lane);
+  __syncthreads();
+  const uint32_t tmem_base = tmem_base_slot;
+  const int tiles = tileCount<G>(p, table);
+  // This CTA's slices of k.
+  const int iters = (p.k + kRowBytes - 1) / kRowBytes;
+  const int kb0 = static_cast<int>(static_cast<long long>(iters) * rank / split);
+  const int kb1 = static_cast<int>(static_cast<long long>(iters) * (rank + 1) / split);
+  const int mine = kb1 - kb0;
+
+  bool ok = true;
+  auto wait = [&](uint64_t *bar, int parity) {
+    if (ok) ok = mbarWait(bar, static_cast<uint32_t>(parity), p.err);
+  };
+
+  if (warp == 0 && electOne()) {
+    // ---------------- TMA producer ----------------
+    int s = 0, parity = 1;
+    for (int i = worker; i < tiles; i += workers) {
+      const Tile t = tileAt<G>(p, table, i);
+      const int boxes = (t.cols + kThinBox - 1) / kThinBox;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        wait(&empty[s], parity);
+        if (!ok) continue;
+        unsigned char *sa = smem + s * kStageBytes;
+        mbarArriveExpectTx(&full[s], G::kABytes + static_cast<uint32_t>(boxes * kThinBox * kRowBytes));
+        tmaLoad3d(sa, &p.tma_a, &full[s], kb * kRowBytes, t.m0, t.group);
+        for (int j = 0; j < boxes; ++j)
+          tmaLoad3d(sa + G::kABytes + j * kThinBox * kRowBytes, &p.tma_b, &full[s], kb * kRowBytes,
+                    t.n0 + j * kThinBox, 0);
+        if (++s == kStages) {
+          s = 0;
+          parity ^= 1;
+        }
+      }
+    }
+    // The last copies have landed and been read (productKernel).
+#pragma unroll 1
+    for (int j = 0; j < kStages; ++j) {
+      wait(&full[s], parity);
+      wait(&empty[s], parity);
+      if (++s == kStages) {
+        s = 0;
+        parity ^= 1;
+      }
+    }
+  } else if (warp == kScaleWarp) {
+    // ---------------- scales ----------------
+    stageScales<G, kStages>(
+        f, table, tiles, worker, workers, 0, kb0, kb1, smem, raw, lane,
+        [&](int s, int parity) { wait(&empty[s], parity); },
+        [&](int s) {
+          if (lane == 0) mbarArrive(&full[s]);
+        });
+    cpAsyncWait<0>();
+  } else if (warp == 1 && electOne()) {
+    // ---------------- MMA issuer ----------------
+    int s = 0, parity = 0;
+    int b = 0, acc_parity = 1;
+    const uint64_t desc_a = smemDesc<false>(smemAddr(smem));
+    const uint64_t desc_b = smemDesc<false>(smemAddr(smem) + G::kABytes);
+    for (int i = worker; i < tiles; i += workers) {
+      const Tile t = tileAt<G>(p, table, i);
+      const int n = (t.cols + 15) / 16 * 16;
+      int in_chunk = 0;
+      for (int j = 0; j < mine; ++j) {
+        const bool first = in_chunk == 0;
+        const bool last = ++in_chunk == p.chunk_iters || j == mine - 1;
+        if (last) in_chunk = 0;
+        if (first) wait(&acc_empty[b], acc_parity);
+        wait(&full[s], parity);
+        tcgenFenceAfter();
+        issueSlice<G>(tmem_base, tmem_base + static_cast<uint32_t>(b * kBN), smemAddr(smem), desc_a, desc_b,
+                      s, n, !first);
+        mmaCommit(&empty[s]);
+        if (last) {
+          mmaCommit(&acc_full[b]);
+          if (++b == G::kAccums) {
+            b = 0;
+            acc_parity ^= 1;
+          }
+        }
+        if (++s == kStages) {
+          s = 0;
+          parity ^= 1;
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue ----------------
+    const int quarter = warp % 4;
+    const int row = quarter * 32 + lane;
+    const int etid = threadIdx.x % kThinEpilogue;
+    const int chunks = mine > 0 ? (mine - 1) / p.chunk_iters + 1 : 0;
+    int b = 0, acc_parity = 0;
+    int part_parity = 0;
+    for (int i = worker; i < tiles; i += workers) {
+      const Tile t = tileAt<G>(p, table, i);
+      float acc[kBN];
+#pragma unroll
+      for (int j = 0; j < kBN; ++j) acc[j] = 0.0F;
+      for (int ch = 0; ch < chunks; ++ch) {
+        wait(&acc_full[b], acc_parity);
+        tcgenFenceAfter();
+        const uint32_t taddr =
+            tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(b * kBN);
+        constexpr int kLoad = kBN < 32 ? kBN : 32;
+#pragma unroll
+        for (int c = 0; c < kBN; c += kLoad) {
+          if (c < t.cols) {
+            uint32_t v[kLoad];
+            if constexpr (kLoad == 16) tmemLoad16(taddr + c, v);
+            else tmemLoad32(taddr + c, v);
+#pragma unroll
+            for (int j = 0; j < kLoad; ++j) acc[c + j] += __uint_as_float(v[j]);
+          }
+        }
+        tcgenFenceBefore();
+        __syncwarp();
+        if (lane == 0) mbarArrive(&acc_empty[b]);
+        if (++b == G::kAccums) {
+          b = 0;
+          acc_parity ^= 1;
+        }
+      }
+      if (split == 1) {
+        if (t.m0 + row < p.m) {
+          const size_t at = static_cast<size_t>(t.n0) * p.ldc + t.m0 + row;
+          if (p.c_bf16) storeRow<kBN>(p, static_cast<__nv_bfloat16 *>(p.c) + at, t.cols, acc);
+          else storeRow<kBN>(p, static_cast<float *>(p.c) + at, t.cols, acc);
+        }
+        continue;
+      }
+      // Each row's sums to the CTA that writes the row (thinProductKernel).
+      if (ok) ok = mbarWaitCluster(part_free, part_parity ^ 1, p.err);
+      const int rows = kBM / split;
+      const int owner = row / rows;
+      const int width = (t.cols + 3) / 4 * 4;
+      if (etid == 0) mbarArriveExpectTx(part_full, static_cast<uint32_t>(kBM * width * 4));
+      const uint32_t to = clusterAddr(
+          smemAddr(part) + static_cast<uint32_t>((rank * rows + row - owner * rows) * kPitch) * 4,
+          static_cast<uint32_t>(owner));
+      const uint32_t bar = clusterAddr(smemAddr(part_full), static_cast<uint32_t>(owner));
+#pragma unroll
+      for (int j = 0; j < kBN; j += 4)
+        if (j < t.cols)
+          storeAsyncCluster4(to + static_cast<uint32_t>(j) * 4, bar, acc[j], acc[j + 1], acc[j + 2],
+                             acc[j + 3]);
+      if (ok) ok = mbarWaitCluster(part_full, part_parity, p.err);
+      for (int e = etid; e < rows * t.cols; e += kThinEpilogue) {
+        const int col = e / rows, r = e - col * rows;
+        float v[kMaxSplit];
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; ++q)
+          v[q] = q < split ? part[(q * rows + r) * kPitch + col] : 0.0F;
+        float sum = v[0];
+#pragma unroll
+        for (int q = 1; q < kMaxSplit; ++q) sum += v[q];
+        const int to_row = t.m0 + rank * rows + r;
+        if (to_row < p.m) {
+          const size_t at = static_cast<size_t>(t.n0 + col) * p.ldc + to_row;
+          if (p.c_bf16) storeScaled(p, static_cast<__nv_bfloat16 *>(p.c) + at, sum);
+          else storeScaled(p, static_cast<float *>(p.c) + at, sum);
+        }
+      }
+      namedBarrier<1, kThinEpilogue>();
+      if (etid < split)
+        mbarArriveCluster(clusterAddr(smemAddr(part_free), static_cast<uint32_t>(etid)));
+      part_parity ^= 1;
+    }
+  }
+
+  tcgenFenceBefore();
+  __syncthreads();
+  if (split > 1) clusterSync();   // no CTA leaves while another reads its part
+  if (warp == 2) {
+    tcgenFenceAfter();
+    tmemDealloc(tmem_base, G::kTmemColumns);
+  }
+}
+
+}  // namespace sgblas::kern::prod
+
+#endif  // SGBLAS_B200_PRODUCT_FP4_CUH_

@@ -284,8 +284,42 @@ __device__ __forceinline__ void mmaNarrow(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
   }
 }
-// Arrives (once) on `bar` when every tcgen05.mma this thread issued so far
-// has completed.
+// 4-bit inputs (e2m1) with a power of two for each 32 of k (kind::mxf4: 64 of k, two
+// scales, per instruction), whose scales lie in TMEM at sfa and sfb; kPair:
+// issued for both CTAs.
+template <bool kPair>
+__device__ __forceinline__ void mmaFp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                       uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
+  if constexpr (kPair) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(sfa),
+        "r"(sfb)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(sfa),
+        "r"(sfb)
+        : "memory");
+  }
+}
+// 32 rows of 16 bytes from shared memory to four TMEM columns of lanes 0-31, and
+// the same to the other three quarters; executed in order with the tcgen05.mma
+// that this thread issues after it.
+template <bool kPair>
+__device__ __forceinline__ void tmemCopyScales(uint32_t taddr, uint64_t desc) {
+  if constexpr (kPair)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Arrives (once) on `bar` when every tcgen05.mma and tcgen05.cp this thread
+// issued so far has completed.
 __device__ __forceinline__ void mmaCommit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    smemAddr(bar))

@@ -137,6 +137,74 @@ def test_gather_backward_has_nothing_to_do(handle, kw):
     assert handle.gather_tokens_backward_status(*move_back_args(**kw)) == OK
 
 
+def quantize4_args(**kw):
+    a = dict(k=301, n=20, x=FAKE, xtype=BF16, ldx=301, q=FAKE, ldq=151, scale=FAKE, ldscale=10, batch=2)
+    a.update(kw)
+    return list(a.values())
+
+
+def fp4_args(**kw):
+    a = dict(m=64, n=32, k=301, groups=4, offsets=FAKE, a=FAKE, lda=151, stride_a=64 * 151, scale_a=FAKE, ldsa=10,
+             stride_sa=640, b=FAKE, ldb=151, scale_b=FAKE, ldsb=10, c=FAKE, ctype=BF16, ldc=64)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("kw", [dict(k=-1), dict(n=-1), dict(batch=-1), dict(xtype=BAD_TYPE), dict(xtype=BYTE),
+                                dict(ldx=300), dict(ldq=150), dict(ldscale=9), dict(x=None), dict(q=None),
+                                dict(scale=None)])
+def test_quantize_fp4_refuses(handle, kw):
+    assert handle.quantize_fp4_status(*quantize4_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.quantize_fp4(*quantize4_args(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(k=0, x=None), dict(n=0, q=None), dict(batch=0, scale=None)])
+def test_quantize_fp4_has_nothing_to_do(handle, kw):
+    assert handle.quantize_fp4_status(*quantize4_args(**kw)) == OK
+
+
+def test_quantize_fp4_limit(handle):
+    big = 2**31 - 1
+    assert handle.quantize_fp4_status(*quantize4_args(k=64, n=big, ldx=64, ldq=32, ldscale=2, batch=1)) == UNSUPPORTED
+
+
+FP4_REFUSALS = [dict(m=-1), dict(n=-1), dict(k=-1), dict(ctype=BAD_TYPE), dict(ctype=BYTE), dict(lda=150), dict(ldb=150),
+                dict(ldc=63), dict(ldsa=9), dict(ldsb=9), dict(a=None), dict(b=None), dict(scale_a=None),
+                dict(scale_b=None), dict(c=None)]
+
+
+@pytest.mark.parametrize("kw", FP4_REFUSALS + [dict(groups=-1), dict(offsets=None)])
+def test_grouped_fp4_refuses(handle, kw):
+    assert handle.grouped_gemm_fp4_status(*fp4_args(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.grouped_gemm_fp4(*fp4_args(**kw))
+
+
+def one_matrix(**kw):
+    names = ("m", "n", "k", "groups", "offsets", "a", "lda", "stride_a", "scale_a", "ldsa", "stride_sa", "b", "ldb",
+             "scale_b", "ldsb", "c", "ctype", "ldc")
+    return [v for name, v in zip(names, fp4_args(**kw)) if name not in ("groups", "offsets", "stride_a", "stride_sa")]
+
+
+@pytest.mark.parametrize("kw", FP4_REFUSALS)
+def test_fp4_refuses(handle, kw):
+    assert handle.gemm_fp4_status(*one_matrix(**kw)) == INVALID
+    with pytest.raises(sg.SgblasError):
+        handle.gemm_fp4(*one_matrix(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(m=0, a=None, ldc=1), dict(n=0, c=None), dict(groups=0, offsets=None)])
+def test_fp4_has_nothing_to_do(handle, kw):
+    assert handle.grouped_gemm_fp4_status(*fp4_args(**kw)) == OK
+    if "groups" not in kw:
+        assert handle.gemm_fp4_status(*one_matrix(**kw)) == OK
+
+
+def test_fp4_groups(handle):
+    assert handle.grouped_gemm_fp4_status(*fp4_args(groups=sg.SGBLAS_MAX_GROUPS + 1)) == UNSUPPORTED
+
+
 def test_bytes_are_no_type_of_products(handle):
     assert handle.quantize_fp8_status(300, 20, 1, FAKE, BYTE, 300, FAKE, 300, FAKE, 3) == INVALID
     assert handle.gemm_fp8_status(64, 32, 300, FAKE, 300, FAKE, 3, FAKE, 300, FAKE, 3, FAKE, BYTE,
@@ -151,5 +219,7 @@ def test_null_handle():
     for name, args in (("sgblasRmsNorm", norm_args()), ("sgblasRmsNormBackward", back),
                        ("sgblasSortTokens", sort_args()), ("sgblasScatterTokens", move_args()),
                        ("sgblasGatherTokens", move_args()),
-                       ("sgblasGatherTokensBackward", move_back_args())):
+                       ("sgblasGatherTokensBackward", move_back_args()),
+                       ("sgblasQuantizeFp4", [300, 20, 1, FAKE, BF16, 300, 0, FAKE, 150, 0, FAKE, 10, 0]),
+                       ("sgblasGemmFp4", one_matrix()), ("sgblasGroupedGemmFp4", fp4_args())):
         assert getattr(sg.lib, name)(none, *args) == sg.SGBLAS_STATUS_NOT_INITIALIZED
