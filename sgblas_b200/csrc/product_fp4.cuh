@@ -73,7 +73,7 @@ struct Fp4Cfg : Fp4Shape<kBN_, kTwo_, false> {
   static constexpr int kFit = (217 * 1024 - kOutBytes - S::kRawBytes) / S::kStageBytes;
   static constexpr int kLess = kFit < S::kFitColumns ? kFit : S::kFitColumns;
   static constexpr int kStages = kLess > 8 ? 8 : kLess;
-  static constexpr int kBarrierBytes = 8 * (2 * kStages + 2 * S::kAccums);
+  static constexpr int kBarrierBytes = 8 * (3 * kStages + 2 * S::kAccums);
   static constexpr int kSmemBytes =
       kStages * S::kStageBytes + kOutBytes + S::kRawBytes + kBarrierBytes + 1024;
   static_assert(kStages >= 3 && kSmemBytes <= 218 * 1024 + 512, "shared memory beside the table");
@@ -226,7 +226,10 @@ __device__ __forceinline__ void issueSlice(uint32_t tmem_base, uint32_t d_tmem, 
 }
 
 // Many tokens: as productKernel.
-//   full[s]   stage s has its operands (TMA) and the scales of each CTA (kScaleWarp)
+//   full[s]     stage s has its operands (TMA) and the scales of each CTA (kScaleWarp)
+//   relayed[s]  a pair's odd CTA has its scales in stage s: its idle warp 1 passes that on,
+//               for a release at cluster scope would wait for the chunks that
+//               kScaleWarp has on their way (1700 clocks a slice instead of 400)
 template <class G>
 __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_constant__ Fp4Params f) {
   constexpr int kBN = G::kBN;
@@ -243,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
   uint64_t *empty = full + kStages;
   uint64_t *acc_full = empty + kStages;
   uint64_t *acc_empty = acc_full + kAccums;
+  uint64_t *relayed = acc_empty + kAccums;
 
   const int warp = uniformWarp(), lane = threadIdx.x % 32;
   const int rank = G::kTwo ? static_cast<int>(blockIdx.x & 1) : 0;
@@ -257,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
     for (int s = 0; s < kStages; ++s) {
       mbarInit(&full[s], G::kTwo ? 3 : 2);
       mbarInit(&empty[s], 1);
+      mbarInit(&relayed[s], 1);
     }
     for (int b = 0; b < kAccums; ++b) {
       mbarInit(&acc_full[b], 1);
@@ -337,11 +342,24 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
           f, table, tiles, worker, workers, rank, 0, iters, smem, raw, lane,
           [&](int s, int parity) { wait(&empty[s], parity); },
           [&](int s) {
-            if (lane != 0) return;
-            if constexpr (G::kTwo) mbarArriveCluster(clusterAddr(smemAddr(&full[s]), 0));
-            else mbarArrive(&full[s]);
+            if (lane == 0) mbarArrive(rank == 0 ? &full[s] : &relayed[s]);
           });
       cpAsyncWait<0>();
+    } else if (warp == 1 && rank == 1) {
+      // ---------------- relay of the odd CTA's scales ----------------
+      if (electOne()) {
+        int s = 0, parity = 0;
+        for (int i = worker; i < tiles; i += workers) {
+          for (int kb = 0; kb < iters; ++kb) {
+            wait(&relayed[s], parity);
+            mbarArriveClusterRelaxed(clusterAddr(smemAddr(&full[s]), 0));
+            if (++s == kStages) {
+              s = 0;
+              parity ^= 1;
+            }
+          }
+        }
+      }
     } else if (warp == 1 && rank == 0) {
       // ---------------- MMA issuer ----------------
       const bool leader = electOne();
@@ -358,11 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
           const bool last = ++in_chunk == p.chunk_iters || kb == iters - 1;
           if (last) in_chunk = 0;
           if (first) wait(&acc_empty[b], acc_parity);
-          if constexpr (G::kTwo) {
-            if (ok) ok = mbarWaitCluster(&full[s], static_cast<uint32_t>(parity), p.err);
-          } else {
-            wait(&full[s], parity);
-          }
+          wait(&full[s], parity);
           if (leader) {
             tcgenFenceAfter();
             issueSlice<G>(tmem_base, tmem_base + static_cast<uint32_t>(b * kBN), smemAddr(smem), desc_a,
