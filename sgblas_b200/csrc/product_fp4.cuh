@@ -8,9 +8,9 @@
 // of k) takes two for every row of A and of B.
 //
 // Scales' way. In global memory they lie as bytes, contiguous along k, a row per
-// column of A or B. A warp of its own (kScaleWarp) copies 16 of a row at once (two
-// slices) into shared memory by cp.async, each lane the rows lane + 32 i, several
-// chunks ahead; it then writes a slice's, four per row and 128 of k, as the 512-byte
+// column of A or B. Two warps in turn copy 16 of a row at once (a chunk: two
+// slices) into shared memory by cp.async, each lane the rows lane + 32 i, a chunk or
+// more ahead; they then write a slice's, four per row and 128 of k, as the 512-byte
 // blocks that tcgen05.cp takes: 32 rows (lanes) of four words, word i for row
 // lane + 32 i. The issuer copies the blocks to TMEM before the slice's four
 // instructions. (Gathering them directly from global memory into the blocks would
@@ -26,8 +26,8 @@
 namespace sgblas::kern::prod {
 
 constexpr int kScaleBlock = 512;     // bytes: four scales of each of 128 rows
-constexpr int kScaleWarp = 3;
-constexpr int kRawChunks = 4;        // chunks of 16 scales per row: one at work, the others on their way
+constexpr int kScaleWarp0 = 2, kScaleWarps = 2;
+constexpr int kRawChunks = 2;        // chunks of 16 scales per row: one at work, the next on its way
 constexpr int kSliceScales = 8;      // of a row in a slice
 
 struct Fp4Params {
@@ -55,7 +55,7 @@ struct Fp4Shape {
   static constexpr int kScaleColumns = kScaleBytes / 128;   // of TMEM
   static constexpr int kStageBytes = kABytes + kBBytes + kScaleBytes;
   static constexpr int kRawRows = kBM + kBN;
-  static constexpr int kRawBytes = kRawChunks * kRawRows * 16;
+  static constexpr int kRawBytes = kScaleWarps * kRawChunks * kRawRows * 16;
   static constexpr int kAccums = kThin_ ? (kBN == 64 ? 4 : 8) : 2;
   static constexpr int kScaleColumn0 = kAccums * kBN;
   static constexpr int kFitColumns = (512 - kScaleColumn0) / kScaleColumns;
@@ -110,96 +110,120 @@ __device__ __forceinline__ uint64_t scaleDesc(uint32_t addr) {
          (static_cast<uint64_t>(8) << 32) | (static_cast<uint64_t>(1) << 46);
 }
 
-// The role of kScaleWarp: the scales of every slice [kb0, kb1) of this worker's tiles into
-// the ring's stages. `ready(s)` announces stage s.
+// The role of the scales' warps: the scales of every slice [kb0, kb1) of this worker's
+// tiles into the ring's stages. Warp `part` of kScaleWarps takes every kScaleWarps-th
+// chunk, with its own raw buffers; `ready(s)` announces stage s.
 template <class G, int kStages, class Wait, class Ready>
 __device__ __forceinline__ void stageScales(const Fp4Params &f, const GroupTable &table, int tiles,
                                             int worker, int workers, int rank, int kb0, int kb1,
-                                            unsigned char *ring, unsigned char *raw, int lane,
-                                            Wait wait, Ready ready) {
+                                            unsigned char *ring, unsigned char *raw, int part,
+                                            int lane, Wait wait, Ready ready) {
   const Params &p = f.p;
   const int chunk0 = kb0 / 2, chunk1 = (kb1 + 1) / 2;
   if (kb0 >= kb1) return;
-  // What is fetched next, chunks ahead of what is at work.
+  raw += part * (kRawChunks * G::kRawRows * 16);
+  // The chunk fetched next, ahead of the one at work: chunks are numbered over all
+  // of this worker's tiles, and every kScaleWarps-th is this warp's.
   int fetch_tile = worker, fetch_chunk = chunk0, fetched = 0;
-  const unsigned char *at_a = nullptr, *at_b = nullptr;
-  int rows_a = 0, rows_b = 0;
+  auto skip = [&](int chunks) {
+    fetch_chunk += chunks;
+    while (fetch_chunk >= chunk1) {
+      fetch_chunk -= chunk1 - chunk0;
+      fetch_tile += workers;
+    }
+  };
   auto fetch = [&]() {
     if (fetch_tile < tiles) {
-      if (fetch_chunk == chunk0) {
-        const Tile t = tileAt<G>(p, table, fetch_tile);
-        const int m0 = t.m0 + rank * kBM;
-        rows_a = p.m - m0;
-        rows_b = t.cols;
-        at_a = f.scale_a + t.group * f.stride_sa + static_cast<long long>(m0 + lane) * f.ldsa;
-        at_b = f.scale_b + static_cast<long long>(t.n0 + lane) * f.ldsb;
-      }
+      const Tile t = tileAt<G>(p, table, fetch_tile);
+      const int m0 = t.m0 + rank * kBM;
+      const unsigned char *a = f.scale_a + t.group * f.stride_sa +
+                               static_cast<long long>(m0 + lane) * f.ldsa + fetch_chunk * 16;
+      const unsigned char *b =
+          f.scale_b + static_cast<long long>(t.n0 + lane) * f.ldsb + fetch_chunk * 16;
       unsigned char *to = raw + (fetched % kRawChunks) * (G::kRawRows * 16) + lane * 16;
       const uint32_t bytes = static_cast<uint32_t>(min(16, f.blocks - fetch_chunk * 16));
 #pragma unroll
       for (int i = 0; i < kBM / 32; ++i) {
-        const bool in = lane + 32 * i < rows_a;
-        cpAsyncN<16>(to + i * 512, in ? at_a + static_cast<long long>(32 * i) * f.ldsa + fetch_chunk * 16 : f.scale_a,
-                     in ? bytes : 0);
+        const bool in = lane + 32 * i < p.m - m0;
+        cpAsync16Cg(to + i * 512, in ? a + static_cast<long long>(32 * i) * f.ldsa : f.scale_a, in ? bytes : 0);
       }
 #pragma unroll
       for (int i = 0; i < (G::kBN + 31) / 32; ++i) {
         if (G::kBN % 32 != 0 && lane >= G::kBN) break;
-        const bool in = lane + 32 * i < rows_b;
-        cpAsyncN<16>(to + (kBM / 32 + i) * 512,
-                     in ? at_b + static_cast<long long>(32 * i) * f.ldsb + fetch_chunk * 16 : f.scale_b,
-                     in ? bytes : 0);
+        const bool in = lane + 32 * i < t.cols;
+        cpAsync16Cg(to + (kBM / 32 + i) * 512, in ? b + static_cast<long long>(32 * i) * f.ldsb : f.scale_b,
+                    in ? bytes : 0);
       }
-      if (++fetch_chunk == chunk1) {
-        fetch_chunk = chunk0;
-        fetch_tile += workers;
-      }
+      skip(kScaleWarps);
     }
     cpAsyncCommit();
     ++fetched;
   };
+  skip(part);
 #pragma unroll 1
   for (int i = 0; i < kRawChunks - 1; ++i) fetch();
-  int s = 0, parity = 1, done = 0;
+  int s = 0, parity = 1, turn = 0, done = 0;
   for (int i = worker; i < tiles; i += workers) {
 #pragma unroll 1
     for (int c = chunk0; c < chunk1; ++c) {
-      fetch();   // into the chunk that this lane read last
-      cpAsyncWait<kRawChunks - 1>();
-      const unsigned char *from = raw + (done % kRawChunks) * (G::kRawRows * 16) + lane * 16;
-      ++done;
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        const int kb = 2 * c + half;
-        if (kb < kb0 || kb >= kb1) continue;
+      const int first = max(2 * c, kb0), slices = min(2 * c + 2, kb1) - first;
+      const bool mine = turn == part;
+      if (++turn == kScaleWarps) turn = 0;
+      int s2 = s + 1, parity2 = parity;   // of a second slice
+      if (s2 == kStages) {
+        s2 = 0;
+        parity2 ^= 1;
+      }
+      if (mine) {
+        fetch();   // into the chunk that this lane read last
+        cpAsyncWait<kRawChunks - 1>();
+        const unsigned char *from = raw + (done % kRawChunks) * (G::kRawRows * 16) + lane * 16;
+        ++done;
         wait(s, parity);
-        unsigned char *to = ring + s * G::kStageBytes + G::kABytes + G::kBBytes + lane * 16;
-        // Blocks: A's of the first and second 128 of k, then B's likewise.
+        if (slices > 1) wait(s2, parity2);
+        unsigned char *blocks = ring + G::kABytes + G::kBBytes + lane * 16;
+        // The chunk's first or second half goes to stage s, its second to s2 where
+        // both are there.
+        unsigned char *to = blocks + s * G::kStageBytes, *to2 = blocks + s2 * G::kStageBytes;
+        const bool upper = first % 2 != 0;
+        // Blocks of a stage: A's of the first and second 128 of k, then B's likewise.
 #pragma unroll
         for (int b = 0; b < 1 + G::kBBlocks; ++b) {
-          uint2 w[4];
+          uint4 w[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int row0 = (b * 4 + r) * 32;   // of the raw rows
-            w[r] = make_uint2(0, 0);
+            w[r] = make_uint4(0, 0, 0, 0);
             if (row0 < G::kRawRows && (row0 + 32 <= G::kRawRows || lane < G::kRawRows - row0))
-              w[r] = *reinterpret_cast<const uint2 *>(from + row0 * 16 + half * kSliceScales);
+              w[r] = *reinterpret_cast<const uint4 *>(from + row0 * 16);
           }
-          const int first = b == 0 ? 0 : 2 + (b - 1), next = b == 0 ? 1 : G::kBBlocks;
-          *reinterpret_cast<uint4 *>(to + first * kScaleBlock) = make_uint4(w[0].x, w[1].x, w[2].x, w[3].x);
-          *reinterpret_cast<uint4 *>(to + (first + next) * kScaleBlock) =
-              make_uint4(w[0].y, w[1].y, w[2].y, w[3].y);
+          const int at = (b == 0 ? 0 : 1 + b) * kScaleBlock;
+          const int next = at + (b == 0 ? 1 : G::kBBlocks) * kScaleBlock;
+          const uint4 low[2] = {make_uint4(w[0].x, w[1].x, w[2].x, w[3].x),
+                                make_uint4(w[0].y, w[1].y, w[2].y, w[3].y)};
+          const uint4 high[2] = {make_uint4(w[0].z, w[1].z, w[2].z, w[3].z),
+                                 make_uint4(w[0].w, w[1].w, w[2].w, w[3].w)};
+          *reinterpret_cast<uint4 *>(to + at) = upper ? high[0] : low[0];
+          *reinterpret_cast<uint4 *>(to + next) = upper ? high[1] : low[1];
+          if (slices > 1) {
+            *reinterpret_cast<uint4 *>(to2 + at) = high[0];
+            *reinterpret_cast<uint4 *>(to2 + next) = high[1];
+          }
         }
         fenceProxyAsyncShared();
         __syncwarp();
         ready(s);
-        if (++s == kStages) {
-          s = 0;
-          parity ^= 1;
-        }
+        if (slices > 1) ready(s2);
+      }
+      s = s2;
+      parity = parity2;
+      if (slices > 1 && ++s == kStages) {
+        s = 0;
+        parity ^= 1;
       }
     }
   }
+  cpAsyncWait<0>();
 }
 
 // One slice: its scales to TMEM, then its instructions (one thread).
@@ -226,10 +250,10 @@ __device__ __forceinline__ void issueSlice(uint32_t tmem_base, uint32_t d_tmem, 
 }
 
 // Many tokens: as productKernel.
-//   full[s]     stage s has its operands (TMA) and the scales of each CTA (kScaleWarp)
+//   full[s]     stage s has its operands (TMA) and the scales of each CTA (the scales' warps)
 //   relayed[s]  a pair's odd CTA has its scales in stage s: its idle warp 1 passes that on,
 //               for a release at cluster scope would wait for the chunks that
-//               kScaleWarp has on their way (1700 clocks a slice instead of 400)
+//               those warps have on their way (1700 clocks a slice instead of 400)
 template <class G>
 __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_constant__ Fp4Params f) {
   constexpr int kBN = G::kBN;
@@ -336,15 +360,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
           parity ^= 1;
         }
       }
-    } else if (warp == kScaleWarp) {
+    } else if (warp >= kScaleWarp0) {
       // ---------------- scales ----------------
       stageScales<G, kStages>(
-          f, table, tiles, worker, workers, rank, 0, iters, smem, raw, lane,
+          f, table, tiles, worker, workers, rank, 0, iters, smem, raw, warp - kScaleWarp0, lane,
           [&](int s, int parity) { wait(&empty[s], parity); },
           [&](int s) {
             if (lane == 0) mbarArrive(rank == 0 ? &full[s] : &relayed[s]);
           });
-      cpAsyncWait<0>();
     } else if (warp == 1 && rank == 1) {
       // ---------------- relay of the odd CTA's scales ----------------
       if (electOne()) {
@@ -562,15 +585,14 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         parity ^= 1;
       }
     }
-  } else if (warp == kScaleWarp) {
+  } else if (warp == kScaleWarp0 || warp == kScaleWarp0 + 1) {
     // ---------------- scales ----------------
     stageScales<G, kStages>(
-        f, table, tiles, worker, workers, 0, kb0, kb1, smem, raw, lane,
+        f, table, tiles, worker, workers, 0, kb0, kb1, smem, raw, warp - kScaleWarp0, lane,
         [&](int s, int parity) { wait(&empty[s], parity); },
         [&](int s) {
           if (lane == 0) mbarArrive(&full[s]);
         });
-    cpAsyncWait<0>();
   } else if (warp == 1 && electOne()) {
     // ---------------- MMA issuer ----------------
     int s = 0, parity = 0;

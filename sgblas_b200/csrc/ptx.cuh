@@ -591,6 +591,13 @@ __device__ __forceinline__ void cpAsyncN(void *dst, const void *src, uint32_t by
                : "memory");
 }
 
+// The same of 16 bytes past the L1 cache.
+__device__ __forceinline__ void cpAsync16Cg(void *dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smemAddr(dst)), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+
 __device__ __forceinline__ void cpAsyncCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 template <int N>
