@@ -12,7 +12,7 @@ namespace sgblas::kern {
 
 constexpr int kLaneBlock = 128;
 
-// Aligned (kVector): consecutive values, one vector of 16 bytes. Otherwise four
+// Columns of whole aligned vectors (kVector): one vector of 16 bytes. Otherwise four
 // values 32 apart, so that a warp holds a block and its scalar accesses are
 // contiguous.
 template <typename T, bool kVector>
@@ -26,19 +26,22 @@ struct Lanes {
   static __device__ __forceinline__ int begin(int slot) {
     return kVector ? slot * kPer : slot / kThreads * kLaneBlock + slot % kThreads;
   }
-  // From `at`; `left` values of the column are there (the rest are zero). With
-  // kVector a thread's last vector may be partial.
+  // From `at`; `left` values of the column are there (whole vectors with kVector),
+  // the rest are zero. One predicated load: a branch to a partial form would keep
+  // a thread's loads from being issued together.
   __device__ __forceinline__ void load(const T *at, int left) {
-    if (kVector && left >= kPer) {
-      *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(at);
+    if constexpr (kVector) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (left > 0) w = *reinterpret_cast<const uint4 *>(at);
+      *reinterpret_cast<uint4 *>(v) = w;
     } else {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) v[j] = j * kStep < left ? at[j * kStep] : T{};
     }
   }
   __device__ __forceinline__ void store(T *at, int left) const {
-    if (kVector && left >= kPer) {
-      *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(v);
+    if constexpr (kVector) {
+      if (left > 0) *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(v);
     } else {
 #pragma unroll
       for (int j = 0; j < kPer; ++j)

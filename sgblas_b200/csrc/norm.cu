@@ -377,7 +377,8 @@ sgblasStatus_t launchBackward(const NormBackwardParams &p, const Shape &s, int c
   }
 }
 
-// Columns of vectors: base and distance multiples of 16 bytes. NULL is no matrix.
+// Columns that begin with whole vectors: base and distance multiples of 16 bytes. NULL
+// is no matrix.
 bool vectorColumns(const void *p, long long ld, int size) {
   return p == nullptr || (aligned16(p) && ld * size % 16 == 0);
 }
@@ -421,9 +422,11 @@ extern "C" sgblasStatus_t sgblasRmsNorm(sgblasHandle_t handle, int k, int n, sgb
   p.ldq = ldq;
   p.ldscale = ldscale;
   const int size = type == SGBLAS_TYPE_BF16 ? 2 : 4;
-  const bool vector = vectorColumns(x, ldx, size) && vectorColumns(residual, ldr, size) &&
+  const bool vector = k * static_cast<long long>(size) % 16 == 0 && vectorColumns(x, ldx, size) && vectorColumns(residual, ldr, size) &&
                       vectorColumns(weight, 0, size) && vectorColumns(sum, ldsum, size) &&
-                      vectorColumns(y, ldy, size) && vectorColumns(q, ldq, 1);
+                      vectorColumns(y, ldy, size) &&
+                      (q == nullptr || (reinterpret_cast<uintptr_t>(q) | static_cast<unsigned>(ldq)) %
+                                               static_cast<unsigned>(16 / size) == 0);
   const auto stream = static_cast<cudaStream_t>(handle->stream);
   if (type == SGBLAS_TYPE_BF16)
     return vector ? launchForward<__nv_bfloat16, true>(p, dev.sms, stream)
@@ -463,7 +466,7 @@ extern "C" sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, in
   p.lddsum = lddsum;
   p.lddx = lddx;
   const int size = type == SGBLAS_TYPE_BF16 ? 2 : 4;
-  const bool vector = vectorColumns(dy, lddy, size) && vectorColumns(sum, ldsum, size) &&
+  const bool vector = k * static_cast<long long>(size) % 16 == 0 && vectorColumns(dy, lddy, size) && vectorColumns(sum, ldsum, size) &&
                       vectorColumns(weight, 0, size) && vectorColumns(dsum, lddsum, size) &&
                       vectorColumns(dx, lddx, size);
   const auto stream = static_cast<cudaStream_t>(handle->stream);

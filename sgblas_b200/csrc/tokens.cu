@@ -346,7 +346,7 @@ sgblasStatus_t launchMoveTyped(Move move, const MoveParams &p, sgblasDataType_t 
   auto whole = [&](const void *at, long long ld) {
     return at == nullptr || (aligned16(at) && ld * size % 16 == 0);
   };
-  const bool vector = whole(p.x, p.ldx) && whole(p.dy, p.lddy) && whole(p.y, p.ldy);
+  const bool vector = p.k * static_cast<long long>(size) % 16 == 0 && whole(p.x, p.ldx) && whole(p.dy, p.lddy) && whole(p.y, p.ldy);
   if (type == SGBLAS_TYPE_FP32)
     return vector ? launchMove<float, true>(move, p, sms, stream)
                   : launchMove<float, false>(move, p, sms, stream);
