@@ -18,17 +18,23 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace sgblas::detail {
 namespace {
 
+using kern::both;
 using kern::Lanes;
 using kern::warpSum;
 
 constexpr int kMaxThreads = 512;
 constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxUnits = 4;          // vectors of a column that a thread holds
-constexpr int kReduceThreads = 256;
+constexpr int kMaxStages = 8;
+// Of the kernels fed by a ring: threads of a CTA, and CTAs that have to fit an SM.
+constexpr int streamThreads(int units) { return units == 4 ? 512 : 256; }
+constexpr int streamResident(int units) { return units == 4 ? 1 : 3; }
+constexpr int kReduceThreads = 1024;
 constexpr int kReduceWarps = kReduceThreads / 32;
 
 struct NormParams {
@@ -52,11 +58,16 @@ struct NormBackwardParams {
 
 // The sums of two values over the threads of one column (blockDim.x of them, a
 // multiple of 32; blockDim.y columns), the same in every thread, in a fixed order.
+// kBarrier: a barrier of the CTA even where a warp has the whole column.
+template <bool kBarrier = false>
 __device__ __forceinline__ float2 columnSum(float2 v, float2 *slots) {
   v.x = warpSum(v.x);
   v.y = warpSum(v.y);
   const int warps = static_cast<int>(blockDim.x) / 32;
-  if (warps == 1) return v;
+  if (warps == 1) {
+    if (kBarrier) __syncthreads();
+    return v;
+  }
   float2 *mine = slots + threadIdx.y * warps;
   if (threadIdx.x % 32 == 0) mine[threadIdx.x / 32] = v;
   __syncthreads();
@@ -77,53 +88,138 @@ __device__ __forceinline__ float inverseLength(float squares, int k, float eps) 
 template <typename T, bool kVector>
 __device__ __forceinline__ void addResidual(Lanes<T, kVector> *h, const Lanes<T, kVector> &r) {
 #pragma unroll
-  for (int j = 0; j < Lanes<T, kVector>::kPer; ++j) h->set(j, h->get(j) + r.get(j));
+  for (int i = 0; i < Lanes<T, kVector>::kPairs; ++i) h->setPair(i, __fadd2_rn(h->pair(i), r.pair(i)));
 }
+
+// What a thread does with its values of a column, whichever way they came: `rest`
+// values of the column are there from the thread's place `at` on.
+template <typename T, bool kVector>
+struct NormOf {
+  using L = Lanes<T, kVector>;
+  // In two sums, of the even and the odd values.
+  static __device__ __forceinline__ void square(const L &h, float2 *sum) {
+#pragma unroll
+    for (int i = 0; i < L::kPairs; ++i) *sum = __ffma2_rn(h.pair(i), h.pair(i), *sum);
+  }
+  // Every thread of a block of 128 values calls it (they share the block's scale).
+  static __device__ __forceinline__ void write(const NormParams &p, long long col, int slot, int rest,
+                                               float s, const L &h, const L &weight) {
+    const int at = L::begin(slot);
+    if (p.sum != nullptr) h.store(static_cast<T *>(p.sum) + col * p.ldsum + at, rest);
+    float2 f[L::kPairs];
+#pragma unroll
+    for (int i = 0; i < L::kPairs; ++i) {
+      f[i] = __fmul2_rn(h.pair(i), both(s));
+      if (p.weight != nullptr) f[i] = __fmul2_rn(f[i], weight.pair(i));
+    }
+    if (p.y != nullptr) {
+      L out;
+#pragma unroll
+      for (int i = 0; i < L::kPairs; ++i) out.setPair(i, f[i]);
+      out.store(static_cast<T *>(p.y) + col * p.ldy + at, rest);
+    }
+    if (p.q != nullptr) {
+      unsigned m = 0;
+#pragma unroll
+      for (int i = 0; i < L::kPairs; ++i) {
+        const unsigned a = __float_as_uint(f[i].x) & 0x7FFFFFFFu, b = __float_as_uint(f[i].y) & 0x7FFFFFFFu;
+        // A thread's values are all there or none with kVector.
+        if (kVector || 2 * i * L::kStep < rest) m = max(m, a);
+        if (kVector || (2 * i + 1) * L::kStep < rest) m = max(m, b);
+      }
+      if (rest <= 0) m = 0;
+#pragma unroll
+      for (int d = L::kThreads / 2; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const float scale = kern::fp8Scale(m);
+      kern::storeFp8<L::kPairs, L::kStep>(p.q + col * p.ldq + at, f, rest, __frcp_rn(scale));
+      if (rest > 0 && slot % L::kThreads == 0) p.scale[col * p.ldscale + slot / L::kThreads] = scale;
+    }
+  }
+};
+
+template <typename T, bool kVector>
+struct NormBackwardOf {
+  using L = Lanes<T, kVector>;
+  // Adds to the sums of h^2 and of h g, each in two parts.
+  static __device__ __forceinline__ void add(bool weighted, const L &h, const L &dy, const L &weight,
+                                             float2 *squares, float2 *products) {
+#pragma unroll
+    for (int i = 0; i < L::kPairs; ++i) {
+      const float2 v = h.pair(i);
+      const float2 g = weighted ? __fmul2_rn(dy.pair(i), weight.pair(i)) : dy.pair(i);
+      *squares = __ffma2_rn(v, v, *squares);
+      *products = __ffma2_rn(v, g, *products);
+    }
+  }
+  // dx to `dx`, and this column's part of dw (zero for a thread without values, whose
+  // dy is zero, unless s is not finite).
+  static __device__ __forceinline__ void finish(bool weighted, bool past, T *dx, int rest, float2 f,
+                                                const L &h, const L &dy, const L &weight, const L &ds,
+                                                float2 *dw) {
+    L out;
+#pragma unroll
+    for (int i = 0; i < L::kPairs; ++i) {
+      const float2 v = h.pair(i), y = dy.pair(i);
+      const float2 g = weighted ? __fmul2_rn(y, weight.pair(i)) : y;
+      const float2 inner = __ffma2_rn(v, both(-f.y), g);
+      out.setPair(i, past ? __fadd2_rn(__fmul2_rn(inner, both(f.x)), ds.pair(i)) : __fmul2_rn(inner, both(f.x)));
+      if (rest > 0) dw[i] = __ffma2_rn(y, __fmul2_rn(v, both(f.x)), dw[i]);
+    }
+    out.store(dx, rest);
+  }
+};
+
+// s, and s^2 times the mean of h g.
+__device__ __forceinline__ float2 backwardFactors(float2 sums, int k, float eps) {
+  const float s = inverseLength(sums.x, k, eps);
+  return make_float2(s, s * s * (sums.y / static_cast<float>(k)));
+}
+
+// ---- few columns, or columns that are not whole vectors ----------------------------
 
 // A column per blockDim.x threads, kUnits vectors (or groups of four values) per
 // thread; kLong: longer columns than that, read twice.
 template <typename T, bool kVector, int kUnits, bool kLong>
 __global__ void __launch_bounds__(kMaxThreads) rmsNormKernel(const NormParams p) {
   using L = Lanes<T, kVector>;
+  using N = NormOf<T, kVector>;
   __shared__ float2 slots[kMaxWarps];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
-  const long long col = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
-  const bool in = col < p.n;
+  const long long at = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
+  const bool in = at < p.n;
+  const long long col = in ? at : 0;
   const int stride = static_cast<int>(blockDim.x);
   // Slots of the column in whole warps: every thread of a warp takes part in its shuffles.
   const int rounds = ((p.k - 1) / kern::kLaneBlock * L::kThreads + L::kThreads + 31) / 32 * 32;
-  const T *x = static_cast<const T *>(p.x) + (in ? col * p.ldx : 0);
-  const T *r = p.residual == nullptr
-                   ? nullptr
-                   : static_cast<const T *>(p.residual) + (in ? col * p.ldr : 0);
+  const T *x = static_cast<const T *>(p.x) + col * p.ldx;
+  const T *r = p.residual == nullptr ? nullptr : static_cast<const T *>(p.residual) + col * p.ldr;
   auto left = [&](int slot) { return in ? p.k - L::begin(slot) : 0; };
-  auto read = [&](int slot, L *h) {
-    const int at = L::begin(slot);
-    h->load(x + at, left(slot));
-    if (r != nullptr) {
-      L v;
-      v.load(r + at, left(slot));
-      addResidual(h, v);
-    }
-  };
-  L h[kUnits], w[kUnits];
-  float squares = 0.0F;
-  auto square = [&](const L &v) {
-#pragma unroll
-    for (int j = 0; j < L::kPer; ++j) squares = fmaf(v.get(j), v.get(j), squares);
-  };
   auto readWeight = [&](int slot, L *v) {
     if (p.weight != nullptr)
       v->load(static_cast<const T *>(p.weight) + L::begin(slot), p.k - L::begin(slot));
   };
+  float2 squares = make_float2(0.0F, 0.0F);
   if constexpr (kLong) {
+    auto read = [&](int slot) {
+      L h;
+      h.load(x + L::begin(slot), left(slot));
+      if (r != nullptr) {
+        L v;
+        v.load(r + L::begin(slot), left(slot));
+        addResidual(&h, v);
+      }
+      return h;
+    };
+    for (int slot = threadIdx.x; slot < rounds; slot += stride) N::square(read(slot), &squares);
+    const float s = inverseLength(columnSum(make_float2(squares.x + squares.y, 0.0F), slots).x, p.k, p.eps);
     for (int slot = threadIdx.x; slot < rounds; slot += stride) {
-      read(slot, &h[0]);
-      square(h[0]);
+      L w;
+      readWeight(slot, &w);
+      N::write(p, col, slot, left(slot), s, read(slot), w);
     }
   } else {
-    L v[kUnits];
+    L h[kUnits], w[kUnits], v[kUnits];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int slot = threadIdx.x + u * stride;
@@ -135,99 +231,105 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormKernel(const NormParams p)
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       if (r != nullptr) addResidual(&h[u], v[u]);
-      square(h[u]);
+      N::square(h[u], &squares);
+    }
+    const float s = inverseLength(columnSum(make_float2(squares.x + squares.y, 0.0F), slots).x, p.k, p.eps);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int slot = threadIdx.x + u * stride;
+      N::write(p, col, slot, left(slot), s, h[u], w[u]);
     }
   }
-  const float s =
-      inverseLength(columnSum(make_float2(squares, 0.0F), slots).x, p.k, p.eps);
-  auto write = [&](int slot, const L &value, const L &weight) {
-    const int at = L::begin(slot), rest = left(slot);
-    if (p.sum != nullptr) value.store(static_cast<T *>(p.sum) + (in ? col * p.ldsum : 0) + at, rest);
-    float f[L::kPer];
+}
+
+// The sums of dw of a CTA's columns of threads (blockDim.y of them) to its row of
+// partial sums, in their order.
+template <typename L, int kUnits>
+__device__ __forceinline__ void storePart(const NormBackwardParams &p, float2 (&dw)[kUnits][L::kPairs],
+                                          float *exchange) {
+  float *part = p.part + static_cast<size_t>(blockIdx.x) * p.part_ld;
+  const int stride = static_cast<int>(blockDim.x);
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int at = L::begin(threadIdx.x + u * stride);
 #pragma unroll
     for (int j = 0; j < L::kPer; ++j) {
-      f[j] = value.get(j) * s;
-      if (p.weight != nullptr) f[j] *= weight.get(j);
+      float sum = j % 2 ? dw[u][j / 2].y : dw[u][j / 2].x;
+      if (blockDim.y > 1) {
+        __syncthreads();
+        exchange[threadIdx.y * stride + threadIdx.x] = sum;
+        __syncthreads();
+        sum = exchange[threadIdx.x];
+        for (unsigned y = 1; y < blockDim.y; ++y) sum += exchange[y * stride + threadIdx.x];
+      }
+      if (threadIdx.y == 0 && at + j * L::kStep < p.k) part[at + j * L::kStep] = sum;
     }
-    if (p.y != nullptr) {
-      L out;
-#pragma unroll
-      for (int j = 0; j < L::kPer; ++j) out.set(j, f[j]);
-      out.store(static_cast<T *>(p.y) + (in ? col * p.ldy : 0) + at, rest);
-    }
-    if (p.q != nullptr) {
-      unsigned m = 0;
-#pragma unroll
-      for (int j = 0; j < L::kPer; ++j)
-        if (j * L::kStep < rest) m = max(m, __float_as_uint(f[j]) & 0x7FFFFFFFu);
-#pragma unroll
-      for (int d = L::kThreads / 2; d > 0; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-      const float scale = kern::fp8Scale(m);
-      kern::storeFp8<L::kPer, L::kStep>(p.q + (in ? col * p.ldq : 0) + at, f, rest, __frcp_rn(scale));
-      if (rest > 0 && slot % L::kThreads == 0) p.scale[col * p.ldscale + slot / L::kThreads] = scale;
-    }
-  };
-  if constexpr (kLong) {
-    for (int slot = threadIdx.x; slot < rounds; slot += stride) {
-      read(slot, &h[0]);
-      readWeight(slot, &w[0]);
-      write(slot, h[0], w[0]);
-    }
-  } else {
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) write(threadIdx.x + u * stride, h[u], w[u]);
   }
 }
 
 // Walks the columns blockIdx.x * blockDim.y + threadIdx.y, ... of a persistent
-// grid; a row of partial sums of dw for each of its columns of threads.
+// grid, each CTA with a row of partial sums of dw.
 template <typename T, bool kVector, int kUnits, bool kLong>
 __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormBackwardParams p) {
   using L = Lanes<T, kVector>;
+  using N = NormBackwardOf<T, kVector>;
   __shared__ float2 slots[kMaxWarps];
+  __shared__ float exchange[kMaxThreads];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const int stride = static_cast<int>(blockDim.x);
   const int rounds = ((p.k - 1) / kern::kLaneBlock + 1) * L::kThreads;
   const long long first = blockIdx.x * static_cast<long long>(blockDim.y);
   const long long step = gridDim.x * static_cast<long long>(blockDim.y);
-  float *part = p.part == nullptr ? nullptr : p.part + (first + threadIdx.y) * p.part_ld;
-  float dw[kLong ? 1 : kUnits][L::kPer];
+  const bool weighted = p.weight != nullptr, past = p.dsum != nullptr;
+  const T *weight = static_cast<const T *>(p.weight);
+  float2 dw[kLong ? 1 : kUnits][L::kPairs];
   L w[kUnits];
   if constexpr (!kLong) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int at = L::begin(threadIdx.x + u * stride);
-      if (p.weight != nullptr) w[u].load(static_cast<const T *>(p.weight) + at, p.k - at);
+      if (weighted) w[u].load(weight + at, p.k - at);
 #pragma unroll
-      for (int j = 0; j < L::kPer; ++j) dw[u][j] = 0.0F;
+      for (int i = 0; i < L::kPairs; ++i) dw[u][i] = make_float2(0.0F, 0.0F);
     }
   }
   for (long long c = first; c < p.n; c += step) {
-    const long long col = c + threadIdx.y;
-    const bool in = col < p.n;
-    const T *h0 = static_cast<const T *>(p.sum) + (in ? col * p.ldsum : 0);
-    const T *dy0 = static_cast<const T *>(p.dy) + (in ? col * p.lddy : 0);
-    const T *ds0 = p.dsum == nullptr ? nullptr
-                                     : static_cast<const T *>(p.dsum) + (in ? col * p.lddsum : 0);
-    T *dx0 = static_cast<T *>(p.dx) + (in ? col * p.lddx : 0);
-    float2 sums = make_float2(0.0F, 0.0F);   // of h^2 and h g
-    auto add = [&](const L &h, const L &dy, const L &weight) {
-#pragma unroll
-      for (int j = 0; j < L::kPer; ++j) {
-        const float g = p.weight != nullptr ? dy.get(j) * weight.get(j) : dy.get(j);
-        sums.x = fmaf(h.get(j), h.get(j), sums.x);
-        sums.y = fmaf(h.get(j), g, sums.y);
-      }
-    };
+    const bool in = c + threadIdx.y < p.n;
+    const long long col = in ? c + threadIdx.y : 0;
+    const T *h0 = static_cast<const T *>(p.sum) + col * p.ldsum;
+    const T *dy0 = static_cast<const T *>(p.dy) + col * p.lddy;
+    const T *ds0 = past ? static_cast<const T *>(p.dsum) + col * p.lddsum : nullptr;
+    T *dx0 = static_cast<T *>(p.dx) + col * p.lddx;
+    float2 squares = make_float2(0.0F, 0.0F), products = squares;
     L h[kUnits], dy[kUnits], ds[kUnits];
     if constexpr (kLong) {
+      float *part = p.part == nullptr ? nullptr : p.part + static_cast<size_t>(blockIdx.x) * p.part_ld;
+      auto read = [&](int at) {
+        h[0].load(h0 + at, p.k - at);
+        dy[0].load(dy0 + at, p.k - at);
+        if (weighted) w[0].load(weight + at, p.k - at);
+      };
       for (int slot = threadIdx.x; slot < rounds; slot += stride) {
-        const int at = L::begin(slot), rest = in ? p.k - at : 0;
-        h[0].load(h0 + at, rest);
-        dy[0].load(dy0 + at, rest);
-        if (p.weight != nullptr) w[0].load(static_cast<const T *>(p.weight) + at, p.k - at);
-        add(h[0], dy[0], w[0]);
+        read(L::begin(slot));
+        N::add(weighted, h[0], dy[0], w[0], &squares, &products);
+      }
+      const float2 f = backwardFactors(columnSum(make_float2(squares.x + squares.y, products.x + products.y), slots), p.k, p.eps);
+      for (int slot = threadIdx.x; slot < rounds; slot += stride) {
+        const int at = L::begin(slot);
+        read(at);
+        if (past) ds[0].load(ds0 + at, p.k - at);
+#pragma unroll
+        for (int i = 0; i < L::kPairs; ++i) dw[0][i] = make_float2(0.0F, 0.0F);
+        N::finish(weighted, past, dx0 + at, p.k - at, f, h[0], dy[0], w[0], ds[0], dw[0]);
+        if (part != nullptr) {
+#pragma unroll
+          for (int j = 0; j < L::kPer; ++j) {
+            const int to = at + j * L::kStep;
+            const float v = j % 2 ? dw[0][j / 2].y : dw[0][j / 2].x;
+            if (to < p.k) part[to] = c != first ? part[to] + v : v;
+          }
+        }
       }
     } else {
 #pragma unroll
@@ -235,68 +337,197 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
         const int at = L::begin(threadIdx.x + u * stride), rest = in ? p.k - at : 0;
         h[u].load(h0 + at, rest);
         dy[u].load(dy0 + at, rest);
-        if (ds0 != nullptr) ds[u].load(ds0 + at, rest);
+        if (past) ds[u].load(ds0 + at, rest);
       }
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) add(h[u], dy[u], w[u]);
-    }
-    sums = columnSum(sums, slots);
-    const float s = inverseLength(sums.x, p.k, p.eps);
-    const float along = s * s * (sums.y / static_cast<float>(p.k));
-    auto finish = [&](const L &hv, const L &dyv, const L &weight, const L &dsv, int at, int rest,
-                      float *acc) {
-      L out;
-#pragma unroll
-      for (int j = 0; j < L::kPer; ++j) {
-        const float g = p.weight != nullptr ? dyv.get(j) * weight.get(j) : dyv.get(j);
-        float d = s * fmaf(-hv.get(j), along, g);
-        if (ds0 != nullptr) d += dsv.get(j);
-        out.set(j, d);
-        if (in) acc[j] = fmaf(dyv.get(j), hv.get(j) * s, acc[j]);
-      }
-      out.store(dx0 + at, rest);
-    };
-    if constexpr (kLong) {
-      for (int slot = threadIdx.x; slot < rounds; slot += stride) {
-        const int at = L::begin(slot), rest = in ? p.k - at : 0;
-        h[0].load(h0 + at, rest);
-        dy[0].load(dy0 + at, rest);
-        if (p.weight != nullptr) w[0].load(static_cast<const T *>(p.weight) + at, p.k - at);
-        if (ds0 != nullptr) ds[0].load(ds0 + at, rest);
-#pragma unroll
-        for (int j = 0; j < L::kPer; ++j)
-          dw[0][j] = part != nullptr && c != first && at + j * L::kStep < p.k ? part[at + j * L::kStep]
-                                                                            : 0.0F;
-        finish(h[0], dy[0], w[0], ds[0], at, rest, dw[0]);
-        if (part != nullptr) {
-#pragma unroll
-          for (int j = 0; j < L::kPer; ++j)
-            if (at + j * L::kStep < p.k) part[at + j * L::kStep] = dw[0][j];
-        }
-      }
-    } else {
+      for (int u = 0; u < kUnits; ++u) N::add(weighted, h[u], dy[u], w[u], &squares, &products);
+      const float2 f = backwardFactors(columnSum(make_float2(squares.x + squares.y, products.x + products.y), slots), p.k, p.eps);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int at = L::begin(threadIdx.x + u * stride);
-        finish(h[u], dy[u], w[u], ds[u], at, in ? p.k - at : 0, dw[u]);
+        N::finish(weighted, past, dx0 + at, in ? p.k - at : 0, f, h[u], dy[u], w[u], ds[u], dw[u]);
       }
     }
   }
   if constexpr (!kLong) {
-    if (part != nullptr) {
+    if (p.part != nullptr) storePart<L, kUnits>(p, dw, exchange);
+  }
+}
+
+// ---- many columns of whole vectors: a persistent grid fed by bulk copies -------------
+
+// A ring of stages in shared memory, each with blockDim.y columns of kRows operands
+// (x and the residual; h, dy and dsum), copied by cp.async.bulk ahead of the columns
+// at work. Registers hold a column only while it is worked on, and the copies do not
+// wait for its sums: with loads straight into registers, each column's latency was
+// uncovered (16384 x 4096 BF16 backward 152 to 192 us, forward 100 to 104).
+template <int kRows>
+struct Ring {
+  unsigned char *stages;
+  uint64_t *full;
+  int row_bytes, count;
+  const unsigned char *from[kRows];   // NULL: no such operand
+  long long ld[kRows];                // bytes
+
+  __device__ __forceinline__ unsigned char *row(int stage, int operand, int y) const {
+    return stages + static_cast<size_t>((stage * kRows + operand) * static_cast<int>(blockDim.y) + y) * row_bytes;
+  }
+  // The columns from `first` on (up to blockDim.y, of n) into a stage: one warp.
+  __device__ __forceinline__ void fill(int stage, long long first, int n) const {
+    const int columns = static_cast<int>(min(static_cast<long long>(blockDim.y), n - first));
+    int operands = 0;
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int at = L::begin(threadIdx.x + u * stride);
+    for (int o = 0; o < kRows; ++o) operands += from[o] != nullptr;
+    const int lane = threadIdx.x % 32;
+    if (lane == 0) kern::mbarArriveExpectTx(&full[stage], static_cast<uint32_t>(columns * operands * row_bytes));
+    __syncwarp();
+    if (lane < columns) {
 #pragma unroll
-        for (int j = 0; j < L::kPer; ++j)
-          if (at + j * L::kStep < p.k) part[at + j * L::kStep] = dw[u][j];
-      }
+      for (int o = 0; o < kRows; ++o)
+        if (from[o] != nullptr)
+          kern::bulkLoad(row(stage, o, lane), from[o] + (first + lane) * ld[o], &full[stage],
+                         static_cast<uint32_t>(row_bytes));
+    }
+  }
+};
+
+// Walks a persistent grid's columns: work(stage, column, in) for blockDim.y of them
+// at a time, which returns after a barrier of the CTA that follows its last read of
+// the stage.
+template <int kRows, class Work>
+__device__ __forceinline__ void walk(const Ring<kRows> &ring, int n, unsigned *err, Work work) {
+  const bool issuer = threadIdx.x < 32 && threadIdx.y == 0;
+  const long long first = blockIdx.x * static_cast<long long>(blockDim.y);
+  const long long step = gridDim.x * static_cast<long long>(blockDim.y);
+  if (issuer) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < ring.count; ++i) kern::mbarInit(&ring.full[i], 1);
+      kern::fenceBarrierInit();
+    }
+    __syncwarp();
+    for (int i = 0; i < ring.count; ++i)
+      if (first + i * step < n) ring.fill(i, first + i * step, n);
+  }
+  __syncthreads();
+  int stage = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  for (long long c = first; c < n; c += step) {
+    if (ok) ok = kern::mbarWait(&ring.full[stage], parity, err);
+    work(stage, c + threadIdx.y, c + threadIdx.y < n);
+    const long long next = c + ring.count * step;
+    if (issuer && next < n && ok) {
+      kern::fenceProxyAsyncShared();   // the reads above come before the copy
+      ring.fill(stage, next, n);
+    }
+    if (++stage == ring.count) {
+      stage = 0;
+      parity ^= 1;
     }
   }
 }
 
+template <typename T, int kUnits>
+__global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
+    rmsNormStreamKernel(const NormParams p, int stages, unsigned *err) {
+  using L = Lanes<T, true>;
+  using N = NormOf<T, true>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float2 slots[kMaxWarps];
+  __shared__ uint64_t full[kMaxStages];
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const int stride = static_cast<int>(blockDim.x);
+  Ring<2> ring = {smem, full, p.k * static_cast<int>(sizeof(T)), stages,
+                  {static_cast<const unsigned char *>(p.x), static_cast<const unsigned char *>(p.residual)},
+                  {p.ldx * static_cast<long long>(sizeof(T)), p.ldr * static_cast<long long>(sizeof(T))}};
+  L w[kUnits];
+  if (p.weight != nullptr) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at = L::begin(threadIdx.x + u * stride);
+      w[u].load(static_cast<const T *>(p.weight) + at, p.k - at);
+    }
+  }
+  walk(ring, p.n, err, [&](int stage, long long col, bool in) {
+    const T *x = reinterpret_cast<const T *>(ring.row(stage, 0, threadIdx.y));
+    const T *r = reinterpret_cast<const T *>(ring.row(stage, 1, threadIdx.y));
+    L h[kUnits];
+    float2 squares = make_float2(0.0F, 0.0F);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at = L::begin(threadIdx.x + u * stride), rest = in ? p.k - at : 0;
+      h[u].load(x + at, rest);
+      if (p.residual != nullptr) {
+        L v;
+        v.load(r + at, rest);
+        addResidual(&h[u], v);
+      }
+      N::square(h[u], &squares);
+    }
+    const float s = inverseLength(columnSum<true>(make_float2(squares.x + squares.y, 0.0F), slots).x, p.k, p.eps);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int slot = threadIdx.x + u * stride;
+      N::write(p, in ? col : 0, slot, in ? p.k - L::begin(slot) : 0, s, h[u], w[u]);
+    }
+  });
+}
+
+template <typename T, int kUnits>
+__global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
+    rmsNormBackwardStreamKernel(const NormBackwardParams p, int stages, unsigned *err) {
+  using L = Lanes<T, true>;
+  using N = NormBackwardOf<T, true>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float2 slots[kMaxWarps];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ float exchange[kMaxThreads];
+  kern::gridDependencyWait();
+  kern::allowDependentLaunch();
+  const int stride = static_cast<int>(blockDim.x);
+  constexpr long long kSize = sizeof(T);
+  Ring<3> ring = {smem, full, p.k * static_cast<int>(sizeof(T)), stages,
+                  {static_cast<const unsigned char *>(p.sum), static_cast<const unsigned char *>(p.dy),
+                   static_cast<const unsigned char *>(p.dsum)},
+                  {p.ldsum * kSize, p.lddy * kSize, p.lddsum * kSize}};
+  const bool weighted = p.weight != nullptr, past = p.dsum != nullptr;
+  float2 dw[kUnits][L::kPairs];
+  L w[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int at = L::begin(threadIdx.x + u * stride);
+    if (weighted) w[u].load(static_cast<const T *>(p.weight) + at, p.k - at);
+#pragma unroll
+    for (int i = 0; i < L::kPairs; ++i) dw[u][i] = make_float2(0.0F, 0.0F);
+  }
+  walk(ring, p.n, err, [&](int stage, long long col, bool in) {
+    const T *h0 = reinterpret_cast<const T *>(ring.row(stage, 0, threadIdx.y));
+    const T *dy0 = reinterpret_cast<const T *>(ring.row(stage, 1, threadIdx.y));
+    const T *ds0 = reinterpret_cast<const T *>(ring.row(stage, 2, threadIdx.y));
+    L h[kUnits], dy[kUnits], ds[kUnits];
+    float2 squares = make_float2(0.0F, 0.0F), products = squares;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at = L::begin(threadIdx.x + u * stride), rest = in ? p.k - at : 0;
+      h[u].load(h0 + at, rest);
+      dy[u].load(dy0 + at, rest);
+      if (past) ds[u].load(ds0 + at, rest);
+      N::add(weighted, h[u], dy[u], w[u], &squares, &products);
+    }
+    const float2 f = backwardFactors(columnSum<true>(make_float2(squares.x + squares.y, products.x + products.y), slots), p.k, p.eps);
+    T *dx0 = static_cast<T *>(p.dx) + (in ? col * p.lddx : 0);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at = L::begin(threadIdx.x + u * stride);
+      N::finish(weighted, past, dx0 + at, in ? p.k - at : 0, f, h[u], dy[u], w[u], ds[u], dw[u]);
+    }
+  });
+  if (p.part != nullptr) storePart<L, kUnits>(p, dw, exchange);
+}
+
 // dw = beta dw + the sum of `rows` rows of partial sums, 32 values per CTA, a
-// warp per eighth of the rows, in a fixed order.
+// warp per kReduceWarps-th row, in a fixed order.
 __global__ void __launch_bounds__(kReduceThreads)
     sumPartsKernel(const float *part, int rows, int part_ld, int k, float beta, float *dw) {
   __shared__ float slots[kReduceWarps][32];
@@ -319,61 +550,120 @@ __global__ void __launch_bounds__(kReduceThreads)
   dw[at] = s;
 }
 
-// How a column is spread over threads.
+// How columns are spread over threads.
 struct Shape {
-  int units;      // 1, 2 or 4; 0: longer than kMaxUnits per thread
+  int units;      // vectors of a thread: 1, 2 or 4; 0: more than kMaxUnits
   int threads;    // of a column, a multiple of 32
-  int columns;    // of a CTA
+  int columns;    // of a CTA at a time
+  int stages;     // of the ring; 0: loads straight into registers
+  int resident;   // CTAs per SM, of a persistent grid
 };
-Shape chooseShape(int k, int per, int n, int sms) {
+// `operands` columns are read for each one written (`vector`: in whole vectors).
+Shape chooseShape(int k, int size, bool vector, int n, int operands, int sms) {
+  const int per = vector ? 16 / size : 4;
   const int lanes = ((k - 1) / kern::kLaneBlock + 1) * (kern::kLaneBlock / per);
+  Shape s = {};
+  // A ring pays where a CTA walks several columns.
+  if (vector && n >= 4 * sms) {
+    s.units = lanes <= 32 ? 1 : lanes <= 2 * streamThreads(2) ? 2 : 4;
+    s.threads = ((lanes - 1) / s.units / 32 + 1) * 32;
+    s.columns = std::max(1, 256 / s.threads);
+    s.resident = s.units < 4 ? streamResident(s.units) : s.threads <= 256 ? 2 : 1;
+    const long long stage = static_cast<long long>(operands) * s.columns * k * size;
+    s.stages = static_cast<int>(std::min<long long>(kMaxStages, (216 * 1024 / s.resident - 6 * 1024) / stage));
+    if (s.threads <= streamThreads(s.units) && s.stages >= 2) return s;
+  }
   // Few columns: all of a column's loads at once, on as many threads.
-  int units = n <= 2 * sms ? 1 : lanes >= 128 ? 4 : 1;
+  int units = n <= 2 * sms ? 1 : lanes >= 128 ? 2 : 1;
   while (units < kMaxUnits && lanes > units * kMaxThreads) units *= 2;
-  Shape s;
   s.units = lanes > units * kMaxThreads ? 0 : units;
   s.threads = s.units == 0 ? kMaxThreads : ((lanes - 1) / units / 32 + 1) * 32;
   s.columns = std::max(1, 128 / s.threads);
+  s.resident = std::max(1, 768 / (s.threads * s.columns));
+  s.stages = 0;
   return s;
 }
 
-template <typename P>
-sgblasStatus_t launchNorm(void (*kernel)(P), const P &p, dim3 grid, dim3 block, cudaStream_t stream) {
+int persistentCtas(const Shape &s, int n, int sms) {
+  return std::min((n - 1) / s.columns + 1, sms * s.resident);
+}
+
+template <typename... Args, typename... Given>
+sgblasStatus_t launchNorm(void (*kernel)(Args...), dim3 grid, const Shape &s, size_t smem,
+                          cudaStream_t stream, const Given &...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = block;
+  cfg.blockDim = dim3(static_cast<unsigned>(s.threads), static_cast<unsigned>(s.columns));
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p));
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, static_cast<Args>(args)...));
+}
+
+template <typename P>
+sgblasStatus_t launchStream(void (*kernel)(P, int, unsigned *), std::atomic<uint64_t> *configured,
+                            const DeviceInfo &dev, int operands, int size, const Shape &s,
+                            cudaStream_t stream, const P &p) {
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, 216 * 1024, configured))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  const size_t smem = static_cast<size_t>(s.stages) * operands * s.columns * p.k * size;
+  return launchNorm(kernel, dim3(static_cast<unsigned>(persistentCtas(s, p.n, dev.sms))), s, smem, stream, p,
+                    s.stages, dev.err);
+}
+
+constexpr int kForwardRows = 2, kBackwardRows = 3;   // of a stage
+
+template <typename T, int kUnits>
+sgblasStatus_t launchForwardStream(const NormParams &p, const Shape &s, const DeviceInfo &dev,
+                                   cudaStream_t stream) {
+  static std::atomic<uint64_t> configured{0};
+  return launchStream(rmsNormStreamKernel<T, kUnits>, &configured, dev, kForwardRows, sizeof(T), s, stream, p);
+}
+template <typename T, int kUnits>
+sgblasStatus_t launchBackwardStream(const NormBackwardParams &p, const Shape &s, const DeviceInfo &dev,
+                                    cudaStream_t stream) {
+  static std::atomic<uint64_t> configured{0};
+  return launchStream(rmsNormBackwardStreamKernel<T, kUnits>, &configured, dev, kBackwardRows, sizeof(T), s,
+                      stream, p);
 }
 
 template <typename T, bool kVector>
-sgblasStatus_t launchForward(const NormParams &p, int sms, cudaStream_t stream) {
-  const Shape s = chooseShape(p.k, Lanes<T, kVector>::kPer, p.n, sms);
-  const dim3 block(static_cast<unsigned>(s.threads), static_cast<unsigned>(s.columns));
+sgblasStatus_t launchForward(const NormParams &p, const DeviceInfo &dev, cudaStream_t stream) {
+  const Shape s = chooseShape(p.k, sizeof(T), kVector, p.n, kForwardRows, dev.sms);
+  if constexpr (kVector) {
+    if (s.stages > 0)
+      return s.units == 1   ? launchForwardStream<T, 1>(p, s, dev, stream)
+             : s.units == 2 ? launchForwardStream<T, 2>(p, s, dev, stream)
+                            : launchForwardStream<T, 4>(p, s, dev, stream);
+  }
   const dim3 grid(static_cast<unsigned>((p.n - 1) / s.columns + 1));
   switch (s.units) {
-    case 1: return launchNorm(rmsNormKernel<T, kVector, 1, false>, p, grid, block, stream);
-    case 2: return launchNorm(rmsNormKernel<T, kVector, 2, false>, p, grid, block, stream);
-    case 4: return launchNorm(rmsNormKernel<T, kVector, 4, false>, p, grid, block, stream);
-    default: return launchNorm(rmsNormKernel<T, kVector, 1, true>, p, grid, block, stream);
+    case 1: return launchNorm(rmsNormKernel<T, kVector, 1, false>, grid, s, 0, stream, p);
+    case 2: return launchNorm(rmsNormKernel<T, kVector, 2, false>, grid, s, 0, stream, p);
+    case 4: return launchNorm(rmsNormKernel<T, kVector, 4, false>, grid, s, 0, stream, p);
+    default: return launchNorm(rmsNormKernel<T, kVector, 1, true>, grid, s, 0, stream, p);
   }
 }
 
 template <typename T, bool kVector>
-sgblasStatus_t launchBackward(const NormBackwardParams &p, const Shape &s, int ctas,
+sgblasStatus_t launchBackward(const NormBackwardParams &p, const Shape &s, const DeviceInfo &dev,
                               cudaStream_t stream) {
-  const dim3 block(static_cast<unsigned>(s.threads), static_cast<unsigned>(s.columns));
-  const dim3 grid(static_cast<unsigned>(ctas));
+  if constexpr (kVector) {
+    if (s.stages > 0)
+      return s.units == 1   ? launchBackwardStream<T, 1>(p, s, dev, stream)
+             : s.units == 2 ? launchBackwardStream<T, 2>(p, s, dev, stream)
+                            : launchBackwardStream<T, 4>(p, s, dev, stream);
+  }
+  const dim3 grid(static_cast<unsigned>(persistentCtas(s, p.n, dev.sms)));
   switch (s.units) {
-    case 1: return launchNorm(rmsNormBackwardKernel<T, kVector, 1, false>, p, grid, block, stream);
-    case 2: return launchNorm(rmsNormBackwardKernel<T, kVector, 2, false>, p, grid, block, stream);
-    case 4: return launchNorm(rmsNormBackwardKernel<T, kVector, 4, false>, p, grid, block, stream);
-    default: return launchNorm(rmsNormBackwardKernel<T, kVector, 1, true>, p, grid, block, stream);
+    case 1: return launchNorm(rmsNormBackwardKernel<T, kVector, 1, false>, grid, s, 0, stream, p);
+    case 2: return launchNorm(rmsNormBackwardKernel<T, kVector, 2, false>, grid, s, 0, stream, p);
+    case 4: return launchNorm(rmsNormBackwardKernel<T, kVector, 4, false>, grid, s, 0, stream, p);
+    default: return launchNorm(rmsNormBackwardKernel<T, kVector, 1, true>, grid, s, 0, stream, p);
   }
 }
 
@@ -429,10 +719,10 @@ extern "C" sgblasStatus_t sgblasRmsNorm(sgblasHandle_t handle, int k, int n, sgb
                                                static_cast<unsigned>(16 / size) == 0);
   const auto stream = static_cast<cudaStream_t>(handle->stream);
   if (type == SGBLAS_TYPE_BF16)
-    return vector ? launchForward<__nv_bfloat16, true>(p, dev.sms, stream)
-                  : launchForward<__nv_bfloat16, false>(p, dev.sms, stream);
-  return vector ? launchForward<float, true>(p, dev.sms, stream)
-                : launchForward<float, false>(p, dev.sms, stream);
+    return vector ? launchForward<__nv_bfloat16, true>(p, dev, stream)
+                  : launchForward<__nv_bfloat16, false>(p, dev, stream);
+  return vector ? launchForward<float, true>(p, dev, stream)
+                : launchForward<float, false>(p, dev, stream);
 }
 
 extern "C" sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, int n,
@@ -472,10 +762,8 @@ extern "C" sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, in
   const auto stream = static_cast<cudaStream_t>(handle->stream);
   int rows = 0;
   if (n > 0) {
-    const Shape s = chooseShape(k, vector ? 16 / size : 4, n, dev.sms);
-    const int threads = s.threads * s.columns;
-    const int ctas = std::min((n - 1) / s.columns + 1, dev.sms * std::max(1, 512 / threads));
-    rows = ctas * s.columns;
+    const Shape s = chooseShape(k, size, vector, n, kBackwardRows, dev.sms);
+    rows = persistentCtas(s, n, dev.sms);
     p.part_ld = (k + 3) / 4 * 4;
     if (dweight != nullptr) {
       const size_t bytes = sizeof(float) * static_cast<size_t>(p.part_ld) * static_cast<size_t>(rows);
@@ -485,11 +773,11 @@ extern "C" sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, in
                                          kCounterRegionBytes);
     }
     if (type == SGBLAS_TYPE_BF16)
-      st = vector ? launchBackward<__nv_bfloat16, true>(p, s, ctas, stream)
-                  : launchBackward<__nv_bfloat16, false>(p, s, ctas, stream);
+      st = vector ? launchBackward<__nv_bfloat16, true>(p, s, dev, stream)
+                  : launchBackward<__nv_bfloat16, false>(p, s, dev, stream);
     else
-      st = vector ? launchBackward<float, true>(p, s, ctas, stream)
-                  : launchBackward<float, false>(p, s, ctas, stream);
+      st = vector ? launchBackward<float, true>(p, s, dev, stream)
+                  : launchBackward<float, false>(p, s, dev, stream);
   }
   if (dweight == nullptr) return st;
   if (st == SGBLAS_STATUS_SUCCESS) {

@@ -174,6 +174,15 @@ __device__ __forceinline__ void tmaLoad3d(void *dst, const CUtensorMap *map, uin
       : "memory");
 }
 
+// `bytes` (a multiple of 16; both addresses, too) global -> shared, counted on `bar`.
+__device__ __forceinline__ void bulkLoad(void *dst, const void *src, uint64_t *bar, uint32_t bytes) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smemAddr(dst)),
+      "l"(src), "r"(bytes), "r"(smemAddr(bar))
+      : "memory");
+}
+
 // 3-D TMA tile store shared -> global, in this thread's bulk group (the
 // shared memory was written before a fenceProxyAsyncShared of its writers);
 // then the group's end, and the waits for its shared-memory reads and for all

@@ -18,24 +18,24 @@ __device__ __forceinline__ float fp8Scale(unsigned amax_bits) {
   return __fdiv_rn(__uint_as_float(max(amax_bits, kAmaxFloorBits)), kFp8Max);
 }
 
-// kPer values times `inverse` to bytes kStep apart, `left` of which exist; kStep
-// 1: as one word where all do (`at` is then aligned to kPer).
-template <int kPer, int kStep>
-__device__ __forceinline__ void storeFp8(unsigned char *at, const float (&f)[kPer], int left,
+// Pairs of values times `inverse` to bytes kStep apart, `left` of which exist; kStep
+// 1: as one word where all do (`at` is then aligned to it).
+template <int kPairs, int kStep>
+__device__ __forceinline__ void storeFp8(unsigned char *at, const float2 (&f)[kPairs], int left,
                                          float inverse) {
-  static_assert(kPer == 4 || kPer == 8, "a word or two");
-  alignas(8) __nv_fp8x2_storage_t q[kPer / 2];
+  static_assert(kPairs == 2 || kPairs == 4, "a word or two");
+  alignas(8) __nv_fp8x2_storage_t q[kPairs];
 #pragma unroll
-  for (int j = 0; j < kPer; j += 2)
-    q[j / 2] = __nv_cvt_float2_to_fp8x2(make_float2(f[j] * inverse, f[j + 1] * inverse),
-                                        __NV_SATFINITE, __NV_E4M3);
-  if (kStep == 1 && left >= kPer) {
-    if constexpr (kPer == 8) *reinterpret_cast<uint2 *>(at) = *reinterpret_cast<const uint2 *>(q);
+  for (int i = 0; i < kPairs; ++i)
+    q[i] = __nv_cvt_float2_to_fp8x2(__fmul2_rn(f[i], make_float2(inverse, inverse)), __NV_SATFINITE,
+                                    __NV_E4M3);
+  if (kStep == 1 && left >= 2 * kPairs) {
+    if constexpr (kPairs == 4) *reinterpret_cast<uint2 *>(at) = *reinterpret_cast<const uint2 *>(q);
     else *reinterpret_cast<uint32_t *>(at) = *reinterpret_cast<const uint32_t *>(q);
-  } else {
+  } else if (kStep > 1) {
     const auto *bytes = reinterpret_cast<const unsigned char *>(q);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
+    for (int j = 0; j < 2 * kPairs; ++j)
       if (j * kStep < left) at[j * kStep] = bytes[j];
   }
 }

@@ -18,6 +18,7 @@
 namespace sgblas::detail {
 namespace {
 
+using kern::both;
 using kern::Lanes;
 using kern::warpSum;
 
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kMoveThreads) scatterTokensKernel(const MovePa
           const float w = __ldg(p.weight + t * p.top + j);
           L out;
 #pragma unroll
-          for (int i = 0; i < L::kPer; ++i) out.set(i, w * v.get(i));
+          for (int i = 0; i < L::kPairs; ++i) out.setPair(i, __fmul2_rn(both(w), v.pair(i)));
           out.store(y, left);
           continue;
         }
@@ -203,9 +204,9 @@ __global__ void __launch_bounds__(kMoveThreads) gatherTokensKernel(const MovePar
   for (int slot = blockIdx.y * blockDim.x + threadIdx.x; slot < p.slots; slot += gridDim.y * blockDim.x) {
     const int at = L::begin(slot), left = p.k - at;
     if (left <= 0) continue;
-    float sum[L::kPer];
+    float2 sum[L::kPairs];
 #pragma unroll
-    for (int i = 0; i < L::kPer; ++i) sum[i] = 0.0F;
+    for (int i = 0; i < L::kPairs; ++i) sum[i] = make_float2(0.0F, 0.0F);
     for (int j0 = 0; j0 < p.top; j0 += kBatch) {
       L v[kBatch];
       float w[kBatch];
@@ -221,12 +222,12 @@ __global__ void __launch_bounds__(kMoveThreads) gatherTokensKernel(const MovePar
       for (int b = 0; b < kBatch; ++b) {
         if (!live[b]) continue;
 #pragma unroll
-        for (int i = 0; i < L::kPer; ++i) sum[i] = fmaf(w[b], v[b].get(i), sum[i]);
+        for (int i = 0; i < L::kPairs; ++i) sum[i] = __ffma2_rn(both(w[b]), v[b].pair(i), sum[i]);
       }
     }
     L out;
 #pragma unroll
-    for (int i = 0; i < L::kPer; ++i) out.set(i, sum[i]);
+    for (int i = 0; i < L::kPairs; ++i) out.setPair(i, sum[i]);
     out.store(static_cast<T *>(p.y) + t * p.ldy + at, left);
   }
 }
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kMoveThreads) gatherTokensKernel(const MovePar
 // dweight(j, t) = sum over k of dy(k, t) x(k, place(j, t)); a CTA's row of
 // blockDim.x threads per token.
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(kMoveThreads) gatherTokensBackwardKernel(const MoveParams p) {
+__global__ void __launch_bounds__(kMoveThreads, 4) gatherTokensBackwardKernel(const MoveParams p) {
   using L = Lanes<T, kVector>;
   __shared__ float partial[kMoveThreads / 32][kBatch];
   kern::gridDependencyWait();
@@ -245,13 +246,14 @@ __global__ void __launch_bounds__(kMoveThreads) gatherTokensBackwardKernel(const
   const int warps = blockDim.x / 32, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   for (int j0 = 0; j0 < p.top; j0 += kBatch) {
     int to[kBatch];
-    float w[kBatch], dot[kBatch];
+    float w[kBatch];
+    float2 dots[kBatch];   // sums of the even and the odd values
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       to[b] = in && j0 + b < p.top ? __ldg(p.place + t * p.top + j0 + b) : -1;
       if (!placed(p, to[b])) to[b] = -1;
       w[b] = to[b] >= 0 && p.weight != nullptr ? __ldg(p.weight + t * p.top + j0 + b) : 1.0F;
-      dot[b] = 0.0F;
+      dots[b] = make_float2(0.0F, 0.0F);
     }
     for (int slot = threadIdx.x; slot < p.slots; slot += blockDim.x) {
       const int at = L::begin(slot), left = p.k - at;
@@ -269,17 +271,18 @@ __global__ void __launch_bounds__(kMoveThreads) gatherTokensBackwardKernel(const
         if (to[b] < 0) continue;
         L out;
 #pragma unroll
-        for (int i = 0; i < L::kPer; ++i) out.set(i, w[b] * dy.get(i));
+        for (int i = 0; i < L::kPairs; ++i) out.setPair(i, __fmul2_rn(both(w[b]), dy.pair(i)));
         out.store(static_cast<T *>(p.y) + static_cast<long long>(to[b]) * p.ldy + at, left);
         if (p.dweight != nullptr) {
 #pragma unroll
-          for (int i = 0; i < L::kPer; ++i) dot[b] = fmaf(dy.get(i), x[b].get(i), dot[b]);
+          for (int i = 0; i < L::kPairs; ++i) dots[b] = __ffma2_rn(dy.pair(i), x[b].pair(i), dots[b]);
         }
       }
     }
     if (p.dweight == nullptr) continue;
+    float dot[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) dot[b] = warpSum(dot[b]);
+    for (int b = 0; b < kBatch; ++b) dot[b] = warpSum(dots[b].x + dots[b].y);
     if (warps > 1) {   // one token
       if (lane == 0) {
 #pragma unroll
