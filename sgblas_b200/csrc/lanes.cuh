@@ -48,6 +48,18 @@ struct Lanes {
         if (j * kStep < left) at[j * kStep] = v[j];
     }
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = T{};
+  }
+  // Keeps the values as they lie: the compiler would otherwise unpack BF16 ahead of
+  // their use, and hold twice the registers across a barrier or a loop.
+  __device__ __forceinline__ void hold() {
+    if constexpr (sizeof(T) == 2 && kVector) {
+      auto *w = reinterpret_cast<uint32_t *>(v);
+      asm volatile("" : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]));
+    }
+  }
   // Two values at a time: packed FP32 arithmetic, and one conversion for both (by
   // single values the norm of 16384 x 4096 took 28 instructions a value, bound by
   // their issue).

@@ -25,15 +25,15 @@ namespace {
 
 using kern::both;
 using kern::Lanes;
-using kern::warpSum;
 
 constexpr int kMaxThreads = 512;
 constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxUnits = 4;          // vectors of a column that a thread holds
 constexpr int kMaxStages = 8;
-// Of the kernels fed by a ring: threads of a CTA, and CTAs that have to fit an SM.
-constexpr int streamThreads(int units) { return units == 4 ? 512 : 256; }
-constexpr int streamResident(int units) { return units == 4 ? 1 : 3; }
+// Of the kernels fed by a ring: threads that have to fit an SM, in CTAs of up to
+// kMaxThreads. The backward pass holds four operands and the sums of dw: with 768
+// threads, 80 registers each, it spilled (16384 x 4096 BF16 270 us for 92).
+constexpr int kForwardThreads = 768, kBackwardThreads = 512;
 constexpr int kReduceThreads = 1024;
 constexpr int kReduceWarps = kReduceThreads / 32;
 
@@ -43,7 +43,7 @@ struct NormParams {
   unsigned char *q;
   float *scale;
   int k, n;
-  float eps;
+  float eps, over_k;   // 1 / k
   int ldx, ldr, ldsum, ldy, ldq, ldscale;
 };
 
@@ -52,36 +52,41 @@ struct NormBackwardParams {
   void *dx;
   float *part;        // NULL: no gradient of the weights
   int k, n, part_ld;
-  float eps;
+  float eps, over_k;
   int lddy, ldsum, lddsum, lddx;
+};
+
+// Room for two values of each warp of a CTA, twice: sums in turn use one and the
+// other, so that one barrier each is enough.
+struct Slots {
+  float2 of[2][kMaxWarps];
 };
 
 // The sums of two values over the threads of one column (blockDim.x of them, a
 // multiple of 32; blockDim.y columns), the same in every thread, in a fixed order.
 // kBarrier: a barrier of the CTA even where a warp has the whole column.
 template <bool kBarrier = false>
-__device__ __forceinline__ float2 columnSum(float2 v, float2 *slots) {
-  v.x = warpSum(v.x);
-  v.y = warpSum(v.y);
+__device__ __forceinline__ float2 columnSum(float2 v, Slots *slots, int turn) {
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2)
+    v = __fadd2_rn(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d)));
   const int warps = static_cast<int>(blockDim.x) / 32;
   if (warps == 1) {
     if (kBarrier) __syncthreads();
     return v;
   }
-  float2 *mine = slots + threadIdx.y * warps;
+  float2 *mine = slots->of[turn] + threadIdx.y * warps;
   if (threadIdx.x % 32 == 0) mine[threadIdx.x / 32] = v;
   __syncthreads();
-  float2 s = make_float2(0.0F, 0.0F);
-  for (int w = 0; w < warps; ++w) {
-    s.x += mine[w].x;
-    s.y += mine[w].y;
-  }
-  __syncthreads();   // the slots are free again
+  float2 s = mine[0];
+#pragma unroll 4
+  for (int w = 1; w < warps; ++w) s = __fadd2_rn(s, mine[w]);
   return s;
 }
 
-__device__ __forceinline__ float inverseLength(float squares, int k, float eps) {
-  return 1.0F / sqrtf(squares / static_cast<float>(k) + eps);
+// 1 / sqrt of the mean plus eps (rsqrtf: two units in the last place at most).
+__device__ __forceinline__ float inverseLength(float squares, float over_k, float eps) {
+  return rsqrtf(fmaf(squares, over_k, eps));
 }
 
 // h = x + r as it is held.
@@ -93,6 +98,19 @@ __device__ __forceinline__ void addResidual(Lanes<T, kVector> *h, const Lanes<T,
 
 // What a thread does with its values of a column, whichever way they came: `rest`
 // values of the column are there from the thread's place `at` on.
+// A thread's weights: ones where there are none.
+template <typename T, bool kVector>
+__device__ __forceinline__ void loadWeight(const void *weight, int k, int slot, Lanes<T, kVector> *w) {
+  using L = Lanes<T, kVector>;
+  const int at = L::begin(slot);
+  if (weight != nullptr) {
+    w->load(static_cast<const T *>(weight) + at, k - at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < L::kPairs; ++i) w->setPair(i, both(1.0F));
+  }
+}
+
 template <typename T, bool kVector>
 struct NormOf {
   using L = Lanes<T, kVector>;
@@ -109,8 +127,7 @@ struct NormOf {
     float2 f[L::kPairs];
 #pragma unroll
     for (int i = 0; i < L::kPairs; ++i) {
-      f[i] = __fmul2_rn(h.pair(i), both(s));
-      if (p.weight != nullptr) f[i] = __fmul2_rn(f[i], weight.pair(i));
+      f[i] = __fmul2_rn(__fmul2_rn(h.pair(i), both(s)), weight.pair(i));
     }
     if (p.y != nullptr) {
       L out;
@@ -141,28 +158,27 @@ template <typename T, bool kVector>
 struct NormBackwardOf {
   using L = Lanes<T, kVector>;
   // Adds to the sums of h^2 and of h g, each in two parts.
-  static __device__ __forceinline__ void add(bool weighted, const L &h, const L &dy, const L &weight,
+  static __device__ __forceinline__ void add(const L &h, const L &dy, const L &weight,
                                              float2 *squares, float2 *products) {
 #pragma unroll
     for (int i = 0; i < L::kPairs; ++i) {
       const float2 v = h.pair(i);
-      const float2 g = weighted ? __fmul2_rn(dy.pair(i), weight.pair(i)) : dy.pair(i);
+      const float2 g = __fmul2_rn(dy.pair(i), weight.pair(i));
       *squares = __ffma2_rn(v, v, *squares);
       *products = __ffma2_rn(v, g, *products);
     }
   }
   // dx to `dx`, and this column's part of dw (zero for a thread without values, whose
   // dy is zero, unless s is not finite).
-  static __device__ __forceinline__ void finish(bool weighted, bool past, T *dx, int rest, float2 f,
+  static __device__ __forceinline__ void finish(T *dx, int rest, float2 f,
                                                 const L &h, const L &dy, const L &weight, const L &ds,
                                                 float2 *dw) {
     L out;
 #pragma unroll
     for (int i = 0; i < L::kPairs; ++i) {
       const float2 v = h.pair(i), y = dy.pair(i);
-      const float2 g = weighted ? __fmul2_rn(y, weight.pair(i)) : y;
-      const float2 inner = __ffma2_rn(v, both(-f.y), g);
-      out.setPair(i, past ? __fadd2_rn(__fmul2_rn(inner, both(f.x)), ds.pair(i)) : __fmul2_rn(inner, both(f.x)));
+      const float2 g = __fmul2_rn(y, weight.pair(i));
+      out.setPair(i, __ffma2_rn(__ffma2_rn(v, both(-f.y), g), both(f.x), ds.pair(i)));
       if (rest > 0) dw[i] = __ffma2_rn(y, __fmul2_rn(v, both(f.x)), dw[i]);
     }
     out.store(dx, rest);
@@ -170,9 +186,9 @@ struct NormBackwardOf {
 };
 
 // s, and s^2 times the mean of h g.
-__device__ __forceinline__ float2 backwardFactors(float2 sums, int k, float eps) {
-  const float s = inverseLength(sums.x, k, eps);
-  return make_float2(s, s * s * (sums.y / static_cast<float>(k)));
+__device__ __forceinline__ float2 backwardFactors(float2 sums, float over_k, float eps) {
+  const float s = inverseLength(sums.x, over_k, eps);
+  return make_float2(s, s * s * (sums.y * over_k));
 }
 
 // ---- few columns, or columns that are not whole vectors ----------------------------
@@ -183,7 +199,7 @@ template <typename T, bool kVector, int kUnits, bool kLong>
 __global__ void __launch_bounds__(kMaxThreads) rmsNormKernel(const NormParams p) {
   using L = Lanes<T, kVector>;
   using N = NormOf<T, kVector>;
-  __shared__ float2 slots[kMaxWarps];
+  __shared__ Slots slots;
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const long long at = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
@@ -195,10 +211,6 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormKernel(const NormParams p)
   const T *x = static_cast<const T *>(p.x) + col * p.ldx;
   const T *r = p.residual == nullptr ? nullptr : static_cast<const T *>(p.residual) + col * p.ldr;
   auto left = [&](int slot) { return in ? p.k - L::begin(slot) : 0; };
-  auto readWeight = [&](int slot, L *v) {
-    if (p.weight != nullptr)
-      v->load(static_cast<const T *>(p.weight) + L::begin(slot), p.k - L::begin(slot));
-  };
   float2 squares = make_float2(0.0F, 0.0F);
   if constexpr (kLong) {
     auto read = [&](int slot) {
@@ -212,10 +224,10 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormKernel(const NormParams p)
       return h;
     };
     for (int slot = threadIdx.x; slot < rounds; slot += stride) N::square(read(slot), &squares);
-    const float s = inverseLength(columnSum(make_float2(squares.x + squares.y, 0.0F), slots).x, p.k, p.eps);
+    const float s = inverseLength(columnSum(make_float2(squares.x + squares.y, 0.0F), &slots, 0).x, p.over_k, p.eps);
     for (int slot = threadIdx.x; slot < rounds; slot += stride) {
       L w;
-      readWeight(slot, &w);
+      loadWeight(p.weight, p.k, slot, &w);
       N::write(p, col, slot, left(slot), s, read(slot), w);
     }
   } else {
@@ -227,13 +239,13 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormKernel(const NormParams p)
       if (r != nullptr) v[u].load(r + L::begin(slot), left(slot));
     }
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) readWeight(threadIdx.x + u * stride, &w[u]);
+    for (int u = 0; u < kUnits; ++u) loadWeight(p.weight, p.k, threadIdx.x + u * stride, &w[u]);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       if (r != nullptr) addResidual(&h[u], v[u]);
       N::square(h[u], &squares);
     }
-    const float s = inverseLength(columnSum(make_float2(squares.x + squares.y, 0.0F), slots).x, p.k, p.eps);
+    const float s = inverseLength(columnSum(make_float2(squares.x + squares.y, 0.0F), &slots, 0).x, p.over_k, p.eps);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int slot = threadIdx.x + u * stride;
@@ -273,7 +285,7 @@ template <typename T, bool kVector, int kUnits, bool kLong>
 __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormBackwardParams p) {
   using L = Lanes<T, kVector>;
   using N = NormBackwardOf<T, kVector>;
-  __shared__ float2 slots[kMaxWarps];
+  __shared__ Slots slots;
   __shared__ float exchange[kMaxThreads];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
@@ -281,20 +293,19 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
   const int rounds = ((p.k - 1) / kern::kLaneBlock + 1) * L::kThreads;
   const long long first = blockIdx.x * static_cast<long long>(blockDim.y);
   const long long step = gridDim.x * static_cast<long long>(blockDim.y);
-  const bool weighted = p.weight != nullptr, past = p.dsum != nullptr;
-  const T *weight = static_cast<const T *>(p.weight);
+  const bool past = p.dsum != nullptr;
   float2 dw[kLong ? 1 : kUnits][L::kPairs];
   L w[kUnits];
   if constexpr (!kLong) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const int at = L::begin(threadIdx.x + u * stride);
-      if (weighted) w[u].load(weight + at, p.k - at);
+      loadWeight(p.weight, p.k, threadIdx.x + u * stride, &w[u]);
 #pragma unroll
       for (int i = 0; i < L::kPairs; ++i) dw[u][i] = make_float2(0.0F, 0.0F);
     }
   }
-  for (long long c = first; c < p.n; c += step) {
+  int turn = 0;
+  for (long long c = first; c < p.n; c += step, turn ^= 1) {
     const bool in = c + threadIdx.y < p.n;
     const long long col = in ? c + threadIdx.y : 0;
     const T *h0 = static_cast<const T *>(p.sum) + col * p.ldsum;
@@ -303,25 +314,28 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
     T *dx0 = static_cast<T *>(p.dx) + col * p.lddx;
     float2 squares = make_float2(0.0F, 0.0F), products = squares;
     L h[kUnits], dy[kUnits], ds[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) ds[u].clear();
     if constexpr (kLong) {
       float *part = p.part == nullptr ? nullptr : p.part + static_cast<size_t>(blockIdx.x) * p.part_ld;
-      auto read = [&](int at) {
+      auto read = [&](int slot) {
+        const int at = L::begin(slot);
         h[0].load(h0 + at, p.k - at);
         dy[0].load(dy0 + at, p.k - at);
-        if (weighted) w[0].load(weight + at, p.k - at);
+        loadWeight(p.weight, p.k, slot, &w[0]);
       };
       for (int slot = threadIdx.x; slot < rounds; slot += stride) {
-        read(L::begin(slot));
-        N::add(weighted, h[0], dy[0], w[0], &squares, &products);
+        read(slot);
+        N::add(h[0], dy[0], w[0], &squares, &products);
       }
-      const float2 f = backwardFactors(columnSum(make_float2(squares.x + squares.y, products.x + products.y), slots), p.k, p.eps);
+      const float2 f = backwardFactors(columnSum(make_float2(squares.x + squares.y, products.x + products.y), &slots, turn), p.over_k, p.eps);
       for (int slot = threadIdx.x; slot < rounds; slot += stride) {
         const int at = L::begin(slot);
-        read(at);
+        read(slot);
         if (past) ds[0].load(ds0 + at, p.k - at);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) dw[0][i] = make_float2(0.0F, 0.0F);
-        N::finish(weighted, past, dx0 + at, p.k - at, f, h[0], dy[0], w[0], ds[0], dw[0]);
+        N::finish(dx0 + at, p.k - at, f, h[0], dy[0], w[0], ds[0], dw[0]);
         if (part != nullptr) {
 #pragma unroll
           for (int j = 0; j < L::kPer; ++j) {
@@ -340,12 +354,12 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
         if (past) ds[u].load(ds0 + at, rest);
       }
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) N::add(weighted, h[u], dy[u], w[u], &squares, &products);
-      const float2 f = backwardFactors(columnSum(make_float2(squares.x + squares.y, products.x + products.y), slots), p.k, p.eps);
+      for (int u = 0; u < kUnits; ++u) N::add(h[u], dy[u], w[u], &squares, &products);
+      const float2 f = backwardFactors(columnSum(make_float2(squares.x + squares.y, products.x + products.y), &slots, turn), p.over_k, p.eps);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int at = L::begin(threadIdx.x + u * stride);
-        N::finish(weighted, past, dx0 + at, in ? p.k - at : 0, f, h[u], dy[u], w[u], ds[u], dw[u]);
+        N::finish(dx0 + at, in ? p.k - at : 0, f, h[u], dy[u], w[u], ds[u], dw[u]);
       }
     }
   }
@@ -391,9 +405,9 @@ struct Ring {
   }
 };
 
-// Walks a persistent grid's columns: work(stage, column, in) for blockDim.y of them
-// at a time, which returns after a barrier of the CTA that follows its last read of
-// the stage.
+// Walks a persistent grid's columns: work(stage, turn, column, in) for blockDim.y of
+// them at a time (turn 0 and 1 by turns), which returns after a barrier of the CTA
+// that follows its last read of the stage.
 template <int kRows, class Work>
 __device__ __forceinline__ void walk(const Ring<kRows> &ring, int n, unsigned *err, Work work) {
   const bool issuer = threadIdx.x < 32 && threadIdx.y == 0;
@@ -409,12 +423,12 @@ __device__ __forceinline__ void walk(const Ring<kRows> &ring, int n, unsigned *e
       if (first + i * step < n) ring.fill(i, first + i * step, n);
   }
   __syncthreads();
-  int stage = 0;
+  int stage = 0, turn = 0;
   uint32_t parity = 0;
   bool ok = true;
-  for (long long c = first; c < n; c += step) {
+  for (long long c = first; c < n; c += step, turn ^= 1) {
     if (ok) ok = kern::mbarWait(&ring.full[stage], parity, err);
-    work(stage, c + threadIdx.y, c + threadIdx.y < n);
+    work(stage, turn, c + threadIdx.y, c + threadIdx.y < n);
     const long long next = c + ring.count * step;
     if (issuer && next < n && ok) {
       kern::fenceProxyAsyncShared();   // the reads above come before the copy
@@ -428,12 +442,12 @@ __device__ __forceinline__ void walk(const Ring<kRows> &ring, int n, unsigned *e
 }
 
 template <typename T, int kUnits>
-__global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
+__global__ void __launch_bounds__(kUnits == 4 ? kMaxThreads : 256, kUnits == 4 ? 1 : kForwardThreads / 256)
     rmsNormStreamKernel(const NormParams p, int stages, unsigned *err) {
   using L = Lanes<T, true>;
   using N = NormOf<T, true>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float2 slots[kMaxWarps];
+  __shared__ Slots slots;
   __shared__ uint64_t full[kMaxStages];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
@@ -442,14 +456,9 @@ __global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
                   {static_cast<const unsigned char *>(p.x), static_cast<const unsigned char *>(p.residual)},
                   {p.ldx * static_cast<long long>(sizeof(T)), p.ldr * static_cast<long long>(sizeof(T))}};
   L w[kUnits];
-  if (p.weight != nullptr) {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int at = L::begin(threadIdx.x + u * stride);
-      w[u].load(static_cast<const T *>(p.weight) + at, p.k - at);
-    }
-  }
-  walk(ring, p.n, err, [&](int stage, long long col, bool in) {
+  for (int u = 0; u < kUnits; ++u) loadWeight(p.weight, p.k, threadIdx.x + u * stride, &w[u]);
+  walk(ring, p.n, err, [&](int stage, int turn, long long col, bool in) {
     const T *x = reinterpret_cast<const T *>(ring.row(stage, 0, threadIdx.y));
     const T *r = reinterpret_cast<const T *>(ring.row(stage, 1, threadIdx.y));
     L h[kUnits];
@@ -465,7 +474,12 @@ __global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
       }
       N::square(h[u], &squares);
     }
-    const float s = inverseLength(columnSum<true>(make_float2(squares.x + squares.y, 0.0F), slots).x, p.k, p.eps);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      h[u].hold();
+      w[u].hold();
+    }
+    const float s = inverseLength(columnSum<true>(make_float2(squares.x + squares.y, 0.0F), &slots, turn).x, p.over_k, p.eps);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int slot = threadIdx.x + u * stride;
@@ -475,12 +489,12 @@ __global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
 }
 
 template <typename T, int kUnits>
-__global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
+__global__ void __launch_bounds__(kBackwardThreads)
     rmsNormBackwardStreamKernel(const NormBackwardParams p, int stages, unsigned *err) {
   using L = Lanes<T, true>;
   using N = NormBackwardOf<T, true>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float2 slots[kMaxWarps];
+  __shared__ Slots slots;
   __shared__ uint64_t full[kMaxStages];
   __shared__ float exchange[kMaxThreads];
   kern::gridDependencyWait();
@@ -491,17 +505,18 @@ __global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
                   {static_cast<const unsigned char *>(p.sum), static_cast<const unsigned char *>(p.dy),
                    static_cast<const unsigned char *>(p.dsum)},
                   {p.ldsum * kSize, p.lddy * kSize, p.lddsum * kSize}};
-  const bool weighted = p.weight != nullptr, past = p.dsum != nullptr;
+  // Long columns are read from the ring again for dx: held, they would not fit the registers.
+  constexpr bool kAgain = kUnits == 4;
+  const bool past = p.dsum != nullptr;
   float2 dw[kUnits][L::kPairs];
   L w[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const int at = L::begin(threadIdx.x + u * stride);
-    if (weighted) w[u].load(static_cast<const T *>(p.weight) + at, p.k - at);
+    loadWeight(p.weight, p.k, threadIdx.x + u * stride, &w[u]);
 #pragma unroll
     for (int i = 0; i < L::kPairs; ++i) dw[u][i] = make_float2(0.0F, 0.0F);
   }
-  walk(ring, p.n, err, [&](int stage, long long col, bool in) {
+  walk(ring, p.n, err, [&](int stage, int turn, long long col, bool in) {
     const T *h0 = reinterpret_cast<const T *>(ring.row(stage, 0, threadIdx.y));
     const T *dy0 = reinterpret_cast<const T *>(ring.row(stage, 1, threadIdx.y));
     const T *ds0 = reinterpret_cast<const T *>(ring.row(stage, 2, threadIdx.y));
@@ -512,16 +527,35 @@ __global__ void __launch_bounds__(streamThreads(kUnits), streamResident(kUnits))
       const int at = L::begin(threadIdx.x + u * stride), rest = in ? p.k - at : 0;
       h[u].load(h0 + at, rest);
       dy[u].load(dy0 + at, rest);
-      if (past) ds[u].load(ds0 + at, rest);
-      N::add(weighted, h[u], dy[u], w[u], &squares, &products);
+      if (!kAgain) {
+        if (past) ds[u].load(ds0 + at, rest);
+        else ds[u].clear();
+      }
+      N::add(h[u], dy[u], w[u], &squares, &products);
     }
-    const float2 f = backwardFactors(columnSum<true>(make_float2(squares.x + squares.y, products.x + products.y), slots), p.k, p.eps);
+    const float2 f = backwardFactors(
+        columnSum<true>(make_float2(squares.x + squares.y, products.x + products.y), &slots, turn), p.over_k, p.eps);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      if (!kAgain) {
+        h[u].hold();
+        dy[u].hold();
+      }
+      w[u].hold();
+    }
     T *dx0 = static_cast<T *>(p.dx) + (in ? col * p.lddx : 0);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const int at = L::begin(threadIdx.x + u * stride);
-      N::finish(weighted, past, dx0 + at, in ? p.k - at : 0, f, h[u], dy[u], w[u], ds[u], dw[u]);
+      const int at = L::begin(threadIdx.x + u * stride), rest = in ? p.k - at : 0;
+      if (kAgain) {
+        h[u].load(h0 + at, rest);
+        dy[u].load(dy0 + at, rest);
+        if (past) ds[u].load(ds0 + at, rest);
+        else ds[u].clear();
+      }
+      N::finish(dx0 + at, rest, f, h[u], dy[u], w[u], ds[u], dw[u]);
     }
+    if (kAgain) __syncthreads();   // the stage has been read
   });
   if (p.part != nullptr) storePart<L, kUnits>(p, dw, exchange);
 }
@@ -550,6 +584,8 @@ __global__ void __launch_bounds__(kReduceThreads)
   dw[at] = s;
 }
 
+constexpr int kForwardRows = 2, kBackwardRows = 3;   // of a stage
+
 // How columns are spread over threads.
 struct Shape {
   int units;      // vectors of a thread: 1, 2 or 4; 0: more than kMaxUnits
@@ -560,26 +596,29 @@ struct Shape {
 };
 // `operands` columns are read for each one written (`vector`: in whole vectors).
 Shape chooseShape(int k, int size, bool vector, int n, int operands, int sms) {
+  const bool backward = operands == kBackwardRows;
   const int per = vector ? 16 / size : 4;
   const int lanes = ((k - 1) / kern::kLaneBlock + 1) * (kern::kLaneBlock / per);
   Shape s = {};
   // A ring pays where a CTA walks several columns.
   if (vector && n >= 4 * sms) {
-    s.units = lanes <= 32 ? 1 : lanes <= 2 * streamThreads(2) ? 2 : 4;
+    s.units = lanes <= 32 ? 1 : lanes <= 2 * (backward ? kMaxThreads : 256) ? 2 : 4;
     s.threads = ((lanes - 1) / s.units / 32 + 1) * 32;
     s.columns = std::max(1, 256 / s.threads);
-    s.resident = s.units < 4 ? streamResident(s.units) : s.threads <= 256 ? 2 : 1;
+    s.resident = std::max(1, (backward || s.units == 4 ? kBackwardThreads : kForwardThreads) /
+                                 (s.threads * s.columns));
     const long long stage = static_cast<long long>(operands) * s.columns * k * size;
     s.stages = static_cast<int>(std::min<long long>(kMaxStages, (216 * 1024 / s.resident - 6 * 1024) / stage));
-    if (s.threads <= streamThreads(s.units) && s.stages >= 2) return s;
+    if (s.threads <= kMaxThreads && s.stages >= 2) return s;
   }
   // Few columns: all of a column's loads at once, on as many threads.
+  const int most = backward ? 2 : kMaxUnits;
   int units = n <= 2 * sms ? 1 : lanes >= 128 ? 2 : 1;
-  while (units < kMaxUnits && lanes > units * kMaxThreads) units *= 2;
+  while (units < most && lanes > units * kMaxThreads) units *= 2;
   s.units = lanes > units * kMaxThreads ? 0 : units;
   s.threads = s.units == 0 ? kMaxThreads : ((lanes - 1) / units / 32 + 1) * 32;
   s.columns = std::max(1, 128 / s.threads);
-  s.resident = std::max(1, 768 / (s.threads * s.columns));
+  s.resident = std::max(1, kForwardThreads / (s.threads * s.columns));
   s.stages = 0;
   return s;
 }
@@ -614,8 +653,6 @@ sgblasStatus_t launchStream(void (*kernel)(P, int, unsigned *), std::atomic<uint
   return launchNorm(kernel, dim3(static_cast<unsigned>(persistentCtas(s, p.n, dev.sms))), s, smem, stream, p,
                     s.stages, dev.err);
 }
-
-constexpr int kForwardRows = 2, kBackwardRows = 3;   // of a stage
 
 template <typename T, int kUnits>
 sgblasStatus_t launchForwardStream(const NormParams &p, const Shape &s, const DeviceInfo &dev,
@@ -662,7 +699,6 @@ sgblasStatus_t launchBackward(const NormBackwardParams &p, const Shape &s, const
   switch (s.units) {
     case 1: return launchNorm(rmsNormBackwardKernel<T, kVector, 1, false>, grid, s, 0, stream, p);
     case 2: return launchNorm(rmsNormBackwardKernel<T, kVector, 2, false>, grid, s, 0, stream, p);
-    case 4: return launchNorm(rmsNormBackwardKernel<T, kVector, 4, false>, grid, s, 0, stream, p);
     default: return launchNorm(rmsNormBackwardKernel<T, kVector, 1, true>, grid, s, 0, stream, p);
   }
 }
@@ -705,6 +741,7 @@ extern "C" sgblasStatus_t sgblasRmsNorm(sgblasHandle_t handle, int k, int n, sgb
   p.k = k;
   p.n = n;
   p.eps = eps;
+  p.over_k = 1.0F / static_cast<float>(k);
   p.ldx = ldx;
   p.ldr = ldr;
   p.ldsum = ldsum;
@@ -751,6 +788,7 @@ extern "C" sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, in
   p.k = k;
   p.n = n;
   p.eps = eps;
+  p.over_k = 1.0F / static_cast<float>(k);
   p.lddy = lddy;
   p.ldsum = ldsum;
   p.lddsum = lddsum;
