@@ -28,6 +28,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortMaxCluster = 8;
 constexpr int kSortWarpEntries = 64;   // of a warp, before another warp (CTA) joins
 
+constexpr int kSortBatch = 8;          // entries of a lane whose loads are issued together
 constexpr int kSortMaxEntries = 1 << 30;
 
 struct SortParams {
@@ -58,41 +59,64 @@ __device__ __forceinline__ int blockScan(int v, int *slots, int *total) {
 }
 
 // A stable counting sort by group: one cluster, whose warps hold consecutive
-// ranges of the entries. Each warp counts its range by group (32 entries at a
-// time: lanes of one group find each other, and their first adds for all); the
-// counts are summed over a CTA's warps, over the cluster's CTAs (through
-// distributed shared memory) and over the groups, and each warp walks its range
-// again, handing out places. Two passes over 4 bytes an entry: bound by the
-// latency of a warp's turns.
-__global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParams p, int ctas) {
-  extern __shared__ int counts[];   // [warps][groups], then the CTA's sums [groups]
+// ranges of the entries. Each warp walks its range, 32 entries at a time: lanes of one
+// group find each other by a ballot for each bit of the group's number, and an entry's
+// place within the warp's part of its group is that group's count so far plus the
+// lanes before. The counts are summed over a CTA's warps, over the cluster's CTAs
+// (through distributed shared memory) and over the groups, and each entry adds where
+// its warp's part of its group begins. Bound by latencies: the loads', the counts'
+// and the cluster's (65536 entries, 64 groups; with __match_any_sync and a second walk
+// 22.5 us).
+__global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParams p, int ctas, int bits) {
+  extern __shared__ int counts[];   // [warps][groups], the CTA's sums, where its groups begin
   __shared__ int slots[kSortThreads / 32];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
   const int rank = static_cast<int>(blockIdx.x);
   int *mine = counts + warp * p.groups;
-  int *sums = counts + warps * p.groups;
+  int *sums = counts + warps * p.groups, *starts = sums + p.groups;
   const int parts = ctas * warps;
   const long long per = ((p.entries + parts - 1LL) / parts + 31) / 32 * 32;
   const int begin = static_cast<int>(min(per * (rank * warps + warp), static_cast<long long>(p.entries)));
   const int end = static_cast<int>(min(begin + per, static_cast<long long>(p.entries)));
+  const bool once = per <= 32 * kSortBatch;   // the range fits the registers
   for (int g = lane; g < p.groups; g += 32) mine[g] = 0;
   __syncwarp();
-  // The entry's group, or -1.
-  auto groupAt = [&](int i) {
-    const int g = i < end ? __ldg(p.group + i) : -1;
-    return g >= 0 && g < p.groups ? g : -1;
+  int group[kSortBatch], local[kSortBatch];   // of entries i0 + 32 b + lane; the group p.groups is none
+  auto readGroups = [&](int i0) {
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+      const int i = i0 + b * 32 + lane;
+      const int g = i < end ? __ldg(p.group + i) : -1;
+      group[b] = static_cast<unsigned>(g) < static_cast<unsigned>(p.groups) ? g : p.groups;
+    }
   };
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int g = groupAt(i0 + lane);
-    const unsigned same = __match_any_sync(0xffffffffu, g);
-    if (g >= 0 && __ffs(same) - 1 == lane) mine[g] += __popc(same);
-    __syncwarp();
+  for (int i0 = begin; i0 < end; i0 += 32 * kSortBatch) {
+    readGroups(i0);
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+      if (i0 + b * 32 >= end) break;
+      const int g = group[b];
+      unsigned same = 0xffffffffu;
+      for (int bit = 0; bit < bits; ++bit) {
+        const unsigned set = __ballot_sync(0xffffffffu, g >> bit & 1);
+        same &= g >> bit & 1 ? set : ~set;
+      }
+      const bool live = g < p.groups;
+      const int before = live ? mine[g] : 0;
+      __syncwarp();
+      if (live && __ffs(same) - 1 == lane) mine[g] = before + __popc(same);
+      __syncwarp();
+      local[b] = before + __popc(same & ((1u << lane) - 1));
+      const int i = i0 + b * 32 + lane;
+      if (!once && i < end) p.place[i] = local[b];
+    }
   }
   __syncthreads();
   for (int g = threadIdx.x; g < p.groups; g += blockDim.x) {
     int sum = 0;
+#pragma unroll 8
     for (int w = 0; w < warps; ++w) {
       const int c = counts[w * p.groups + g];
       counts[w * p.groups + g] = sum;
@@ -102,13 +126,14 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
   }
   if (ctas > 1) kern::clusterSync();
   else __syncthreads();
-  // Where each group begins, and this CTA's part of it.
-  int carry = 0;
+  int carry = 0;   // entries of the groups so far
   for (int g0 = 0; g0 < p.groups; g0 += blockDim.x) {
     const int g = g0 + threadIdx.x;
     int total = 0, before = 0;
     if (g < p.groups) {
-      for (int c = 0; c < ctas; ++c) {
+#pragma unroll
+      for (int c = 0; c < kSortMaxCluster; ++c) {
+        if (c == ctas) break;
         const int there = ctas > 1 ? kern::ldCluster(kern::clusterAddr(kern::smemAddr(sums + g), c)) : sums[g];
         if (c < rank) before += there;
         total += there;
@@ -118,21 +143,24 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
     const int at = carry + blockScan(total, slots, &all);
     if (g < p.groups) {
       if (rank == 0) p.offsets[g] = at;
-      for (int w = 0; w < warps; ++w) counts[w * p.groups + g] += at + before;
+      starts[g] = at + before;
     }
     carry += all;
   }
   if (rank == 0 && threadIdx.x == 0) p.offsets[p.groups] = carry;
   __syncthreads();
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int g = groupAt(i0 + lane);
-    const unsigned same = __match_any_sync(0xffffffffu, g);
-    const int base = g >= 0 ? mine[g] : 0;
-    __syncwarp();
-    if (g >= 0 && __ffs(same) - 1 == lane) mine[g] = base + __popc(same);
-    __syncwarp();
-    if (i0 + lane < end)
-      p.place[i0 + lane] = g >= 0 ? base + __popc(same & ((1u << lane) - 1)) : -1;
+  for (int i0 = begin; i0 < end; i0 += 32 * kSortBatch) {
+    if (!once) {
+      readGroups(i0);
+#pragma unroll
+      for (int b = 0; b < kSortBatch; ++b)
+        if (i0 + b * 32 + lane < end) local[b] = p.place[i0 + b * 32 + lane];
+    }
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+      const int i = i0 + b * 32 + lane, g = group[b];
+      if (i < end) p.place[i] = g < p.groups ? starts[g] + mine[g] + local[b] : -1;
+    }
   }
   if (ctas > 1) kern::clusterSync();   // no CTA leaves while another reads its sums
 }
@@ -324,8 +352,8 @@ template <typename T, bool kVector>
 sgblasStatus_t launchMove(Move move, MoveParams p, int sms, cudaStream_t stream) {
   using L = Lanes<T, kVector>;
   p.slots = ((p.k - 1) / kern::kLaneBlock + 1) * L::kThreads;
-  const int threads = std::min(kMoveThreads, (p.slots + 31) / 32 * 32);
   const bool whole = move == Move::kBackward;   // a token's threads share its sums
+  const int threads = std::min(kMoveThreads, (p.slots + 31) / 32 * 32);
   const int tokens = whole && threads > 32 ? 1 : kMoveThreads / threads;
   const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(tokens));
   const int across = (p.n - 1) / tokens + 1;
@@ -375,7 +403,7 @@ extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top
   const sgblasStatus_t st = currentDevice(&dev);
   if (st != SGBLAS_STATUS_SUCCESS) return st;
   static std::atomic<uint64_t> configured{0};
-  constexpr int kMost = (kSortThreads / 32 + 1) * SGBLAS_MAX_GROUPS * 4;
+  constexpr int kMost = (kSortThreads / 32 + 2) * SGBLAS_MAX_GROUPS * 4;
   if (!configureKernel(reinterpret_cast<const void *>(sortTokensKernel), dev.device, kMost, &configured))
     return SGBLAS_STATUS_EXECUTION_FAILED;
   SortParams p = {};
@@ -391,7 +419,7 @@ extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(static_cast<unsigned>(32 * warps));
-  cfg.dynamicSmemBytes = sizeof(int) * static_cast<size_t>(warps + 1) * std::max(groups, 1);
+  cfg.dynamicSmemBytes = sizeof(int) * static_cast<size_t>(warps + 2) * std::max(groups, 1);
   cfg.stream = static_cast<cudaStream_t>(handle->stream);
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -402,7 +430,9 @@ extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ctas > 1 ? 2 : 1;
-  return launchStatus(cudaLaunchKernelEx(&cfg, sortTokensKernel, p, ctas));
+  int bits = 0;   // of a group's number, none among them
+  while (groups >> bits != 0) ++bits;
+  return launchStatus(cudaLaunchKernelEx(&cfg, sortTokensKernel, p, ctas, bits));
 }
 
 extern "C" sgblasStatus_t sgblasScatterTokens(sgblasHandle_t handle, int k, int n, int top, int rows,
