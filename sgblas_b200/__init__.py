@@ -402,8 +402,12 @@ class Handle:
                                  _ptr(weight), eps, _ptr(sum), ldsum, _ptr(y), ldy, _ptr(q), ldq,
                                  _ptr(scale), ldscale)
 
-    def rms_norm(self, *args, **kwargs) -> None:
-        status = self.rms_norm_status(*args, **kwargs)
+    def rms_norm(self, k, n, type, x, ldx, residual, ldr, weight, eps, sum=None, ldsum=0, y=None,
+                 ldy=0, q=None, ldq=0, scale=None, ldscale=0) -> None:
+        # Not by way of rms_norm_status: a third of a microsecond where a call takes five.
+        status = lib.sgblasRmsNorm(self._h, k, n, type, _ptr(x), ldx, _ptr(residual), ldr,
+                                   _ptr(weight), eps, _ptr(sum), ldsum, _ptr(y), ldy, _ptr(q), ldq,
+                                   _ptr(scale), ldscale)
         if status:
             raise SgblasError("sgblasRmsNorm", status)
 

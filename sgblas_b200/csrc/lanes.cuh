@@ -84,6 +84,33 @@ struct Lanes {
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// kWords words from any address of whole values (of 2 or 4 bytes): the aligned vectors
+// of 16 bytes that hold them, moved into place. Reads up to 15 bytes beside them, inside
+// their first and last vector.
+template <int kWords>
+__device__ __forceinline__ void loadShifted(const void *at, uint32_t (&w)[kWords]) {
+  static_assert(kWords % 4 == 0, "whole vectors");
+  const auto address = reinterpret_cast<uintptr_t>(at);
+  const auto *from = reinterpret_cast<const uint4 *>(address & ~uintptr_t{15});
+  const unsigned shift = static_cast<unsigned>(address & 15);
+  uint32_t in[kWords + 4];
+#pragma unroll
+  for (int j = 0; j <= kWords / 4; ++j) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (j < kWords / 4 || shift != 0) v = __ldg(from + j);
+    in[4 * j] = v.x;
+    in[4 * j + 1] = v.y;
+    in[4 * j + 2] = v.z;
+    in[4 * j + 3] = v.w;
+  }
+#pragma unroll
+  for (int i = 0; i < kWords + 2; ++i) in[i] = shift & 8 ? in[i + 2] : in[i];
+#pragma unroll
+  for (int i = 0; i < kWords + 1; ++i) in[i] = shift & 4 ? in[i + 1] : in[i];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(in[i], in[i + 1], shift % 4 * 8);
+}
+
 __device__ __forceinline__ float warpSum(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
