@@ -136,9 +136,9 @@ sgblasStatus_t sgblasQuantizeFp4(sgblasHandle_t handle, int k, int n, int batch,
  *
  * A is k x m (weights, scale_a ceil(k/32) x m), B is k x n (tokens, scale_b ceil(k/32) x
  * n), C is m x n of type ctype; lda and ldb count bytes. Products and scales are
- * exact, sums are FP32, chained in the tensor core over at most 512 of k for an
- * FP32 C and 4096 for a BF16 C, as in sgblasGroupedGemmN; a block's two scales together
- * should be in FP32's range. With an odd k, the last half byte of every column has to
+ * exact, sums are FP32, chained in the tensor core over at most 2048 of k for an
+ * FP32 C (32 instructions, as in sgblasGroupedGemmN) and 4096 for a BF16 C; a block's two
+ * scales together should be in FP32's range. With an odd k, the last half byte of every column has to
  * be zero. k == 0 writes zeros. Any alignment: operands and scales whose base is not
  * 16-byte aligned, or whose leading dimension (or stride) is not a multiple of 16
  * bytes, are first copied into the handle's workspace. */

@@ -145,6 +145,49 @@ sgblasStatus_t launchQuantize(void (*kernel)(QuantParams), const QuantParams &p,
 
 // ---- products --------------------------------------------------------------------
 
+constexpr int kPairWidth = 192;
+using PairCfg = t::Fp4Cfg<kPairWidth, true, false>;   // or true: the same tiles
+
+// Workspace of the laid-out scales of a pair product: those of A, then those of B.
+struct LaidSize {
+  long long a, b;   // bytes
+};
+LaidSize laidSize(const t::Params &p) {
+  const long long iters = (p.k + t::kRowBytes - 1) / t::kRowBytes;
+  const long long tiles = p.n / kPairWidth + std::min<long long>(p.groups, p.n);
+  LaidSize s;
+  s.a = static_cast<long long>(p.groups) * t::scaleBlocksA(p.m) * iters * t::kScaleRowsA * t::kScaleRowBytes;
+  s.b = tiles * iters * t::kScaleRowsB * t::kScaleRowBytes;
+  return s;
+}
+
+// Lays out the scales in the workspace at `at` and sets the maps.
+sgblasStatus_t layScales(const DeviceInfo &dev, t::Fp4Params &f, unsigned char *at, cudaStream_t stream) {
+  t::Params &p = f.p;
+  const LaidSize size = laidSize(p);
+  f.laid_a = at;
+  f.laid_b = at + size.a;
+  p.tiles_m = (p.m - 1) / PairCfg::kTileM + 1;
+  auto encode = [](CUtensorMap *map, const void *from, long long bytes, int rows) {
+    return encodeTyped3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, from, t::kScaleRowBytes, bytes / t::kScaleRowBytes, 1,
+                         t::kScaleRowBytes, bytes, t::kScaleRowBytes, rows, CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
+  if (!encode(&f.tma_sa, f.laid_a, size.a, t::kScaleRowsA) || !encode(&f.tma_sb, f.laid_b, size.b, t::kScaleRowsB))
+    return SGBLAS_STATUS_EXECUTION_FAILED;
+  constexpr long long kWarps = t::kLayThreads / 32;
+  const long long items = (size.a + size.b) / (4 * t::kScaleBlock) + 1;   // four blocks each, about
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>((items - 1) / kWarps + 1, 8LL * dev.sms)));
+  cfg.blockDim = dim3(t::kLayThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return launchStatus(cudaLaunchKernelEx(&cfg, t::layScalesKernel<PairCfg>, f));
+}
+
 template <class G>
 sgblasStatus_t launchTile(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
                           t::Fp4Params &f, cudaStream_t stream) {
@@ -250,38 +293,47 @@ sgblasStatus_t launchThin(const DeviceInfo &dev, const NarrowOperand &a, const N
   return launchStatus(cudaLaunchKernelEx(&cfg, kernel, f, split));
 }
 
-// Width (columns of tokens) of the tiles: 16, 32 or 64 for the thin kernel, 128 for
-// single CTAs, 192 for pairs.
+// Width (columns of tokens) of the tiles: 16 or 32 for the thin kernel, 128 for single
+// CTAs, 192 for pairs. The host knows the number of tokens, not how they fall to the
+// groups: a group is taken to end in half a tile.
+//
+// Thin tiles, whose k several CTAs may share, pay while a group has few tokens (4 x
+// 4096 x 4096, 8 tokens each: 7.9 us, 11.8 in 128 columns; 16: 8.0 and 7.9; 1 x 4096 x
+// 4096, 32 tokens: 8.1 and 7.4), those of 32 columns where groups of more than 16 are to
+// be expected (384 tokens unevenly over 32 x 2048 x 2048, with their quantisation:
+// 16.3 us in 16 columns, 15.4 in 32, 17.6 in 128). A wave of single tiles takes 0.40 us
+// a slice of k and no less than 2.2, of pairs 0.44 and 3.1, with 3 us for the scales'
+// blocks (32 x 2048 x 2048, 256 tokens each: singles 27.7 us, pairs 32.1; 512: 48.3 and
+// 44.5; 2048: 180 and 142; 16 x 1024 x 2048, 1024: 24.8 and 25.9).
 int chooseWidth(const DeviceInfo &dev, const t::Params &p) {
   const int active = std::min(p.groups, p.n);
   const double mean = static_cast<double>(p.n) / std::max(p.groups, 1);
-  auto tiles = [&](int rows, int width) {
+  if (mean <= 6) return 16;
+  if (mean <= 14) return 32;
+  auto waves = [&](int rows, int width, int workers) {
     const double columns = p.groups == 1
                                ? static_cast<double>((p.n - 1) / width + 1)
                                : std::max<double>(active, static_cast<double>(p.n) / width + 0.5 * active);
-    return columns * ((p.m - 1) / rows + 1);
+    return std::ceil(columns * ((p.m - 1) / rows + 1) / workers);
   };
-  if (mean <= 6) return 16;
-  const double single = tiles(t::kBM, 128);
-  if (mean <= 12 || (mean <= 64 && 4 * single <= dev.sms)) return mean <= 16 ? 32 : 64;
-  const double waves = std::ceil(single / dev.sms);
-  const double pair_waves = std::ceil(tiles(2 * t::kBM, 192) / (dev.sms / 2));
-  return pair_waves * 1.35 < waves ? 192 : 128;
+  const int iters = (p.k - 1) / t::kRowBytes + 1;   // slices of k
+  const double single = waves(t::kBM, 128, dev.sms) * std::max(0.40 * iters, 2.2);
+  const double pair = waves(2 * t::kBM, kPairWidth, dev.sms / 2) * std::max(0.44 * iters, 3.1) + 3.0;
+  return pair < single ? kPairWidth : 128;
 }
 
-sgblasStatus_t launchFp4(const DeviceInfo &dev, const NarrowOperand &a, const NarrowOperand &b,
+sgblasStatus_t launchFp4(const DeviceInfo &dev, int width, const NarrowOperand &a, const NarrowOperand &b,
                          t::Fp4Params &f, cudaStream_t stream) {
   const bool fp32 = !f.p.c_bf16;
-  switch (chooseWidth(dev, f.p)) {
+  switch (width) {
     case 16: return launchThin<t::Fp4ThinCfg<16>>(dev, a, b, f, stream);
     case 32: return launchThin<t::Fp4ThinCfg<32>>(dev, a, b, f, stream);
-    case 64: return launchThin<t::Fp4ThinCfg<64>>(dev, a, b, f, stream);
     case 128:
       return fp32 ? launchTile<t::Fp4Cfg<128, false, true>>(dev, a, b, f, stream)
                   : launchTile<t::Fp4Cfg<128, false, false>>(dev, a, b, f, stream);
     default:
-      return fp32 ? launchTile<t::Fp4Cfg<192, true, true>>(dev, a, b, f, stream)
-                  : launchTile<t::Fp4Cfg<192, true, false>>(dev, a, b, f, stream);
+      return fp32 ? launchTile<t::Fp4Cfg<kPairWidth, true, true>>(dev, a, b, f, stream)
+                  : launchTile<PairCfg>(dev, a, b, f, stream);
   }
 }
 
@@ -315,16 +367,18 @@ sgblasStatus_t gemmFp4(sgblasHandle_t handle, int m, int n, int k, int groups, c
   p.ldc = ldc;
   p.alpha = 1.0F;
   p.err = dev.err;
-  // Chains of 512 of k for an FP32 result, of 4096 for a BF16 one (launchNarrow).
-  p.chunk_iters = p.c_bf16 ? 16 : 2;
+  // Chains of 32 instructions, 2048 of k, for an FP32 result, as the BF16 products have
+  // (launchNarrow), and of 4096 of k for a BF16 one (in chains of 512 an FP32 result of
+  // 8192 x 8192 x 4096 took 136 us).
+  p.chunk_iters = p.c_bf16 ? 16 : 8;
   // Operands, then their scales, whose rows the kernels read 16 bytes at a time.
   NarrowOperand op[4];
   const void *ptr[4] = {a, b, scale_a, scale_b};
-  const int width[4] = {bytes, bytes, blocks, blocks};
+  const int row[4] = {bytes, bytes, blocks, blocks};
   const int ld[4] = {lda, ldb, ldsa, ldsb};
   for (int i = 0; i < 4; ++i) {
     op[i].ptr = ptr[i];
-    op[i].dim0 = width[i];
+    op[i].dim0 = row[i];
     op[i].dim1 = i % 2 == 0 ? m : n;
     op[i].ld = ld[i];
     op[i].count = i % 2 == 0 ? groups : 1;
@@ -332,14 +386,28 @@ sgblasStatus_t gemmFp4(sgblasHandle_t handle, int m, int n, int k, int groups, c
   }
   const auto stream = static_cast<cudaStream_t>(handle->stream);
   bool used_workspace = false;
+  int width = chooseWidth(dev, p);
+  unsigned char *laid = nullptr;
   if (k > 0) {
     size_t size[4], all = 0;
     for (int i = 0; i < 4; ++i) {
       size[i] = tmaReadable(op[i], 1) ? 0 : copyBytes(op[i], 1);
       all += size[i];
     }
+    const LaidSize extra = laidSize(p);
+    if (width == kPairWidth) {
+      // Without a workspace for the scales, single CTAs, which stage them.
+      if (std::max(extra.a, extra.b) / t::kScaleRowBytes <= INT_MAX &&
+          ensureWorkspace(handle, kCounterRegionBytes + all + static_cast<size_t>(extra.a + extra.b),
+                          dev.device, stream)) {
+        used_workspace = true;
+        laid = static_cast<unsigned char *>(handle->workspace) + kCounterRegionBytes + all;
+      } else {
+        width = 128;
+      }
+    }
     if (all > 0) {
-      if (!ensureWorkspace(handle, kCounterRegionBytes + all, dev.device, stream))
+      if (!used_workspace && !ensureWorkspace(handle, kCounterRegionBytes + all, dev.device, stream))
         return SGBLAS_STATUS_NOT_SUPPORTED;
       used_workspace = true;
       auto *to = static_cast<unsigned char *>(handle->workspace) + kCounterRegionBytes;
@@ -350,13 +418,14 @@ sgblasStatus_t gemmFp4(sgblasHandle_t handle, int m, int n, int k, int groups, c
       }
     }
   }
-  f.scale_a = static_cast<const unsigned char *>(op[2].ptr);
+  f.scale_a = static_cast<const unsigned char *>(op[2].ptr);   // of the copies, where there are any
   f.scale_b = static_cast<const unsigned char *>(op[3].ptr);
   f.ldsa = static_cast<int>(op[2].ld);
   f.ldsb = static_cast<int>(op[3].ld);
   f.stride_sa = op[2].count == 1 ? 0 : op[2].stride;
   f.blocks = blocks;
-  if (st == SGBLAS_STATUS_SUCCESS) st = launchFp4(dev, op[0], op[1], f, stream);
+  if (st == SGBLAS_STATUS_SUCCESS && laid != nullptr) st = layScales(dev, f, laid, stream);
+  if (st == SGBLAS_STATUS_SUCCESS) st = launchFp4(dev, width, op[0], op[1], f, stream);
   // Failed or not: a copy may be on its way, and later users wait for it.
   if (used_workspace && !markWorkspaceUse(handle, stream) && st == SGBLAS_STATUS_SUCCESS)
     return SGBLAS_STATUS_EXECUTION_FAILED;

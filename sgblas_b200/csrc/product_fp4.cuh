@@ -8,13 +8,16 @@
 // of k) takes two for every row of A and of B.
 //
 // Scales' way. In global memory they lie as bytes, contiguous along k, a row per
-// column of A or B. Two warps in turn copy 16 of a row at once (a chunk: two
-// slices) into shared memory by cp.async, each lane the rows lane + 32 i, a chunk or
-// more ahead; they then write a slice's, four per row and 128 of k, as the 512-byte
-// blocks that tcgen05.cp takes: 32 rows (lanes) of four words, word i for row
-// lane + 32 i. The issuer copies the blocks to TMEM before the slice's four
-// instructions. (Gathering them directly from global memory into the blocks would
-// take a 4-byte access per row and 128 of k, twice what the L1 cache can look up.)
+// column of A or B; tcgen05.cp takes them to TMEM in 512-byte blocks: 32 rows (lanes)
+// of four words, word i the four scales of row lane + 32 i for 128 of k. The issuer copies
+// a slice's blocks before its four instructions. Single CTAs stage them as they go: two
+// warps in turn copy 16 of a row at once (a chunk: two slices) into shared memory by
+// cp.async, each lane the rows lane + 32 i, a chunk or more ahead, and then write the
+// slices' blocks. (Gathering them directly from global memory into the blocks would
+// take a 4-byte access per row and 128 of k, twice what the L1 cache can look up.) A
+// pair's tensor cores leave no time for that: each row's 16 bytes cost shared memory
+// a clock of their own, in every tile again (8192 x 8192 x 4096 121 us, 99 without). For
+// pairs layScalesKernel writes all blocks once, into the workspace, and TMA loads them.
 // A stage of the ring holds a slice of A, of B and of the blocks; its TMEM columns
 // are the stage's, too, so one barrier frees all of it.
 #ifndef SGBLAS_B200_PRODUCT_FP4_CUH_
@@ -28,13 +31,19 @@ namespace sgblas::kern::prod {
 constexpr int kScaleBlock = 512;     // bytes: four scales of each of 128 rows
 constexpr int kScaleWarp0 = 2, kScaleWarps = 2;
 constexpr int kRawChunks = 2;        // chunks of 16 scales per row: one at work, the next on its way
-constexpr int kSliceScales = 8;      // of a row in a slice
+constexpr int kScaleRowBytes = 256;  // of the laid-out scales
+constexpr int kScaleRowsA = 2 * kScaleBlock / kScaleRowBytes;
+constexpr int kScaleRowsB = 2 * kScaleRowsA;
 
 struct Fp4Params {
   Params p;                          // k in bytes
   const unsigned char *scale_a, *scale_b;
   int ldsa, ldsb, blocks;            // blocks of 32 along k
   long long stride_sa;
+  // Pairs: the scales' blocks, and the maps they are read by: rows of 256 bytes, a slice's
+  // kScaleRowsA of each 128 rows of a matrix of A, and kScaleRowsB of each tile's columns.
+  unsigned char *laid_a, *laid_b;
+  CUtensorMap tma_sa, tma_sb;
 };
 
 // Shared layout of both forms: kBN columns of the tile, all of whose scales each
@@ -55,13 +64,13 @@ struct Fp4Shape {
   static constexpr int kScaleColumns = kScaleBytes / 128;   // of TMEM
   static constexpr int kStageBytes = kABytes + kBBytes + kScaleBytes;
   static constexpr int kRawRows = kBM + kBN;
-  static constexpr int kRawBytes = kScaleWarps * kRawChunks * kRawRows * 16;
-  static constexpr int kAccums = kThin_ ? (kBN == 64 ? 4 : 8) : 2;
+  static constexpr int kRawBytes = kTwo ? 0 : kScaleWarps * kRawChunks * kRawRows * 16;
+  static constexpr int kAccums = kThin_ ? 8 : 2;
   static constexpr int kScaleColumn0 = kAccums * kBN;
   static constexpr int kFitColumns = (512 - kScaleColumn0) / kScaleColumns;
   static constexpr int kTmemColumns = 512;
   static_assert(kBN % 16 == 0 && kBN <= 256, "the instruction's N");
-  static_assert(!kTwo || kBN % 32 == 0, "halves of whole swizzle groups");
+  static_assert(!kTwo || (kBN % 32 == 0 && kBBlocks == 2), "halves of whole swizzle groups, kScaleRowsB");
 };
 
 template <int kBN_, bool kTwo_, bool kFp32_>
@@ -73,7 +82,7 @@ struct Fp4Cfg : Fp4Shape<kBN_, kTwo_, false> {
   static constexpr int kFit = (217 * 1024 - kOutBytes - S::kRawBytes) / S::kStageBytes;
   static constexpr int kLess = kFit < S::kFitColumns ? kFit : S::kFitColumns;
   static constexpr int kStages = kLess > 8 ? 8 : kLess;
-  static constexpr int kBarrierBytes = 8 * (3 * kStages + 2 * S::kAccums);
+  static constexpr int kBarrierBytes = 8 * (2 * kStages + 2 * S::kAccums);
   static constexpr int kSmemBytes =
       kStages * S::kStageBytes + kOutBytes + S::kRawBytes + kBarrierBytes + 1024;
   static_assert(kStages >= 3 && kSmemBytes <= 218 * 1024 + 512, "shared memory beside the table");
@@ -90,7 +99,7 @@ struct Fp4ThinCfg : Fp4Shape<kBN_, false, true> {
   static constexpr int kBarrierBytes = 8 * (2 * kStages + 2 * S::kAccums + 2);
   static constexpr int kSmemBytes =
       kStages * S::kStageBytes + kPartBytes + S::kRawBytes + kBarrierBytes + 1024;
-  static_assert(S::kBN == 16 || S::kBN == 32 || S::kBN == 64, "tile width");
+  static_assert(S::kBN == 16 || S::kBN == 32, "tile width");
   static_assert(kSmemBytes <= 218 * 1024, "shared memory beside the table");
 };
 
@@ -115,7 +124,7 @@ __device__ __forceinline__ uint64_t scaleDesc(uint32_t addr) {
 // chunk, with its own raw buffers; `ready(s)` announces stage s.
 template <class G, int kStages, class Wait, class Ready>
 __device__ __forceinline__ void stageScales(const Fp4Params &f, const GroupTable &table, int tiles,
-                                            int worker, int workers, int rank, int kb0, int kb1,
+                                            int worker, int workers, int kb0, int kb1,
                                             unsigned char *ring, unsigned char *raw, int part,
                                             int lane, Wait wait, Ready ready) {
   const Params &p = f.p;
@@ -135,7 +144,7 @@ __device__ __forceinline__ void stageScales(const Fp4Params &f, const GroupTable
   auto fetch = [&]() {
     if (fetch_tile < tiles) {
       const Tile t = tileAt<G>(p, table, fetch_tile);
-      const int m0 = t.m0 + rank * kBM;
+      const int m0 = t.m0;
       const unsigned char *a = f.scale_a + t.group * f.stride_sa +
                                static_cast<long long>(m0 + lane) * f.ldsa + fetch_chunk * 16;
       const unsigned char *b =
@@ -249,11 +258,83 @@ __device__ __forceinline__ void issueSlice(uint32_t tmem_base, uint32_t d_tmem, 
   }
 }
 
+// Blocks of 128 rows of a matrix of A.
+__host__ __device__ __forceinline__ int scaleBlocksA(int m) { return (m + kBM - 1) / kBM; }
+
+// Writes the scales' blocks of pairs of width G::kBN: a warp per chunk (16 scales) of
+// 128 rows of A, of groups that have columns, or of half a tile's columns.
+constexpr int kLayThreads = 256;
+template <class G>
+__global__ void __launch_bounds__(kLayThreads) layScalesKernel(const __grid_constant__ Fp4Params f) {
+  const Params &p = f.p;
+  __shared__ GroupTable table;
+  gridDependencyWait();
+  allowDependentLaunch();
+  const int lane = threadIdx.x % 32;
+  if (threadIdx.x < 32) readGroups<G>(p, &table, lane);
+  __syncthreads();
+  const int iters = (p.k + kRowBytes - 1) / kRowBytes, chunks = (iters + 1) / 2;
+  const int blocks_a = scaleBlocksA(p.m);
+  const long long items_a = static_cast<long long>(p.groups) * blocks_a * chunks;
+  const long long items = items_a + static_cast<long long>(table.first[p.groups]) * G::kBBlocks * chunks;
+  const long long step = gridDim.x * static_cast<long long>(kLayThreads / 32);
+  for (long long i = blockIdx.x * (kLayThreads / 32LL) + threadIdx.x / 32; i < items; i += step) {
+    const bool is_a = i < items_a;
+    const long long at = is_a ? i : i - items_a;
+    const int chunk = static_cast<int>(at % chunks), block = static_cast<int>(at / chunks);
+    const unsigned char *from;
+    unsigned char *to;     // of the chunk's first slice
+    int rows, ld, slice, next;   // bytes of a slice, and from its first 128 of k to its second
+    if (is_a) {
+      const int group = block / blocks_a, row0 = (block - group * blocks_a) * kBM;
+      if (table.offset[group + 1] <= table.offset[group]) continue;
+      from = f.scale_a + group * f.stride_sa + static_cast<long long>(row0) * f.ldsa;
+      rows = p.m - row0;
+      ld = f.ldsa;
+      slice = kScaleRowsA * kScaleRowBytes;
+      next = kScaleBlock;
+      to = f.laid_a + (static_cast<long long>(block) * iters + 2 * chunk) * slice;
+    } else {
+      const int tile = block / G::kBBlocks, half = block - tile * G::kBBlocks;
+      const Tile t = tileAt<G>(p, table, tile * p.tiles_m);
+      from = f.scale_b + static_cast<long long>(t.n0 + half * kBM) * f.ldsb;
+      rows = t.cols - half * kBM;
+      ld = f.ldsb;
+      slice = kScaleRowsB * kScaleRowBytes;
+      next = G::kBBlocks * kScaleBlock;
+      to = f.laid_b + (static_cast<long long>(tile) * iters + 2 * chunk) * slice + half * kScaleBlock;
+    }
+    const int bytes = min(16, f.blocks - chunk * 16);
+    uint4 w[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      w[r] = make_uint4(0, 0, 0, 0);
+      const unsigned char *row = from + static_cast<long long>(lane + 32 * r) * ld + chunk * 16;
+      if (lane + 32 * r >= rows) continue;
+      if (bytes == 16) {
+        w[r] = __ldg(reinterpret_cast<const uint4 *>(row));
+      } else {
+        uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 15; ++j)
+          if (j < bytes) v[j / 4] |= static_cast<uint32_t>(row[j]) << (j % 4 * 8);
+        w[r] = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    uint4 *out = reinterpret_cast<uint4 *>(to) + lane;
+    out[0] = make_uint4(w[0].x, w[1].x, w[2].x, w[3].x);
+    out[next / 16] = make_uint4(w[0].y, w[1].y, w[2].y, w[3].y);
+    if (2 * chunk + 1 < iters) {
+      out += slice / 16;
+      out[0] = make_uint4(w[0].z, w[1].z, w[2].z, w[3].z);
+      out[next / 16] = make_uint4(w[0].w, w[1].w, w[2].w, w[3].w);
+    }
+  }
+}
+
 // Many tokens: as productKernel.
-//   full[s]     stage s has its operands (TMA) and the scales of each CTA (the scales' warps)
-//   relayed[s]  a pair's odd CTA has its scales in stage s: its idle warp 1 passes that on,
-//               for a release at cluster scope would wait for the chunks that
-//               those warps have on their way (1700 clocks a slice instead of 400)
+//   full[s]   stage s has its operands and scales: TMA's bytes (of both CTAs of a pair),
+//             and a single CTA's scales' warps
 template <class G>
 __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_constant__ Fp4Params f) {
   constexpr int kBN = G::kBN;
@@ -270,7 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
   uint64_t *empty = full + kStages;
   uint64_t *acc_full = empty + kStages;
   uint64_t *acc_empty = acc_full + kAccums;
-  uint64_t *relayed = acc_empty + kAccums;
 
   const int warp = uniformWarp(), lane = threadIdx.x % 32;
   const int rank = G::kTwo ? static_cast<int>(blockIdx.x & 1) : 0;
@@ -282,10 +362,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
       prefetchTensorMap(&p.tma_b);
     }
     if (p.c_tma) prefetchTensorMap(&p.tma_c);
+    if (G::kTwo && p.k > 0) {
+      prefetchTensorMap(&f.tma_sa);
+      prefetchTensorMap(&f.tma_sb);
+    }
     for (int s = 0; s < kStages; ++s) {
-      mbarInit(&full[s], G::kTwo ? 3 : 2);
+      mbarInit(&full[s], G::kTwo ? 1 : 2);
       mbarInit(&empty[s], 1);
-      mbarInit(&relayed[s], 1);
     }
     for (int b = 0; b < kAccums; ++b) {
       mbarInit(&acc_full[b], 1);
@@ -329,18 +412,24 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
         const Tile t = tileAt<G>(p, table, i);
         const int m0 = t.m0 + rank * kBM;
         const int n0 = t.n0 + (G::kTwo ? rank * (widthOf(t.cols) / 2) : 0);
+        // A pair's: where the laid-out scales of this tile begin, in slices. Rows past
+        // the matrix's last block are the next one's, or zeros; they reach no row of C.
+        const int scale_a = (t.group * scaleBlocksA(p.m) + m0 / kBM) * iters;
+        const int scale_b = i / p.tiles_m * iters;
         for (int kb = 0; kb < iters; ++kb) {
           wait(&empty[s], parity);
           if (!ok) continue;
           unsigned char *stage = smem + s * kStageBytes;
-          constexpr uint32_t kBytes = G::kABytes + G::kBBytes;
           if constexpr (G::kTwo) {
-            if (rank == 0) mbarArriveExpectTx(&full[s], 2 * kBytes);
+            if (rank == 0) mbarArriveExpectTx(&full[s], 2 * kStageBytes);
             const uint32_t bar = clusterAddr(smemAddr(&full[s]), 0);
             tmaLoad3dPair(stage, &p.tma_a, bar, kb * kRowBytes, m0, t.group);
             tmaLoad3dPair(stage + G::kABytes, &p.tma_b, bar, kb * kRowBytes, n0, 0);
+            unsigned char *scales = stage + G::kABytes + G::kBBytes;
+            tmaLoad3dPair(scales, &f.tma_sa, bar, 0, (scale_a + kb) * kScaleRowsA, 0);
+            tmaLoad3dPair(scales + 2 * kScaleBlock, &f.tma_sb, bar, 0, (scale_b + kb) * kScaleRowsB, 0);
           } else {
-            mbarArriveExpectTx(&full[s], kBytes);
+            mbarArriveExpectTx(&full[s], G::kABytes + G::kBBytes);
             tmaLoad3d(stage, &p.tma_a, &full[s], kb * kRowBytes, m0, t.group);
             tmaLoad3d(stage + G::kABytes, &p.tma_b, &full[s], kb * kRowBytes, n0, 0);
           }
@@ -360,29 +449,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp4TileKernel(const __grid_consta
           parity ^= 1;
         }
       }
-    } else if (warp >= kScaleWarp0) {
+    } else if (!G::kTwo && warp >= kScaleWarp0) {
       // ---------------- scales ----------------
-      stageScales<G, kStages>(
-          f, table, tiles, worker, workers, rank, 0, iters, smem, raw, warp - kScaleWarp0, lane,
-          [&](int s, int parity) { wait(&empty[s], parity); },
-          [&](int s) {
-            if (lane == 0) mbarArrive(rank == 0 ? &full[s] : &relayed[s]);
-          });
-    } else if (warp == 1 && rank == 1) {
-      // ---------------- relay of the odd CTA's scales ----------------
-      if (electOne()) {
-        int s = 0, parity = 0;
-        for (int i = worker; i < tiles; i += workers) {
-          for (int kb = 0; kb < iters; ++kb) {
-            wait(&relayed[s], parity);
-            mbarArriveClusterRelaxed(clusterAddr(smemAddr(&full[s]), 0));
-            if (++s == kStages) {
-              s = 0;
-              parity ^= 1;
-            }
-          }
-        }
-      }
+      if constexpr (!G::kTwo)
+        stageScales<G, kStages>(
+            f, table, tiles, worker, workers, 0, iters, smem, raw, warp - kScaleWarp0, lane,
+            [&](int s, int parity) { wait(&empty[s], parity); },
+            [&](int s) {
+              if (lane == 0) mbarArrive(&full[s]);
+            });
     } else if (warp == 1 && rank == 0) {
       // ---------------- MMA issuer ----------------
       const bool leader = electOne();
@@ -588,7 +663,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
   } else if (warp == kScaleWarp0 || warp == kScaleWarp0 + 1) {
     // ---------------- scales ----------------
     stageScales<G, kStages>(
-        f, table, tiles, worker, workers, 0, kb0, kb1, smem, raw, warp - kScaleWarp0, lane,
+        f, table, tiles, worker, workers, kb0, kb1, smem, raw, warp - kScaleWarp0, lane,
         [&](int s, int parity) { wait(&empty[s], parity); },
         [&](int s) {
           if (lane == 0) mbarArrive(&full[s]);
