@@ -1,5 +1,5 @@
 """A mixture-of-experts layer on the library's products: trained in BF16, its
-experts' updates orthogonalised, then served in 8 bits.
+experts' updates orthogonalised, then served in 8 and in 4 bits.
 
     python examples/moe_layer.py [--tokens 2048] [--width 512] [--hidden 1024] [--experts 8]
 
@@ -7,8 +7,10 @@ Each token goes to one expert e: y = W2[e] relu(W1[e] x). The forward and token
 gradient products are sgblasGroupedGemmN, the weight gradients
 sgblasGroupedGemmK (into FP32), the update of every expert's matrices one
 sgblasOrthogonalize per weight tensor, and serving quantises the weights once
-(128 x 128 blocks) and the tokens per call (1 x 128) for sgblasGroupedGemmFp8.
-Routing, the activation and the loss are torch's.
+(128 x 128 blocks) and the tokens per call (1 x 128) for sgblasGroupedGemmFp8, or both
+to 4 bits (blocks of 32) for sgblasGroupedGemmFp4. Tokens are sorted by expert and
+moved by sgblasSortTokens and sgblasScatterTokens. The router, the activation and the
+loss are torch's.
 
 Tensors are row-major; the library reads the same memory as column-major
 matrices, so a [tokens, k] tensor is a k x tokens matrix.
@@ -114,15 +116,43 @@ class Experts:
         return self.product_fp8(quantized[1], torch.relu(self.product_fp8(quantized[0], x, offsets)),
                                 offsets)
 
+    # ---- in 4 bits: rows padded to 16 bytes, which the products read in place -----
 
-def route(x, router):
-    """Tokens sorted by expert, and where each expert's begin (on the device)."""
-    expert = (x @ router).argmax(dim=1)
-    order = torch.argsort(expert, stable=True)
-    counts = torch.bincount(expert, minlength=router.shape[1])
-    offsets = torch.zeros(router.shape[1] + 1, dtype=torch.int32, device="cuda")
-    offsets[1:] = counts.cumsum(0)
-    return order, offsets
+    def quantize_fp4(self, x):
+        """(values, scales) of the last two axes' rows."""
+        batch, (rows, cols) = x.shape[0] if x.dim() == 3 else 1, x.shape[-2:]
+        ldq, lds = -(-cols // 32) * 16, -(-cols // 512) * 16
+        q = torch.empty(*x.shape[:-1], ldq, dtype=torch.uint8, device="cuda")
+        s = torch.empty(*x.shape[:-1], lds, dtype=torch.uint8, device="cuda")
+        self.h.quantize_fp4(cols, rows, x, BF16, cols, q, ldq, s, lds, batch=batch, stride_x=rows * cols,
+                            stride_q=rows * ldq, stride_scale=rows * lds)
+        return q, s
+
+    def product_fp4(self, weights, x, offsets):
+        (q, s), (xq, xs) = weights, self.quantize_fp4(x)
+        e, m, ldq = q.shape
+        lds = s.shape[2]
+        y = torch.empty(x.shape[0], m, dtype=torch.bfloat16, device="cuda")
+        self.h.grouped_gemm_fp4(m, x.shape[0], x.shape[1], e, offsets, q, ldq, m * ldq, s, lds, m * lds, xq, ldq,
+                                xs, lds, y, BF16, m)
+        return y
+
+    def serve_fp4(self, quantized, x, offsets):
+        return self.product_fp4(quantized[1], torch.relu(self.product_fp4(quantized[0], x, offsets)), offsets)
+
+
+def route(h, x, router):
+    """Tokens (in BF16) sorted by expert, and where each expert's begin (on the device)."""
+    tokens, width = x.shape
+    experts = router.shape[1]
+    expert = (x @ router).argmax(dim=1).to(torch.int32)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+    place = torch.empty(tokens, 1, dtype=torch.int32, device="cuda")
+    h.sort_tokens(tokens, 1, experts, expert, offsets, place)
+    x = x.to(torch.bfloat16)
+    y = torch.empty_like(x)
+    h.scatter_tokens(width, tokens, 1, tokens, place, None, x, BF16, width, y, width)
+    return y, offsets
 
 
 def main(tokens=2048, width=512, hidden=1024, experts=8, steps=30, seed=0, quiet=False):
@@ -136,24 +166,23 @@ def main(tokens=2048, width=512, hidden=1024, experts=8, steps=30, seed=0, quiet
         h.set_stream(torch.cuda.current_stream())
         layer = Experts(h, experts, width, hidden, gen)
         for step in range(steps):
-            x = torch.randn(tokens, width, generator=gen, device="cuda")
-            order, offsets = route(x, router)
-            x = x[order].to(torch.bfloat16)
+            x, offsets = route(h, torch.randn(tokens, width, generator=gen, device="cuda"), router)
             want = x.float() @ target
             hid, act, y = layer.forward(x, offsets)
             diff = y.float() - want
             losses.append(diff.square().mean().item())
             dy = (2.0 / diff.numel() * diff).to(torch.bfloat16)
             layer.step(x, dy, hid, act, offsets, rate=0.02)
-        x = torch.randn(64, width, generator=gen, device="cuda")   # a batch being decoded
-        order, offsets = route(x, router)
-        x = x[order].to(torch.bfloat16)
+        # A batch being decoded.
+        x, offsets = route(h, torch.randn(64, width, generator=gen, device="cuda"), router)
         full = layer.forward(x, offsets)[2].float()
         small = layer.serve(layer.quantize(), x, offsets).float()
         deviation = ((small - full).norm() / full.norm()).item()
+        smaller = layer.serve_fp4([layer.quantize_fp4(w) for w in layer.weights], x, offsets).float()
+        deviation4 = ((smaller - full).norm() / full.norm()).item()
     if not quiet:
         print(f"loss {losses[0]:.4f} -> {losses[-1]:.4f} in {steps} steps; "
-              f"8-bit serving is {100 * deviation:.2f} % off BF16; "
+              f"serving in 8 bits is {100 * deviation:.2f} % off BF16, in 4 bits {100 * deviation4:.1f} %; "
               f"device errors {sg.get_device_errors()}")
     return losses, deviation
 

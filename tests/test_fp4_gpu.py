@@ -185,14 +185,25 @@ def test_small_products(cuda, handle, ctype, case, ld, shift):
     check_product(handle, ops, ctype, ldc=ld, shift=shift)
 
 
+# Pairs of CTAs: tiles of 256 x 192, groups that end inside either half of one, rows and
+# columns that are no multiple of anything, k from a chunk of scales to several chains.
+PAIRS = [dict(name="pairs", lengths=[2999, 1, 0, 2303, 777, 3333, 193, 191, 97], m=3999, k=2120),
+         dict(name="pairs, edges", lengths=[192, 384, 96, 1920, 2000, 3600, 1111, 2222], m=4112, k=4100),
+         dict(name="pairs, one group", lengths=[7777], m=6001, k=1543)]
+
+
 @pytest.mark.parametrize("ctype", ["fp32", "bf16"])
-@pytest.mark.parametrize("case", RAGGED, ids=lambda c: c["name"])
+@pytest.mark.parametrize("case", RAGGED + PAIRS, ids=lambda c: c["name"])
 def test_ragged_products(cuda, handle, ctype, case):
     check_product(handle, Operands(case["m"], case["k"], case["lengths"], seed=1), ctype)
 
 
+ONE_MATRIX = [(4096, 1, 4096), (2048, 40, 4000), (4096, 600, 700), (4104, 2500, 520), (1999, 3001, 390),
+              (4096, 4100, 1100), (6008, 6100, 1542)]
+
+
 @pytest.mark.parametrize("ctype", ["fp32", "bf16"])
-@pytest.mark.parametrize("m,n,k", [(4096, 1, 4096), (2048, 40, 4000), (4096, 600, 700), (4104, 2500, 520), (1999, 3001, 390)])
+@pytest.mark.parametrize("m,n,k", ONE_MATRIX)
 def test_one_matrix(cuda, handle, ctype, m, n, k):
     ops = Operands(m, k, [n], seed=n)
     c = Matrix(n, m, TYPES[ctype])
@@ -201,11 +212,13 @@ def test_one_matrix(cuda, handle, ctype, m, n, k):
     assert not c.unmarked()
 
 
-@pytest.mark.parametrize("lengths", [[300, 0, 40], [3, 1, 0, 5], [1500, 700]])
-def test_columns_of_no_group_stay(cuda, handle, lengths):
-    for m in (520, 1001):
+@pytest.mark.parametrize("lengths,sizes", [([300, 0, 40], (520, 1001)), ([3, 1, 0, 5], (520, 1001)),
+                                           ([20] * 3, (520, 1001)), ([2500, 3700, 0, 2800], (4096, 4001))])
+def test_columns_of_no_group_stay(cuda, handle, lengths, sizes):
+    for m in sizes:
         for ctype in ("fp32", "bf16"):
-            check_product(handle, Operands(m, 300, lengths, seed=2, lead=5, tail=77), ctype)
+            k = 300 if m < 4000 else 1542
+            check_product(handle, Operands(m, k, lengths, seed=2, lead=5, tail=77), ctype)
 
 
 def test_offsets_outside_count_as_the_nearer_end(cuda, handle):
@@ -219,12 +232,12 @@ def test_offsets_outside_count_as_the_nearer_end(cuda, handle):
 
 def test_neighbours_do_not_reach_a_column(cuda, handle):
     """NaN scales of one group's tokens and weights stay in that group."""
-    for lengths in ([200, 100, 300], [3, 2, 4]):
-        ops = Operands(300, 520, lengths, seed=4)
+    for m, lengths in ((300, [200, 100, 300]), (300, [3, 2, 4]), (300, [8, 13, 9]), (4001, [2500, 3000, 3700])):
+        ops = Operands(m, 1544, lengths, seed=4)
         want = ops.want()
         ops.sb.view[ops.ends[1]:ops.ends[2]] = 255
-        ops.sa.view[300:600] = 255
-        c = Matrix(ops.n, 300, torch.float32)
+        ops.sa.view[m:2 * m] = 255
+        c = Matrix(ops.n, m, torch.float32)
         ops.run(handle, "fp32", c)
         assert bool(c.view[ops.ends[1]:ops.ends[2]].isnan().all())
         for lo, hi in ((0, ops.ends[1]), (ops.ends[2], ops.n)):
@@ -240,7 +253,8 @@ def test_no_products(cuda, handle):
 
 
 @pytest.mark.parametrize("ctype", ["fp32", "bf16"])
-@pytest.mark.parametrize("m,k,lengths", [(1024, 4096, [1]), (2048, 2048, [12] * 16), (2048, 4096, [1500, 900])])
+@pytest.mark.parametrize("m,k,lengths", [(1024, 4096, [1]), (2048, 2048, [12] * 16), (2048, 4096, [1500, 900]),
+                                         (4096, 4608, [3500, 4000])])
 def test_real_values(cuda, handle, ctype, m, k, lengths):
     """Quantised activations and weights: sums of any size. An FP32 C is chained over
     32 instructions (2^-22 of the terms each, truncated) and pieces of 2048 of k (2^-24
@@ -269,16 +283,23 @@ def test_real_values(cuda, handle, ctype, m, k, lengths):
         at += length
 
 
-def test_fp4_in_a_graph_and_on_a_stream(cuda, lib):
-    """A captured step reads new tokens and offsets on each replay."""
-    m, k, lengths = 512, 1024, [3, 40, 0, 21]
+@pytest.mark.parametrize("m,lengths", [(512, [3, 40, 0, 21]), (512, [1, 0, 9, 2]), (4096, [2500, 0, 4000, 3000])])
+@pytest.mark.parametrize("prepared", [True, False])
+def test_fp4_in_a_graph_and_on_a_stream(cuda, lib, m, lengths, prepared):
+    """A captured step reads new tokens, weights and offsets on each replay, with the
+    workspace for a pair's scales or without."""
+    k = 1536
     ops = Operands(m, k, lengths, seed=6)
-    other = Operands(m, k, [40, 0, 21, 3], seed=7)
+    other = Operands(m, k, lengths[1:] + lengths[:1], seed=7)
     c = Matrix(ops.n, m, torch.float32)
     stream = torch.cuda.Stream()
     torch.cuda.synchronize()
     with lib.Handle() as h:
         h.set_stream(stream)
+        if prepared:
+            ops.run(h, "fp32", c)
+            torch.cuda.synchronize()
+            assert torch.equal(c.view, ops.want().float())
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
             ops.run(h, "fp32", c)
@@ -305,6 +326,7 @@ def test_unaligned_operands_in_a_capture_need_a_workspace(cuda, lib):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
             assert h.gemm_fp4_status(*args) == lib.SGBLAS_STATUS_NOT_SUPPORTED
+            c.fresh.zero_()   # a graph of something
         graph.reset()
         h.gemm_fp4(*args)
         torch.cuda.synchronize()
