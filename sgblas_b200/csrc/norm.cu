@@ -30,10 +30,15 @@ constexpr int kMaxThreads = 512;
 constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxUnits = 4;          // vectors of a column that a thread holds
 constexpr int kMaxStages = 8;
-// Of the kernels fed by a ring: threads that have to fit an SM, in CTAs of up to
-// kMaxThreads. The backward pass holds four operands and the sums of dw: with 768
+// Of the kernels fed by a ring: threads that have to fit an SM, in CTAs of at most
+// streamCta. The backward pass holds four operands and the sums of dw: with 768
 // threads, 80 registers each, it spilled (16384 x 4096 BF16 270 us for 92).
-constexpr int kForwardThreads = 768, kBackwardThreads = 512;
+constexpr int streamThreads(int units, bool backward) {
+  return units == 1 ? 1024 : backward ? 512 : 768;
+}
+constexpr int streamCta(int units, bool backward) {
+  return backward && units > 1 ? kMaxThreads : 256;
+}
 constexpr int kReduceThreads = 1024;
 constexpr int kReduceWarps = kReduceThreads / 32;
 
@@ -255,26 +260,40 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormKernel(const NormParams p)
 }
 
 // The sums of dw of a CTA's columns of threads (blockDim.y of them) to its row of
-// partial sums, in their order.
-template <typename L, int kUnits>
-__device__ __forceinline__ void storePart(const NormBackwardParams &p, float2 (&dw)[kUnits][L::kPairs],
-                                          float *exchange) {
+// partial sums, in their order: kVector as vectors, whose rows are padded to 32 values.
+template <typename T, bool kVector, int kUnits>
+__device__ __forceinline__ void storePart(const NormBackwardParams &p,
+                                          float2 (&dw)[kUnits][Lanes<T, kVector>::kPairs],
+                                          float2 *exchange) {
+  using L = Lanes<T, kVector>;
   float *part = p.part + static_cast<size_t>(blockIdx.x) * p.part_ld;
   const int stride = static_cast<int>(blockDim.x);
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
     const int at = L::begin(threadIdx.x + u * stride);
+    if (blockDim.y > 1) {
 #pragma unroll
-    for (int j = 0; j < L::kPer; ++j) {
-      float sum = j % 2 ? dw[u][j / 2].y : dw[u][j / 2].x;
-      if (blockDim.y > 1) {
+      for (int i = 0; i < L::kPairs; ++i) {
         __syncthreads();
-        exchange[threadIdx.y * stride + threadIdx.x] = sum;
+        exchange[threadIdx.y * stride + threadIdx.x] = dw[u][i];
         __syncthreads();
-        sum = exchange[threadIdx.x];
-        for (unsigned y = 1; y < blockDim.y; ++y) sum += exchange[y * stride + threadIdx.x];
+        float2 sum = exchange[threadIdx.x];
+        for (unsigned y = 1; y < blockDim.y; ++y) sum = __fadd2_rn(sum, exchange[y * stride + threadIdx.x]);
+        dw[u][i] = sum;
       }
-      if (threadIdx.y == 0 && at + j * L::kStep < p.k) part[at + j * L::kStep] = sum;
+    }
+    if (threadIdx.y != 0) continue;
+    if constexpr (kVector) {
+      if (at < p.k) {
+#pragma unroll
+        for (int i = 0; i < L::kPairs; i += 2)
+          *reinterpret_cast<float4 *>(part + at + 2 * i) =
+              make_float4(dw[u][i].x, dw[u][i].y, dw[u][i + 1].x, dw[u][i + 1].y);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < L::kPer; ++j)
+        if (at + j * L::kStep < p.k) part[at + j * L::kStep] = j % 2 ? dw[u][j / 2].y : dw[u][j / 2].x;
     }
   }
 }
@@ -286,7 +305,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
   using L = Lanes<T, kVector>;
   using N = NormBackwardOf<T, kVector>;
   __shared__ Slots slots;
-  __shared__ float exchange[kMaxThreads];
+  __shared__ float2 exchange[kMaxThreads];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const int stride = static_cast<int>(blockDim.x);
@@ -364,7 +383,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
     }
   }
   if constexpr (!kLong) {
-    if (p.part != nullptr) storePart<L, kUnits>(p, dw, exchange);
+    if (p.part != nullptr) storePart<T, kVector, kUnits>(p, dw, exchange);
   }
 }
 
@@ -442,7 +461,7 @@ __device__ __forceinline__ void walk(const Ring<kRows> &ring, int n, unsigned *e
 }
 
 template <typename T, int kUnits>
-__global__ void __launch_bounds__(kUnits == 4 ? kMaxThreads : 256, kUnits == 4 ? 1 : kForwardThreads / 256)
+__global__ void __launch_bounds__(streamCta(kUnits, false), streamThreads(kUnits, false) / streamCta(kUnits, false))
     rmsNormStreamKernel(const NormParams p, int stages, unsigned *err) {
   using L = Lanes<T, true>;
   using N = NormOf<T, true>;
@@ -489,14 +508,14 @@ __global__ void __launch_bounds__(kUnits == 4 ? kMaxThreads : 256, kUnits == 4 ?
 }
 
 template <typename T, int kUnits>
-__global__ void __launch_bounds__(kBackwardThreads)
+__global__ void __launch_bounds__(streamCta(kUnits, true), streamThreads(kUnits, true) / streamCta(kUnits, true))
     rmsNormBackwardStreamKernel(const NormBackwardParams p, int stages, unsigned *err) {
   using L = Lanes<T, true>;
   using N = NormBackwardOf<T, true>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Slots slots;
   __shared__ uint64_t full[kMaxStages];
-  __shared__ float exchange[kMaxThreads];
+  __shared__ float2 exchange[kMaxThreads];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const int stride = static_cast<int>(blockDim.x);
@@ -557,7 +576,7 @@ __global__ void __launch_bounds__(kBackwardThreads)
     }
     if (kAgain) __syncthreads();   // the stage has been read
   });
-  if (p.part != nullptr) storePart<L, kUnits>(p, dw, exchange);
+  if (p.part != nullptr) storePart<T, true, kUnits>(p, dw, exchange);
 }
 
 // dw = beta dw + the sum of `rows` rows of partial sums, 32 values per CTA, a
@@ -594,22 +613,24 @@ struct Shape {
   int stages;     // of the ring; 0: loads straight into registers
   int resident;   // CTAs per SM, of a persistent grid
 };
-// `operands` columns are read for each one written (`vector`: in whole vectors).
-Shape chooseShape(int k, int size, bool vector, int n, int operands, int sms) {
-  const bool backward = operands == kBackwardRows;
+// For columns read `vector`-wise or not, whichever results are asked for. A ring pays
+// where a CTA walks several columns. More vectors per thread mean fewer instructions a
+// column: forward 16384 x 4096 BF16 94 us with four, 101 with two, without a residual 43
+// and 54, with e4m3 results 76 and 83.
+Shape chooseShape(int k, int size, bool vector, int n, bool backward, int sms) {
   const int per = vector ? 16 / size : 4;
   const int lanes = ((k - 1) / kern::kLaneBlock + 1) * (kern::kLaneBlock / per);
+  const int operands = backward ? kBackwardRows : kForwardRows;
   Shape s = {};
-  // A ring pays where a CTA walks several columns.
   if (vector && n >= 4 * sms) {
-    s.units = lanes <= 32 ? 1 : lanes <= 2 * (backward ? kMaxThreads : 256) ? 2 : 4;
+    const int two = backward ? 2 * kMaxThreads : 128;   // lanes for two vectors each
+    s.units = lanes <= 32 ? 1 : lanes <= two ? 2 : 4;
     s.threads = ((lanes - 1) / s.units / 32 + 1) * 32;
     s.columns = std::max(1, 256 / s.threads);
-    s.resident = std::max(1, (backward || s.units == 4 ? kBackwardThreads : kForwardThreads) /
-                                 (s.threads * s.columns));
+    s.resident = std::max(1, streamThreads(s.units, backward) / (s.threads * s.columns));
     const long long stage = static_cast<long long>(operands) * s.columns * k * size;
     s.stages = static_cast<int>(std::min<long long>(kMaxStages, (216 * 1024 / s.resident - 6 * 1024) / stage));
-    if (s.threads <= kMaxThreads && s.stages >= 2) return s;
+    if (s.threads <= streamCta(s.units, backward) && s.stages >= 2) return s;
   }
   // Few columns: all of a column's loads at once, on as many threads.
   const int most = backward ? 2 : kMaxUnits;
@@ -618,7 +639,7 @@ Shape chooseShape(int k, int size, bool vector, int n, int operands, int sms) {
   s.units = lanes > units * kMaxThreads ? 0 : units;
   s.threads = s.units == 0 ? kMaxThreads : ((lanes - 1) / units / 32 + 1) * 32;
   s.columns = std::max(1, 128 / s.threads);
-  s.resident = std::max(1, kForwardThreads / (s.threads * s.columns));
+  s.resident = std::max(1, 768 / (s.threads * s.columns));
   s.stages = 0;
   return s;
 }
@@ -670,7 +691,7 @@ sgblasStatus_t launchBackwardStream(const NormBackwardParams &p, const Shape &s,
 
 template <typename T, bool kVector>
 sgblasStatus_t launchForward(const NormParams &p, const DeviceInfo &dev, cudaStream_t stream) {
-  const Shape s = chooseShape(p.k, sizeof(T), kVector, p.n, kForwardRows, dev.sms);
+  const Shape s = chooseShape(p.k, sizeof(T), kVector, p.n, false, dev.sms);
   if constexpr (kVector) {
     if (s.stages > 0)
       return s.units == 1   ? launchForwardStream<T, 1>(p, s, dev, stream)
@@ -800,9 +821,9 @@ extern "C" sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, in
   const auto stream = static_cast<cudaStream_t>(handle->stream);
   int rows = 0;
   if (n > 0) {
-    const Shape s = chooseShape(k, size, vector, n, kBackwardRows, dev.sms);
+    const Shape s = chooseShape(k, size, vector, n, true, dev.sms);
     rows = persistentCtas(s, n, dev.sms);
-    p.part_ld = (k + 3) / 4 * 4;
+    p.part_ld = (k + 31) / 32 * 32;
     if (dweight != nullptr) {
       const size_t bytes = sizeof(float) * static_cast<size_t>(p.part_ld) * static_cast<size_t>(rows);
       if (!ensureWorkspace(handle, kCounterRegionBytes + bytes, dev.device, stream))
