@@ -9,7 +9,6 @@
 #include "sgemm_launch.hpp"
 
 #include <cuda_bf16.h>
-#include <cuda_fp4.h>
 
 #include <algorithm>
 #include <atomic>
@@ -44,8 +43,20 @@ __device__ __forceinline__ unsigned scaleByte(unsigned amax_bits) {
 // 2^(127 - byte), exact: byte is 0 to 252 for numbers.
 __device__ __forceinline__ float inverseOf(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
 
-__device__ __forceinline__ unsigned pairOf(float2 v) {
-  return __nv_cvt_float2_to_fp4x2(v, __NV_E2M1, cudaRoundNearest);
+// Eight values to e2m1, the first in the lowest half byte: rounded to nearest, ties to
+// even, at most 6.
+__device__ __forceinline__ uint32_t eightOf(const float2 (&f)[4]) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(f[0].x), "f"(f[0].y), "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x),
+        "f"(f[3].y));
+  return w;
 }
 
 // Two threads to a block of 32, 16 consecutive values each, kUnroll blocks per
@@ -115,16 +126,20 @@ __global__ void __launch_bounds__(kQuantThreads) quantizeFp4Kernel(const QuantPa
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     const unsigned byte = scaleByte(m);
     const float inverse = inverseOf(byte);
-    alignas(8) unsigned char b[kPer / 2];
+    uint32_t q[2];
 #pragma unroll
-    for (int j = 0; j < kPer / 2; ++j)
-      b[j] = static_cast<unsigned char>(pairOf(__fmul2_rn(f[j], make_float2(inverse, inverse))));
+    for (int half = 0; half < 2; ++half) {
+      float2 scaled[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) scaled[j] = __fmul2_rn(f[half * 4 + j], make_float2(inverse, inverse));
+      q[half] = eightOf(scaled);
+    }
     if (left[u] >= kPer && p.q_words) {
-      *reinterpret_cast<uint2 *>(q_to[u]) = *reinterpret_cast<const uint2 *>(b);
+      *reinterpret_cast<uint2 *>(q_to[u]) = make_uint2(q[0], q[1]);
     } else {
 #pragma unroll
       for (int j = 0; j < kPer / 2; ++j)
-        if (2 * j < left[u]) q_to[u][j] = b[j];
+        if (2 * j < left[u]) q_to[u][j] = static_cast<unsigned char>(q[j / 4] >> (j % 4 * 8));
     }
     if (scale_to[u] != nullptr) *scale_to[u] = static_cast<unsigned char>(byte);
   }
