@@ -1,5 +1,5 @@
 // A column's values spread over threads, for the memory-bound operators: what
-// one thread holds of a block of 128 values, and sums over a column's threads.
+// one thread holds of a block of 128 values.
 #ifndef SGBLAS_B200_LANES_CUH_
 #define SGBLAS_B200_LANES_CUH_
 
@@ -109,12 +109,6 @@ __device__ __forceinline__ void loadShifted(const void *at, uint32_t (&w)[kWords
   for (int i = 0; i < kWords + 1; ++i) in[i] = shift & 4 ? in[i + 1] : in[i];
 #pragma unroll
   for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(in[i], in[i + 1], shift % 4 * 8);
-}
-
-__device__ __forceinline__ float warpSum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
 }
 
 }  // namespace sgblas::kern

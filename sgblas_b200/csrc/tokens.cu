@@ -20,7 +20,6 @@ namespace {
 
 using kern::both;
 using kern::Lanes;
-using kern::warpSum;
 
 // ---- the sort ------------------------------------------------------------------
 
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
 // ---- moving columns ------------------------------------------------------------
 
 constexpr int kMoveThreads = 256;
-constexpr int kBatch = 4;   // choices whose columns are on their way at once
+constexpr int kBatch = 4;   // choices whose columns are on their way at once (sumFour)
 
 struct MoveParams {
   const int *place;
@@ -261,6 +260,19 @@ __global__ void __launch_bounds__(kMoveThreads) gatherTokensKernel(const MovePar
   }
 }
 
+// The sums over a warp of four values; lanes 8 b to 8 b + 7 get the b-th.
+__device__ __forceinline__ float sumFour(const float (&v)[4], int lane) {
+  const bool upper = (lane & 16) != 0, odd = (lane & 8) != 0;
+  float a = upper ? v[2] : v[0], b = upper ? v[3] : v[1];
+  a += __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], 16);
+  b += __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], 16);
+  float s = odd ? b : a;
+  s += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+  for (int d = 4; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+  return s;
+}
+
 // y(:, place(j, t)) = weight(j, t) dy(:, t) and, with dweight,
 // dweight(j, t) = sum over k of dy(k, t) x(k, place(j, t)); a CTA's row of
 // blockDim.x threads per token.
@@ -311,12 +323,10 @@ __global__ void __launch_bounds__(kMoveThreads, 4) gatherTokensBackwardKernel(co
     if (p.dweight == nullptr) continue;
     float dot[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) dot[b] = warpSum(dots[b].x + dots[b].y);
+    for (int b = 0; b < kBatch; ++b) dot[b] = dots[b].x + dots[b].y;
+    const float sum = sumFour(dot, lane);   // of choice lane / 8
     if (warps > 1) {   // one token
-      if (lane == 0) {
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) partial[warp][b] = dot[b];
-      }
+      if (lane % 8 == 0) partial[warp][lane / 8] = sum;
       __syncthreads();
       if (threadIdx.x < kBatch) {
         float s = 0.0F;
@@ -324,10 +334,8 @@ __global__ void __launch_bounds__(kMoveThreads, 4) gatherTokensBackwardKernel(co
         if (j0 + static_cast<int>(threadIdx.x) < p.top) p.dweight[t * p.top + j0 + threadIdx.x] = s;
       }
       __syncthreads();
-    } else if (in && lane == 0) {
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-        if (j0 + b < p.top) p.dweight[t * p.top + j0 + b] = dot[b];
+    } else if (in && lane % 8 == 0 && j0 + lane / 8 < p.top) {
+      p.dweight[t * p.top + j0 + lane / 8] = sum;
     }
   }
 }
@@ -354,7 +362,9 @@ sgblasStatus_t launchMove(Move move, MoveParams p, int sms, cudaStream_t stream)
   using L = Lanes<T, kVector>;
   p.slots = ((p.k - 1) / kern::kLaneBlock + 1) * L::kThreads;
   const bool whole = move == Move::kBackward;   // a token's threads share its sums
-  const int threads = std::min(kMoveThreads, (p.slots + 31) / 32 * 32);
+  // Threads in whole warps, as busy in their last turn as in the others.
+  const int turns = (p.slots - 1) / kMoveThreads + 1;
+  const int threads = ((p.slots - 1) / turns / 32 + 1) * 32;
   const int tokens = whole && threads > 32 ? 1 : kMoveThreads / threads;
   const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(tokens));
   const int across = (p.n - 1) / tokens + 1;
