@@ -315,6 +315,34 @@ def test_fp4_in_a_graph_and_on_a_stream(cuda, lib, m, lengths, prepared):
         graph.reset()
 
 
+@pytest.mark.parametrize("ctype", ["fp32", "bf16"])
+def test_products_without_a_workspace_are_the_same(cuda, lib, ctype):
+    """Inside a capture without a workspace large products take smaller tiles, whose sums
+    are made in the same order: equal results for values of any size."""
+    m, k, lengths = 4096, 4608, [3500, 4000]
+    n = sum(lengths)
+    gen = generator(7)
+    q = [torch.randint(0, 256, (rows, k // 2), generator=gen, device="cuda").to(torch.uint8) for rows in (2 * m, n)]
+    s = [torch.randint(110, 140, (rows, k // 32), generator=gen, device="cuda").to(torch.uint8) for rows in (2 * m, n)]
+    offsets = torch.tensor([0, 3500, 7500], dtype=torch.int32, device="cuda")
+    out = [torch.zeros(n, m, dtype=TYPES[ctype], device="cuda") for _ in range(2)]
+    with lib.Handle() as h:
+        run = lambda c: h.grouped_gemm_fp4(m, n, k, 2, offsets, q[0], k // 2, m * k // 2, s[0], k // 32, m * k // 32,  # noqa: E731
+                                           q[1], k // 2, s[1], k // 32, c, CODE[ctype], m)
+        stream = torch.cuda.Stream()
+        h.set_stream(stream)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run(out[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        run(out[1])
+        torch.cuda.synchronize()
+        graph.reset()
+    assert torch.equal(out[0], out[1])
+
+
 def test_unaligned_operands_in_a_capture_need_a_workspace(cuda, lib):
     ops = Operands(64, 77, [20], seed=8, ld=1, shift=1)
     c = Matrix(20, 64, torch.float32)
