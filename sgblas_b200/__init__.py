@@ -175,6 +175,22 @@ def _load() -> ctypes.CDLL:
 
 lib = _load()
 
+# The compiled caller (calls.c) of the entry points whose own time is a few
+# microseconds; `_direct` is the library it is bound to, None where it was not built.
+try:
+    from . import _calls
+except ImportError:
+    _calls, _direct = None, None
+else:
+    _direct = lib
+    for _name, _symbol in (("rms_norm", "RmsNorm"), ("rms_norm_backward", "RmsNormBackward"),
+                           ("sort_tokens", "SortTokens"), ("scatter_tokens", "ScatterTokens"),
+                           ("gather_tokens", "GatherTokens"),
+                           ("gather_tokens_backward", "GatherTokensBackward"),
+                           ("quantize_fp4", "QuantizeFp4"), ("gemm_fp4", "GemmFp4"),
+                           ("grouped_gemm_fp4", "GroupedGemmFp4")):
+        _calls.bind(_name, ctypes.cast(getattr(lib, "sgblas" + _symbol), ctypes.c_void_p).value)
+
 
 def status_string(status: int) -> str:
     return lib.sgblasGetStatusString(status).decode()
@@ -219,6 +235,7 @@ class Handle:
         raw = ctypes.c_void_p()
         _check("sgblasCreate", lib.sgblasCreate(ctypes.byref(raw)))
         self._h = raw
+        self._address = raw.value   # for the compiled caller
 
     @property
     def raw(self) -> ctypes.c_void_p:
@@ -227,7 +244,7 @@ class Handle:
     def close(self) -> None:
         if self._h is not None and self._h.value is not None:
             _check("sgblasDestroy", lib.sgblasDestroy(self._h))
-        self._h = None
+        self._h = self._address = None
 
     def __enter__(self) -> "Handle":
         return self
@@ -355,8 +372,14 @@ class Handle:
         return lib.sgblasQuantizeFp4(self._h, k, n, batch, _ptr(x), xtype, ldx, stride_x, _ptr(q),
                                      ldq, stride_q, _ptr(scale), ldscale, stride_scale)
 
-    def quantize_fp4(self, *args, **kwargs) -> None:
-        status = self.quantize_fp4_status(*args, **kwargs)
+    def quantize_fp4(self, k, n, x, xtype, ldx, q, ldq, scale, ldscale, batch=1, stride_x=0, stride_q=0,
+                     stride_scale=0) -> None:
+        if lib is _direct:
+            status = _calls.quantize_fp4(self._address, k, n, batch, x, xtype, ldx, stride_x, q, ldq,
+                                         stride_q, scale, ldscale, stride_scale)
+        else:
+            status = self.quantize_fp4_status(k, n, x, xtype, ldx, q, ldq, scale, ldscale, batch,
+                                              stride_x, stride_q, stride_scale)
         if status:
             raise SgblasError("sgblasQuantizeFp4", status)
 
@@ -367,7 +390,7 @@ class Handle:
                                  _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
 
     def gemm_fp4(self, *args) -> None:
-        status = self.gemm_fp4_status(*args)
+        status = _calls.gemm_fp4(self._address, *args) if lib is _direct else self.gemm_fp4_status(*args)
         if status:
             raise SgblasError("sgblasGemmFp4", status)
 
@@ -379,7 +402,7 @@ class Handle:
                                         _ptr(scale_b), ldsb, _ptr(c), ctype, ldc)
 
     def grouped_gemm_fp4(self, *args) -> None:
-        status = self.grouped_gemm_fp4_status(*args)
+        status = _calls.grouped_gemm_fp4(self._address, *args) if lib is _direct else self.grouped_gemm_fp4_status(*args)
         if status:
             raise SgblasError("sgblasGroupedGemmFp4", status)
 
@@ -404,10 +427,12 @@ class Handle:
 
     def rms_norm(self, k, n, type, x, ldx, residual, ldr, weight, eps, sum=None, ldsum=0, y=None,
                  ldy=0, q=None, ldq=0, scale=None, ldscale=0) -> None:
-        # Not by way of rms_norm_status: a third of a microsecond where a call takes five.
-        status = lib.sgblasRmsNorm(self._h, k, n, type, _ptr(x), ldx, _ptr(residual), ldr,
-                                   _ptr(weight), eps, _ptr(sum), ldsum, _ptr(y), ldy, _ptr(q), ldq,
-                                   _ptr(scale), ldscale)
+        if lib is _direct:
+            status = _calls.rms_norm(self._address, k, n, type, x, ldx, residual, ldr, weight, eps, sum,
+                                     ldsum, y, ldy, q, ldq, scale, ldscale)
+        else:
+            status = self.rms_norm_status(k, n, type, x, ldx, residual, ldr, weight, eps, sum, ldsum,
+                                          y, ldy, q, ldq, scale, ldscale)
         if status:
             raise SgblasError("sgblasRmsNorm", status)
 
@@ -418,8 +443,14 @@ class Handle:
                                          _ptr(weight), eps, _ptr(dsum), lddsum, _ptr(dx), lddx,
                                          _fp(beta), _ptr(dweight))
 
-    def rms_norm_backward(self, *args, **kwargs) -> None:
-        status = self.rms_norm_backward_status(*args, **kwargs)
+    def rms_norm_backward(self, k, n, type, dy, lddy, sum, ldsum, weight, eps, dsum, lddsum, dx, lddx,
+                          beta=None, dweight=None) -> None:
+        if lib is _direct:
+            status = _calls.rms_norm_backward(self._address, k, n, type, dy, lddy, sum, ldsum, weight,
+                                              eps, dsum, lddsum, dx, lddx, beta, dweight)
+        else:
+            status = self.rms_norm_backward_status(k, n, type, dy, lddy, sum, ldsum, weight, eps, dsum,
+                                                   lddsum, dx, lddx, beta, dweight)
         if status:
             raise SgblasError("sgblasRmsNormBackward", status)
 
@@ -428,7 +459,7 @@ class Handle:
         return lib.sgblasSortTokens(self._h, n, top, groups, _ptr(group), _ptr(offsets), _ptr(place))
 
     def sort_tokens(self, *args) -> None:
-        status = self.sort_tokens_status(*args)
+        status = _calls.sort_tokens(self._address, *args) if lib is _direct else self.sort_tokens_status(*args)
         if status:
             raise SgblasError("sgblasSortTokens", status)
 
@@ -438,7 +469,7 @@ class Handle:
                                        type, ldx, _ptr(y), ldy)
 
     def scatter_tokens(self, *args) -> None:
-        status = self.scatter_tokens_status(*args)
+        status = _calls.scatter_tokens(self._address, *args) if lib is _direct else self.scatter_tokens_status(*args)
         if status:
             raise SgblasError("sgblasScatterTokens", status)
 
@@ -448,7 +479,7 @@ class Handle:
                                       type, ldx, _ptr(y), ldy)
 
     def gather_tokens(self, *args) -> None:
-        status = self.gather_tokens_status(*args)
+        status = _calls.gather_tokens(self._address, *args) if lib is _direct else self.gather_tokens_status(*args)
         if status:
             raise SgblasError("sgblasGatherTokens", status)
 
@@ -459,8 +490,14 @@ class Handle:
                                               _ptr(dy), type, lddy, _ptr(x), ldx, _ptr(dx), lddx,
                                               _ptr(dweights))
 
-    def gather_tokens_backward(self, *args, **kwargs) -> None:
-        status = self.gather_tokens_backward_status(*args, **kwargs)
+    def gather_tokens_backward(self, k, n, top, rows, place, weights, dy, type, lddy, x, ldx, dx, lddx,
+                               dweights=None) -> None:
+        if lib is _direct:
+            status = _calls.gather_tokens_backward(self._address, k, n, top, rows, place, weights, dy,
+                                                   type, lddy, x, ldx, dx, lddx, dweights)
+        else:
+            status = self.gather_tokens_backward_status(k, n, top, rows, place, weights, dy, type, lddy,
+                                                        x, ldx, dx, lddx, dweights)
         if status:
             raise SgblasError("sgblasGatherTokensBackward", status)
 

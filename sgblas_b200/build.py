@@ -8,6 +8,8 @@ Every translation unit under sgblas_b200/csrc is compiled for
 ``sgblas_b200/lib/libsgblas.so`` together with a static CUDA runtime, so the
 library does not depend on whichever libcudart another package (torch) loaded.
 Objects are rebuilt only when a source or header is newer than the object.
+Where Python's headers are installed, calls.c becomes sgblas_b200/_calls*.so, the
+compiled caller of the shortest entry points (without it they go by ctypes).
 """
 from __future__ import annotations
 
@@ -17,6 +19,7 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
@@ -65,9 +68,26 @@ def _compile(src: pathlib.Path, verbose: bool) -> pathlib.Path:
     return obj
 
 
+def _build_calls() -> None:
+    include = pathlib.Path(sysconfig.get_paths()["include"])
+    src, out = PKG / "calls.c", PKG / f"_calls{sysconfig.get_config_var('EXT_SUFFIX')}"
+    if not (include / "Python.h").exists():
+        return
+    newest = max(p.stat().st_mtime for p in (src, INCLUDE / "sgblas" / "sgblas.h", INCLUDE / "sgblas" / "sgblas_lm.h"))
+    if out.exists() and out.stat().st_mtime >= newest:
+        return
+    tmp = out.with_suffix(".tmp")
+    res = subprocess.run(["gcc", "-std=gnu11", "-O2", "-fPIC", "-shared", "-Wall", "-Wextra", f"-I{include}",
+                          f"-I{INCLUDE}", str(src), "-o", str(tmp)], capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compiling calls.c failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, out)
+
+
 def build(verbose: bool = False) -> pathlib.Path:
     OBJ.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
+    _build_calls()
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
