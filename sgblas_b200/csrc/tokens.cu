@@ -65,9 +65,10 @@ __device__ __forceinline__ int blockScan(int v, int *slots, int *total) {
 // lanes before. The counts are summed over a CTA's warps, over the cluster's CTAs
 // (through distributed shared memory) and over the groups, and each entry adds where
 // its warp's part of its group begins. Bound by latencies: the loads', the counts'
-// and the cluster's (65536 entries, 64 groups: 11.4 us; with __match_any_sync and a
+// and the cluster's (65536 entries, 64 groups: 10.2 us; with __match_any_sync and a
 // second walk 22.5).
-__global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParams p, int ctas, int bits) {
+template <int kBits>   // of a group's number, p.groups (none) among them
+__global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParams p, int ctas) {
   extern __shared__ int counts[];   // [warps][groups], the CTA's sums, where its groups begin
   __shared__ int slots[kSortThreads / 32];
   kern::gridDependencyWait();
@@ -76,10 +77,10 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
   const int rank = static_cast<int>(blockIdx.x);
   int *mine = counts + warp * p.groups;
   int *sums = counts + warps * p.groups, *starts = sums + p.groups;
+  // 2^30 entries at most, and 2^8 warps of 32 of them more.
   const int parts = ctas * warps;
-  const long long per = ((p.entries + parts - 1LL) / parts + 31) / 32 * 32;
-  const int begin = static_cast<int>(min(per * (rank * warps + warp), static_cast<long long>(p.entries)));
-  const int end = static_cast<int>(min(begin + per, static_cast<long long>(p.entries)));
+  const int per = ((p.entries + parts - 1) / parts + 31) / 32 * 32;
+  const int begin = min(per * (rank * warps + warp), p.entries), end = min(begin + per, p.entries);
   const bool once = per <= 32 * kSortBatch;   // the range fits the registers
   for (int g = lane; g < p.groups; g += 32) mine[g] = 0;
   __syncwarp();
@@ -99,9 +100,10 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
       if (i0 + b * 32 >= end) break;
       const int g = group[b];
       unsigned same = 0xffffffffu;
-      for (int bit = 0; bit < bits; ++bit) {
-        const unsigned set = __ballot_sync(0xffffffffu, g >> bit & 1);
-        same &= g >> bit & 1 ? set : ~set;
+#pragma unroll
+      for (int bit = 0; bit < kBits; ++bit) {
+        const int unset = (g >> bit & 1) - 1;   // all ones where the bit is zero
+        same &= __ballot_sync(0xffffffffu, unset == 0) ^ static_cast<unsigned>(unset);
       }
       const bool live = g < p.groups;
       const int before = live ? mine[g] : 0;
@@ -131,12 +133,18 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
     const int g = g0 + threadIdx.x;
     int total = 0, before = 0;
     if (g < p.groups) {
+      // All CTAs' sums at once: one latency of the cluster's, not eight.
+      int there[kSortMaxCluster];
 #pragma unroll
       for (int c = 0; c < kSortMaxCluster; ++c) {
-        if (c == ctas) break;
-        const int there = ctas > 1 ? kern::ldCluster(kern::clusterAddr(kern::smemAddr(sums + g), c)) : sums[g];
-        if (c < rank) before += there;
-        total += there;
+        there[c] = 0;
+        if (ctas == 1 && c == 0) there[c] = sums[g];
+        if (ctas > 1 && c < ctas) there[c] = kern::ldCluster(kern::clusterAddr(kern::smemAddr(sums + g), c));
+      }
+#pragma unroll
+      for (int c = 0; c < kSortMaxCluster; ++c) {
+        if (c < rank) before += there[c];
+        total += there[c];
       }
     }
     int all;
@@ -417,9 +425,11 @@ extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top
   DeviceInfo dev;
   const sgblasStatus_t st = currentDevice(&dev);
   if (st != SGBLAS_STATUS_SUCCESS) return st;
-  static std::atomic<uint64_t> configured{0};
   constexpr int kMost = (kSortThreads / 32 + 2) * SGBLAS_MAX_GROUPS * 4;
-  if (!configureKernel(reinterpret_cast<const void *>(sortTokensKernel), dev.device, kMost, &configured))
+  static_assert(SGBLAS_MAX_GROUPS < 1 << 11, "a group's bits");
+  static std::atomic<uint64_t> configured[2];
+  auto *kernel = groups < 256 ? sortTokensKernel<8> : sortTokensKernel<11>;
+  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, kMost, &configured[groups < 256 ? 0 : 1]))
     return SGBLAS_STATUS_EXECUTION_FAILED;
   SortParams p = {};
   p.group = group;
@@ -447,9 +457,7 @@ extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ctas > 1 ? 2 : 1;
-  int bits = 0;   // of a group's number, none among them
-  while (groups >> bits != 0) ++bits;
-  return launchStatus(cudaLaunchKernelEx(&cfg, sortTokensKernel, p, ctas, bits));
+  return launchStatus(cudaLaunchKernelEx(&cfg, kernel, p, ctas));
 }
 
 extern "C" sgblasStatus_t sgblasScatterTokens(sgblasHandle_t handle, int k, int n, int top, int rows,

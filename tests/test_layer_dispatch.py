@@ -126,10 +126,11 @@ def test_every_norm_and_token_kernel_is_tested(log):
                     h.gather_tokens_backward(k, n, top, n * top, at, at, at, type_, k + ld, at, k + ld, at, k + ld, at)
         for k in (16, 37):
             h.scatter_tokens(k, 50, 3, 150, FAKE, None, FAKE, BYTE, k, FAKE, k)
-        h.sort_tokens(10, 2, 4, FAKE, FAKE, FAKE)
+        for groups in (4, 1000):
+            h.sort_tokens(10, 2, groups, FAKE, FAKE, FAKE)
         for ldx in (64, 65):
             for type_ in (BF16, FP32):
                 h.quantize_fp4(64, 5, FAKE, type_, ldx, FAKE, 32, FAKE, 2)
-    for part, count in (("rmsNorm", 30), ("sumParts", 1), ("scatterTokens", 6), ("gatherTokens", 8), ("sortTokens", 1), ("quantizeFp4", 4)):
+    for part, count in (("rmsNorm", 30), ("sumParts", 1), ("scatterTokens", 6), ("gatherTokens", 8), ("sortTokens", 2), ("quantizeFp4", 4)):
         every, left = reached(log, part)
         assert len(every) >= count and not left, (len(every), left)

@@ -40,7 +40,7 @@ def check_sort(handle, group, groups):
 
 @pytest.mark.parametrize("n,top,groups", [
     (0, 2, 5), (3, 0, 4), (1, 1, 1), (5, 3, 7), (31, 1, 2), (32, 2, 1024), (100, 8, 64), (129, 1, 3),
-    (1000, 8, 128), (777, 3, 1000), (4096, 4, 33), (16384, 8, 64), (50001, 5, 1024)])
+    (1000, 8, 128), (777, 3, 1000), (300, 2, 255), (300, 2, 256), (700, 3, 1023), (4096, 4, 33), (16384, 8, 64), (50001, 5, 1024)])
 def test_sort(cuda, handle, n, top, groups):
     gen = generator(n + top)
     group = torch.randint(-2, groups + 2, (n, top), generator=gen, device="cuda", dtype=torch.int32)
