@@ -188,7 +188,8 @@ sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int n, int batc
  * are h to sum (NULL: not), v to y (NULL: not), and v in e4m3 to q (NULL: not),
  * with the scales in `scale`, as sgblasQuantizeFp8 with block_n = 1 writes them;
  * y or q has to be given. Everything between h and the roundings to y and q is
- * FP32, so squares of h have to stay in its range (magnitudes above 2^63 give 0).
+ * FP32, so squares of h have to stay in its range: magnitudes above 2^63 give 0, and
+ * without an eps those below 2^-60 are inexact.
  * sum may be x or residual itself (the same address and leading dimension):
  * the residual is then updated in place. */
 sgblasStatus_t sgblasRmsNorm(sgblasHandle_t handle, int k, int n, sgblasDataType_t type,

@@ -5,7 +5,8 @@ reference sgBLAS API (``include/sgblas/sgblas.h``). This module is a thin
 ctypes mirror of that API for Python callers and for the test-suite: the same
 entry-point names, the same argument meaning and the same status codes
 (``sgblasCreate`` ... ``sgblasSgemm``; reference ``include/sgblas/sgblas.h:38-62``
-of AG0708/sgBLAS), plus a small object wrapper (:class:`Handle`).
+of AG0708/sgBLAS), plus a small object wrapper (:class:`Handle`). The shortest entry
+points go through a compiled caller (``calls.c``) instead of ctypes where it was built.
 
 There is no CPU fallback: importing this module fails loudly when the library
 has not been built (``python sgblas_b200/build.py``).

@@ -231,3 +231,62 @@ def test_the_example_serves_in_4_bits(cuda):
     losses, deviation = example.main(300, 256, 512, 6, steps=3, quiet=True)
     assert len(losses) == 3 and all(loss == loss for loss in losses) and 0 < deviation < 0.08
     assert sg.get_device_errors() == 0
+
+
+def test_one_handle_on_two_streams(cuda, lib):
+    """Calls that use the handle's workspace (partial sums, laid-out scales) wait for
+    each other, whichever streams they are on."""
+    n, k = 20000, 1024
+    gen = generator(5)
+    rand = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(torch.bfloat16)  # noqa: E731
+    h_, dy = [rand(n, k) for _ in range(2)], [rand(n, k) for _ in range(2)]
+    codes = [[torch.randint(0, 256, (6144, k), generator=gen, device="cuda").to(torch.uint8) for _ in range(2)] for _ in range(2)]
+    scales = [[torch.randint(118, 128, (6144, k // 16), generator=gen, device="cuda").to(torch.uint8) for _ in range(2)] for _ in range(2)]
+    new = lambda: ([torch.empty(k, device="cuda") for _ in range(2)], [torch.empty(n, k, dtype=torch.bfloat16, device="cuda") for _ in range(2)],  # noqa: E731
+                   [torch.empty(6144, 6144, dtype=torch.bfloat16, device="cuda") for _ in range(2)])
+
+    def call(h, i, dw, dx, y):
+        h.rms_norm_backward(k, n, BF16, dy[i], k, h_[i], k, None, EPS, None, k, dx[i], k, 0.0, dw[i])
+        h.gemm_fp4(6144, 6144, 2 * k, codes[i][0], k, scales[i][0], k // 16, codes[i][1], k, scales[i][1], k // 16, y[i], BF16, 6144)
+
+    with lib.Handle() as h:
+        want = new()
+        for i in range(2):
+            call(h, i, *want)
+            torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = new()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for i in range(2):
+                h.set_stream(streams[i])
+                call(h, i, *got)
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_two_handles_at_once(cuda, lib):
+    """Two layers on two streams, each with its own handle."""
+    made_ = [made(500, 256, 320, 6, seed) for seed in (3, 4)]
+    handles = [lib.Handle() for _ in range(2)]
+    try:
+        layers = [Layer(h, *m[:-1]) for h, m in zip(handles, made_)]
+        for layer, m in zip(layers, made_):
+            layer.forward(), layer.backward(m[-1])
+        torch.cuda.synchronize()
+        want = [[v.clone() for v in (layer.out, layer.dx, layer.dw, layer.dw1, layer.dw2, layer.dgate)] for layer in layers]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        for h, s in zip(handles, streams):
+            h.set_stream(s)
+        for _ in range(5):
+            for layer, m, s in zip(layers, made_, streams):
+                with torch.cuda.stream(s):
+                    layer.forward(), layer.backward(m[-1])
+        torch.cuda.synchronize()
+        for layer, w in zip(layers, want):
+            got = (layer.out, layer.dx, layer.dw, layer.dw1, layer.dw2, layer.dgate)
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
+    finally:
+        for h in handles:
+            h.close()
