@@ -175,7 +175,12 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
 
 // ---- moving columns ------------------------------------------------------------
 
-constexpr int kMoveThreads = 256;
+// A CTA's threads. With sums over choices more and smaller CTAs have columns on their way
+// while others wait for places or shuffle: 8192 tokens with 8 choices, 2048 values, on 256,
+// 128 and 64 threads combined in 51, 47 and 46 us, their gradients in 94, 86 and 90;
+// sorted and scattered in 57.5 and 58.7. 16 tokens' gradients 2.6, 2.9.
+constexpr int kScatterThreads = 256;
+constexpr int kGatherThreads = 128;
 constexpr int kBatch = 4;   // choices whose columns are on their way at once (sumFour)
 
 struct MoveParams {
@@ -197,7 +202,7 @@ constexpr bool kNumber = sizeof(T) > 1;   // bytes move as they are
 // y(:, place(j, t)) = weight(j, t) x(:, t). Bound by its stores: 8192 tokens with 8
 // choices, 2048 BF16 values, 48 us (293 MB, 6.1 TB/s).
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(kMoveThreads) scatterTokensKernel(const MoveParams p) {
+__global__ void __launch_bounds__(kScatterThreads) scatterTokensKernel(const MoveParams p) {
   using L = Lanes<T, kVector>;
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
@@ -229,9 +234,9 @@ __global__ void __launch_bounds__(kMoveThreads) scatterTokensKernel(const MovePa
 }
 
 // y(:, t) = sum over j of weight(j, t) x(:, place(j, t)), in the order of j. Bound by its
-// loads, kBatch columns of a token at a time: the same tokens 51 us (5.8 TB/s).
+// loads, kBatch columns of a token at a time: the same tokens 47 us (6.2 TB/s).
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(kMoveThreads) gatherTokensKernel(const MoveParams p) {
+__global__ void __launch_bounds__(kGatherThreads) gatherTokensKernel(const MoveParams p) {
   using L = Lanes<T, kVector>;
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
@@ -286,12 +291,12 @@ __device__ __forceinline__ float sumFour(const float (&v)[4], int lane) {
 // y(:, place(j, t)) = weight(j, t) dy(:, t) and, with dweight,
 // dweight(j, t) = sum over k of dy(k, t) x(k, place(j, t)); a CTA's row of
 // blockDim.x threads per token, so that dy is read once for kBatch choices and dweight
-// needs no second pass. Bound by HBM: the same tokens 95 us (5.8 TB/s); 3001 tokens with
-// 3 choices, 1537 values on odd addresses, 22 us (2.8 TB/s).
+// needs no second pass. Bound by HBM: the same tokens 86 us (6.4 TB/s); 3001 tokens with
+// 3 choices, 1537 values on odd addresses, 20 us (3.1 TB/s).
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(kMoveThreads, 4) gatherTokensBackwardKernel(const MoveParams p) {
+__global__ void __launch_bounds__(kGatherThreads, 8) gatherTokensBackwardKernel(const MoveParams p) {
   using L = Lanes<T, kVector>;
-  __shared__ float partial[kMoveThreads / 32][kBatch];
+  __shared__ float partial[kGatherThreads / 32][kBatch];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
   const long long t = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
@@ -375,9 +380,10 @@ sgblasStatus_t launchMove(Move move, MoveParams p, int sms, cudaStream_t stream)
   p.slots = ((p.k - 1) / kern::kLaneBlock + 1) * L::kThreads;
   const bool whole = move == Move::kBackward;   // a token's threads share its sums
   // Threads in whole warps, as busy in their last turn as in the others.
-  const int turns = (p.slots - 1) / kMoveThreads + 1;
+  const int limit = move == Move::kScatter ? kScatterThreads : kGatherThreads;
+  const int turns = (p.slots - 1) / limit + 1;
   const int threads = ((p.slots - 1) / turns / 32 + 1) * 32;
-  const int tokens = whole && threads > 32 ? 1 : kMoveThreads / threads;
+  const int tokens = whole && threads > 32 ? 1 : limit / threads;
   const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(tokens));
   const int across = (p.n - 1) / tokens + 1;
   // Long columns of few tokens are cut, so that every SM has some.
