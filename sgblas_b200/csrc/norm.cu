@@ -56,7 +56,8 @@ struct NormBackwardParams {
   const void *dy, *sum, *weight, *dsum;
   void *dx;
   float *part;        // NULL: no gradient of the weights
-  int k, n, part_ld;
+  long long part_ld;
+  int k, n;
   float eps, over_k;
   int lddy, ldsum, lddsum, lddx;
 };
@@ -268,7 +269,7 @@ __device__ __forceinline__ void storePart(const NormBackwardParams &p,
                                           float2 (&dw)[kUnits][Lanes<T, kVector>::kPairs],
                                           float2 *exchange) {
   using L = Lanes<T, kVector>;
-  float *part = p.part + static_cast<size_t>(blockIdx.x) * p.part_ld;
+  float *part = p.part + blockIdx.x * p.part_ld;
   const int stride = static_cast<int>(blockDim.x);
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) ds[u].clear();
     if constexpr (kLong) {
-      float *part = p.part == nullptr ? nullptr : p.part + static_cast<size_t>(blockIdx.x) * p.part_ld;
+      float *part = p.part == nullptr ? nullptr : p.part + blockIdx.x * p.part_ld;
       auto read = [&](int slot) {
         const int at = L::begin(slot);
         h[0].load(h0 + at, p.k - at);
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(streamCta(kUnits, true), streamThreads(kUnits,
 // warp per kReduceWarps-th row, in a fixed order. Bound by latency: 296 rows of 4096
 // values, which lie in L2, 3 us.
 __global__ void __launch_bounds__(kReduceThreads)
-    sumPartsKernel(const float *part, int rows, int part_ld, int k, float beta, float *dw) {
+    sumPartsKernel(const float *part, int rows, long long part_ld, int k, float beta, float *dw) {
   __shared__ float slots[kReduceWarps][32];
   kern::gridDependencyWait();
   kern::allowDependentLaunch();
@@ -600,7 +601,7 @@ __global__ void __launch_bounds__(kReduceThreads)
   float s = 0.0F;
   if (at < k) {
 #pragma unroll 8
-    for (int r = warp; r < rows; r += kReduceWarps) s += part[static_cast<size_t>(r) * part_ld + at];
+    for (int r = warp; r < rows; r += kReduceWarps) s += part[r * part_ld + at];
   }
   slots[warp][lane] = s;
   __syncthreads();
@@ -832,7 +833,7 @@ extern "C" sgblasStatus_t sgblasRmsNormBackward(sgblasHandle_t handle, int k, in
   if (n > 0) {
     const Shape s = chooseShape(k, size, vector, n, true, dev.sms);
     rows = persistentCtas(s, n, dev.sms);
-    p.part_ld = (k + 31) / 32 * 32;
+    p.part_ld = (k + 31LL) / 32 * 32;
     if (dweight != nullptr) {
       const size_t bytes = sizeof(float) * static_cast<size_t>(p.part_ld) * static_cast<size_t>(rows);
       if (!ensureWorkspace(handle, kCounterRegionBytes + bytes, dev.device, stream))

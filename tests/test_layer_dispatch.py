@@ -113,6 +113,15 @@ def test_a_failed_weight_gradient_is_a_use(log, at):
         assert log.lines()[-1] == "record"
 
 
+def test_the_longest_columns_partial_sums(log):
+    """Four bytes for each of 2^31 values: their size is not counted in 32 bits."""
+    k = 2**31 - 1
+    with sg.Handle() as h:
+        h.rms_norm_backward(k, 1, BF16, FAKE, k, FAKE, k, FAKE, 1e-6, FAKE, k, FAKE, k, 0.0, FAKE)
+    sizes = [int(line.split()[2]) for line in log.lines() if line.startswith("malloc")]
+    assert 2**33 <= max(sizes) < 2**34, sizes   # with room for larger calls
+
+
 def test_every_norm_and_token_kernel_is_tested(log):
     with sg.Handle() as h:
         for type_ in (BF16, FP32):
