@@ -456,6 +456,13 @@ __device__ __forceinline__ void clusterSync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same in two parts, where nothing written before the first is read after the second.
+__device__ __forceinline__ void clusterArriveRelaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void clusterWait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // mbarWait for a barrier that other CTAs of the cluster arrive on: acquires at
 // cluster scope what they released.
 __device__ __forceinline__ bool mbarWaitCluster(uint64_t *bar, uint32_t parity, unsigned *err) {

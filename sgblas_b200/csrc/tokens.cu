@@ -24,7 +24,7 @@ using kern::Lanes;
 // ---- the sort ------------------------------------------------------------------
 
 constexpr int kSortThreads = 1024;
-constexpr int kSortMaxCluster = 8;
+constexpr int kSortMaxCluster = 16;      // 8 where the device has no room for 16 (clusterLimit)
 constexpr int kSortCtaWarps = 8;
 constexpr int kSortWarpEntries = 64;   // of a warp, before another warp (CTA) joins
 
@@ -65,8 +65,8 @@ __device__ __forceinline__ int blockScan(int v, int *slots, int *total) {
 // lanes before. The counts are summed over a CTA's warps, over the cluster's CTAs
 // (through distributed shared memory) and over the groups, and each entry adds where
 // its warp's part of its group begins. Bound by latencies: the loads', the counts'
-// and the cluster's (65536 entries, 64 groups: 10.2 us; with __match_any_sync and a
-// second walk 22.5).
+// and the cluster's (65536 entries, 64 groups: 7.0 us, in clusters of 8 CTAs 10.1; 524288
+// entries 25 and 51; with 8, __match_any_sync and a second walk 65536 took 22.5).
 template <int kBits>   // of a group's number, p.groups (none) among them
 __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParams p, int ctas) {
   extern __shared__ int counts[];   // [warps][groups], the CTA's sums, where its groups begin
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
   const int rank = static_cast<int>(blockIdx.x);
   int *mine = counts + warp * p.groups;
   int *sums = counts + warps * p.groups, *starts = sums + p.groups;
-  // 2^30 entries at most, and 2^8 warps of 32 of them more.
+  // 2^30 entries at most, and 2^9 warps of 32 of them more.
   const int parts = ctas * warps;
   const int per = ((p.entries + parts - 1) / parts + 31) / 32 * 32;
   const int begin = min(per * (rank * warps + warp), p.entries), end = min(begin + per, p.entries);
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
     const int g = g0 + threadIdx.x;
     int total = 0, before = 0;
     if (g < p.groups) {
-      // All CTAs' sums at once: one latency of the cluster's, not eight.
+      // All CTAs' sums at once: one latency of the cluster's, not one each.
       int there[kSortMaxCluster];
 #pragma unroll
       for (int c = 0; c < kSortMaxCluster; ++c) {
@@ -157,6 +157,8 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
   }
   if (rank == 0 && threadIdx.x == 0) p.offsets[p.groups] = carry;
   __syncthreads();
+  // No CTA leaves while another reads its sums; this one has them, in `starts`.
+  if (ctas > 1) kern::clusterArriveRelaxed();
   for (int i0 = begin; i0 < end; i0 += 32 * kSortBatch) {
     if (!once) {
       readGroups(i0);
@@ -170,7 +172,34 @@ __global__ void __launch_bounds__(kSortThreads) sortTokensKernel(const SortParam
       if (i < end) p.place[i] = g < p.groups ? starts[g] + mine[g] + local[b] : -1;
     }
   }
-  if (ctas > 1) kern::clusterSync();   // no CTA leaves while another reads its sums
+  if (ctas > 1) kern::clusterWait();
+}
+
+// The largest cluster that the kernel can have on the device: 16 CTAs are allowed to
+// kernels that ask for them, not promised (a part of a GPU may have no 16 SMs together).
+int clusterLimit(const void *kernel, int device, int smem, std::atomic<int> *known) {
+  int limit = known[device].load(std::memory_order_relaxed);
+  if (limit > 0) return limit;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kSortMaxCluster;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSortMaxCluster);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    clusters = 0;
+  }
+  limit = clusters > 0 ? kSortMaxCluster : kSortMaxCluster / 2;
+  known[device].store(limit, std::memory_order_relaxed);
+  return limit;
 }
 
 // ---- moving columns ------------------------------------------------------------
@@ -434,9 +463,12 @@ extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top
   constexpr int kMost = (kSortThreads / 32 + 2) * SGBLAS_MAX_GROUPS * 4;
   static_assert(SGBLAS_MAX_GROUPS < 1 << 11, "a group's bits");
   static std::atomic<uint64_t> configured[2];
+  static std::atomic<int> known[2][kMaxDevices];
   auto *kernel = groups < 256 ? sortTokensKernel<8> : sortTokensKernel<11>;
-  if (!configureKernel(reinterpret_cast<const void *>(kernel), dev.device, kMost, &configured[groups < 256 ? 0 : 1]))
-    return SGBLAS_STATUS_EXECUTION_FAILED;
+  const auto *entry = reinterpret_cast<const void *>(kernel);
+  const int which = groups < 256 ? 0 : 1;
+  if (!configureKernel(entry, dev.device, kMost, &configured[which])) return SGBLAS_STATUS_EXECUTION_FAILED;
+  const int most = clusterLimit(entry, dev.device, kMost, known[which]);
   SortParams p = {};
   p.group = group;
   p.offsets = offsets;
@@ -447,7 +479,7 @@ extern "C" sgblasStatus_t sgblasSortTokens(sgblasHandle_t handle, int n, int top
   // cluster's, then more warps.
   const long long wanted = std::max(1LL, (entries + kSortWarpEntries - 1) / kSortWarpEntries);
   int ctas = 1;
-  while (ctas < kSortMaxCluster && static_cast<long long>(ctas) * kSortCtaWarps < wanted) ctas *= 2;
+  while (ctas < most && static_cast<long long>(ctas) * kSortCtaWarps < wanted) ctas *= 2;
   const int warps = static_cast<int>(std::min<long long>(kSortThreads / 32, std::max((wanted - 1) / ctas + 1, 4LL)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));

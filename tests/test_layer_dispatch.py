@@ -113,6 +113,13 @@ def test_a_failed_weight_gradient_is_a_use(log, at):
         assert log.lines()[-1] == "record"
 
 
+@pytest.mark.parametrize("n,top,ctas", [(16, 4, 1), (1024, 2, 4), (1024, 8, 16), (65536, 8, 16)])
+def test_ctas_of_a_sort(log, n, top, ctas):
+    with sg.Handle() as h:
+        h.sort_tokens(n, top, 64, FAKE, FAKE, FAKE)
+    assert [grid for _, grid in log.launches()] == [ctas]
+
+
 def test_the_longest_columns_partial_sums(log):
     """Four bytes for each of 2^31 values: their size is not counted in 32 bits."""
     k = 2**31 - 1
