@@ -163,25 +163,13 @@ sgblasStatus_t launchQuantize(void (*kernel)(QuantParams), const QuantParams &p,
 constexpr int kPairWidth = 192;
 using PairCfg = t::Fp4Cfg<kPairWidth, true, false>;   // or true: the same tiles
 
-// Workspace of the laid-out scales of a pair product: those of A, then those of B.
-struct LaidSize {
-  long long a, b;   // bytes
-};
-LaidSize laidSize(const t::Params &p) {
-  const long long iters = (p.k + t::kRowBytes - 1) / t::kRowBytes;
-  const long long tiles = p.n / kPairWidth + std::min<long long>(p.groups, p.n);
-  LaidSize s;
-  s.a = static_cast<long long>(p.groups) * t::scaleBlocksA(p.m) * iters * t::kScaleRowsA * t::kScaleRowBytes;
-  s.b = tiles * iters * t::kScaleRowsB * t::kScaleRowBytes;
-  return s;
-}
-
 // Lays out the scales in the workspace at `at` and sets the maps.
 sgblasStatus_t layScales(const DeviceInfo &dev, t::Fp4Params &f, unsigned char *at, cudaStream_t stream) {
   t::Params &p = f.p;
-  const LaidSize size = laidSize(p);
+  const t::LaidSize size = t::laidSize<PairCfg>(p);
   f.laid_a = at;
   f.laid_b = at + size.a;
+  f.laid_tiles = static_cast<int>(size.tiles);
   p.tiles_m = (p.m - 1) / PairCfg::kTileM + 1;
   auto encode = [](CUtensorMap *map, const void *from, long long bytes, int rows) {
     return encodeTyped3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, from, t::kScaleRowBytes, bytes / t::kScaleRowBytes, 1,
@@ -409,7 +397,7 @@ sgblasStatus_t gemmFp4(sgblasHandle_t handle, int m, int n, int k, int groups, c
       size[i] = tmaReadable(op[i], 1) ? 0 : copyBytes(op[i], 1);
       all += size[i];
     }
-    const LaidSize extra = laidSize(p);
+    const t::LaidSize extra = t::laidSize<PairCfg>(p);
     if (width == kPairWidth) {
       // Without a workspace for the scales, single CTAs, which stage them.
       if (std::max(extra.a, extra.b) / t::kScaleRowBytes <= INT_MAX &&

@@ -43,6 +43,7 @@ struct Fp4Params {
   // Pairs: the scales' blocks, and the maps they are read by: rows of 256 bytes, a slice's
   // kScaleRowsA of each 128 rows of a matrix of A, and kScaleRowsB of each tile's columns.
   unsigned char *laid_a, *laid_b;
+  int laid_tiles;                    // tiles of columns that laid_b has room for
   CUtensorMap tma_sa, tma_sb;
 };
 
@@ -261,9 +262,75 @@ __device__ __forceinline__ void issueSlice(uint32_t tmem_base, uint32_t d_tmem, 
 // Blocks of 128 rows of a matrix of A.
 __host__ __device__ __forceinline__ int scaleBlocksA(int m) { return (m + kBM - 1) / kBM; }
 
+// Room for the laid-out scales of pairs of width G::kBN: those of A, then those of B, in
+// bytes. Groups whose offsets do not decrease have no more tiles than that.
+struct LaidSize {
+  long long a, b, tiles;
+};
+template <class G>
+__host__ __device__ __forceinline__ LaidSize laidSize(const Params &p) {
+  const long long iters = (p.k + kRowBytes - 1) / kRowBytes;
+  LaidSize s;
+  s.tiles = p.n / G::kBN + (p.groups < p.n ? p.groups : p.n);
+  s.a = static_cast<long long>(p.groups) * scaleBlocksA(p.m) * iters * kScaleRowsA * kScaleRowBytes;
+  s.b = s.tiles * iters * kScaleRowsB * kScaleRowBytes;
+  return s;
+}
+
+// The scales' blocks in items: a chunk (16 scales) of 128 rows of A, or of half a tile's
+// columns. Offsets that decrease, which the host cannot see, give more tiles than it has
+// counted: blocks past its room are left out.
+__host__ __device__ __forceinline__ long long laidItemsA(const Params &p) {
+  const int iters = (p.k + kRowBytes - 1) / kRowBytes;
+  return static_cast<long long>(p.groups) * scaleBlocksA(p.m) * ((iters + 1) / 2);
+}
+template <class G>
+__host__ __device__ __forceinline__ long long laidItems(const Fp4Params &f, const GroupTable &table) {
+  const int iters = (f.p.k + kRowBytes - 1) / kRowBytes;
+  const int tiles = table.first[f.p.groups] < f.laid_tiles ? table.first[f.p.groups] : f.laid_tiles;
+  return laidItemsA(f.p) + static_cast<long long>(tiles) * G::kBBlocks * ((iters + 1) / 2);
+}
+
+struct LaidItem {
+  const unsigned char *from;
+  unsigned char *to;           // of the chunk's first slice
+  int rows, ld, chunk;         // no rows: nothing to lay out
+  int slice, next;             // bytes of a slice, and from its first 128 of k to its second
+};
+template <class G>
+__host__ __device__ __forceinline__ LaidItem laidItem(const Fp4Params &f, const GroupTable &table, long long i) {
+  const Params &p = f.p;
+  const int iters = (p.k + kRowBytes - 1) / kRowBytes, chunks = (iters + 1) / 2;
+  const int blocks_a = scaleBlocksA(p.m);
+  const long long items_a = laidItemsA(p);
+  const bool is_a = i < items_a;
+  const long long at = is_a ? i : i - items_a;
+  const int block = static_cast<int>(at / chunks);
+  LaidItem r;
+  r.chunk = static_cast<int>(at % chunks);
+  if (is_a) {
+    const int group = block / blocks_a, row0 = (block - group * blocks_a) * kBM;
+    r.from = f.scale_a + group * f.stride_sa + static_cast<long long>(row0) * f.ldsa;
+    r.rows = table.offset[group + 1] <= table.offset[group] ? 0 : p.m - row0;
+    r.ld = f.ldsa;
+    r.slice = kScaleRowsA * kScaleRowBytes;
+    r.next = kScaleBlock;
+    r.to = f.laid_a + (static_cast<long long>(block) * iters + 2 * r.chunk) * r.slice;
+  } else {
+    const int tile = block / G::kBBlocks, half = block - tile * G::kBBlocks;
+    const Tile t = tileAt<G>(p, table, tile * p.tiles_m);
+    r.from = f.scale_b + static_cast<long long>(t.n0 + half * kBM) * f.ldsb;
+    r.rows = t.cols - half * kBM;
+    r.ld = f.ldsb;
+    r.slice = kScaleRowsB * kScaleRowBytes;
+    r.next = G::kBBlocks * kScaleBlock;
+    r.to = f.laid_b + (static_cast<long long>(tile) * iters + 2 * r.chunk) * r.slice + half * kScaleBlock;
+  }
+  return r;
+}
+
 // Writes the scales' blocks of pairs of width G::kBN (1 MB of each operand's for 8192 x
-// 8192 x 4096: 4 us): a warp per chunk (16 scales) of
-// 128 rows of A, of groups that have columns, or of half a tile's columns.
+// 8192 x 4096: 4 us): a warp per item, of groups that have columns.
 constexpr int kLayThreads = 256;
 template <class G>
 __global__ void __launch_bounds__(kLayThreads) layScalesKernel(const __grid_constant__ Fp4Params f) {
@@ -274,44 +341,19 @@ __global__ void __launch_bounds__(kLayThreads) layScalesKernel(const __grid_cons
   const int lane = threadIdx.x % 32;
   if (threadIdx.x < 32) readGroups<G>(p, &table, lane);
   __syncthreads();
-  const int iters = (p.k + kRowBytes - 1) / kRowBytes, chunks = (iters + 1) / 2;
-  const int blocks_a = scaleBlocksA(p.m);
-  const long long items_a = static_cast<long long>(p.groups) * blocks_a * chunks;
-  const long long items = items_a + static_cast<long long>(table.first[p.groups]) * G::kBBlocks * chunks;
+  const int iters = (p.k + kRowBytes - 1) / kRowBytes;
+  const long long items = laidItems<G>(f, table);
   const long long step = gridDim.x * static_cast<long long>(kLayThreads / 32);
   for (long long i = blockIdx.x * (kLayThreads / 32LL) + threadIdx.x / 32; i < items; i += step) {
-    const bool is_a = i < items_a;
-    const long long at = is_a ? i : i - items_a;
-    const int chunk = static_cast<int>(at % chunks), block = static_cast<int>(at / chunks);
-    const unsigned char *from;
-    unsigned char *to;     // of the chunk's first slice
-    int rows, ld, slice, next;   // bytes of a slice, and from its first 128 of k to its second
-    if (is_a) {
-      const int group = block / blocks_a, row0 = (block - group * blocks_a) * kBM;
-      if (table.offset[group + 1] <= table.offset[group]) continue;
-      from = f.scale_a + group * f.stride_sa + static_cast<long long>(row0) * f.ldsa;
-      rows = p.m - row0;
-      ld = f.ldsa;
-      slice = kScaleRowsA * kScaleRowBytes;
-      next = kScaleBlock;
-      to = f.laid_a + (static_cast<long long>(block) * iters + 2 * chunk) * slice;
-    } else {
-      const int tile = block / G::kBBlocks, half = block - tile * G::kBBlocks;
-      const Tile t = tileAt<G>(p, table, tile * p.tiles_m);
-      from = f.scale_b + static_cast<long long>(t.n0 + half * kBM) * f.ldsb;
-      rows = t.cols - half * kBM;
-      ld = f.ldsb;
-      slice = kScaleRowsB * kScaleRowBytes;
-      next = G::kBBlocks * kScaleBlock;
-      to = f.laid_b + (static_cast<long long>(tile) * iters + 2 * chunk) * slice + half * kScaleBlock;
-    }
-    const int bytes = min(16, f.blocks - chunk * 16);
+    const LaidItem it = laidItem<G>(f, table, i);
+    if (i < laidItemsA(p) && it.rows <= 0) continue;
+    const int bytes = min(16, f.blocks - it.chunk * 16);
     uint4 w[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       w[r] = make_uint4(0, 0, 0, 0);
-      const unsigned char *row = from + static_cast<long long>(lane + 32 * r) * ld + chunk * 16;
-      if (lane + 32 * r >= rows) continue;
+      const unsigned char *row = it.from + static_cast<long long>(lane + 32 * r) * it.ld + it.chunk * 16;
+      if (lane + 32 * r >= it.rows) continue;
       if (bytes == 16) {
         w[r] = __ldg(reinterpret_cast<const uint4 *>(row));
       } else {
@@ -322,13 +364,13 @@ __global__ void __launch_bounds__(kLayThreads) layScalesKernel(const __grid_cons
         w[r] = make_uint4(v[0], v[1], v[2], v[3]);
       }
     }
-    uint4 *out = reinterpret_cast<uint4 *>(to) + lane;
+    uint4 *out = reinterpret_cast<uint4 *>(it.to) + lane;
     out[0] = make_uint4(w[0].x, w[1].x, w[2].x, w[3].x);
-    out[next / 16] = make_uint4(w[0].y, w[1].y, w[2].y, w[3].y);
-    if (2 * chunk + 1 < iters) {
-      out += slice / 16;
+    out[it.next / 16] = make_uint4(w[0].y, w[1].y, w[2].y, w[3].y);
+    if (2 * it.chunk + 1 < iters) {
+      out += it.slice / 16;
       out[0] = make_uint4(w[0].z, w[1].z, w[2].z, w[3].z);
-      out[next / 16] = make_uint4(w[0].w, w[1].w, w[2].w, w[3].w);
+      out[it.next / 16] = make_uint4(w[0].w, w[1].w, w[2].w, w[3].w);
     }
   }
 }

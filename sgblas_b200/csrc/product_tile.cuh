@@ -231,7 +231,7 @@ __device__ __forceinline__ int tileCount(const Params &p, const GroupTable &t) {
 }
 
 template <class G>
-__device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int index) {
+__host__ __device__ __forceinline__ Tile tileAt(const Params &p, const GroupTable &t, int index) {
   Tile r;
   if constexpr (G::kSymmetric) {
     constexpr int kWays = G::kTileM / G::kBN;

@@ -230,6 +230,31 @@ def test_offsets_outside_count_as_the_nearer_end(cuda, handle):
     assert torch.equal(c.view, want.float()) and not c.unmarked()
 
 
+# Of pairs of CTAs (test_layer_dispatch.py).
+DECREASING = dict(m=4096, k=1544, n=20000, groups=64)
+
+
+@pytest.mark.parametrize("way", ["swinging", "backwards", "anything"])
+def test_offsets_that_decrease_reach_nothing_else(cuda, handle, way):
+    """They give no result, but more tiles than the host has counted: all that is written
+    is the workspace and C, and the next product is right."""
+    m, k, n, groups = (DECREASING[key] for key in ("m", "k", "n", "groups"))
+    ops = Operands(m, k, [n // groups] * groups, seed=12, tail=n % groups)
+    g = torch.arange(groups + 1, device="cuda")
+    good = ops.offsets.clone()
+    bad = {"swinging": g % 2 * n, "backwards": n - g * (n // groups),
+           "anything": torch.randint(-2**31, 2**31 - 1, (groups + 1,), generator=generator(1), device="cuda")}[way]
+    for ctype in ("bf16", "fp32"):
+        c = Matrix(n, m, TYPES[ctype])
+        ops.offsets.copy_(bad)
+        ops.run(handle, ctype, c)
+        torch.cuda.synchronize()
+        assert not any(v.unmarked() for v in (c, ops.a, ops.b, ops.sa, ops.sb))
+        ops.offsets.copy_(good)
+        check_product(handle, ops, ctype)
+    assert sg.get_device_errors() == 0
+
+
 def test_neighbours_do_not_reach_a_column(cuda, handle):
     """NaN scales of one group's tokens and weights stay in that group."""
     for m, lengths in ((300, [200, 100, 300]), (300, [3, 2, 4]), (300, [8, 13, 9]), (4001, [2500, 3000, 3700])):

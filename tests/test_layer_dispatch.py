@@ -6,7 +6,7 @@ import sgblas_b200 as sg
 from tests import fake_cuda
 from tests.fake_cuda import FAKE
 from tests.lm_cases import RAGGED
-from tests.test_fp4_gpu import ONE_MATRIX, PAIRS, SMALL
+from tests.test_fp4_gpu import DECREASING, ONE_MATRIX, PAIRS, SMALL
 from tests.test_norm_gpu import SIZES as NORM_SIZES
 from tests.test_tokens_gpu import SIZES as TOKEN_SIZES
 
@@ -60,6 +60,13 @@ def test_cases_of_pairs_are_pairs(log, case):
     with sg.Handle() as h:
         fp4(h, case["m"], sum(case["lengths"]), case["k"], len(case["lengths"]), BF16)
     assert "fp4TileKernel<Fp4Cfg<192" in log.launches()[-1][0]
+
+
+def test_decreasing_offsets_are_tested_on_pairs(log):
+    with sg.Handle() as h:
+        for ctype in (BF16, FP32):
+            fp4(h, DECREASING["m"], DECREASING["n"], DECREASING["k"], DECREASING["groups"], ctype)
+            assert "fp4TileKernel<Fp4Cfg<192" in log.launches()[-1][0]
 
 
 @pytest.mark.parametrize("m,n,k,groups,kernel", [
