@@ -17,9 +17,10 @@ extern "C" {
  * No counterpart in the reference (it has no device-side waits). */
 sgblasStatus_t sgblasGetDeviceErrors(unsigned *flags, int clear);
 
-/* Self-test of the kernels' bounded waits: a one-thread kernel waits on a
- * barrier that nothing completes, giving up after `polls` polls. On return
- * *timed_out is 1 when the wait gave up (and the device error flags then hold
+/* Self-test of the kernels' bounded waits: a thread waits on a barrier that
+ * nothing completes, giving up after `polls` polls, and a warp half of whose
+ * lanes gave up has to start no further copy. On return
+ * *timed_out is 1 when both were so (and the device error flags then hold
  * bit 0, which sgblasGetDeviceErrors reads and may clear); the device stays
  * usable. Synchronizes the current device. No counterpart in the reference. */
 sgblasStatus_t sgblasSelfTestWaitTimeout(unsigned polls, int *timed_out);

@@ -1,6 +1,7 @@
 // Device error word and the diagnostics entry point that reads it.
 #include "device.hpp"
 #include "ptx.cuh"
+#include "ring.cuh"
 
 #include <cuda.h>
 
@@ -71,17 +72,36 @@ unsigned *deviceErrorWord(int device) {
 
 namespace {
 
+__device__ uint4 g_ring_source = {1, 2, 3, 4};
+
 // Waits on an mbarrier that nothing will ever complete, with a short poll
 // limit: the wait must give up, raise the error flag and let the kernel
-// return normally. Reports whether the wait returned false.
+// return normally. Then a ring's stage is filled by a warp half of whose lanes gave up
+// before (nothing may be copied, and all lanes have to know), and by one that did not.
+// Reports whether all of it was so.
 __global__ void waitTimeoutKernel(unsigned *err, unsigned polls, int *gave_up) {
-  __shared__ uint64_t bar;
+  __shared__ uint64_t bars[2];
+  __shared__ uint4 stage;
   if (threadIdx.x == 0) {
-    kern::mbarInit(&bar, 1);
+    kern::mbarInit(&bars[0], 1);
+    kern::mbarInit(&bars[1], 1);
     kern::fenceBarrierInit();
+    stage = make_uint4(0, 0, 0, 0);
   }
+  kern::fenceProxyAsyncShared();
   __syncthreads();
-  if (threadIdx.x == 0) *gave_up = kern::mbarWait(&bar, 0, err, polls) ? 0 : 1;
+  bool right = true;
+  if (threadIdx.x == 0) right = !kern::mbarWait(&bars[0], 0, err, polls);
+  __syncwarp();
+  const kern::Ring<1> ring = {reinterpret_cast<unsigned char *>(&stage), &bars[1], sizeof(uint4), 1,
+                              {reinterpret_cast<const unsigned char *>(&g_ring_source)}, {sizeof(uint4)}};
+  const bool some = ring.fill(0, 0, 1, threadIdx.x % 2 != 0);
+  right = right && !some && stage.x == 0 && !kern::mbarTestWait(&bars[1], 0);
+  __syncwarp();
+  right = ring.fill(0, 0, 1, true) && right;
+  right = kern::mbarWait(&bars[1], 0, err) && right && stage.x == 1 && stage.w == 4;
+  const bool all = __all_sync(0xffffffffu, right) != 0;
+  if (threadIdx.x == 0) *gave_up = all ? 1 : 0;
 }
 
 }  // namespace

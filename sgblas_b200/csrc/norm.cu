@@ -14,6 +14,7 @@
 #include "product.hpp"
 #include "ptx.cuh"
 #include "quantize.cuh"
+#include "ring.cuh"
 
 #include <cuda_bf16.h>
 
@@ -24,12 +25,14 @@ namespace sgblas::detail {
 namespace {
 
 using kern::both;
+using kern::kMaxStages;
 using kern::Lanes;
+using kern::Ring;
+using kern::walk;
 
 constexpr int kMaxThreads = 512;
 constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxUnits = 4;          // vectors of a column that a thread holds
-constexpr int kMaxStages = 8;
 // Of the kernels fed by a ring: threads that have to fit an SM, in CTAs of at most
 // streamCta. The backward pass holds four operands and the sums of dw: with 768
 // threads, 80 registers each, it spilled (16384 x 4096 BF16 270 us for 92).
@@ -396,78 +399,9 @@ __global__ void __launch_bounds__(kMaxThreads) rmsNormBackwardKernel(const NormB
 
 // ---- many columns of whole vectors: a persistent grid fed by bulk copies -------------
 
-// A ring of stages in shared memory, each with blockDim.y columns of kRows operands
-// (x and the residual; h, dy and dsum), copied by cp.async.bulk ahead of the columns
-// at work. Registers hold a column only while it is worked on, and the copies do not
-// wait for its sums: with loads straight into registers, each column's latency was
-// uncovered (16384 x 4096 BF16 backward 152 to 192 us, forward 100 to 104). Bound by HBM:
-// that backward 86 to 93 us (5.8 to 6.2 TB/s), forward 94 (5.7), in e4m3 76 (6.2).
-template <int kRows>
-struct Ring {
-  unsigned char *stages;
-  uint64_t *full;
-  int row_bytes, count;
-  const unsigned char *from[kRows];   // NULL: no such operand
-  long long ld[kRows];                // bytes
-
-  __device__ __forceinline__ unsigned char *row(int stage, int operand, int y) const {
-    return stages + static_cast<size_t>((stage * kRows + operand) * static_cast<int>(blockDim.y) + y) * row_bytes;
-  }
-  // The columns from `first` on (up to blockDim.y, of n) into a stage: one warp.
-  __device__ __forceinline__ void fill(int stage, long long first, int n) const {
-    const int columns = static_cast<int>(min(static_cast<long long>(blockDim.y), n - first));
-    int operands = 0;
-#pragma unroll
-    for (int o = 0; o < kRows; ++o) operands += from[o] != nullptr;
-    const int lane = threadIdx.x % 32;
-    if (lane == 0) kern::mbarArriveExpectTx(&full[stage], static_cast<uint32_t>(columns * operands * row_bytes));
-    __syncwarp();
-    if (lane < columns) {
-#pragma unroll
-      for (int o = 0; o < kRows; ++o)
-        if (from[o] != nullptr)
-          kern::bulkLoad(row(stage, o, lane), from[o] + (first + lane) * ld[o], &full[stage],
-                         static_cast<uint32_t>(row_bytes));
-    }
-  }
-};
-
-// Walks a persistent grid's columns: work(stage, turn, column, in) for blockDim.y of
-// them at a time (turn 0 and 1 by turns), which returns after a barrier of the CTA
-// that follows its last read of the stage.
-template <int kRows, class Work>
-__device__ __forceinline__ void walk(const Ring<kRows> &ring, int n, unsigned *err, Work work) {
-  const bool issuer = threadIdx.x < 32 && threadIdx.y == 0;
-  const long long first = blockIdx.x * static_cast<long long>(blockDim.y);
-  const long long step = gridDim.x * static_cast<long long>(blockDim.y);
-  if (issuer) {
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < ring.count; ++i) kern::mbarInit(&ring.full[i], 1);
-      kern::fenceBarrierInit();
-    }
-    __syncwarp();
-    for (int i = 0; i < ring.count; ++i)
-      if (first + i * step < n) ring.fill(i, first + i * step, n);
-  }
-  __syncthreads();
-  int stage = 0, turn = 0;
-  uint32_t parity = 0;
-  bool ok = true;
-  for (long long c = first; c < n; c += step, turn ^= 1) {
-    if (ok) ok = kern::mbarWait(&ring.full[stage], parity, err);
-    work(stage, turn, c + threadIdx.y, c + threadIdx.y < n);
-    const long long next = c + ring.count * step;
-    if (issuer && next < n && ok) {
-      kern::fenceProxyAsyncShared();   // the reads above come before the copy
-      ring.fill(stage, next, n);
-    }
-    if (++stage == ring.count) {
-      stage = 0;
-      parity ^= 1;
-    }
-  }
-}
-
+// With loads straight into registers, each column's latency was uncovered (16384 x 4096
+// BF16 backward 152 to 192 us, forward 100 to 104). Bound by HBM: that backward 86 to 93
+// us (5.8 to 6.2 TB/s), forward 94 (5.7), in e4m3 76 (6.2).
 template <typename T, int kUnits>
 __global__ void __launch_bounds__(streamCta(kUnits, false), streamThreads(kUnits, false) / streamCta(kUnits, false))
     rmsNormStreamKernel(const NormParams p, int stages, unsigned *err) {

@@ -8,6 +8,8 @@ v adds two. So y is within half a step plus 2^-16 of v, relative; the sums of th
 backward pass alike, relative to the sums of their terms' magnitudes (dw: a CTA's
 columns one after another, 17 here, 32 warps of 19 rows, 32 sums: 2^-24 * 180 < 2^-16).
 """
+import ctypes
+
 import pytest
 import torch
 
@@ -267,3 +269,14 @@ def test_norm_past_32_bits(cuda, handle):
     handle.rms_norm_backward(k, n, CODE["bf16"], rows, k, x, ld, None, EPS, None, 0 + k, x, ld)
     handle.rms_norm_backward(k, n, CODE["bf16"], rows, k, rows, k, None, EPS, None, k, want, k)
     assert torch.equal(x.view(n, ld)[:, :k], want.view)
+
+
+@pytest.mark.parametrize("polls", [1, 100, 5000])
+def test_a_warp_that_gave_up_in_part_copies_nothing(cuda, lib, polls):
+    """A ring is filled by a warp whose lanes wait for themselves: after a wait that ran out
+    for some of them, none fills it (and none waits for the others)."""
+    gave_up = ctypes.c_int(-1)
+    assert lib.get_device_errors(clear=True) == 0
+    assert lib.lib.sgblasSelfTestWaitTimeout(polls, ctypes.byref(gave_up)) == 0
+    assert gave_up.value == 1
+    assert lib.get_device_errors(clear=True) & 1
