@@ -239,8 +239,8 @@ sgblasStatus_t sgblasScatterTokens(sgblasHandle_t handle, int k, int n, int top,
 /* And back: y(:, t) = sum over j of weights(j, t) * x(:, place(j, t)), x k x rows and
  * y k x n. Sums are FP32, in the order of j, rounded once; a choice without a
  * place adds nothing, whatever its weight, and a token without any gets zeros.
- * Choices may share a place. With weights NULL, the gradient of
- * sgblasScatterTokens without weights. */
+ * Choices may share a place; a token has at most 2^30 of them. With weights NULL,
+ * the gradient of sgblasScatterTokens without weights. */
 sgblasStatus_t sgblasGatherTokens(sgblasHandle_t handle, int k, int n, int top, int rows,
                                   const int *place, const float *weights, const void *x,
                                   sgblasDataType_t type, int ldx, void *y, int ldy);
@@ -251,7 +251,7 @@ sgblasStatus_t sgblasGatherTokens(sgblasHandle_t handle, int k, int n, int top, 
  *   dweights(j, t)     = sum over k of dy(k, t) * x(k, place(j, t))       (FP32; 0 for none)
  *
  * dweights NULL: not computed, x unused. No two choices may have the same place;
- * columns of dx that none has are left as they were. */
+ * columns of dx that none has are left as they were. At most 2^30 choices of a token. */
 sgblasStatus_t sgblasGatherTokensBackward(sgblasHandle_t handle, int k, int n, int top, int rows,
                                           const int *place, const float *weights, const void *dy,
                                           sgblasDataType_t type, int lddy, const void *x, int ldx,

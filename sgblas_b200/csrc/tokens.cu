@@ -30,6 +30,7 @@ constexpr int kSortWarpEntries = 64;   // of a warp, before another warp (CTA) j
 
 constexpr int kSortBatch = 8;          // entries of a lane whose loads are issued together
 constexpr int kSortMaxEntries = 1 << 30;
+constexpr int kMaxTop = 1 << 30;       // kBatch choices past the last are counted in 32 bits, too
 
 struct SortParams {
   const int *group;
@@ -537,6 +538,7 @@ extern "C" sgblasStatus_t sgblasGatherTokens(sgblasHandle_t handle, int k, int n
   if (k == 0 || n == 0) return SGBLAS_STATUS_SUCCESS;
   if (y == nullptr || (top > 0 && place == nullptr) || (top > 0 && rows > 0 && x == nullptr))
     return SGBLAS_STATUS_INVALID_VALUE;
+  if (top > kMaxTop) return SGBLAS_STATUS_NOT_SUPPORTED;
   DeviceInfo dev;
   const sgblasStatus_t st = currentDevice(&dev);
   if (st != SGBLAS_STATUS_SUCCESS) return st;
@@ -570,6 +572,7 @@ extern "C" sgblasStatus_t sgblasGatherTokensBackward(sgblasHandle_t handle, int 
       (rows > 0 && dweights != nullptr && x == nullptr))
     return SGBLAS_STATUS_INVALID_VALUE;
   if (rows == 0 && dweights == nullptr) return SGBLAS_STATUS_SUCCESS;
+  if (top > kMaxTop) return SGBLAS_STATUS_NOT_SUPPORTED;
   DeviceInfo dev;
   const sgblasStatus_t st = currentDevice(&dev);
   if (st != SGBLAS_STATUS_SUCCESS) return st;

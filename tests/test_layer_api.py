@@ -137,6 +137,13 @@ def test_gather_backward_has_nothing_to_do(handle, kw):
     assert handle.gather_tokens_backward_status(*move_back_args(**kw)) == OK
 
 
+def test_choices_of_a_token(handle):
+    """More are not counted in 32 bits, and would never end."""
+    for top in ((1 << 30) + 1, 2**31 - 1):
+        assert handle.gather_tokens_status(*move_args(top=top)) == UNSUPPORTED
+        assert handle.gather_tokens_backward_status(*move_back_args(top=top)) == UNSUPPORTED
+
+
 def quantize4_args(**kw):
     a = dict(k=301, n=20, x=FAKE, xtype=BF16, ldx=301, q=FAKE, ldq=151, scale=FAKE, ldscale=10, batch=2)
     a.update(kw)
