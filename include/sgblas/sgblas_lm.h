@@ -188,8 +188,8 @@ sgblasStatus_t sgblasOrthogonalize(sgblasHandle_t handle, int m, int n, int batc
  * are h to sum (NULL: not), v to y (NULL: not), and v in e4m3 to q (NULL: not),
  * with the scales in `scale`, as sgblasQuantizeFp8 with block_n = 1 writes them;
  * y or q has to be given. Everything between h and the roundings to y and q is
- * FP32, so squares of h have to stay in its range: magnitudes above 2^63 give 0, and
- * without an eps those below 2^-60 are inexact.
+ * FP32: the sum of h^2 over a column has to stay below 2^128 (4096 values of 2^57 do;
+ * from there on v is 0), and their mean, where eps is 0, at 2^-126 or above.
  * sum may be x or residual itself (the same address and leading dimension):
  * the residual is then updated in place. */
 sgblasStatus_t sgblasRmsNorm(sgblasHandle_t handle, int k, int n, sgblasDataType_t type,
@@ -203,6 +203,8 @@ sgblasStatus_t sgblasRmsNorm(sgblasHandle_t handle, int k, int n, sgblasDataType
  *   dx      = dsum + s * (g - h * s^2 * mean of (h * g))
  *   dweight = (*beta) * dweight + sum over the columns of dy * h * s       (FP32)
  *
+ * The sums of h^2 and of h * g over a column have to stay below 2^128 in magnitude,
+ * and the mean of h^2, where eps is 0, at 2^-126 or above.
  * dx is the gradient of x and of the residual alike; dsum (NULL: zero) that which
  * reaches h past the norm. dweight NULL: not computed, beta unused; *beta == 0
  * writes it without reading. Sums are FP32 in an order that depends on the sizes

@@ -9,6 +9,7 @@ backward pass alike, relative to the sums of their terms' magnitudes (dw: a CTA'
 columns one after another, 17 here, 32 warps of 19 rows, 32 sums: 2^-24 * 180 < 2^-16).
 """
 import ctypes
+import math
 
 import pytest
 import torch
@@ -182,6 +183,36 @@ def test_norm_special_values(cuda, handle):
         handle.rms_norm(k, n, CODE[type_], x, k, None, 0, w, 0.0, None, 0, y, k)
         assert bool(y.view[1].isnan().all())
         check_y(y.view[[0, 5]], definition(x.view, w.view, 0.0)[1][[0, 5]])
+
+
+@pytest.mark.parametrize("type_", ["bf16", "fp32"])
+@pytest.mark.parametrize("k,n", [(1, 3), (300, 4), (4096, 2), (4096, 800), (20011, 2)])
+def test_norm_to_the_ends_of_its_range(cuda, handle, type_, k, n):
+    """Sums of h^2 up to 2^128 (the values are +-1.75 * 2^e) and means from 2^-126 on."""
+    high = math.floor((127.9 - math.log2(1.75 ** 2 * k)) / 2)
+    _, _, dy, _, w = inputs(k, n, type_, seed=k)
+    sign = 1 - 2 * torch.randint(0, 2, (n, k), generator=generator(k), device="cuda").float()
+    blocks = -(-k // 128)
+    for size, eps in ((1.75 * 2.0 ** high, EPS), (2.0 ** -63, 0.0)):
+        x = Matrix(n, k, TYPES[type_], data=size * sign)
+        y, q, scale = Matrix(n, k, TYPES[type_]), Matrix(n, k, torch.uint8), Matrix(n, blocks, torch.float32)
+        handle.rms_norm(k, n, CODE[type_], x, k, None, 0, w, eps, None, 0, y, k, q, k, scale, blocks)
+        s, v = definition(x.view, w.view, eps)
+        check_y(y.view, v)
+        check_q(q.view, scale.view, v)
+        dx, dw = Matrix(n, k, TYPES[type_]), Matrix(1, k, torch.float32)
+        handle.rms_norm_backward(k, n, CODE[type_], dy, k, x, k, w, eps, None, k, dx, k, 0.0, dw)
+        h, d = x.view.double(), dy.view.double()
+        g = d * w.view.double()
+        want = s * (g - h * s * s * (h * g).mean(dim=1, keepdim=True))
+        sizes = s * (g.abs() + h.abs() * s * s * (h * g).abs().mean(dim=1, keepdim=True))
+        # Past 2^126 s^2 is subnormal: 2^-22 more.
+        assert bool(((dx.view.double() - want).abs() <= HALF[TYPES[type_]] * want.abs() + (SUMS + 2.0 ** -22) * sizes).all())
+        terms = d * h * s
+        assert bool(((dw.view[0].double() - terms.sum(dim=0)).abs() <= SUMS * terms.abs().sum(dim=0)).all())
+    x = Matrix(n, k, TYPES[type_], data=1.75 * 2.0 ** (high + 2) * sign)   # sums past 2^129
+    handle.rms_norm(k, n, CODE[type_], x, k, None, 0, w, EPS, None, 0, y, k)
+    assert bool((y.view == 0).all())
 
 
 def test_norm_backward_without_columns(cuda, handle):
