@@ -59,6 +59,11 @@ class Log:
         found = [line.split()[1:] for line in self.lines() if line.startswith("launch ")]
         return list(zip(demangled(f[0] for f in found), (int(f[1]) for f in found)))
 
+    def shapes(self):
+        """(kernel, grid.x, block.x, block.y, dynamic shared memory) of each launch."""
+        found = [line.split()[1:] for line in self.lines() if line.startswith("launch ")]
+        return [(name, *map(int, f[1:])) for name, f in zip(demangled(f[0] for f in found), found)]
+
     def kernels(self):
         """Every kernel that the library has."""
         return set(demangled(self.dll.fakeKernels().decode().split()))

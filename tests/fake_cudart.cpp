@@ -3,7 +3,7 @@
 // capability 10.0 with 148 SMs, memory that nothing reads, launches that run
 // nothing. What the library does is written to a log, a line per call:
 //
-//   launch <mangled kernel> <grid.x>     record     wait
+//   launch <mangled kernel> <grid.x> <block.x> <block.y> <shared bytes>     record     wait
 //   malloc <address> <bytes>             free <address>
 //
 // fakeFailLaunch(n) makes the n-th launch from now fail, fakeCapture(1) makes
@@ -40,9 +40,10 @@ std::string hex(const void *p) {
   return text;
 }
 
-cudaError_t launch(const void *kernel, dim3 grid) {
+cudaError_t launch(const void *kernel, dim3 grid, dim3 block, size_t smem) {
   if (fail_launch > 0 && --fail_launch == 0) return cudaErrorLaunchOutOfResources;
-  say("launch " + kernels()[kernel] + " " + std::to_string(grid.x));
+  say("launch " + kernels()[kernel] + " " + std::to_string(grid.x) + " " + std::to_string(block.x) + " " +
+      std::to_string(block.y) + " " + std::to_string(smem));
   return cudaSuccess;
 }
 
@@ -107,10 +108,10 @@ cudaError_t __cudaPopCallConfiguration(dim3 *grid, dim3 *block, size_t *smem, vo
 }
 
 cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t *config, const void *kernel, void **) {
-  return launch(kernel, config->gridDim);
+  return launch(kernel, config->gridDim, config->blockDim, config->dynamicSmemBytes);
 }
-cudaError_t cudaLaunchKernel(const void *kernel, dim3 grid, dim3, void **, size_t, cudaStream_t) {
-  return launch(kernel, grid);
+cudaError_t cudaLaunchKernel(const void *kernel, dim3 grid, dim3 block, void **, size_t smem, cudaStream_t) {
+  return launch(kernel, grid, block, smem);
 }
 cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int) { return cudaSuccess; }
 cudaError_t cudaOccupancyMaxActiveClusters(int *clusters, const void *,

@@ -7,6 +7,7 @@ from tests import fake_cuda
 from tests.fake_cuda import FAKE
 from tests.lm_cases import RAGGED
 from tests.test_fp4_gpu import DECREASING, ONE_MATRIX, PAIRS, SMALL
+from tests.test_norm_gpu import RINGS
 from tests.test_norm_gpu import SIZES as NORM_SIZES
 from tests.test_tokens_gpu import SIZES as TOKEN_SIZES
 
@@ -118,6 +119,28 @@ def test_a_failed_weight_gradient_is_a_use(log, at):
         assert h.rms_norm_backward_status(256, 100, BF16, FAKE, 256, FAKE, 256, FAKE, 1e-6, FAKE, 256, FAKE, 256, 0.0,
                                           FAKE) == sg.SGBLAS_STATUS_EXECUTION_FAILED
         assert log.lines()[-1] == "record"
+
+
+@pytest.mark.parametrize("type_,size", [(BF16, 2), (FP32, 4)])
+def test_rings_are_tested_past_their_stages(log, type_, size):
+    """Of each kernel fed by a ring a test's CTAs walk more than twice as many sets of
+    columns as it has stages, and one ends in part of a set where a set has several."""
+    turns, parts = {}, {}
+    with sg.Handle() as h:
+        for k, n in RINGS:
+            for residual in (FAKE, None):   # the stages are the same without
+                log.dll.fakeReset()
+                h.rms_norm(k, n, type_, FAKE, k, residual, k, FAKE, 1e-6, FAKE, k, FAKE, k)
+                h.rms_norm_backward(k, n, type_, FAKE, k, FAKE, k, FAKE, 1e-6, residual, k, FAKE, k, 0.0, FAKE)
+                for name, grid, _, columns, smem in log.shapes():
+                    if "Stream" not in name:
+                        continue
+                    stages = smem // ((3 if "Backward" in name else 2) * columns * k * size)
+                    turns[name] = max(turns.get(name, 0), -(-n // columns) / grid / stages)
+                    parts[name] = parts.get(name, False) or columns == 1 or n % columns != 0
+    every = {name for name in log.kernels() if "Stream" in name and ("<float" in name) == (type_ == FP32)}
+    assert len(every) == 6 and set(turns) == every
+    assert min(turns.values()) > 2 and all(parts.values()), turns
 
 
 @pytest.mark.parametrize("n,top,ctas", [(16, 4, 1), (1024, 2, 4), (1024, 8, 16), (65536, 8, 16)])

@@ -30,6 +30,13 @@ SIZES = [(1, 1), (1, 700), (7, 5), (8, 1), (8, 2500), (127, 3), (128, 2), (129, 
          (16384, 600), (16392, 3), (20011, 2)]
 
 
+# So many columns of whole vectors that each CTA's ring goes round more than twice, the
+# last set of columns in part (test_layer_dispatch.py). The gradients of the weights are
+# then sums of up to 40 columns in turn, 8 of a CTA, 19 rows of a warp, 32 warps, and s is
+# off as above: 2^-24 * (99 + 106) < 2^-16.
+RINGS = [(64, 100003), (504, 20001), (1000, 20001), (4096, 7001), (5120, 2001), (8200, 1501), (10240, 1501)]
+
+
 def inputs(k, n, type_, ld=0, shift=0, seed=0, scale=1.0):
     gen = generator(seed)
     make = lambda f: Matrix(n, k, TYPES[type_], k + ld, shift, (f * torch.randn(n, k, generator=gen, device="cuda")))  # noqa: E731
@@ -160,6 +167,58 @@ def test_norm_in_place(cuda, handle):
             ops = [Matrix(n, k, torch.bfloat16, data=dy.view), Matrix(n, k, torch.bfloat16, data=ds.view)]
             handle.rms_norm_backward(k, n, CODE["bf16"], ops[0], k, x, k, w, EPS, ops[1], k, ops[place], k, 0.0, dw2)
             assert torch.equal(ops[place].view, dx.view) and torch.equal(dw2.view, dw.view)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "fp32"])
+@pytest.mark.parametrize("k,n", RINGS)
+def test_norm_of_many_columns(cuda, handle, type_, k, n):
+    x, r, _, _, w = inputs(k, n, type_, seed=k)
+    t, blocks = TYPES[type_], -(-k // 128)
+    h, y = Matrix(n, k, t), Matrix(n, k, t)
+    q, scale = Matrix(n, k, torch.uint8), Matrix(n, blocks, torch.float32)
+    handle.rms_norm(k, n, CODE[type_], x, k, r, k, w, EPS, h, k, y, k, q, k, scale, blocks)
+    want_h = (x.view.float() + r.view.float()).to(t)
+    assert torch.equal(h.view, want_h)
+    v = definition(want_h, w.view)[1]
+    check_y(y.view, v)
+    check_q(q.view, scale.view, v)
+    assert not any(m.unmarked() for m in (x, r, w, h, y, q, scale))
+    y2 = Matrix(n, k, t)
+    handle.rms_norm(k, n, CODE[type_], h, k, None, 0, w, EPS, y=y2, ldy=k)   # one operand in the ring
+    assert torch.equal(y2.view, y.view)
+    for place in (0, 1):   # in place: columns ahead are on their way meanwhile
+        ops = [Matrix(n, k, t, data=x.view), Matrix(n, k, t, data=r.view)]
+        y2 = Matrix(n, k, t)
+        handle.rms_norm(k, n, CODE[type_], ops[0], k, ops[1], k, w, EPS, ops[place], k, y2, k)
+        assert torch.equal(ops[place].view, want_h) and torch.equal(y2.view, y.view)
+        assert torch.equal(ops[1 - place].view, (r if place == 0 else x).view)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "fp32"])
+@pytest.mark.parametrize("k,n", RINGS)
+def test_norm_gradients_of_many_columns(cuda, handle, type_, k, n):
+    x, _, dy, ds, w = inputs(k, n, type_, seed=k + 1)
+    t = TYPES[type_]
+    h, d = x.view.double(), dy.view.double()
+    s, _ = definition(x.view, None)
+    g = d * w.view.double()
+    want = s * (g - h * s * s * (h * g).mean(dim=1, keepdim=True))
+    size = s * (g.abs() + h.abs() * s * s * (h * g).abs().mean(dim=1, keepdim=True))
+    terms = d * h * s
+    want_w, size_w = terms.sum(dim=0), terms.abs().sum(dim=0)
+    for past in (False, True):
+        dx, dw = Matrix(n, k, t), Matrix(1, k, torch.float32)
+        handle.rms_norm_backward(k, n, CODE[type_], dy, k, x, k, w, EPS, ds if past else None, k, dx, k, 0.0, dw)
+        if past:
+            want, size = want + ds.view.double(), size + ds.view.double().abs()
+        assert bool(((dx.view.double() - want).abs() <= HALF[t] * want.abs() + SUMS * size).all())
+        assert bool(((dw.view[0].double() - want_w).abs() <= SUMS * size_w).all())
+        assert not any(m.unmarked() for m in (x, dy, ds, w, dx, dw))
+    for place in (0, 1):
+        ops = [Matrix(n, k, t, data=dy.view), Matrix(n, k, t, data=ds.view)]
+        dw2 = Matrix(1, k, torch.float32)
+        handle.rms_norm_backward(k, n, CODE[type_], ops[0], k, x, k, w, EPS, ops[1], k, ops[place], k, 0.0, dw2)
+        assert torch.equal(ops[place].view, dx.view) and torch.equal(dw2.view, dw.view)
 
 
 def test_norm_special_values(cuda, handle):
