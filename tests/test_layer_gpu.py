@@ -233,6 +233,18 @@ def test_the_example_serves_in_4_bits(cuda):
     assert sg.get_device_errors() == 0
 
 
+@pytest.mark.parametrize("tokens,width,hidden,experts", [(300, 256, 512, 6), (257, 130, 264, 5)])
+def test_the_example_in_4_bits_is_near_bf16(cuda, tokens, width, hidden, experts):
+    path = pathlib.Path(__file__).resolve().parent.parent / "examples" / "moe_layer.py"
+    spec = importlib.util.spec_from_file_location("moe_layer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    _, _, deviation = example.train_and_serve(tokens, width, hidden, experts, steps=2)
+    # Two products of two operands each, whose values are off by 2^-2 of themselves at most
+    # (test_a_layer_served_in_4_bits); outputs of nothing are off by 1, wrong ones by more.
+    assert 0 < deviation < 4 * 0.25 / 3 ** 0.5
+
+
 def test_one_handle_on_two_streams(cuda, lib):
     """Calls that use the handle's workspace (partial sums, laid-out scales) wait for
     each other, whichever streams they are on."""
