@@ -8,8 +8,9 @@ Every translation unit under sgblas_b200/csrc is compiled for
 ``sgblas_b200/lib/libsgblas.so`` together with a static CUDA runtime, so the
 library does not depend on whichever libcudart another package (torch) loaded.
 Objects are rebuilt only when a source or header is newer than the object.
-Where Python's headers are installed, calls.c becomes sgblas_b200/_calls*.so, the
-compiled caller of the shortest entry points (without it they go by ctypes).
+Where it compiles (Python's headers, 3.10 or newer, and a C compiler), calls.c becomes
+sgblas_b200/_calls*.so, the compiled caller of the shortest entry points; without it
+they go by ctypes.
 """
 from __future__ import annotations
 
@@ -69,19 +70,31 @@ def _compile(src: pathlib.Path, verbose: bool) -> pathlib.Path:
 
 
 def _build_calls() -> None:
+    """calls.c, or nothing: without Python's headers, a C compiler or a Python that it
+    compiles for, the package goes by ctypes. What an older source left is not kept."""
     include = pathlib.Path(sysconfig.get_paths()["include"])
     src, out = PKG / "calls.c", PKG / f"_calls{sysconfig.get_config_var('EXT_SUFFIX')}"
-    if not (include / "Python.h").exists():
-        return
     newest = max(p.stat().st_mtime for p in (src, INCLUDE / "sgblas" / "sgblas.h", INCLUDE / "sgblas" / "sgblas_lm.h"))
     if out.exists() and out.stat().st_mtime >= newest:
         return
-    tmp = out.with_suffix(".tmp")
-    res = subprocess.run(["gcc", "-std=gnu11", "-O2", "-fPIC", "-shared", "-Wall", "-Wextra", f"-I{include}",
-                          f"-I{INCLUDE}", str(src), "-o", str(tmp)], capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"compiling calls.c failed:\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, out)
+    problem = None
+    cc = next(filter(None, map(shutil.which, filter(None, (os.environ.get("CC"), "gcc", "cc")))), None)
+    tmp = out.with_name(f"{out.name}.{os.getpid()}.tmp")   # of this process: several may build at once
+    if not (include / "Python.h").exists():
+        problem = f"no Python.h in {include}"
+    elif cc is None:
+        problem = "no C compiler"
+    else:
+        res = subprocess.run([cc, "-std=gnu11", "-O2", "-fPIC", "-shared", "-Wall", "-Wextra", f"-I{include}",
+                              f"-I{INCLUDE}", str(src), "-o", str(tmp)], capture_output=True, text=True)
+        if res.returncode != 0:
+            problem = f"{cc} failed:\n{res.stdout}\n{res.stderr}"
+    if problem is None:
+        os.replace(tmp, out)
+        return
+    tmp.unlink(missing_ok=True)
+    out.unlink(missing_ok=True)
+    sys.stderr.write(f"calls.c was not compiled, its entry points go by ctypes: {problem}\n")
 
 
 def build(verbose: bool = False) -> pathlib.Path:
