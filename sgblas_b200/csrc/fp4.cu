@@ -60,9 +60,11 @@ __device__ __forceinline__ uint32_t eightOf(const float2 (&f)[4]) {
 }
 
 // Two threads to a block of 32, 16 consecutive values each, kUnroll blocks per
-// thread whose loads are issued together. Memory-bound (16384 x 8192 BF16 57 us,
-// 5.9 TB/s). kAligned: 16 values start on 16 bytes of x; otherwise they are read as
-// vectors all the same, and moved into place (8192 x 4095 by single values 195 us).
+// thread whose loads are issued together. Memory-bound (16384 x 8192 BF16 51 to 53 us, 6.4
+// to 6.6 TB/s). kAligned: 16 values start on 16 bytes of x; otherwise they are read as
+// vectors all the same, and moved into place: 8192 x 4095 20 us in a row, 23 from HBM, for
+// a floor of 13 (by single values 195), bound by neither HBM nor issue (61 % of the slots)
+// alone.
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kQuantThreads) quantizeFp4Kernel(const QuantParams p) {
   constexpr int kPer = 16, kVectors = kPer * static_cast<int>(sizeof(T)) / 16;
@@ -301,13 +303,20 @@ sgblasStatus_t launchThin(const DeviceInfo &dev, const NarrowOperand &a, const N
 // groups: a group is taken to end in half a tile.
 //
 // Thin tiles, whose k several CTAs may share, pay while a group has few tokens (4 x
-// 4096 x 4096, 8 tokens each: 7.9 us, 11.8 in 128 columns; 16: 8.0 and 7.9; 1 x 4096 x
-// 4096, 32 tokens: 8.1 and 7.4), those of 32 columns where groups of more than 16 are to
-// be expected (384 tokens unevenly over 32 x 2048 x 2048, with their quantisation:
-// 16.3 us in 16 columns, 15.4 in 32, 17.6 in 128). A wave of single tiles takes 0.40 us
-// a slice of k and no less than 2.2, of pairs 0.44 and 3.1, with 3 us for the scales'
-// blocks (32 x 2048 x 2048, 256 tokens each: singles 27.7 us, pairs 32.1; 512: 48.3 and
-// 44.5; 2048: 180 and 142; 16 x 1024 x 2048, 1024: 24.8 and 25.9).
+// 4096 x 4096, 8 tokens each: 11.0 us in 16 columns, 16.8 in 128; 16: 10.4 and 8.2), those
+// of 32 columns where groups of more than 16 are to be expected (384 tokens unevenly over
+// 32 x 2048 x 2048, with their quantisation: 16.3 us in 16 columns, 15.4 in 32, 17.6 in
+// 128). A wave of single tiles takes 0.40 us a slice of k and no less than 2.2, of pairs
+// 0.44 and 3.1, with 3 us for the scales' blocks (32 x 2048 x 2048, 512 tokens each:
+// singles 48.7 us, pairs 44.8; 2048: 181 and 145; 16 x 1024 x 2048, 2048: 46 and 41).
+//
+// Against the best of the four widths the rule loses 2.6 % in the geometric mean over 153
+// shapes with even groups, 1.4 % over 85 with uneven ones, more than 10 % in 11 and 5 of
+// them. It errs towards pairs where a wave or two of them stand against full waves of single
+// tiles (4 x 4096 x 4096, 96 tokens each: pairs taken, 14.3 us, singles 9.2; 256: 19.3 and
+// 14.3; 32 x 2048 x 2048, 256: 32.0 and 27.2), and towards thin tiles where m and k are
+// small (1 x 1024 x 1024, 12 tokens: 5.5 in 32 columns, 4.2 in 128): its least times are
+// those of long waves, and below 14 tokens it looks at the mean alone.
 int chooseWidth(const DeviceInfo &dev, const t::Params &p) {
   const int active = std::min(p.groups, p.n);
   const double mean = static_cast<double>(p.n) / std::max(p.groups, 1);

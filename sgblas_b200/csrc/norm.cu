@@ -105,8 +105,6 @@ __device__ __forceinline__ void addResidual(Lanes<T, kVector> *h, const Lanes<T,
   for (int i = 0; i < Lanes<T, kVector>::kPairs; ++i) h->setPair(i, __fadd2_rn(h->pair(i), r.pair(i)));
 }
 
-// What a thread does with its values of a column, whichever way they came: `rest`
-// values of the column are there from the thread's place `at` on.
 // A thread's weights: ones where there are none.
 template <typename T, bool kVector>
 __device__ __forceinline__ void loadWeight(const void *weight, int k, int slot, Lanes<T, kVector> *w) {
@@ -120,6 +118,8 @@ __device__ __forceinline__ void loadWeight(const void *weight, int k, int slot, 
   }
 }
 
+// What a thread does with its values of a column, whichever way they came: `rest`
+// values of the column are there from the thread's place `at` on.
 template <typename T, bool kVector>
 struct NormOf {
   using L = Lanes<T, kVector>;
@@ -201,6 +201,10 @@ __device__ __forceinline__ float2 backwardFactors(float2 sums, float over_k, flo
 }
 
 // ---- few columns, or columns that are not whole vectors ----------------------------
+
+// Many columns of odd places are bound by their accesses of single values, latency and
+// issue, not by HBM: 16384 x 4095 BF16 forward 173 us (floor 82), e4m3 190 (72), backward 240
+// (82); 8192 x 4095 FP32 106, 99 (67) and 126.
 
 // A column per blockDim.x threads, kUnits vectors (or groups of four values) per
 // thread; kLong: longer columns than that, read twice.

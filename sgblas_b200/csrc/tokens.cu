@@ -321,8 +321,9 @@ __device__ __forceinline__ float sumFour(const float (&v)[4], int lane) {
 // y(:, place(j, t)) = weight(j, t) dy(:, t) and, with dweight,
 // dweight(j, t) = sum over k of dy(k, t) x(k, place(j, t)); a CTA's row of
 // blockDim.x threads per token, so that dy is read once for kBatch choices and dweight
-// needs no second pass. Bound by HBM: the same tokens 86 us (6.4 TB/s); 3001 tokens with
-// 3 choices, 1537 values on odd addresses, 20 us (3.1 TB/s).
+// needs no second pass. Bound by HBM: the same tokens 86 to 89 us (6.4 TB/s); 3001 tokens with
+// 3 choices, 1537 values on odd addresses, by accesses of one value: 19 us (3.3 TB/s), 12.5
+// where L2 has them; 8192 with 8, 2047 values, 133 (scattered 68, gathered 71).
 template <typename T, bool kVector>
 __global__ void __launch_bounds__(kGatherThreads, 8) gatherTokensBackwardKernel(const MoveParams p) {
   using L = Lanes<T, kVector>;
